@@ -168,7 +168,8 @@ def run(state):
     if own:
         got = state["thunk"](*state["arrays"])
         got = got if isinstance(got, tuple) else (got,)
-        return tuple(t.mT if t.dim() == 2 else t for t in map(torch.from_dlpack, got))
+        stream = torch.cuda.current_stream().cuda_stream or 1
+        return tuple(t.mT if t.dim() == 2 else t for t in (torch.from_dlpack(x.__dlpack__(stream=stream)) for x in got))
     case = state["case"]
     return {"embedding": _embedding, "embedding_grad": _embedding_grad, "dropout": _dropout, "token_logprobs": _token_logprobs,
             "token_logprobs_grad": _token_logprobs_grad}[case["op"]](case, *state["in"])
