@@ -125,6 +125,23 @@ RxBuffer* CopyBufferToDevice(RxBuffer* buffer, RxDevice* dst_device);
 void CopyToBuffer(RxClient* client, RxBuffer* buffer, void* data, size_t offset, size_t size, RxBuffer** bufferP);
 void CopyFromBuffer(RxClient* client, RxBuffer* buffer, void* data, size_t offset, size_t size, RxBuffer** bufferP);
 
+/* Exchange of arrays with other libraries on the same device, without a copy, as
+ * DLPack tensors (no counterpart in the reference, whose CUDA arrays are wrapped
+ * by pointer, ext/ReactantCUDAExt.jl).  Both carry the Julia view of an array:
+ * dims reversed, first dim contiguous.
+ * RxBufferToDLPack returns a DLManagedTensor that shares the buffer's memory and
+ * makes `consumer_stream` (a cudaStream_t; 1 = the legacy default stream, 2 = the
+ * per-thread one, -1 = no ordering wanted) wait for the work queued so far.  The
+ * consumer calls its deleter, after which the memory is used again only behind
+ * what that stream held at that time.
+ * RxBufferFromDLPack makes a buffer over the tensor's memory and, if it succeeds,
+ * takes the tensor over: its deleter is called once the buffer is freed and the
+ * work queued with it is done.  The producer has to have ordered the device's
+ * stream (RxDeviceStream) behind its own writes.  The array has to be dense and
+ * start on a 16-byte boundary; other arrays are refused and stay the caller's. */
+void* RxBufferToDLPack(RxBuffer* buffer, void* consumer_stream);
+RxBuffer* RxBufferFromDLPack(RxDevice* device, void* dl_managed_tensor);
+
 /* ---- futures (API.cpp:1357-1373) ------------------------------------------ */
 void FreeFuture(RxFuture* future);
 uint8_t FutureIsReady(RxFuture* future);

@@ -522,6 +522,8 @@ class Interpreter:
             return self._reduce_window(op, env)
         if short == "while":
             return self._while(op, env)
+        if short == "custom_call":
+            return self._custom_call(op, env)
         if short == "all_reduce":
             # single-address-space evaluation: the operand already is the global value
             return _operands(text, env, len(name))[0]
@@ -601,6 +603,71 @@ class Interpreter:
             r = piece if r is None else ufunc(r, piece)
         return make(np.asarray(r).reshape(oshape), et)
 
+    def _custom_call(self, op, env):
+        """The token-model operators, in float64 from their definitions (no counterpart in the reference)."""
+        target = re.search(r"@([\w.]+)\(([^)]*)\)", op.text)
+        args = [env[n.strip()] for n in target.group(2).split(",")]
+        cfg = {k: float(v) for k, v in re.findall(r"(\w+)\s*=\s*([-+.\w]+)\s*:\s*(?:f64|f32|i64|i32)\b", re.search(r"backend_config\s*=\s*\{([^}]*)\}", op.text).group(1))}
+        outs = _types_after_colon(op.text)
+        name = target.group(1)
+        if name == "rx.embedding":
+            table, ids = args
+            i = ids.a.astype(np.int64)
+            live = (i >= 0) & (i < table.shape[0])
+            padded = np.concatenate([_wide(table), np.zeros((1, table.shape[1]))])
+            return [make(cfg.get("scale", 1.0) * padded[np.where(live, i, table.shape[0])], outs[0][1])]
+        if name == "rx.embedding_grad":
+            dy, ids = args
+            i = ids.a.astype(np.int64).reshape(-1)
+            rows = _wide(dy).reshape(len(i), -1) if len(i) else np.zeros((0, outs[0][0][1]))
+            total = np.zeros(outs[0][0])
+            live = (i >= 0) & (i < total.shape[0])
+            np.add.at(total, i[live], rows[live])
+            return [make(cfg.get("scale", 1.0) * total, outs[0][1])]
+        if name == "rx.dropout":
+            x = args[0]
+            keep = dropout_mask(x.a.size, args[1].a, cfg["rate"], int(cfg.get("site", 0))).reshape(x.shape)
+            cut = math.floor(cfg["rate"] * 65536 + 0.5)
+            y = np.where(keep, _wide(x) * (65536.0 / (65536.0 - cut)), 0.0)
+            return [make(y + _wide(args[2]) if len(args) > 2 else y, outs[0][1])]
+        if name == "rx.token_logprobs":
+            logits, ids = args
+            with np.errstate(invalid="ignore", divide="ignore"):
+                z = _wide(logits) / cfg.get("temperature", 1.0)
+                top = z.max(axis=-1, keepdims=True)
+                e = np.where(z == -np.inf, 0.0, np.exp(z - np.where(top == -np.inf, 0.0, top)))
+                s = e.sum(axis=-1)
+                empty = top[..., 0] == -np.inf
+                lse = np.where(empty, -np.inf, top[..., 0] + np.log(s))
+                h = np.where(empty, 0.0, np.log(s) - np.where(e > 0, e * (z - top), np.where(np.isnan(e), np.nan, 0.0)).sum(axis=-1) / s)
+                i = ids.a.astype(np.int64)
+                live = (i >= 0) & (i < z.shape[-1])
+                chosen = np.take_along_axis(z, np.where(live, i, 0)[..., None], -1)[..., 0]
+                lp = np.where(live, np.where(empty, -np.inf, chosen - lse), 0.0)
+                res = [make(lp, "f32"), make(h, "f32"), make(lse, "f32")]
+                k = int(cfg.get("top_k", 0))
+                if k:
+                    # larger value first (NaN above everything), then the lower index; ranked on the logits themselves
+                    rank = np.where(np.isnan(logits.a), np.inf, logits.a.astype(np.float64))
+                    order = np.lexsort((np.broadcast_to(np.arange(z.shape[-1]), z.shape), -rank, ~np.isnan(logits.a)), axis=-1)[..., :k]
+                    res += [make(np.where(empty[..., None], -np.inf, np.take_along_axis(z, order, -1) - lse[..., None]), "f32"), make(order, "i32")]
+            return res
+        if name == "rx.token_logprobs_grad":
+            logits, ids, lse, h, g, gh, gl = args
+            t = cfg.get("temperature", 1.0)
+            i = ids.a.astype(np.int64)
+            live = (i >= 0) & (i < logits.shape[-1])
+            col = lambda v: _wide(v)[..., None]  # noqa: E731
+            g64 = np.where(live, _wide(g), 0.0)[..., None]
+            empty = (lse.a == -np.inf)[..., None]
+            with np.errstate(invalid="ignore"):
+                logp = _wide(logits) / t - col(lse)
+                p = np.where(empty, 0.0, np.exp(logp))
+                dz = np.where(p == 0, 0.0, p * (col(gl) - g64 - col(gh) * (np.where(p == 0, 0.0, logp) + col(h))))
+                dz = dz + np.where(empty, 0.0, (np.arange(logits.shape[-1]) == i[..., None]) * g64)
+            return [make(dz / t, outs[0][1])]
+        raise NotImplementedError(f"oracle: unsupported custom_call @{name}")
+
     def _while(self, op, env):
         text = op.text
         pairs = re.findall(r"(%[\w#.$-]+)\s*=\s*(%[\w#.$-]+)", text[text.index("(") + 1:text.index(")")])
@@ -620,6 +687,22 @@ class Interpreter:
             guard += 1
             assert guard < 1_000_000, "runaway loop"
         return list(state)
+
+
+def dropout_mask(n, key, rate, site=0, first=0):
+    """Which of the elements first .. first + n - 1 stay: 16 bits each of Philox4x32-10 (Salmon, Moraes, Dror and Shaw,
+    SC 2011) at the counters (element // 8, site), low halves of words first."""
+    lo, groups = first // 8, (first + n + 7) // 8 - first // 8
+    g = np.arange(lo, lo + groups, dtype=np.uint64)
+    mask, sh = np.uint64(0xFFFFFFFF), np.uint64(32)
+    c = [g & mask, g >> sh, np.full(groups, site, np.uint64), np.zeros(groups, np.uint64)]
+    k = [np.uint64(int(v) & 0xFFFFFFFF) for v in np.asarray(key).reshape(-1)]
+    for _ in range(10):
+        a, b = c[0] * np.uint64(0xD2511F53), c[2] * np.uint64(0xCD9E8D57)
+        c = [(b >> sh) ^ c[1] ^ k[0], b & mask, (a >> sh) ^ c[3] ^ k[1], a & mask]
+        k = [(k[0] + np.uint64(0x9E3779B9)) & mask, (k[1] + np.uint64(0xBB67AE85)) & mask]
+    half = np.ascontiguousarray(np.stack(c, 1).astype("<u4")).view("<u2").reshape(-1)
+    return half[first - 8 * lo:first - 8 * lo + n] >= math.floor(rate * 65536 + 0.5)
 
 
 def run_module(text, inputs, func="main"):

@@ -303,6 +303,54 @@ class ConcreteRArray:
             b.device.synchronize()
 
 
+    # The array API's exchange of device arrays (DLPack): `torch.from_dlpack(y)` and the like see the same memory.
+    def __dlpack_device__(self):
+        return (_DL_CUDA, lib().PjRtDeviceGetLocalHardwareId(self._single().device.handle))
+
+    def __dlpack__(self, *, stream=None, max_version=None, dl_device=None, copy=None):
+        """Hand the array out without a copy, in its Julia shape (first dimension contiguous).  `stream` is the consumer's
+        stream, which is made to wait for the work queued here: None or 1 the legacy default one, -1 no waiting."""
+        if copy or (dl_device is not None and tuple(dl_device) != self.__dlpack_device__()):
+            raise BufferError("the array can only be handed out as it is, on its own device")
+        p = lib().RxBufferToDLPack(self._single().handle, (1 if stream is None else stream) & 0xFFFFFFFFFFFFFFFF)
+        if not p:
+            check()
+        return _PyCapsule_New(p, b"dltensor", _dl_drop)
+
+    def _single(self) -> "_Buffer":
+        if len(self.data) != 1 or (self.sharding is not None and not self.replicated and self.sharding.sharded_dim() is not None):
+            raise BufferError("an array spread over several devices has no single memory to exchange")
+        return self.data[0]
+
+
+# DLPack capsules: the names and the rule that the consumer renames the capsule are the specification's.
+_DL_CUDA = 2
+_PyCapsule_New = C.pythonapi.PyCapsule_New
+_PyCapsule_New.restype, _PyCapsule_New.argtypes = C.py_object, [C.c_void_p, C.c_char_p, C.c_void_p]
+_PyCapsule_GetPointer = C.pythonapi.PyCapsule_GetPointer
+_PyCapsule_GetPointer.restype, _PyCapsule_GetPointer.argtypes = C.c_void_p, [C.py_object, C.c_char_p]
+_PyCapsule_SetName = C.pythonapi.PyCapsule_SetName
+_PyCapsule_SetName.restype, _PyCapsule_SetName.argtypes = C.c_int, [C.py_object, C.c_char_p]
+_DL_USED = b"used_dltensor"
+
+
+_capsules = C.PyDLL(None)  # its own function objects: a capsule that is being destroyed is only an address
+_capsules.PyCapsule_IsValid.argtypes = _capsules.PyCapsule_GetPointer.argtypes = [C.c_void_p, C.c_char_p]
+_capsules.PyCapsule_GetPointer.restype = C.c_void_p
+
+
+@C.CFUNCTYPE(None, C.c_void_p)
+def _dl_drop_unused(capsule):
+    # a capsule that nobody consumed still owns its tensor, whose last field (after the 48 bytes of the tensor's
+    # description and the context) is its deleter
+    if _capsules.PyCapsule_IsValid(capsule, b"dltensor"):
+        tensor = _capsules.PyCapsule_GetPointer(capsule, b"dltensor")
+        C.CFUNCTYPE(None, C.c_void_p)(C.c_void_p.from_address(tensor + 56).value)(tensor)
+
+
+_dl_drop = C.cast(_dl_drop_unused, C.c_void_p)
+
+
 class ConcreteRNumber(ConcreteRArray):
     """ConcretePJRTNumber{T,D}: a rank-0 array (src/Types.jl:155-211)."""
 
@@ -352,6 +400,29 @@ def to_rarray(x, client: Client | None = None, device: Device | None = None, sha
             piece = a[tuple(sl)]
         bufs.append(_upload(client, dev, piece))
     return ConcreteRArray(bufs, a.shape, a.dtype, sharding=sharding, replicated=d is None)
+
+
+def from_dlpack(x, client: Client | None = None, device: Device | None = None) -> ConcreteRArray:
+    """An array of another library (a torch tensor, say) on one of this client's devices, as a ConcreteRArray over the
+    same memory.  Its shape is the Julia shape, so its first dimension has to be the contiguous one: a row-major matrix
+    is handed over as its transposed view.  The array has to be dense and start on a 16-byte boundary.  Work queued here
+    waits for what the producer's current stream holds; the memory goes back to its owner when the array is gone and
+    the work that uses it is done."""
+    client = client or default_client()
+    kind, ordinal = x.__dlpack_device__()
+    if device is None:
+        device = next((d for d in client.addressable_devices if kind == _DL_CUDA and lib().PjRtDeviceGetLocalHardwareId(d.handle) == ordinal), None)
+        if device is None:
+            raise ReactantError(12, f"the array is on device ({int(kind)}, {ordinal}), which is not one of this client's")
+    capsule = x.__dlpack__(stream=lib().RxDeviceStream(device.handle))
+    h = lib().RxBufferFromDLPack(device.handle, _PyCapsule_GetPointer(capsule, b"dltensor"))
+    if not h:
+        check()
+    _PyCapsule_SetName(capsule, _DL_USED)
+    buf = _Buffer(h, device)
+    dims = buf.dims
+    cls = ConcreteRNumber if not dims else ConcreteRArray
+    return cls([buf], tuple(reversed(dims)), buf.dtype)
 
 
 def from_local_shards(pieces, global_shape, sharding: NamedSharding, client: Client | None = None):

@@ -69,6 +69,8 @@ PROTOTYPES = {
     "CopyBufferToDevice": (P, [P, P]),
     "CopyToBuffer": (None, [P, P, P, C.c_size_t, C.c_size_t, PP]),
     "CopyFromBuffer": (None, [P, P, P, C.c_size_t, C.c_size_t, PP]),
+    "RxBufferToDLPack": (P, [P, P]),
+    "RxBufferFromDLPack": (P, [P, P]),
     "FreeFuture": (None, [P]),
     "FutureIsReady": (C.c_uint8, [P]),
     "FutureAwait": (None, [P]),

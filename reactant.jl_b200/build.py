@@ -18,6 +18,7 @@ OBJ = os.path.join(HERE, "build")
 SOURCES = [
     "rx_parser.cpp", "rx_plan.cpp", "rx_kernels.cu", "rx_wide.cu", "rx_gemm.cu", "rx_gemm_tc.cu",
     "rx_stencil.cu", "rx_stencil_tma.cu", "rx_collective.cu", "rx_runtime.cu", "rx_noalloc.cu", "rx_abi_extra.cu", "rx_jit.cpp",
+    "rx_embedding.cu", "rx_dropout.cu", "rx_logprobs.cu",
 ]
 
 # Device headers handed to NVRTC by name when a fused chain is specialised at run time.

@@ -46,7 +46,7 @@ struct Type {
 enum class OpK {
   Constant, Iota, Unary, Binary, Convert, Compare, Select, Clamp,
   BroadcastInDim, Transpose, Reshape, Slice, DynamicSlice, DynamicUpdateSlice, Pad, Concatenate,
-  DotGeneral, Reduce, ReduceWindow, While, AllReduce, Return
+  DotGeneral, Reduce, ReduceWindow, While, AllReduce, CustomCall, Return
 };
 
 enum class RedK { Add, Max, Min, Mul, Or, And };
@@ -74,6 +74,9 @@ struct Op {
   // dot_general
   std::vector<int64_t> lbatch, rbatch, lcontract, rcontract;
   RedK red = RedK::Add;
+  // custom_call: the target's name and the entries of its backend_config dictionary
+  std::string target;
+  std::map<std::string, double> config;
   std::vector<Region> regions;  // while: {cond, body}
   int line = 0;
 };

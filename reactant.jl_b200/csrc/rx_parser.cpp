@@ -596,6 +596,59 @@ struct Parser {
     }
   }
 
+  // %r:2 = stablehlo.custom_call @rx.name(%a, %b) {api_version = 4 : i32, backend_config = {key = 1.0 : f32, ..}}
+  //          : (tensor<..>, tensor<..>) -> (tensor<..>, tensor<..>)
+  // -- the typed form of the op: its settings are the entries of the backend_config dictionary, numbers and truth
+  // values each.  Which targets exist, and what they take, is the planner's business.
+  void parse_custom_call(Op& op, std::vector<Type>* ins, std::vector<Type>* outs) {
+    op.kind = OpK::CustomCall;
+    expect("@");
+    op.target = ident();
+    expect("(");
+    if (!accept(")")) {
+      do op.in.push_back(use()); while (accept(","));
+      expect(")");
+    }
+    ws();
+    if (peek("{"))
+      for (auto& kv : split_top(balanced_text('{', '}'))) {
+        const size_t eq = kv.find('=');
+        const std::string key = trim(eq == std::string::npos ? kv : kv.substr(0, eq));
+        const std::string value = eq == std::string::npos ? "" : trim(kv.substr(eq + 1));
+        if (key == "backend_config") {
+          if (value.size() < 2 || value.front() != '{' || value.back() != '}')
+            fail(RX_ERR_PARSE, "stablehlo.custom_call @" + op.target + ": backend_config is not a dictionary");
+          for (auto& entry : split_top(value.substr(1, value.size() - 2))) {
+            const size_t e2 = entry.find('=');
+            if (e2 == std::string::npos) fail(RX_ERR_PARSE, "stablehlo.custom_call @" + op.target + ": malformed backend_config entry '" + trim(entry) + "'");
+            const std::string name = trim(entry.substr(0, e2)), rest = trim(entry.substr(e2 + 1));
+            const size_t colon = rest.find(':');
+            const std::string number = trim(rest.substr(0, colon)), et = colon == std::string::npos ? "" : trim(rest.substr(colon + 1));
+            double f = 0;
+            int64_t i = 0;
+            bool is_float = false;
+            if (number == "true" || number == "false") {
+              f = number == "true";
+            } else if (number.compare(0, 2, "0x") == 0 || number.compare(0, 2, "0X") == 0) {
+              scalar_token(number, elem_type(et), &f, &i, &is_float);
+            } else {
+              char* end = nullptr;
+              f = strtod(number.c_str(), &end);
+              if (number.empty() || *end) fail(RX_ERR_PARSE, "stablehlo.custom_call @" + op.target + ": backend_config entry '" + name + "' is not a number");
+            }
+            if (!op.config.emplace(name, f).second) fail(RX_ERR_PARSE, "stablehlo.custom_call @" + op.target + ": backend_config entry '" + name + "' is given twice");
+          }
+        } else if (key == "called_computations" || key == "output_operand_aliases" || key == "operand_layouts" || key == "result_layouts") {
+          if (value != "[]") fail(RX_ERR_UNSUPPORTED_OP, "unsupported op stablehlo.custom_call @" + op.target + " with " + key);
+        }
+      }
+    signature(ins, outs);
+    if (ins->size() != op.in.size()) fail(RX_ERR_PARSE, "stablehlo.custom_call @" + op.target + ": " + std::to_string(ins->size()) + " operand types for " + std::to_string(op.in.size()) + " operands");
+    for (size_t k = 0; k < ins->size(); ++k)
+      if (!((*ins)[k] == m->values[op.in[k]].type))
+        fail(RX_ERR_PARSE, "stablehlo.custom_call @" + op.target + ": operand " + std::to_string(k) + " is " + m->values[op.in[k]].type.str() + ", its signature says " + (*ins)[k].str());
+  }
+
   void parse_op(Region& region, bool* saw_return) {
     ws();
     int line = line_at(p);
@@ -868,6 +921,9 @@ struct Parser {
       bool ok = false;
       for (auto& r : reds) if (applied == r.first) { op.red = r.second; ok = true; }
       if (!ok) fail(RX_ERR_UNSUPPORTED_OP, "unsupported op stablehlo.reduce applying " + applied);
+      finish(op, res, outs);
+    } else if (shortn == "custom_call") {
+      parse_custom_call(op, &ins, &outs);
       finish(op, res, outs);
     } else if (shortn == "while") {
       op.kind = OpK::While;

@@ -2555,6 +2555,288 @@ struct Planner {
       }
     }
   }
+  // ---- custom calls: the operators of a token model (rx_token.h) ------------------------------------------------
+  // A call's operands are read from memory: values that are still lazy expressions are materialised first.  The
+  // operand that is read row by row may stay a window of a wider array (logits padded to a multiple of something and
+  // cut to the vocabulary): only its innermost dim has to be contiguous and the others have to merge into one.
+  //
+  // On a mesh the calls are local to a token, so operands and results split along a token dimension stay split the
+  // same way; the lookup's gradient then is a sum over the devices (all-reduced), and dropout numbers the elements as
+  // they lie in the whole array, so that the mask does not depend on the number of devices.
+  std::string call_error(const Op& op, const std::string& what) { return op.name + " @" + op.target + ": " + what; }
+  void call_arity(const Op& op, size_t lo, size_t hi, size_t outs_lo, size_t outs_hi) {
+    if (op.in.size() < lo || op.in.size() > hi || op.out.size() < outs_lo || op.out.size() > outs_hi)
+      throw Error(RX_ERR_ARG, call_error(op, "takes " + std::to_string(lo) + (hi > lo ? " to " + std::to_string(hi) : "") + " operands and has " + std::to_string(outs_lo) +
+                                                 (outs_hi > outs_lo ? " or " + std::to_string(outs_hi) : "") + " results, got " + std::to_string(op.in.size()) + " and " + std::to_string(op.out.size())));
+  }
+  // the entries of backend_config this call knows; anything else is refused rather than ignored
+  double call_setting(const Op& op, const std::string& key, double otherwise) {
+    auto it = op.config.find(key);
+    return it == op.config.end() ? otherwise : it->second;
+  }
+  void call_known_settings(const Op& op, std::initializer_list<const char*> known) {
+    for (auto& kv : op.config) {
+      bool ok = false;
+      for (const char* k : known) ok = ok || kv.first == k;
+      if (!ok) throw Error(RX_ERR_ARG, call_error(op, "unknown setting '" + kv.first + "'"));
+    }
+  }
+  void call_dtype(const Op& op, int v, std::initializer_list<DT> allowed, const char* what) {
+    const DT dt = m.values[v].type.dt;
+    for (DT a : allowed)
+      if (dt == a) return;
+    throw Error(RX_ERR_UNSUPPORTED_TYPE, "unsupported element type " + std::string(dt_name(dt)) + " for " + what + " of " + op.name + " @" + op.target);
+  }
+  void call_shape(const Op& op, int v, const std::vector<int64_t>& want, const char* what) {
+    const Type& t = m.values[v].type;
+    if (t.shape != want) throw Error(RX_ERR_SHAPE, call_error(op, std::string(what) + " is " + t.str() + ", expected " + Type{t.dt, want}.str()));
+  }
+  // operand -> (slot, element offset), dense; `zero_ok`: a constant zero need not exist in memory
+  void call_operand(Step& st, int v, const Type& local, const char* why, bool zero_ok = false) {
+    ExprP e = env[v];
+    if (e->k == Expr::Const) {
+      if (zero_ok && e->f == 0.0) {
+        st.leaf_slot.push_back(-1);
+        st.call.off.push_back(0);
+        return;
+      }
+      e = konst(local, e->f, e->i);  // a constant has no sharding: this device's share of it
+    }
+    if (!contiguous_leaf(e)) {
+      e = materialised(e, why);
+      if (!contiguous_leaf(e)) {  // a strided window: copied into place
+        const Type t{e->dt, e->shape};
+        const int s = new_slot(t);
+        emit_map(e, s, 0, canon_strides(t.shape), why);
+        e = leaf(s, t);
+      }
+    }
+    st.leaf_slot.push_back(e->slot);
+    st.call.off.push_back(e->loffset);
+  }
+  // the row-wise operand: also sets call.ld
+  void call_rows_operand(Step& st, int v, const Type& local, const char* why) {
+    MatView mv;
+    const size_t rank = local.shape.size();
+    if (env[v]->k != Expr::Const && as_strided_leaf(env[v], &mv)) {
+      bool ok = local.shape[rank - 1] <= 1 || mv.stride[rank - 1] == 1;
+      int64_t ld = -1, span = 1;
+      for (int d = (int)rank - 2; d >= 0; --d) {
+        if (local.shape[d] == 1) continue;
+        if (ld < 0) ld = mv.stride[d];
+        else ok = ok && mv.stride[d] == ld * span;
+        span *= local.shape[d];
+      }
+      if (ok && ld >= -1) {
+        st.leaf_slot.push_back(mv.slot);
+        st.call.off.push_back(mv.off);
+        st.call.ld = ld < 0 ? local.shape[rank - 1] : ld;
+        return;
+      }
+    }
+    call_operand(st, v, local, why);
+    st.call.ld = local.shape[rank - 1];
+  }
+  // The common token dimension along which the given operands are split, or -1.  Constants take any sharding.
+  int call_shard(const Op& op, const std::vector<int>& vs, size_t token_rank) {
+    int s = -1;
+    for (int v : vs) s = std::max(s, shard[v]);
+    if (s < 0) return -1;
+    if (s >= (int)token_rank) throw Error(RX_ERR_UNSUPPORTED_OP, "unsupported op " + op.name + " @" + op.target + " with an operand sharded along the rows' own dimension");
+    for (int v : vs)
+      if (shard[v] != s && env[v]->k != Expr::Const)
+        throw Error(RX_ERR_UNSUPPORTED_OP, "unsupported op " + op.name + " @" + op.target + ": operands are not sharded alike");
+    return s;
+  }
+  Type call_local(int v, int s) const {
+    Type t = m.values[v].type;
+    if (s >= 0) t.shape[s] /= nparts;
+    return t;
+  }
+
+  void plan_custom_call(const Op& op) {
+    struct Target { const char* name; CallK k; };
+    static const Target targets[] = {{"rx.embedding", CallK::Embedding}, {"rx.embedding_grad", CallK::EmbeddingGrad}, {"rx.dropout", CallK::Dropout},
+                                     {"rx.token_logprobs", CallK::LogProbs}, {"rx.token_logprobs_grad", CallK::LogProbsGrad}};
+    Step st;
+    st.kind = StepK::Call;
+    CallDesc& c = st.call;
+    for (auto& t : targets)
+      if (op.target == t.name) c.op = t.k;
+    if (c.op == CallK::None) throw Error(RX_ERR_UNSUPPORTED_OP, "unsupported op " + op.name + " @" + op.target);
+    auto shape_of = [&](int v) -> const std::vector<int64_t>& { return m.values[v].type.shape; };
+    auto dtype_of = [&](int v) { return m.values[v].type.dt; };
+    auto positive = [&](const char* key, double v) {
+      if (!(v > 0) || std::isinf(v)) throw Error(RX_ERR_ARG, call_error(op, std::string(key) + " has to be a positive finite number"));
+      return v;
+    };
+    std::ostringstream note;
+    int s = -1;
+    bool all_reduce = false;
+    switch (c.op) {
+      case CallK::Embedding: {
+        call_arity(op, 2, 2, 1, 1);
+        call_known_settings(op, {"scale"});
+        const int table = op.in[0], ids = op.in[1], out = op.out[0];
+        call_dtype(op, table, {DT::F32, DT::BF16}, "the table");
+        call_dtype(op, ids, {DT::S32, DT::S64}, "the ids");
+        call_dtype(op, out, {DT::F32, DT::BF16}, "the result");
+        if (shape_of(table).size() != 2) throw Error(RX_ERR_SHAPE, call_error(op, "the table is " + m.values[table].type.str() + ", expected a matrix"));
+        std::vector<int64_t> want = shape_of(ids);
+        want.push_back(shape_of(table)[1]);
+        call_shape(op, out, want, "the result");
+        if (shard[table] >= 0) throw Error(RX_ERR_UNSUPPORTED_OP, "unsupported op " + op.name + " @" + op.target + " of a sharded table");
+        s = call_shard(op, {ids}, want.size() - 1);
+        c.scale = call_setting(op, "scale", 1);
+        if (!std::isfinite(c.scale)) throw Error(RX_ERR_ARG, call_error(op, "scale has to be finite"));
+        c.in_dt = dtype_of(table);
+        c.out_dt = dtype_of(out);
+        c.ids_dt = dtype_of(ids);
+        c.vocab = shape_of(table)[0];
+        c.cols = shape_of(table)[1];
+        c.rows = prod(call_local(ids, s).shape);
+        call_rows_operand(st, table, m.values[table].type, "embedding table");
+        call_operand(st, ids, call_local(ids, s), "token ids");
+        note << "embedding of " << c.rows << " tokens, table " << c.vocab << " x " << c.cols;
+        break;
+      }
+      case CallK::EmbeddingGrad: {
+        call_arity(op, 2, 2, 1, 1);
+        call_known_settings(op, {"scale"});
+        const int dy = op.in[0], ids = op.in[1], out = op.out[0];
+        call_dtype(op, dy, {DT::F32, DT::BF16}, "the gradient");
+        call_dtype(op, ids, {DT::S32, DT::S64}, "the ids");
+        call_dtype(op, out, {DT::F32, DT::BF16}, "the result");
+        if (shape_of(out).size() != 2) throw Error(RX_ERR_SHAPE, call_error(op, "the result is " + m.values[out].type.str() + ", expected a matrix"));
+        std::vector<int64_t> want = shape_of(ids);
+        want.push_back(shape_of(out)[1]);
+        call_shape(op, dy, want, "the gradient");
+        s = call_shard(op, {dy, ids}, want.size() - 1);
+        if (s >= 0 && dtype_of(out) != DT::F32) throw Error(RX_ERR_UNSUPPORTED_TYPE, "unsupported element type " + std::string(dt_name(dtype_of(out))) + " for a gradient that is summed over the mesh");
+        c.scale = call_setting(op, "scale", 1);
+        if (!std::isfinite(c.scale)) throw Error(RX_ERR_ARG, call_error(op, "scale has to be finite"));
+        c.in_dt = dtype_of(dy);
+        c.out_dt = dtype_of(out);
+        c.ids_dt = dtype_of(ids);
+        c.vocab = shape_of(out)[0];
+        c.cols = shape_of(out)[1];
+        c.rows = prod(call_local(ids, s).shape);
+        call_rows_operand(st, dy, call_local(dy, s), "gradient of the looked-up rows");
+        call_operand(st, ids, call_local(ids, s), "token ids");
+        all_reduce = s >= 0;
+        s = -1;  // the result is replicated
+        note << "embedding gradient of " << c.rows << " tokens, table " << c.vocab << " x " << c.cols;
+        break;
+      }
+      case CallK::Dropout: {
+        call_arity(op, 2, 3, 1, 1);
+        call_known_settings(op, {"rate", "site"});
+        const int x = op.in[0], key = op.in[1], out = op.out[0];
+        call_dtype(op, x, {DT::F32, DT::BF16}, "the operand");
+        call_dtype(op, key, {DT::S32}, "the key");
+        call_shape(op, key, {2}, "the key");
+        call_shape(op, out, shape_of(x), "the result");
+        call_dtype(op, out, {dtype_of(x)}, "the result");
+        std::vector<int> like = {x};
+        if (op.in.size() == 3) {
+          call_shape(op, op.in[2], shape_of(x), "the residual");
+          call_dtype(op, op.in[2], {dtype_of(x)}, "the residual");
+          like.push_back(op.in[2]);
+        }
+        if (!op.config.count("rate")) throw Error(RX_ERR_ARG, call_error(op, "needs a rate"));
+        c.rate = call_setting(op, "rate", 0);
+        if (!(c.rate >= 0 && c.rate < 1) || dropout_threshold(c.rate) > 65535)
+          throw Error(RX_ERR_ARG, call_error(op, "the rate is kept in steps of 1/65536 and has to be at least 0 and below 1 - 1/131072"));
+        const double site = call_setting(op, "site", 0);
+        if (!(site >= 0 && site < 4294967296.0) || site != std::floor(site)) throw Error(RX_ERR_ARG, call_error(op, "site has to be a whole number from 0 to 2^32 - 1"));
+        c.site = (int64_t)site;
+        if (shard[key] >= 0) throw Error(RX_ERR_UNSUPPORTED_OP, "unsupported op " + op.name + " @" + op.target + " with a sharded key");
+        s = call_shard(op, like, shape_of(x).size());
+        if (s >= 0)
+          for (int d = 0; d < s; ++d)
+            if (shape_of(x)[d] != 1) throw Error(RX_ERR_UNSUPPORTED_OP, "unsupported op " + op.name + " @" + op.target + " sharded along a dimension other than the first");
+        const Type t = call_local(x, s);
+        c.sharded = s >= 0;
+        c.in_dt = c.out_dt = t.dt;
+        c.rows = 1;
+        c.cols = prod(t.shape);
+        call_operand(st, x, t, "dropout operand");
+        call_operand(st, key, m.values[key].type, "dropout key");
+        if (op.in.size() == 3) call_operand(st, op.in[2], t, "dropout residual");
+        note << "dropout(" << c.rate << ") of " << c.cols << " elements" << (op.in.size() == 3 ? " + residual" : "");
+        break;
+      }
+      case CallK::LogProbs:
+      case CallK::LogProbsGrad: {
+        const bool grad = c.op == CallK::LogProbsGrad;
+        if (grad) {
+          call_arity(op, 7, 7, 1, 1);
+          call_known_settings(op, {"temperature"});
+        } else {
+          call_arity(op, 2, 2, 3, 5);
+          call_known_settings(op, {"temperature", "top_k"});
+        }
+        const int logits = op.in[0], ids = op.in[1];
+        call_dtype(op, logits, {DT::F32, DT::BF16}, "the logits");
+        call_dtype(op, ids, {DT::S32, DT::S64}, "the ids");
+        if (shape_of(logits).empty()) throw Error(RX_ERR_SHAPE, call_error(op, "the logits are a scalar"));
+        std::vector<int64_t> tokens = shape_of(logits);
+        c.cols = c.vocab = tokens.back();
+        tokens.pop_back();
+        call_shape(op, ids, tokens, "the ids operand");
+        c.scale = 1.0 / positive("temperature", call_setting(op, "temperature", 1));
+        if (!(c.scale < INFINITY) || (float)c.scale <= 0.f || std::isinf((float)c.scale)) throw Error(RX_ERR_ARG, call_error(op, "temperature is out of the range of 32-bit floats"));
+        std::vector<int> like = {logits, ids};
+        for (size_t k = 2; k < op.in.size(); ++k) {
+          static const char* names[] = {"lse", "entropy", "dlogprob", "dentropy", "dlse"};
+          call_dtype(op, op.in[k], {DT::F32}, names[k - 2]);
+          call_shape(op, op.in[k], tokens, names[k - 2]);
+          like.push_back(op.in[k]);
+        }
+        s = call_shard(op, like, tokens.size());
+        c.in_dt = dtype_of(logits);
+        c.ids_dt = dtype_of(ids);
+        c.rows = prod(call_local(ids, s).shape);
+        if (grad) {
+          call_shape(op, op.out[0], shape_of(logits), "the result");
+          call_dtype(op, op.out[0], {c.in_dt}, "the result");
+          c.out_dt = c.in_dt;
+        } else {
+          const double k = call_setting(op, "top_k", 0);
+          if (!(k >= 0 && k <= kMaxTopK) || k != std::floor(k) || k > (double)c.vocab)
+            throw Error(RX_ERR_ARG, call_error(op, "top_k has to be a whole number from 0 to " + std::to_string(kMaxTopK) + ", and no more than the vocabulary"));
+          c.top_k = (int)k;
+          if ((op.out.size() == 5) != (c.top_k > 0) || op.out.size() == 4) throw Error(RX_ERR_ARG, call_error(op, "has three results without top_k and five with it"));
+          for (size_t q = 0; q < op.out.size(); ++q) {
+            std::vector<int64_t> want = tokens;
+            if (q >= 3) want.push_back(c.top_k);
+            call_shape(op, op.out[q], want, "a result");
+            call_dtype(op, op.out[q], {q == 4 ? DT::S32 : DT::F32}, "a result");
+          }
+        }
+        call_rows_operand(st, logits, call_local(logits, s), "logits");
+        call_operand(st, ids, call_local(ids, s), "token ids");
+        for (size_t k = 2; k < op.in.size(); ++k) call_operand(st, op.in[k], call_local(op.in[k], s), "row value", k >= 4);
+        note << (grad ? "gradient of token log probabilities, " : "token log probabilities, ") << c.rows << " tokens, vocabulary " << c.vocab;
+        if (c.top_k) note << ", top " << c.top_k;
+        break;
+      }
+      default: break;
+    }
+    if (c.rows > INT32_MAX || c.vocab > INT32_MAX) throw Error(RX_ERR_TOO_LARGE, call_error(op, "more than 2^31 - 1 tokens or entries of the vocabulary"));
+    for (int v : op.out) {
+      shard[v] = s;
+      const Type t = local_type(v);
+      const int slot = new_slot(t);
+      st.out_slot.push_back(slot);
+      env[v] = leaf(slot, t);
+    }
+    st.note = note.str();
+    cur->push_back(std::move(st));
+    last_map.where = nullptr;
+    if (all_reduce) emit_allreduce(env[op.out[0]]->slot, local_type(op.out[0]));
+  }
+
   int materialise_copy(const ExprP& e) {
     Type t{e->dt, e->shape};
     int s = new_slot(t);
@@ -2584,6 +2866,7 @@ struct Planner {
         case OpK::Concatenate: plan_concat(op); break;
         case OpK::DotGeneral: plan_dot(op); break;
         case OpK::While: plan_while(op); break;
+        case OpK::CustomCall: plan_custom_call(op); break;
         default: throw Error(RX_ERR_UNSUPPORTED_OP, "unsupported op " + op.name);
       }
       if (op.kind != OpK::While)
@@ -2670,8 +2953,8 @@ struct Planner {
   }
 };
 
-const char* step_name(StepK k) {
-  switch (k) {
+const char* step_name(const Step& s) {
+  switch (s.kind) {
     case StepK::Map: return "map";
     case StepK::ReduceFull: return "reduce_full";
     case StepK::ReduceRow: return "reduce_row";
@@ -2688,6 +2971,7 @@ const char* step_name(StepK k) {
     case StepK::RowsIn: return "rows_in";
     case StepK::RowsOut: return "rows_out";
     case StepK::DynSlice: return "dyn_slice";
+    case StepK::Call: return call_name(s.call.op);
   }
   return "?";
 }
@@ -2707,7 +2991,7 @@ void describe_steps(std::ostringstream& os, const std::vector<Step>& steps) {
   for (size_t k = 0; k < steps.size(); ++k) {
     const Step& s = steps[k];
     if (k) os << ",";
-    os << "{\"kind\":\"" << step_name(s.kind) << "\",\"note\":\"" << s.note << "\"";
+    os << "{\"kind\":\"" << step_name(s) << "\",\"note\":\"" << s.note << "\"";
     if (s.kind == StepK::Map || s.kind == StepK::ReduceFull || s.kind == StepK::ReduceRow || s.kind == StepK::ReduceCol || s.kind == StepK::Stencil || s.kind == StepK::LogSumExp) {
       os << ",\"chain\":\"" << fast_name(s.prog.fast_id) << "\",\"instrs\":" << s.prog.n_instr << ",\"leaves\":" << s.prog.n_leaves
          << ",\"linear\":" << s.prog.all_linear << ",\"rank\":" << s.prog.rank << ",\"dims\":[";

@@ -8,6 +8,7 @@
 #include <vector>
 
 #include "rx_ir.h"
+#include "rx_token.h"
 #include "rx_vm.h"
 
 namespace rx {
@@ -29,7 +30,7 @@ struct Slot {
   int64_t bytes() const { return type.numel() * (int64_t)dt_size(type.dt); }
 };
 
-enum class StepK { Map, ReduceFull, ReduceRow, ReduceCol, LogSumExp, Stencil, Gemm, Copy, Fill, Loop, AllReduce, Scan, SumPartials, RowsIn, RowsOut, DynSlice };
+enum class StepK { Map, ReduceFull, ReduceRow, ReduceCol, LogSumExp, Stencil, Gemm, Copy, Fill, Loop, AllReduce, Scan, SumPartials, RowsIn, RowsOut, DynSlice, Call };
 
 struct GemmDesc {
   // D[m][n] = sum_k A(m,k) * B(k,n); strides in elements of the operand slots.
@@ -76,6 +77,7 @@ struct Step {
   int st_radius = 0;
   std::vector<int> st_dy, st_dx;  // per leaf
   GemmDesc gemm;
+  CallDesc call;                  // Call: leaf_slot = operands, out_slot = results
   // Copy / Fill
   int src_slot = -1, dst_slot = -1;
   int64_t bytes = 0;

@@ -15,9 +15,11 @@
 
 #include "../../include/rx_b200.h"
 #include "rx_collective.h"
+#include "rx_dlpack.h"
 #include "rx_gemm.h"
 #include "rx_jit.h"
 #include "rx_stencil.h"
+#include "rx_token.h"
 
 using namespace rx;
 
@@ -151,6 +153,50 @@ void RxDevice::trim() {
     for (void* p : kv.second) cudaFree(p);
 }
 
+void RxDevice::hand_back(void* tensor) {
+  auto* t = (rx::DLManagedTensor*)tensor;
+  if (closed.load()) {  // everything that was queued has drained
+    if (t->deleter) t->deleter(t);
+    return;
+  }
+  int cur = 0;
+  cudaGetDevice(&cur);
+  cudaSetDevice(ordinal);
+  Returned r{tensor, nullptr};
+  if (cudaEventCreateWithFlags(&r.done, cudaEventDisableTiming) != cudaSuccess || cudaEventRecord(r.done, stream) != cudaSuccess) {
+    cudaGetLastError();
+    cudaStreamSynchronize(stream);
+  }
+  {
+    std::lock_guard<std::mutex> lk(mu);
+    returned.push_back(r);
+    n_returned.store((int)returned.size());
+  }
+  reap(false);
+  cudaSetDevice(cur);
+}
+
+void RxDevice::reap(bool all) {
+  if (!n_returned.load()) return;
+  std::vector<Returned> done;
+  {
+    std::lock_guard<std::mutex> lk(mu);
+    size_t kept = 0;
+    for (auto& r : returned) {
+      if (all || !r.done || cudaEventQuery(r.done) == cudaSuccess) done.push_back(r);
+      else returned[kept++] = r;
+    }
+    returned.resize(kept);
+    n_returned.store((int)kept);
+  }
+  cudaGetLastError();  // "not ready" is no error
+  for (auto& r : done) {  // outside the lock: the owner's code runs here
+    if (r.done) cudaEventDestroy(r.done);
+    auto* t = (rx::DLManagedTensor*)r.tensor;
+    if (t->deleter) t->deleter(t);
+  }
+}
+
 cudaEvent_t EventState::event() {
   std::lock_guard<std::mutex> g(ev_mu);
   if (ev) return ev;
@@ -185,6 +231,7 @@ namespace {
 
 struct DevRun {
   RxDevice* dev;
+  const Plan* plan;
   std::vector<std::shared_ptr<Storage>> table;  // per slot
   // slots with an all-reduce still running on the device's communication stream, and the event that ends it
   std::map<int, cudaEvent_t> pending;
@@ -202,7 +249,8 @@ void join_pending(DevRun& r, int slot) {
 }
 void join_pending_of(DevRun& r, const Step& st) {
   if (r.pending.empty()) return;
-  for (int s : st.leaf_slot) join_pending(r, s);
+  for (int s : st.leaf_slot)
+    if (s >= 0) join_pending(r, s);
   for (int s : st.out_slot) join_pending(r, s);
   for (int s : {st.gemm.a_slot, st.gemm.b_slot, st.gemm.d_slot, st.src_slot, st.dst_slot})
     if (s >= 0) join_pending(r, s);
@@ -324,6 +372,7 @@ const char* kind_name(StepK k) {
     case StepK::RowsIn: return "rows_in";
     case StepK::RowsOut: return "rows_out";
     case StepK::DynSlice: return "dyn_slice";
+    case StepK::Call: return "call";
   }
   return "?";
 }
@@ -414,6 +463,44 @@ bool operands_settled(DevRun& r, const Step& st) {
       if (w == p) return false;
   }
   return true;
+}
+
+// The operators of a token model (rx_token.h).  The workspace goes back to the pool as soon as the launches are queued:
+// whoever gets the block next uses it in stream order, after them.
+void run_call(DevRun& r, const Step& st) {
+  RxDevice* d = r.dev;
+  const CallDesc& c = st.call;
+  const LaunchCtx ctx = d->ctx();
+  auto in = [&](size_t k) -> const void* {
+    const int slot = st.leaf_slot[k];
+    if (slot < 0) return nullptr;
+    return (const char*)slot_ptr(r, slot) + c.off[k] * (int64_t)dt_size(r.plan->slots[slot].type.dt);
+  };
+  auto out = [&](size_t k) { return k < st.out_slot.size() ? slot_ptr(r, st.out_slot[k]) : nullptr; };
+  std::shared_ptr<Storage> work;
+  auto workspace = [&](int64_t bytes) -> void* {
+    if (!bytes) return nullptr;
+    work = std::make_shared<Storage>(d, d->alloc((size_t)bytes), (size_t)bytes);
+    return work->ptr;
+  };
+  switch (c.op) {
+    case CallK::Embedding: CK(launch_embedding(ctx, c, in(0), in(1), out(0))); break;
+    case CallK::EmbeddingGrad: CK(launch_embedding_grad(ctx, c, in(0), in(1), out(0), workspace(embedding_grad_workspace(c, d->sm_count)))); break;
+    case CallK::Dropout:
+      CK(launch_dropout(ctx, c, in(0), in(1), st.leaf_slot.size() > 2 ? in(2) : nullptr, out(0), c.sharded ? (int64_t)d->global_id * c.cols : 0));
+      break;
+    case CallK::LogProbs: {
+      const LogProbsOut o{(float*)out(0), (float*)out(1), (float*)out(2), (float*)out(3), (int32_t*)out(4)};
+      CK(launch_logprobs(ctx, c, in(0), in(1), o, workspace(logprobs_workspace(c, d->sm_count))));
+      break;
+    }
+    case CallK::LogProbsGrad: {
+      const LogProbsGradIn g{(const float*)in(2), (const float*)in(3), (const float*)in(4), (const float*)in(5), (const float*)in(6)};
+      CK(launch_logprobs_grad(ctx, c, in(0), in(1), g, out(0)));
+      break;
+    }
+    default: throw Error(RX_ERR_PLAN, "internal: unknown call");
+  }
 }
 
 void run_one(RxExecutable* ex, const Step& st, DevRun& r, const FusedAllReduce* fused = nullptr) {
@@ -546,6 +633,11 @@ void run_one(RxExecutable* ex, const Step& st, DevRun& r, const FusedAllReduce* 
         off += start * st.dyn_stride[k];
       }
       CK(cudaMemcpyAsync(slot_ptr(r, st.dst_slot), (const char*)slot_ptr(r, st.src_slot) + off * st.dyn_elem_bytes, (size_t)st.bytes, cudaMemcpyDeviceToDevice, d->stream));
+      break;
+    }
+    case StepK::Call: {
+      run_call(r, st);
+      if (!by_note) ps.kind = call_name(st.call.op);
       break;
     }
     default:
@@ -805,12 +897,16 @@ void execute(RxExecutable* ex, const std::vector<RxDevice*>& devs, RxBuffer** ar
   std::sort(order.begin(), order.end(), [](RxDevice* a, RxDevice* b) { return a->ordinal < b->ordinal; });
   order.erase(std::unique(order.begin(), order.end()), order.end());
   std::vector<std::unique_lock<std::mutex>> held;
-  for (RxDevice* d : order) held.emplace_back(d->exec_mu);
+  for (RxDevice* d : order) {
+    d->reap(false);
+    held.emplace_back(d->exec_mu);
+  }
   std::vector<DevRun> runs(devs.size());
   for (size_t k = 0; k < devs.size(); ++k) {
     RxDevice* d = devs[k];
     DevRun& r = runs[k];
     r.dev = d;
+    r.plan = &p;
     r.table.resize(p.slots.size());
     CK(cudaSetDevice(d->ordinal));
     for (int i = 0; i < nargs_per_dev; ++i) check_arg(p, i, args[k * nargs_per_dev + i], d);
@@ -852,6 +948,7 @@ void execute(RxExecutable* ex, const std::vector<RxDevice*>& devs, RxBuffer** ar
       }
     }
   }
+  for (RxDevice* d : order) d->enqueued.fetch_add(1);
   run_steps(ex, p.steps, runs);
   // All-reduces still in flight on the communication stream: a result keeps the event (its future and its next user
   // wait for it), so the compute stream is free to start the next execution; anything else is joined now.
@@ -1023,7 +1120,10 @@ void FreeClient(RxClient* client) {
     cudaSetDevice(d->ordinal);
     cudaStreamSynchronize(d->stream);
     if (d->comm_stream) cudaStreamSynchronize(d->comm_stream);
+    d->reap(true);
     d->trim();
+    if (d->order) cudaEventDestroy(d->order);
+    d->order = nullptr;
     if (d->scratch) cudaFree(d->scratch);
     if (d->flush_buf) cudaFree(d->flush_buf);
     if (d->status) cudaFreeHost(d->status);
@@ -1191,6 +1291,134 @@ void* UnsafeBufferPointer(RxBuffer* b) {
     check_device_status(b->dev);
   }
   return b->st->ptr;
+  API_END(nullptr)
+}
+
+// ---- exchange with other libraries on the same device ------------------------------------------------------------
+namespace {
+constexpr intptr_t kNoOrder = -1;  // the array API's "no synchronisation wanted"
+
+struct HandedOut {
+  rx::DLManagedTensor t;
+  std::vector<int64_t> shape, strides;
+  std::shared_ptr<Storage> st;
+  cudaStream_t consumer;
+  bool ordered;
+};
+
+// The consumer is done with the tensor on the host, but its stream may still be reading: the memory carries an event
+// of that stream, which the next use here (or the pool, before it hands the block out again) waits for.
+void handed_out_deleter(rx::DLManagedTensor* t) {
+  std::unique_ptr<HandedOut> h((HandedOut*)t->manager_ctx);
+  RxDevice* d = h->st->dev;
+  if (!h->ordered || d->closed.load()) return;
+  int cur = 0;
+  cudaGetDevice(&cur);
+  if (cur != d->ordinal) cudaSetDevice(d->ordinal);
+  cudaEvent_t ev = nullptr;
+  if (cudaEventCreateWithFlags(&ev, cudaEventDisableTiming) != cudaSuccess || cudaEventRecord(ev, h->consumer) != cudaSuccess) {
+    cudaGetLastError();  // the consumer's stream is gone: everything it had queued is waited for instead
+    if (ev) cudaEventDestroy(ev);
+    cudaDeviceSynchronize();
+  } else {
+    h->st->make_ready();
+    std::lock_guard<std::mutex> g(h->st->pending_mu);
+    if (h->st->pending) {
+      cudaStreamWaitEvent(d->stream, h->st->pending, 0);
+      cudaEventDestroy(h->st->pending);
+    }
+    h->st->pending = ev;
+  }
+  h.reset();
+  if (cur != d->ordinal) cudaSetDevice(cur);
+}
+
+rx::DLDataType dl_type(DT t) {
+  const uint8_t bits = (uint8_t)(8 * dt_size(t));
+  if (t == DT::PRED) return {rx::kDLBool, 8, 1};
+  if (t == DT::BF16) return {rx::kDLBfloat, 16, 1};
+  if (dt_is_float(t)) return {rx::kDLFloat, bits, 1};
+  return {t >= DT::U8 ? rx::kDLUInt : rx::kDLInt, bits, 1};
+}
+}  // namespace
+
+void* RxBufferToDLPack(RxBuffer* b, void* consumer_stream) {
+  API_BEGIN
+  live(b);
+  RxDevice* d = b->dev;
+  if (d->closed.load()) throw Error(RX_ERR_BAD_HANDLE, "the client that owns this device was freed");
+  if (b->dt == DT::C64 || b->dt == DT::C128) throw Error(RX_ERR_UNSUPPORTED_TYPE, std::string("unsupported element type ") + dt_name(b->dt) + " in an exchange of arrays");
+  if (!consumer_stream) throw Error(RX_ERR_ARG, "a consumer's stream of 0 is ambiguous: 1 is the legacy default stream, 2 the per-thread one, -1 none");
+  auto h = std::make_unique<HandedOut>();
+  h->st = b->st;
+  h->ordered = (intptr_t)consumer_stream != kNoOrder;
+  h->consumer = (cudaStream_t)consumer_stream;
+  if (h->ordered) {
+    int cur = 0;
+    cudaGetDevice(&cur);
+    if (cur != d->ordinal) CK(cudaSetDevice(d->ordinal));
+    const bool late = b->st->pending != nullptr;
+    b->st->make_ready();
+    std::lock_guard<std::mutex> g(d->order_mu);
+    if (!d->order) CK(cudaEventCreateWithFlags(&d->order, cudaEventDisableTiming));
+    const uint64_t now = d->enqueued.load();
+    if (now != d->ordered || late) {
+      CK(cudaEventRecord(d->order, d->stream));
+      d->ordered = now;
+    }
+    CK(cudaStreamWaitEvent(h->consumer, d->order, 0));
+    if (cur != d->ordinal) CK(cudaSetDevice(cur));
+  }
+  // the Julia view of the array: dims reversed, first dim contiguous
+  const size_t n = b->dims.size();
+  h->shape.assign(b->dims.rbegin(), b->dims.rend());
+  h->strides.resize(n);
+  int64_t step = 1;
+  for (size_t k = 0; k < n; ++k) {
+    h->strides[k] = step;
+    step *= std::max<int64_t>(1, h->shape[k]);
+  }
+  h->t.dl_tensor = {b->st->ptr, {rx::kDLCUDA, d->ordinal}, (int32_t)n, dl_type(b->dt), h->shape.data(), h->strides.data(), 0};
+  h->t.manager_ctx = h.get();
+  h->t.deleter = handed_out_deleter;
+  return &h.release()->t;
+  API_END(nullptr)
+}
+
+RxBuffer* RxBufferFromDLPack(RxDevice* d, void* tensor) {
+  API_BEGIN
+  if (!d || !d->addressable) throw Error(RX_ERR_BAD_HANDLE, "device is null or not addressable from this process");
+  if (!tensor) throw Error(RX_ERR_BAD_HANDLE, "null tensor");
+  const rx::DLTensor& t = ((rx::DLManagedTensor*)tensor)->dl_tensor;
+  if (t.device.device_type != rx::kDLCUDA || t.device.device_id != d->ordinal)
+    throw Error(RX_ERR_ARG, "the array is not in the memory of CUDA device " + std::to_string(d->ordinal));
+  DT dt = DT::INVALID;
+  for (DT k : {DT::PRED, DT::S8, DT::S16, DT::S32, DT::S64, DT::U8, DT::U16, DT::U32, DT::U64, DT::F16, DT::F32, DT::F64, DT::BF16}) {
+    const rx::DLDataType q = dl_type(k);
+    if (q.code == t.dtype.code && q.bits == t.dtype.bits && t.dtype.lanes == 1) dt = k;
+  }
+  if (dt == DT::INVALID) throw Error(RX_ERR_UNSUPPORTED_TYPE, "unsupported element type in an exchange of arrays (code " + std::to_string(t.dtype.code) + ", " + std::to_string(t.dtype.bits) + " bits)");
+  auto b = std::make_unique<RxBuffer>();
+  b->dt = dt;
+  b->dev = d;
+  int64_t step = 1, row_major = 1;
+  std::vector<int64_t> dense((size_t)t.ndim);
+  for (int k = t.ndim - 1; k >= 0; --k) {  // the strides that a missing array of strides stands for
+    dense[k] = row_major;
+    row_major *= t.shape[k];
+  }
+  for (int k = 0; k < t.ndim; ++k) {
+    const int64_t stride = t.strides ? t.strides[k] : dense[k];
+    if (row_major != 0 && t.shape[k] != 1 && stride != step)
+      throw Error(RX_ERR_ARG, "the array is not dense with its first dimension contiguous (dimension " + std::to_string(k) + " has stride " + std::to_string(stride) + ", expected " + std::to_string(step) + ")");
+    step *= t.shape[k];
+  }
+  for (int k = t.ndim - 1; k >= 0; --k) b->dims.push_back(t.shape[k]);
+  char* ptr = (char*)t.data + t.byte_offset;
+  if (row_major != 0 && (uintptr_t)ptr % 16) throw Error(RX_ERR_ARG, "the array does not start on a 16-byte boundary: hand over a copy of it");
+  b->st = std::make_shared<Storage>(d, ptr, b->bytes());
+  b->st->foreign = tensor;
+  return own(b.release());
   API_END(nullptr)
 }
 

@@ -75,6 +75,18 @@ struct RxDevice : std::enable_shared_from_this<RxDevice> {
   bool mail_own[kMaxRanks] = {};          // entry maps one of this process's own mailboxes (no IPC mapping to close)
   bool mail_ready = false;
   std::map<const void*, std::vector<uint8_t>> tmaps;  // tensor-map cache keyed by base pointer
+  // Exchange of arrays with other libraries on the same device (DLPack).  Memory that was taken over goes back to its
+  // owner only when the work queued here has passed `done`; memory that was handed out carries the event its consumer
+  // left (Storage::pending).
+  struct Returned { void* tensor; cudaEvent_t done; };
+  std::vector<Returned> returned;          // guarded by mu
+  std::atomic<int> n_returned{0};
+  std::mutex order_mu;                     // guards the next two
+  cudaEvent_t order = nullptr;             // recorded on `stream` when a consumer needs to wait for it and executions were queued since the last time
+  uint64_t ordered = 0;                    // value of `enqueued` then
+  std::atomic<uint64_t> enqueued{1};       // executions queued so far
+  void hand_back(void* tensor);            // memory taken over is no longer used by anything that will be queued
+  void reap(bool all);                     // owners whose memory is free now get it back
 
   void* alloc(size_t bytes);
   void release(void* p, size_t bytes);
@@ -103,6 +115,7 @@ struct Storage {
   // -- the next execution, a copy to the host, or the release of the memory -- waits for this event first.
   std::mutex pending_mu;
   cudaEvent_t pending = nullptr;
+  void* foreign = nullptr;  // the DLPack tensor that owns this memory, when it was taken over from another library
   Storage(RxDevice* d, void* p, size_t b) : dev(d), keep(d->shared_from_this()), ptr(p), bytes(b) {}
   void make_ready() {  // call with the owning device current
     std::lock_guard<std::mutex> g(pending_mu);
@@ -119,7 +132,8 @@ struct Storage {
       make_ready();  // the pool hands the block out again in compute-stream order
       cudaSetDevice(cur);
     }
-    dev->release(ptr, bytes);
+    if (foreign) dev->hand_back(foreign);
+    else dev->release(ptr, bytes);
   }
 };
 

@@ -254,6 +254,151 @@ def mlp_grad(features: int = 1024, hidden: int = 4096, out: int = 1024, batch: i
 """
 
 
+# ---- the operators at the two ends of a token model ------------------------------------------------------------------
+# StableHLO has no op for these; they are custom_calls with a typed backend_config, which pass through Reactant's
+# pipeline untouched.  Shapes below are the module's (row-major) ones; in Julia the dims come in reverse: a table is
+# features x vocabulary, logits are vocabulary x tokens.  Token ids count from 0.
+def _call(target: str, operands, results, **config) -> str:
+    """One `stablehlo.custom_call`: operands are (name, type) pairs; settings are written as f64 or i64."""
+    cfg = ", ".join(f"{k} = {v!r} : f64" if isinstance(v, float) else f"{k} = {int(v)} : i64" for k, v in config.items())
+    res = results[0] if len(results) == 1 else "(" + ", ".join(results) + ")"
+    return (f"stablehlo.custom_call @{target}({', '.join(n for n, _ in operands)}) {{api_version = 4 : i32, backend_config = {{{cfg}}}}} : "
+            f"({', '.join(t for _, t in operands)}) -> {res}")
+
+
+def _dims(tokens) -> list:
+    return list(tokens) if isinstance(tokens, (tuple, list)) else [tokens]
+
+
+def _one_call(name: str, target: str, types, results, num_partitions: int = 1, split=(), **config) -> str:
+    """A module whose @main is one custom call; arguments whose index is in `split` are split along their first dim."""
+    args = [(f"%arg{k}", t) for k, t in enumerate(types)]
+    mesh = f'  sdy.mesh @mesh = <["x"={num_partitions}]>\n' if num_partitions > 1 else ""
+
+    def attr(k, t):
+        if num_partitions == 1 or k not in split:
+            return ""
+        rank = t.count("x")
+        return " {sdy.sharding = #sdy.sharding<@mesh, [" + ", ".join(['{"x"}'] + ["{}"] * (rank - 1)) + "]>}"
+
+    sig = ", ".join(f"{n}: {t}{attr(k, t)}" for k, (n, t) in enumerate(args))
+    res = results[0] if len(results) == 1 else "(" + ", ".join(results) + ")"
+    lhs = "%0" if len(results) == 1 else f"%0:{len(results)}"
+    outs = "%0" if len(results) == 1 else ", ".join(f"%0#{k}" for k in range(len(results)))
+    return (f"module @reactant_{name} attributes {{mhlo.num_partitions = {num_partitions} : i64, mhlo.num_replicas = 1 : i64}} {{\n{mesh}"
+            f"  func.func @main({sig}) -> {res} {{\n    {lhs} = {_call(target, args, results, **config)}\n    return {outs} : {', '.join(results)}\n  }}\n}}\n")
+
+
+def embedding(vocab: int, features: int, tokens, et: str = "bf16", out_et: str | None = None, ids_et: str = "i32", scale: float = 1.0, num_partitions: int = 1) -> str:
+    """out[t, :] = scale * table[ids[t], :] for a table of `vocab` rows; `tokens` is a count or a tuple of dims.
+    A token outside the table (padding) is a row of zeros.  Products are formed in 32 bits and rounded once.
+    Arguments: table, ids.  With num_partitions > 1 the tokens are split along their first dim."""
+    n = _dims(tokens)
+    return _one_call("embedding", "rx.embedding", [_t([vocab, features], et), _t(n, ids_et)], [_t(n + [features], out_et or et)], num_partitions, (1,), scale=float(scale))
+
+
+def embedding_grad(vocab: int, features: int, tokens, et: str = "bf16", out_et: str = "f32", ids_et: str = "i32", scale: float = 1.0, num_partitions: int = 1) -> str:
+    """The gradient of `embedding` with respect to the table: row v is scale times the sum, in 32 bits and in a fixed
+    order, of the gradients of the tokens with id v; zeros where there are none.  Arguments: dy, ids."""
+    n = _dims(tokens)
+    return _one_call("embedding_grad", "rx.embedding_grad", [_t(n + [features], et), _t(n, ids_et)], [_t([vocab, features], out_et)], num_partitions, (0, 1), scale=float(scale))
+
+
+def dropout(shape, rate: float, et: str = "bf16", site: int = 0, residual: bool = False, num_partitions: int = 1) -> str:
+    """x with a share `rate` of its elements set to zero and the others scaled to keep the mean, plus a residual if
+    there is one.  Arguments: x, key (two 32-bit words), [residual].  The mask is a function of the key, the number
+    `site` (one for each place in a model) and the element's index only -- the same call on a gradient is the gradient:
+    element i has 16 of the 128 bits Philox4x32-10 gives at the counter (i // 8, site), and stays if they reach
+    round(65536 * rate), so rates are kept in steps of 1 / 65536."""
+    t = _t(_dims(shape), et)
+    return _one_call("dropout", "rx.dropout", [t, _t([2], "i32")] + ([t] if residual else []), [t], num_partitions, (0, 2), rate=float(rate), site=site)
+
+
+def token_logprobs(tokens, vocab: int, et: str = "bf16", ids_et: str = "i32", top_k: int = 0, temperature: float = 1.0, num_partitions: int = 1) -> str:
+    """Of every row of logits / temperature: the log probability of its token, the entropy, and the log-sum-exp; with
+    top_k the largest log probabilities and their tokens too (equal ones by the lower token).  Arguments: logits, ids.
+    All results are f32 (tokens i32).  A token outside the vocabulary (padding) has log probability 0.  A row of
+    nothing but -inf has the entropy 0, and -inf for everything else."""
+    n = _dims(tokens)
+    f = _t(n)
+    return _one_call("token_logprobs", "rx.token_logprobs", [_t(n + [vocab], et), _t(n, ids_et)], [f, f, f] + ([_t(n + [top_k]), _t(n + [top_k], "i32")] if top_k else []),
+                     num_partitions, (0, 1), temperature=float(temperature), top_k=top_k)
+
+
+def token_logprobs_grad(tokens, vocab: int, et: str = "bf16", ids_et: str = "i32", temperature: float = 1.0, num_partitions: int = 1) -> str:
+    """The gradient of the first three results of `token_logprobs` with respect to the logits.  Arguments: logits, ids,
+    the entropy's and the log-sum-exp's values in the order (lse, entropy), then the gradients that arrive at the log
+    probability, the entropy and the log-sum-exp.  Padding rows take no gradient through their log probability."""
+    n = _dims(tokens)
+    return _one_call("token_logprobs_grad", "rx.token_logprobs_grad", [_t(n + [vocab], et), _t(n, ids_et)] + [_t(n)] * 5, [_t(n + [vocab], et)], num_partitions, tuple(range(7)),
+                     temperature=float(temperature))
+
+
+def token_model_grad(vocab: int = 32768, features: int = 1024, hidden: int = 4096, tokens: int = 4096, rate: float = 0.1, num_partitions: int = 1) -> str:
+    """One training step of a small token model, as it reaches the runtime with its reverse program: embedding lookup,
+    a tanh layer with dropout on the residual stream, a vocabulary projection, and the mean negative log probability
+    of the next tokens.
+
+    Arguments: E vocab x features, W1 features x hidden, W2 hidden x features, U features x vocab (all bf16, module
+    dims), ids and targets (i32, `tokens` of each; a target of -1 is padding), key (two i32).
+    Results: dE (f32), dW1, dW2, dU (bf16), loss, mean entropy (f32).
+
+        x = sqrt(features) E[ids];  h = tanh(x W1);  y = x + dropout(h W2);  loss = -sum(log softmax(y U)[targets]) / tokens
+    """
+    V, F, H, T = vocab, features, hidden, tokens
+    b = lambda *d: _t(d, "bf16")  # noqa: E731
+    tE, tW1, tW2, tU, tI, tK = b(V, F), b(F, H), b(H, F), b(F, V), _t([T], "i32"), _t([2], "i32")
+    tX, tH, tL, tR, tS = b(T, F), b(T, H), b(T, V), _t([T]), "tensor<f32>"
+    scale = math.sqrt(F)
+    sh = ' {sdy.sharding = #sdy.sharding<@mesh, [{"x"}]>}' if num_partitions > 1 else ""
+    mesh = f'  sdy.mesh @mesh = <["x"={num_partitions}]>\n' if num_partitions > 1 else ""
+
+    def dot(a, ta, c, tc, ac, cc, out):
+        return f"stablehlo.dot_general {a}, {c}, contracting_dims = [{ac}] x [{cc}], precision = [DEFAULT, DEFAULT] : ({ta}, {tc}) -> {out}"
+
+    tHf, tLp = _t([T, H]), [tR, tR, tR]
+    return f"""module @reactant_token_model_grad attributes {{mhlo.num_partitions = {num_partitions} : i64, mhlo.num_replicas = 1 : i64}} {{
+{mesh}  func.func @main(%E: {tE}, %W1: {tW1}, %W2: {tW2}, %U: {tU}, %ids: {tI}{sh}, %targets: {tI}{sh}, %key: {tK}) -> ({_t([V, F])}, {tW1}, {tW2}, {tU}, {tS}, {tS}) {{
+    %zero = stablehlo.constant dense<0.000000e+00> : {tS}
+    %none = stablehlo.constant dense<0.000000e+00> : {tR}
+    %one = stablehlo.constant dense<1.000000e+00> : {tHf}
+    %inv = stablehlo.constant dense<{1.0 / T:.9e}> : {tS}
+    %minus = stablehlo.constant dense<{-1.0 / T:.9e}> : {tS}
+    %g = stablehlo.constant dense<{-1.0 / T:.9e}> : {tR}
+    %x = {_call("rx.embedding", [("%E", tE), ("%ids", tI)], [tX], scale=scale)}
+    %0 = {dot("%x", tX, "%W1", tW1, 1, 0, tH)}
+    %1 = stablehlo.convert %0 : ({tH}) -> {tHf}
+    %2 = stablehlo.tanh %1 : {tHf}
+    %h = stablehlo.convert %2 : ({tHf}) -> {tH}
+    %3 = {dot("%h", tH, "%W2", tW2, 1, 0, tX)}
+    %y = {_call("rx.dropout", [("%3", tX), ("%key", tK), ("%x", tX)], [tX], rate=rate, site=1)}
+    %logits = {dot("%y", tX, "%U", tU, 1, 0, tL)}
+    %lp:3 = {_call("rx.token_logprobs", [("%logits", tL), ("%targets", tI)], tLp)}
+    %4 = stablehlo.reduce(%lp#0 init: %zero) applies stablehlo.add across dimensions = [0] : ({tR}, {tS}) -> {tS}
+    %loss = stablehlo.multiply %4, %minus : {tS}
+    %5 = stablehlo.reduce(%lp#1 init: %zero) applies stablehlo.add across dimensions = [0] : ({tR}, {tS}) -> {tS}
+    %entropy = stablehlo.multiply %5, %inv : {tS}
+    %dl = {_call("rx.token_logprobs_grad", [("%logits", tL), ("%targets", tI), ("%lp#2", tR), ("%lp#1", tR), ("%g", tR), ("%none", tR), ("%none", tR)], [tL])}
+    %dU = {dot("%y", tX, "%dl", tL, 0, 0, tU)}
+    %dy = {dot("%dl", tL, "%U", tU, 1, 1, tX)}
+    %d3 = {_call("rx.dropout", [("%dy", tX), ("%key", tK)], [tX], rate=rate, site=1)}
+    %dW2 = {dot("%h", tH, "%d3", tX, 0, 0, tW2)}
+    %6 = {dot("%d3", tX, "%W2", tW2, 1, 1, tH)}
+    %7 = stablehlo.convert %6 : ({tH}) -> {tHf}
+    %8 = stablehlo.multiply %2, %2 : {tHf}
+    %9 = stablehlo.subtract %one, %8 : {tHf}
+    %10 = stablehlo.multiply %7, %9 : {tHf}
+    %dz = stablehlo.convert %10 : ({tHf}) -> {tH}
+    %dW1 = {dot("%x", tX, "%dz", tH, 0, 0, tW1)}
+    %11 = {dot("%dz", tH, "%W1", tW1, 1, 1, tX)}
+    %dx = stablehlo.add %dy, %11 : {tX}
+    %dE = {_call("rx.embedding_grad", [("%dx", tX), ("%ids", tI)], [_t([V, F])], scale=scale)}
+    return %dE, %dW1, %dW2, %dU, %loss, %entropy : {_t([V, F])}, {tW1}, {tW2}, {tU}, {tS}, {tS}
+  }}
+}}
+"""
+
+
 def matmul(m: int, k: int, n: int, et: str = "f32") -> str:
     """C = A * B for Julia A (m x k), B (k x n): the arguments arrive as k x m and
     n x k tensors and the product as n x m (test/core/compile.jl:350-355)."""

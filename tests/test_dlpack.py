@@ -1,0 +1,123 @@
+"""Arrays exchanged with another library on the same device without a copy (DLPack): shapes and bytes both ways, the
+order between the two libraries' streams, lifetimes on either side, and what is refused."""
+import gc
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+
+def scale_module(n, et="f32"):
+    t = f"tensor<{n}x{et}>"
+    return f"""module {{
+  func.func @main(%arg0: {t}) -> {t} {{
+    %c = stablehlo.constant dense<2.000000e+00> : {t}
+    %0 = stablehlo.multiply %arg0, %c : {t}
+    return %0 : {t}
+  }}
+}}
+"""
+
+
+@pytest.mark.parametrize("dt", ["float32", "bfloat16", "int32", "int64", "float64", "bool"])
+@pytest.mark.parametrize("shape", [(), (5,), (3, 4), (2, 3, 4), (0, 4), (1, 7)])
+def test_round_trip_shares_memory(rx, client, dt, shape):
+    n = int(np.prod(shape))
+    x = torch.arange(n, device="cuda").reshape(shape).to(getattr(torch, dt))
+    turned = x.permute(tuple(reversed(range(len(shape)))))  # first dimension contiguous: the Julia view
+    a = rx.from_dlpack(turned, client)
+    assert a.shape == tuple(turned.shape)
+    back = torch.from_dlpack(a)
+    assert back.dtype == x.dtype and back.shape == turned.shape and torch.equal(back, turned)
+    if n:
+        assert back.data_ptr() == x.data_ptr()
+        x.fill_(1)
+        torch.cuda.synchronize()
+        assert back.bool().all()
+
+
+def test_results_and_inputs_follow_the_streams(rx, client):
+    """A long chain on a stream of torch's feeds the engine, whose result feeds the chain again, with no wait on the host."""
+    n = 1 << 22
+    f = rx.compile(scale_module(n), client)
+    side = torch.cuda.Stream()
+    for where in (torch.cuda.current_stream(), side):
+        with torch.cuda.stream(where):
+            x = torch.ones(n, device="cuda")
+            for _ in range(10):
+                big = torch.randn(2048, 2048, device="cuda")
+                for _ in range(5):
+                    big = big @ big * 1e-3  # keeps the stream busy
+                x = x + 1
+                x = torch.from_dlpack(f(rx.from_dlpack(x, client)))
+                gc.collect()
+        torch.cuda.synchronize()
+        want = 1.0
+        for _ in range(10):
+            want = (want + 1) * 2
+        assert (x == want).all()
+
+
+def test_memory_goes_back_when_both_sides_are_done(rx, client):
+    n = 1 << 24
+    f = rx.compile(scale_module(n), client)
+    base = client.addressable_devices[0].allocator_stats()["bytes_in_use"]
+    torch.cuda.synchronize()
+    held = torch.cuda.memory_allocated()
+    x = torch.ones(n, device="cuda")
+    a = rx.from_dlpack(x, client)
+    y = f(a)
+    out = torch.from_dlpack(y)
+    del x, a, y  # the engine's view keeps the input, torch's view the result
+    assert (out == 2).all()
+    del out
+    client.addressable_devices[0].synchronize()
+    rx.from_dlpack(torch.ones(4, device="cuda"), client)  # any later call hands back what is free by now
+    f(rx.to_rarray(np.ones(n, np.float32), client))
+    gc.collect()
+    client.addressable_devices[0].synchronize()
+    f(rx.to_rarray(np.ones(n, np.float32), client))
+    assert client.addressable_devices[0].allocator_stats()["bytes_in_use"] <= base
+    assert torch.cuda.memory_allocated() <= held + 4096
+
+
+def test_unused_capsules_and_many_views(rx, client):
+    a = rx.to_rarray(np.arange(8, dtype=np.float32), client)
+    for _ in range(100):
+        a.__dlpack__()            # nobody takes it
+        a.__dlpack__(stream=-1)
+    views = [torch.from_dlpack(a) for _ in range(10)]
+    del a
+    gc.collect()
+    assert all(v.tolist() == list(range(8)) for v in views)
+
+
+def test_refusals(rx, client):
+    with pytest.raises(rx.ReactantError, match="first dimension contiguous"):
+        rx.from_dlpack(torch.ones(3, 4, device="cuda"), client)  # row-major: its transposed view would do
+    with pytest.raises(rx.ReactantError, match="first dimension contiguous"):
+        rx.from_dlpack(torch.ones(8, device="cuda")[::2], client)
+    with pytest.raises(rx.ReactantError, match="16-byte"):
+        rx.from_dlpack(torch.ones(8, device="cuda")[1:], client)
+    with pytest.raises(rx.ReactantError, match="not one of this client's"):
+        rx.from_dlpack(torch.ones(8), client)
+    with pytest.raises(rx.ReactantError, match="element type"):
+        rx.from_dlpack(torch.ones(8, device="cuda", dtype=torch.complex64), client)
+    a = rx.to_rarray(np.ones(4, np.float32), client)
+    with pytest.raises(BufferError):
+        a.__dlpack__(copy=True)
+    with pytest.raises(rx.ReactantError, match="ambiguous"):
+        a.__dlpack__(stream=0)
+
+
+def test_donated_arrays_are_not_handed_out(rx, client):
+    text = scale_module(16).replace("%arg0: tensor<16xf32>", "%arg0: tensor<16xf32> {tf.aliasing_output = 0 : i32}")
+    f = rx.compile(text, client)
+    a = rx.to_rarray(np.ones(16, np.float32), client)
+    old = rx.ConcreteRArray(list(a.data), a.shape, a.dtype)
+    f(a)
+    with pytest.raises(rx.ReactantError, match="donated"):
+        old.__dlpack__()
+    assert torch.from_dlpack(a).tolist() == [2.0] * 16

@@ -1,0 +1,451 @@
+"""The operators at the two ends of a token model (custom calls): embedding lookup and its gradient, counter-based
+dropout, log probabilities of given tokens and their gradient.  CPU: the oracle against direct formulas, against
+differences and against torch's autograd; plans, sharding rules and refusals.  GPU: the engine against the oracle.
+
+Tolerances are bounds on the arithmetic, with u = 2^-24 the rounding of a 32-bit operation (2^-8 for a bf16 result):
+  lookup      scale and product are rounded once each, the result once
+  gradient    n terms summed in any order are off by at most n u times the sum of their magnitudes
+  dropout     scale, product and sum; the mask is exact
+  logprobs    see `logprob_bounds`
+"""
+import math
+
+import numpy as np
+import pytest
+
+U = 2.0 ** -24
+HALF = {"f32": U, "bf16": 2.0 ** -8}  # half a step, relative to the value: finfo.eps / 2
+
+
+def np_et(rx, et):
+    return {"f32": np.float32, "bf16": rx.bfloat16, "i32": np.int32, "i64": np.int64}[et]
+
+
+def run(rx, client, text, inputs):
+    """Row-major in, row-major out (the module's own dims)."""
+    out = rx.compile(text, client)(*[rx.to_rarray(np.asarray(x).T, client) for x in inputs])
+    return [np.asarray(o).T for o in (out if isinstance(out, tuple) else (out,))]
+
+
+def close(got, want, bound, what=""):
+    got, want = np.asarray(got, np.float64), np.asarray(want, np.float64)
+    assert got.shape == want.shape
+    same = (got == want) | (np.isnan(got) & np.isnan(want))
+    with np.errstate(invalid="ignore"):
+        bad = ~same & ~(np.abs(got - want) <= bound)
+    assert not bad.any(), (what, int(bad.sum()), got[bad][:4], want[bad][:4], np.broadcast_to(bound, got.shape)[bad][:4])
+
+
+def some_ids(rng, tokens, vocab, et, odd=True):
+    """Few distinct tokens take most of the places; some are outside the table."""
+    n = int(np.prod(tokens))
+    ids = np.minimum((vocab * rng.random(n) ** 3).astype(np.int64), vocab - 1)
+    if odd and n > 3:
+        ids[rng.integers(n)] = -1
+        ids[rng.integers(n)] = vocab
+        if et == "i64":
+            ids[rng.integers(n)] = 2 ** 32 + 1  # its low word is a token
+    return ids.astype(np.int32 if et == "i32" else np.int64).reshape(tokens)
+
+
+def values(rx, rng, shape, et, scale=1.0):
+    return (scale * rng.standard_normal(shape)).astype(np.float32).astype(np_et(rx, et))
+
+
+def f64(a):
+    return np.asarray(a).astype(np.float64)
+
+
+# ---- CPU: the oracle itself ---------------------------------------------------------------------------------------------
+def test_oracle_generator_known_answers(ref):
+    # the published known-answer vectors of Philox4x32-10 for the zero and the all-ones counter are checked in torch-free
+    # integer arithmetic; the counters reachable here have a zero fourth word
+    def philox(c, k):
+        c, k = list(c), list(k)
+        for _ in range(10):
+            a, b = 0xD2511F53 * c[0], 0xCD9E8D57 * c[2]
+            c = [(b >> 32) ^ c[1] ^ k[0], b & 0xFFFFFFFF, (a >> 32) ^ c[3] ^ k[1], a & 0xFFFFFFFF]
+            k = [(k[0] + 0x9E3779B9) & 0xFFFFFFFF, (k[1] + 0xBB67AE85) & 0xFFFFFFFF]
+        return c
+    assert philox([0] * 4, [0] * 2) == [0x6627E8D5, 0xE169C58D, 0xBC57AC4C, 0x9B00DBD8]
+    words = philox([5, 1, 7, 0], [0xFFFFFFFE, 3])
+    bits = [w >> s & 0xFFFF for w in words for s in (0, 16)]
+    first = (5 + (1 << 32)) * 8
+    for rate in (0.1, 0.5, 0.9):
+        got = ref.dropout_mask(8, np.array([-2, 3], np.int32), rate, site=7, first=first)
+        assert got.tolist() == [b >= math.floor(rate * 65536 + 0.5) for b in bits]
+
+
+def test_oracle_gradients_against_differences(ref, rx):
+    rng = np.random.default_rng(0)
+    T, V, temp = 5, 13, 0.7
+    x = rng.standard_normal((T, V))
+    ids = np.array([0, 12, -1, 4, 7], np.int32)
+    g, gh, gl = rng.standard_normal((3, T))
+
+    def forward(x):
+        z = x / temp
+        lse = np.log(np.exp(z).sum(1))
+        lp = np.where(ids < 0, 0, z[np.arange(T), np.maximum(ids, 0)] - lse)
+        p = np.exp(z - lse[:, None])
+        return lp, -(p * np.log(p)).sum(1), lse
+
+    lp, h, lse = forward(x)
+    text = rx.programs.token_logprobs(T, V, et="f64", temperature=temp)  # the oracle takes any type
+    got = ref.run_module(text, [x, ids])
+    for a, b in zip(got, (lp, h, lse)):
+        np.testing.assert_allclose(a, b, rtol=3e-7, atol=1e-7)
+    text = rx.programs.token_logprobs_grad(T, V, et="f64", temperature=temp)
+    dx = ref.run_module(text, [x, ids, lse, h, g, gh, gl])[0]
+    loss = lambda x: sum((a * b).sum() for a, b in zip(forward(x), (g, gh, gl)))  # noqa: E731
+    num = np.zeros_like(x)
+    for i in np.ndindex(*x.shape):
+        e = np.zeros_like(x)
+        e[i] = 1e-5
+        num[i] = (loss(x + e) - loss(x - e)) / 2e-5
+    # lse, entropy and the incoming gradients reach the oracle rounded to f32 values
+    np.testing.assert_allclose(dx, num, rtol=2e-5, atol=2e-6)
+
+
+def test_oracle_lookup_gradient_is_the_transpose(ref, rx):
+    rng = np.random.default_rng(1)
+    V, D, T = 11, 3, 9
+    table, dy = rng.standard_normal((V, D)), rng.standard_normal((T, D))
+    ids = np.array([3, 3, -1, 10, 0, 11, 3, 10, 5], np.int32)
+    y = ref.run_module(rx.programs.embedding(V, D, T, et="f64", scale=2.5), [table, ids])[0]
+    dt = ref.run_module(rx.programs.embedding_grad(V, D, T, et="f64", out_et="f64", scale=2.5), [dy, ids])[0]
+    np.testing.assert_allclose((y * dy).sum(), (table * dt).sum(), rtol=1e-12)
+    assert not dt[[1, 2, 4, 6, 7, 8, 9]].any() and not y[[2, 5]].any()
+
+
+# ---- CPU: plans and refusals ------------------------------------------------------------------------------------------------
+def steps(rx, text):
+    return [s["kind"] for s in rx.plan_describe(text)["steps"]]
+
+
+def test_calls_are_single_steps(rx):
+    p = rx.programs
+    assert steps(rx, p.embedding(100, 64, (3, 5), ids_et="i64")) == ["embedding"]
+    assert steps(rx, p.embedding_grad(100, 64, 7)) == ["embedding_grad"]
+    assert steps(rx, p.dropout((3, 5), 0.1, residual=True)) == ["dropout"]
+    assert steps(rx, p.token_logprobs((2, 3), 50, top_k=5)) == ["token_logprobs"]
+    assert steps(rx, p.token_logprobs_grad(6, 50)) == ["token_logprobs_grad"]
+
+
+def test_mesh_rules(rx):
+    p = rx.programs
+    assert steps(rx, p.embedding(100, 64, 8, num_partitions=2)) == ["embedding"]
+    assert steps(rx, p.embedding_grad(100, 64, 8, num_partitions=2)) == ["embedding_grad", "all_reduce"]
+    assert steps(rx, p.token_logprobs_grad(6, 50, num_partitions=2)) == ["token_logprobs_grad"]
+    assert "20 elements" in rx.plan_describe(p.dropout((8, 5), 0.1, num_partitions=2))["steps"][0]["note"]
+    kinds = steps(rx, p.token_model_grad(512, 256, 512, 512, num_partitions=2))
+    assert kinds.count("all_reduce") == 6  # four gradients, two means
+    with pytest.raises(rx.ReactantError, match="bf16"):
+        rx.plan_describe(p.embedding_grad(100, 64, 8, out_et="bf16", num_partitions=2))
+    text = p.token_logprobs(6, 50, num_partitions=2)
+    with pytest.raises(rx.ReactantError, match="sharded along the rows' own dimension"):
+        rx.plan_describe(text.replace('[{"x"}, {}]', '[{}, {"x"}]', 1))
+    text = p.dropout((8, 6), 0.1, num_partitions=2)
+    with pytest.raises(rx.ReactantError, match="other than the first"):
+        rx.plan_describe(text.replace('[{"x"}, {}]', '[{}, {"x"}]'))
+    text = p.embedding(100, 64, 8, num_partitions=2)
+    with pytest.raises(rx.ReactantError, match="sharded table"):
+        rx.plan_describe(text.replace("tensor<100x64xbf16>,", 'tensor<100x64xbf16> {sdy.sharding = #sdy.sharding<@mesh, [{"x"}, {}]>},', 1))
+
+
+REFUSALS = [
+    ("unknown target", lambda p: p.embedding(8, 4, 3).replace("@rx.embedding", "@rx.other"), 2, "@rx.other"),
+    ("unknown setting", lambda p: p.embedding(8, 4, 3).replace("scale =", "scales ="), 12, "scales"),
+    ("infinite scale", lambda p: p.embedding(8, 4, 3, scale=math.inf).replace("inf", "0x7FF0000000000000"), 12, "scale"),
+    ("half-precision table", lambda p: p.embedding(8, 4, 3, et="f16"), 3, "f16"),
+    ("double table", lambda p: p.embedding(8, 4, 3, et="f64"), 3, "f64"),
+    ("float ids", lambda p: p.embedding(8, 4, 3, ids_et="f32"), 3, "ids"),
+    ("result of another shape", lambda p: p.embedding(8, 4, 3).replace("tensor<3x4xbf16>", "tensor<3x5xbf16>"), 6, "the result"),
+    ("one operand", lambda p: p.embedding(8, 4, 3).replace("(%arg0, %arg1)", "(%arg0)").replace("(tensor<8x4xbf16>, tensor<3xi32>) ->", "(tensor<8x4xbf16>) ->"), 12, "operands"),
+    ("gradient of another length", lambda p: p.embedding_grad(8, 4, 3).replace("tensor<3xi32>", "tensor<2xi32>"), 6, "the gradient"),
+    ("signature that is not the operands'", lambda p: p.embedding_grad(8, 4, 3).replace(": (tensor<3x4xbf16>, tensor<3xi32>)", ": (tensor<3x4xbf16>, tensor<2xi32>)"), 1, "signature"),
+    ("rate of one", lambda p: p.dropout(8, 1.0), 12, "rate"),
+    ("rate that rounds to one", lambda p: p.dropout(8, 0.999999), 12, "rate"),
+    ("negative rate", lambda p: p.dropout(8, -0.1), 12, "rate"),
+    ("rate that is no number", lambda p: p.dropout(8, 0.5).replace("0.5 : f64", "0x7FF8000000000000 : f64"), 12, "rate"),
+    ("no rate", lambda p: p.dropout(8, 0.5).replace("rate = 0.5 : f64, ", ""), 12, "rate"),
+    ("negative site", lambda p: p.dropout(8, 0.5, site=-1), 12, "site"),
+    ("site of 33 bits", lambda p: p.dropout(8, 0.5, site=2 ** 32), 12, "site"),
+    ("key of one word", lambda p: p.dropout(8, 0.5).replace("tensor<2xi32>", "tensor<1xi32>"), 6, "key"),
+    ("residual of another type", lambda p: p.dropout(8, 0.5, residual=True).replace("%arg2: tensor<8xbf16>", "%arg2: tensor<8xf32>").replace("tensor<2xi32>, tensor<8xbf16>) ->", "tensor<2xi32>, tensor<8xf32>) ->"), 3, "residual"),
+    ("temperature of zero", lambda p: p.token_logprobs(3, 8, temperature=0.0), 12, "temperature"),
+    ("negative temperature", lambda p: p.token_logprobs_grad(3, 8, temperature=-1.0), 12, "temperature"),
+    ("temperature below the range of floats", lambda p: p.token_logprobs(3, 8, temperature=1e-300), 12, "temperature"),
+    ("more alternatives than tokens", lambda p: p.token_logprobs(3, 8, top_k=9), 12, "top_k"),
+    ("more alternatives than are kept", lambda p: p.token_logprobs(3, 800, top_k=65), 12, "top_k"),
+    ("five results without alternatives", lambda p: p.token_logprobs(3, 8, top_k=2).replace("top_k = 2", "top_k = 0"), 12, "results"),
+    ("double logits", lambda p: p.token_logprobs(3, 8, et="f64"), 3, "logits"),
+    ("ids of another shape", lambda p: p.token_logprobs(3, 8).replace("tensor<3xi32>", "tensor<4xi32>"), 6, "ids"),
+    ("narrow row values", lambda p: p.token_logprobs_grad(3, 8).replace("tensor<3xf32>", "tensor<3xbf16>"), 3, "lse"),
+    ("config that is no dictionary", lambda p: p.embedding(8, 4, 3).replace("{scale = 1.0 : f64}", '"scale=1"'), 1, "dictionary"),
+    ("aliased results", lambda p: p.embedding(8, 4, 3).replace("api_version = 4 : i32", "output_operand_aliases = [#stablehlo.alias<0>]"), 2, "output_operand_aliases"),
+]
+
+
+@pytest.mark.parametrize("what,text,code,match", REFUSALS, ids=[r[0] for r in REFUSALS])
+def test_refusals(rx, what, text, code, match):
+    with pytest.raises(rx.ReactantError, match=match) as e:
+        rx.plan_describe(text(rx.programs))
+    assert e.value.code == code
+
+
+def test_operands_are_windows_or_copies(rx):
+    """Logits cut out of a padded array are read in place; a transposed array is copied first; a constant zero gradient is not made."""
+    p = rx.programs
+    cut = p.token_logprobs(4, 50, et="f32").replace("%arg0: tensor<4x50xf32>", "%arg0: tensor<4x64xf32>").replace(
+        "    %0:3 =", "    %w = stablehlo.slice %arg0 [0:4, 0:50] : (tensor<4x64xf32>) -> tensor<4x50xf32>\n    %0:3 =").replace("custom_call @rx.token_logprobs(%arg0", "custom_call @rx.token_logprobs(%w")
+    assert steps(rx, cut) == ["token_logprobs"]
+    turned = p.token_logprobs(4, 50, et="f32").replace("%arg0: tensor<4x50xf32>", "%arg0: tensor<50x4xf32>").replace(
+        "    %0:3 =", "    %w = stablehlo.transpose %arg0, dims = [1, 0] : (tensor<50x4xf32>) -> tensor<4x50xf32>\n    %0:3 =").replace("custom_call @rx.token_logprobs(%arg0", "custom_call @rx.token_logprobs(%w")
+    assert steps(rx, turned) == ["map", "token_logprobs"]
+    kinds = steps(rx, p.token_model_grad(512, 256, 512, 256))
+    assert kinds.count("map") == 3  # the loss's share of each row, and the two means
+
+
+# ---- GPU: the engine against the oracle ---------------------------------------------------------------------------------------
+SIZES = [(1, 1, 1), (1, 8, 5), (7, 33, 100), ((2, 3), 128, 50), (300, 1000, 999), (129, 2048, 40), (0, 8, 5), (5, 0, 7)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("et,out_et,ids_et", [("f32", "f32", "i32"), ("bf16", "bf16", "i64"), ("bf16", "f32", "i32"), ("f32", "bf16", "i64")])
+@pytest.mark.parametrize("tokens,features,vocab", SIZES)
+def test_embedding(rx, ref, client, tokens, features, vocab, et, out_et, ids_et):
+    rng = np.random.default_rng(3)
+    table = values(rx, rng, (vocab, features), et)
+    ids = some_ids(rng, tokens, vocab, ids_et)
+    text = rx.programs.embedding(vocab, features, tokens, et=et, out_et=out_et, ids_et=ids_et, scale=math.sqrt(7.0))
+    got, = run(rx, client, text, [table, ids])
+    want = ref.run_module(text, [table.astype(np.float32), ids])[0]
+    close(f64(got), f64(want), (2 * HALF[out_et] + 2 * U) * np.abs(f64(want)))
+    assert not f64(got)[(ids < 0) | (ids >= vocab)].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("et,out_et,ids_et", [("f32", "f32", "i64"), ("bf16", "f32", "i32"), ("bf16", "bf16", "i32")])
+@pytest.mark.parametrize("tokens,features,vocab", SIZES + [(5000, 24, 3), (4097, 65, 70000), (20000, 8, 300)])
+def test_embedding_grad(rx, ref, client, tokens, features, vocab, et, out_et, ids_et):
+    rng = np.random.default_rng(4)
+    n = int(np.prod(tokens))
+    dy = values(rx, rng, (tuple(tokens) if isinstance(tokens, tuple) else (tokens,)) + (features,), et)
+    ids = some_ids(rng, tokens, vocab, ids_et)
+    text = rx.programs.embedding_grad(vocab, features, tokens, et=et, out_et=out_et, ids_et=ids_et, scale=3.0)
+    got, = run(rx, client, text, [dy, ids])
+    want = ref.run_module(text, [dy.astype(np.float32), ids])[0]
+    size = ref.run_module(rx.programs.embedding_grad(vocab, features, tokens, et="f64", out_et="f64", ids_et=ids_et, scale=3.0), [np.abs(f64(dy)), ids])[0]
+    live = ids.reshape(-1)[(ids.reshape(-1) >= 0) & (ids.reshape(-1) < vocab)]
+    counts = np.bincount(live.astype(np.int64), minlength=vocab)[:, None] if n else np.zeros((vocab, 1))
+    close(f64(got), f64(want), (counts + 2) * U * size + 2 * HALF[out_et] * np.abs(f64(want)))
+    again, = run(rx, client, text, [dy, ids])
+    assert np.array_equal(f64(got), f64(again))  # a fixed order of additions
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("et", ["f32", "bf16"])
+@pytest.mark.parametrize("shape,rate,site,residual", [(1, 0.5, 0, False), (7, 0.3, 1, True), ((3, 5), 0.1, 2 ** 32 - 1, False), (1000, 0.0, 3, True), ((129, 255), 0.25, 0, True), ((512, 1024), 0.9, 5, False), (0, 0.5, 0, False),
+                                                     (70001, 1e-6, 0, False), (4099, 65535 / 65536, 0, True)])
+def test_dropout(rx, ref, client, shape, rate, site, residual, et):
+    rng = np.random.default_rng(5)
+    x, r = values(rx, rng, shape, et), values(rx, rng, shape, et)
+    key = rng.integers(-2 ** 31, 2 ** 31, 2).astype(np.int32)
+    text = rx.programs.dropout(shape, rate, et=et, site=site, residual=residual)
+    ins = [x, key] + ([r] if residual else [])
+    got, = run(rx, client, text, ins)
+    want = ref.run_module(text, [a.astype(np.float32) if a.dtype != np.int32 else a for a in ins])[0]
+    scale = 65536 / (65536 - math.floor(rate * 65536 + 0.5))
+    close(f64(got), f64(want), 2 * U * np.abs(f64(x)) * scale + 2 * HALF[et] * np.abs(f64(want)))
+    if not residual and rate:
+        mask = ref.dropout_mask(x.size, key, rate, site).reshape(x.shape)
+        assert np.array_equal(f64(got) != 0, mask & (f64(x) != 0))
+
+
+@pytest.mark.gpu
+def test_dropout_drops_what_is_not_finite(rx, client, ref):
+    key = np.array([1, 2], np.int32)
+    mask = ref.dropout_mask(64, key, 0.5)
+    for bad in (np.inf, -np.inf, np.nan):
+        got, = run(rx, client, rx.programs.dropout(64, 0.5, et="f32"), [np.full(64, bad, np.float32), key])
+        assert not got[~mask].any() and not np.isfinite(got[mask]).any()
+
+
+def logprob_bounds(z, top, h):
+    """How far lse, entropy and log probabilities may be off, from u = 2^-24, per row.  z' = z (1 + 2u) of two roundings;
+    an exponential of an argument of size R is off by 3 R u of its argument's roundings and 4 u of its own; a thread adds
+    at most V / 32 terms and a few levels of merges, each of which rounds (and rescales) once."""
+    counts = np.isfinite(z) & (top[..., None] - np.where(np.isfinite(z), z, 0.0) < 105)  # exp(-105) is no 32-bit number any more
+    finite = np.where(counts, z, 0.0)
+    zmax = np.abs(finite).max(-1)
+    spread = (np.where(counts, top[..., None] - z, 0.0)).max(-1)
+    s = (3 * spread + z.shape[-1] / 32 + 64) * U
+    dz = 2 * 2 * U * zmax
+    lse = s + dz + 2 * U * (zmax + np.log(max(2, z.shape[-1])))
+    ent = s * (1 + 2 * spread) + 2 * dz + 4 * U * (np.abs(h) + 2 * np.log(max(2, z.shape[-1])) + spread)
+    far = np.where(np.isfinite(z), np.abs(z), 0.0).max(-1)  # a token's own logit may lie anywhere
+    return lse, ent, lse + dz + 6 * U * (far + zmax + np.log(max(2, z.shape[-1])))
+
+
+def masked_logits(rx, rng, shape, et, scale=3.0):
+    x = (scale * rng.standard_normal(shape)).astype(np.float32)
+    if shape[-1] > 4:
+        x[rng.random(shape) < 0.1] = -np.inf
+    return x.astype(np_et(rx, et))
+
+
+LOGPROB_SIZES = [(1, 1, 1), (1, 8, 3), ((2, 3), 33, 5), (5, 1000, 64), (3, 1025, 20), (2, 50021, 7), (64, 259, 0), (0, 16, 2), (1, 131072, 32), (300, 64, 1)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("et,ids_et,temperature", [("f32", "i32", 1.0), ("bf16", "i64", 0.7), ("bf16", "i32", 1.0)])
+@pytest.mark.parametrize("tokens,vocab,top_k", LOGPROB_SIZES)
+def test_token_logprobs(rx, ref, client, tokens, vocab, top_k, et, ids_et, temperature):
+    rng = np.random.default_rng(6)
+    shape = (tuple(tokens) if isinstance(tokens, tuple) else (tokens,)) + (vocab,)
+    x = masked_logits(rx, rng, shape, et)
+    ids = some_ids(rng, tokens, vocab, ids_et)
+    text = rx.programs.token_logprobs(tokens, vocab, et=et, ids_et=ids_et, top_k=top_k, temperature=temperature)
+    check_logprobs(run(rx, client, text, [x, ids]), ref.run_module(text, [x.astype(np.float32), ids]), x, temperature, top_k)
+
+
+def check_logprobs(got, want, x, temperature, top_k):
+    z = f64(x) / temperature
+    b_lse, b_ent, b_lp = logprob_bounds(z, z.max(-1), f64(want[1]))
+    close(got[2], want[2], b_lse, "lse")
+    close(got[1], want[1], b_ent, "entropy")
+    close(got[0], want[0], b_lp, "logprob")
+    if top_k:
+        assert np.array_equal(got[4], want[4])
+        close(got[3], want[3], b_lp[..., None], "top")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("et", ["f32", "bf16"])
+@pytest.mark.parametrize("pattern", ["equal", "rising", "falling", "two values", "zeros of both signs", "one finite", "nothing", "huge", "far apart", "lowest"])
+@pytest.mark.parametrize("vocab", [37, 9001])
+def test_token_logprobs_patterns(rx, ref, client, pattern, vocab, et):
+    """Ties, orders that defeat a running threshold, rows that a mask empties, values at the ends of the range."""
+    t, lowest = 3, -3.3895313892515355e38  # the largest finite bf16
+    rows = {"equal": np.full(vocab, 1.25), "rising": np.arange(vocab) * 0.125, "falling": np.arange(vocab) * -0.125, "two values": np.arange(vocab) % 2.0,
+            "zeros of both signs": np.where(np.arange(vocab) % 3 == 0, 0.0, -0.0), "one finite": np.where(np.arange(vocab) == vocab - 2, -7.0, -np.inf), "nothing": np.full(vocab, -np.inf),
+            "huge": np.where(np.arange(vocab) % 5 == 0, 1e30, -1e30), "far apart": np.arange(vocab) % 7 * 40.0, "lowest": np.where(np.arange(vocab) % 4 == 0, 1.0, lowest)}[pattern]
+    x = np.broadcast_to(rows, (t, vocab)).astype(np.float32).astype(np_et(rx, et))
+    ids = np.array([0, vocab - 2, -1], np.int32)
+    text = rx.programs.token_logprobs(t, vocab, et=et, top_k=20)
+    got, want = run(rx, client, text, [x, ids]), ref.run_module(text, [x.astype(np.float32), ids])
+    if pattern == "nothing":
+        assert (got[2] == -np.inf).all() and not got[1].any() and got[0].tolist() == [-np.inf, -np.inf, 0.0]
+        assert (got[3] == -np.inf).all() and (got[4] == np.arange(20)).all()
+    else:
+        check_logprobs(got, want, x, 1.0, 20)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+@pytest.mark.parametrize("vocab", [40, 5000])
+def test_token_logprobs_not_finite(rx, ref, client, bad, vocab):
+    """A row with a NaN or +inf has no probabilities; the rows around it are untouched; NaN ranks above everything."""
+    rng = np.random.default_rng(7)
+    x = rng.standard_normal((3, vocab)).astype(np.float32)
+    x[1, vocab - 3] = bad
+    ids = np.array([1, 1, 1], np.int32)
+    text = rx.programs.token_logprobs(3, vocab, et="f32", top_k=4)
+    got, want = run(rx, client, text, [x, ids]), ref.run_module(text, [x, ids])
+    assert np.isnan(got[0][1]) and np.isnan(got[1][1]) and np.isnan(got[2][1]) and np.isnan(got[3][1]).all()
+    assert np.array_equal(got[4], want[4]) and got[4][1, 0] == vocab - 3
+    keep = [0, 2]
+    check_logprobs([g[keep] for g in got], [w[keep] for w in want], x[keep], 1.0, 4)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("et,ids_et,temperature", [("f32", "i32", 1.0), ("bf16", "i64", 0.7)])
+@pytest.mark.parametrize("tokens,vocab,top_k", [s for s in LOGPROB_SIZES if s[0] != 0] + [(0, 5, 1), (2049, 130, 0)])
+def test_token_logprobs_grad(rx, ref, client, tokens, vocab, top_k, et, ids_et, temperature):
+    rng = np.random.default_rng(8)
+    shape = tuple(tokens) if isinstance(tokens, tuple) else (tokens,)
+    x = masked_logits(rx, rng, shape + (vocab,), et)
+    if shape[0] > 1:
+        x[-1] = -np.inf  # a row that a mask empties
+    ids = some_ids(rng, tokens, vocab, ids_et)
+    lp, h, lse = ref.run_module(rx.programs.token_logprobs(tokens, vocab, et=et, ids_et=ids_et, temperature=temperature), [x.astype(np.float32), ids])
+    g, gh, gl = (rng.standard_normal((3,) + shape) * np.array([1, 0.1, 0.01]).reshape((3,) + (1,) * len(shape))).astype(np.float32)
+    text = rx.programs.token_logprobs_grad(tokens, vocab, et=et, ids_et=ids_et, temperature=temperature)
+    got, = run(rx, client, text, [x, ids, lse, h, g, gh, gl])
+    want = ref.run_module(text, [x.astype(np.float32), ids, lse, h, g, gh, gl])[0]
+    z = f64(x) / temperature
+    far = np.where(np.isfinite(z) & np.isfinite(lse)[..., None], np.abs(z - np.where(np.isfinite(lse), f64(lse), 0)[..., None]), 0.0)
+    p = np.exp(-np.minimum(far, 700.0)) * np.isfinite(z)
+    dlogp = 4 * U * (np.abs(np.where(np.isfinite(z), z, 0)) + np.abs(np.where(np.isfinite(lse), f64(lse), 0))[..., None] + far)
+    col = lambda v: np.abs(f64(v))[..., None]  # noqa: E731
+    size = col(gl) + col(g) + col(gh) * (far + col(h))
+    bound = (p * size * (dlogp + 12 * U) + p * col(gh) * dlogp + 4 * U * col(g)) / temperature + 2 * HALF[et] * np.abs(f64(want)) + 2.0 ** -126
+    close(f64(got), f64(want), bound)
+    if shape[0] > 1:
+        assert not f64(got)[-1].any()
+
+
+@pytest.mark.gpu
+def test_windows_of_wider_arrays(rx, ref, client):
+    """Operands that are windows (padded vocabulary, odd starts and pitches) or transposed give what their copies give."""
+    rng = np.random.default_rng(9)
+    for et in ("f32", "bf16"):
+        wide = masked_logits(rx, rng, (6, 1111), et)
+        ids = np.array([0, 3, -1, 700], np.int32)
+        base = rx.programs.token_logprobs(4, 1001, et=et, top_k=6)
+        cut = base.replace(f"%arg0: tensor<4x1001x{et}>", f"%arg0: tensor<6x1111x{et}>").replace(
+            "    %0:5 =", f"    %w = stablehlo.slice %arg0 [1:5, 7:1008] : (tensor<6x1111x{et}>) -> tensor<4x1001x{et}>\n    %0:5 =").replace("custom_call @rx.token_logprobs(%arg0", "custom_call @rx.token_logprobs(%w")
+        for a, b in zip(run(rx, client, cut, [wide, ids]), run(rx, client, base, [np.ascontiguousarray(wide[1:5, 7:1008]), ids])):
+            close(a, b, 64 * U * np.maximum(1, np.abs(b)))  # the two may split their sums differently
+        table = values(rx, rng, (50, 77), et)
+        base = rx.programs.embedding(40, 33, 4, et=et)
+        cut = base.replace(f"%arg0: tensor<40x33x{et}>", f"%arg0: tensor<50x77x{et}>").replace(
+            "    %0 =", f"    %w = stablehlo.slice %arg0 [3:43, 5:38] : (tensor<50x77x{et}>) -> tensor<40x33x{et}>\n    %0 =").replace("custom_call @rx.embedding(%arg0", "custom_call @rx.embedding(%w")
+        ids = np.array([0, 39, 40, 7], np.int32)
+        a, = run(rx, client, cut, [table, ids])
+        b, = run(rx, client, base, [np.ascontiguousarray(table[3:43, 5:38]), ids])
+        assert np.array_equal(f64(a), f64(b)) and f64(a)[0].any()
+        dy = values(rx, rng, (9, 77), et)
+        ids = np.array([1, 1, 5, 1, 0], np.int32)
+        base = rx.programs.embedding_grad(6, 33, 5, et=et)
+        cut = base.replace(f"%arg0: tensor<5x33x{et}>", f"%arg0: tensor<9x77x{et}>").replace(
+            "    %0 =", f"    %w = stablehlo.slice %arg0 [3:8, 5:38] : (tensor<9x77x{et}>) -> tensor<5x33x{et}>\n    %0 =").replace("custom_call @rx.embedding_grad(%arg0", "custom_call @rx.embedding_grad(%w")
+        a, = run(rx, client, cut, [dy, ids])
+        b, = run(rx, client, base, [np.ascontiguousarray(dy[3:8, 5:38]), ids])
+        assert np.array_equal(f64(a), f64(b))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab,features,hidden,tokens", [(512, 256, 512, 256), (300, 96, 160, 77)])
+def test_token_model_step(rx, ref, client, vocab, features, hidden, tokens):
+    """All of them in one program with the matrix products between, against the float64 oracle.  Every value between
+    two steps is rounded to bf16 in both, so what differs is a rounding that falls the other way here and there."""
+    rng = np.random.default_rng(10)
+    E, U_ = values(rx, rng, (vocab, features), "bf16", features ** -0.5), values(rx, rng, (features, vocab), "bf16", features ** -0.5)
+    W1, W2 = values(rx, rng, (features, hidden), "bf16", features ** -0.5), values(rx, rng, (hidden, features), "bf16", hidden ** -0.5)
+    ids, targets = some_ids(rng, tokens, vocab, "i32", odd=False), some_ids(rng, tokens, vocab, "i32", odd=False)
+    targets[-3:] = -1
+    key = np.array([11, -12], np.int32)
+    text = rx.programs.token_model_grad(vocab, features, hidden, tokens, rate=0.2)
+    ins = [E, W1, W2, U_, ids, targets, key]
+    got = run(rx, client, text, ins)
+    want = ref.run_module(text, [a.astype(np.float32) if a.dtype not in (np.int32,) else a for a in ins])
+    for name, a, b in zip(("dE", "dW1", "dW2", "dU", "loss", "entropy"), got, want):
+        a, b = f64(a), f64(b)
+        # a bf16 value's half step is 2^-8; a gradient passes through at most six of them in a row
+        assert np.linalg.norm(a - b) <= 6 * 2.0 ** -8 * np.linalg.norm(b), name
+
+
+@pytest.mark.gpu
+def test_step_repeats_itself_and_follows_its_key(rx, client):
+    rng = np.random.default_rng(11)
+    V, F, H, T = 256, 256, 256, 256
+    text = rx.programs.token_model_grad(V, F, H, T, rate=0.1)
+    p = [values(rx, rng, s, "bf16", F ** -0.5) for s in ((V, F), (F, H), (H, F), (F, V))]
+    ids = rng.integers(0, V, T).astype(np.int32)
+    ins = p + [ids, np.roll(ids, -1), np.array([1, 2], np.int32)]
+    a, b = run(rx, client, text, ins), run(rx, client, text, ins)
+    assert all(np.array_equal(f64(x), f64(y)) for x, y in zip(a, b))
+    c = run(rx, client, text, p + [ids, np.roll(ids, -1), np.array([1, 3], np.int32)])
+    assert not np.array_equal(f64(a[0]), f64(c[0]))  # another key, another mask
