@@ -1,0 +1,69 @@
+// Device-side pieces shared by the token-model kernels: eight elements at a time as 32-bit floats, and division by a
+// row length known at launch.
+#pragma once
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "rx_device.cuh"
+
+namespace rx {
+
+// bf16 is handled as its 16-bit pattern throughout
+__device__ __forceinline__ float widen(float v) { return v; }
+__device__ __forceinline__ float widen(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
+__device__ __forceinline__ float2 widen_pair(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u)); }
+__device__ __forceinline__ void put(float* p, float v) { *p = v; }
+__device__ __forceinline__ void put(uint16_t* p, float v) { *p = bf16_bits(v); }
+
+// Eight consecutive elements as they lie in memory, and as floats.  Loads and stores bypass or leave L1 early (.cs):
+// every one of these operators touches its large operand once.
+struct Raw8f { uint4 a, b; };
+struct Raw8h { uint4 a; };
+template <class T> struct Raw8T;
+template <> struct Raw8T<float> { using type = Raw8f; };
+template <> struct Raw8T<uint16_t> { using type = Raw8h; };
+template <class T> using Raw8 = typename Raw8T<T>::type;
+
+__device__ __forceinline__ Raw8f load8(const float* p) { return {__ldcs((const uint4*)p), __ldcs((const uint4*)p + 1)}; }
+__device__ __forceinline__ Raw8h load8(const uint16_t* p) { return {__ldcs((const uint4*)p)}; }
+__device__ __forceinline__ Raw8f load8_cached(const float* p) { return {__ldg((const uint4*)p), __ldg((const uint4*)p + 1)}; }
+__device__ __forceinline__ Raw8h load8_cached(const uint16_t* p) { return {__ldg((const uint4*)p)}; }
+__device__ __forceinline__ void widen8(const Raw8f& r, float (&v)[8]) {
+  v[0] = u2f(r.a.x); v[1] = u2f(r.a.y); v[2] = u2f(r.a.z); v[3] = u2f(r.a.w);
+  v[4] = u2f(r.b.x); v[5] = u2f(r.b.y); v[6] = u2f(r.b.z); v[7] = u2f(r.b.w);
+}
+__device__ __forceinline__ void widen8(const Raw8h& r, float (&v)[8]) {
+  const uint32_t w[4] = {r.a.x, r.a.y, r.a.z, r.a.w};
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    v[2 * k] = __uint_as_float(w[k] << 16);
+    v[2 * k + 1] = __uint_as_float(w[k] & 0xFFFF0000u);
+  }
+}
+__device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
+  __stcs((uint4*)p, make_uint4(f2u(v[0]), f2u(v[1]), f2u(v[2]), f2u(v[3])));
+  __stcs((uint4*)p + 1, make_uint4(f2u(v[4]), f2u(v[5]), f2u(v[6]), f2u(v[7])));
+}
+__device__ __forceinline__ void store8(uint16_t* p, const float (&v)[8]) {
+  __stcs((uint4*)p, make_uint4(bf16x2_bits(v[0], v[1]), bf16x2_bits(v[2], v[3]), bf16x2_bits(v[4], v[5]), bf16x2_bits(v[6], v[7])));
+}
+
+// Quotients of numbers below 2^31 by a fixed divisor with one multiplication (Granlund and Montgomery, "Division by
+// invariant integers using multiplication", 1994): with l = ceil(log2 d) and m = ceil(2^(31 + l) / d), which is below
+// 2^32, n / d = (n m) >> (31 + l) for every n < 2^31.
+struct Divisor {
+  uint32_t d, m;
+  int shift;
+  explicit Divisor(int64_t divisor) : d((uint32_t)divisor), m(0), shift(0) {
+    if (divisor <= 0 || divisor >= (int64_t)1 << 31) return;  // not used
+    int l = 0;
+    while (((uint64_t)1 << l) < d) ++l;
+    m = (uint32_t)((((uint64_t)1 << (31 + l)) + d - 1) / d);
+    shift = l - 1;
+  }
+  __device__ __forceinline__ uint32_t quotient(uint32_t n) const { return d == 1 ? n : __umulhi(n, m) >> shift; }
+};
+
+inline bool aligned16(const void* p) { return (uintptr_t)p % 16 == 0; }
+
+}  // namespace rx
