@@ -2,6 +2,8 @@
 #include "rx_token.cuh"
 #include "rx_token.h"
 
+#include <cooperative_groups.h>
+
 #include <algorithm>
 #include <type_traits>
 
@@ -10,74 +12,459 @@ namespace rx {
 namespace {
 
 constexpr int kBlock = 256;
+constexpr int kWarpRow = 4096;       // rows up to this long are one warp's
+constexpr int kMaxRanksPerRow = 8;   // blocks of a cluster that share a row
 
-// m = max z, s = sum exp(z - m), w = sum exp(z - m) (z - m) of some of a row's elements; m = -inf: nothing but -inf
+__device__ __forceinline__ float exp2_fast(float x) {  // within two units of the last place; results below 2^-126 are 0
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float nan_max3(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// two floats in one 64-bit register, one instruction for both
+using Pair = uint64_t;
+__device__ __forceinline__ Pair pair(float lo, float hi) {
+  Pair r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void split(Pair p, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(p)); }
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+  Pair r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+  Pair r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  Pair r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+// ---- the sums of a row -------------------------------------------------------------------------------------------
+// With c = log2(e) / temperature and a reference ref, one pass keeps
+//     s = sum 2^a,   w = sum 2^a a,   a = c (x - ref),
+// from which lse = ref / temperature + ln s and H = ln s - ln(2) w / s.  The reference need not be the maximum: it is
+// the maximum of the first vector a thread meets, and moves only when a logit lies 2^kSlack above it, so the sums are
+// almost never rescaled and cannot overflow.  x - ref is exact where it matters, whatever the size of the logits.
+// Arguments are cut at kFloor, where 2^a is 0 already: -inf, and a mask of the type's lowest value, add 0 and not
+// 0 * inf.  NaN and +inf go through (cut and maxima propagate NaN; inf - inf is NaN).
+constexpr float kSlack = 16.f, kFloor = -300.f;
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
+
 struct RowSum {
-  float m, s, w;
+  float ref, s, w;
 };
-__device__ __forceinline__ void merge(RowSum& a, const RowSum& b) {
-  const float m = nan_max(a.m, b.m);
-  if (m == -INFINITY) return;
-  const float da = a.m - m, db = b.m - m;
-  const float fa = expf(da), fb = expf(db);
-  // w was taken against the old maximum: sum e (z - m) = f (w + s (m_old - m))
-  // (a part far below the maximum, a mask of the type's lowest value say, counts nothing: s (m_old - m) may be infinite there)
-  const float wa = fa != 0.f ? fa * (a.w + a.s * da) : 0.f, wb = fb != 0.f ? fb * (b.w + b.s * db) : 0.f;
-  a.s = (a.m == -INFINITY ? 0.f : a.s * fa) + (b.m == -INFINITY ? 0.f : b.s * fb);
-  a.w = (a.m == -INFINITY ? 0.f : wa) + (b.m == -INFINITY ? 0.f : wb);
-  a.m = m;
+__device__ __forceinline__ void rescale(RowSum& a, float ref, float c) {
+  const float d = nan_max((a.ref - ref) * c, kFloor), f = exp2_fast(d);
+  a.w = f * fmaf(a.s, d, a.w);
+  a.s *= f;
+  a.ref = ref;
+}
+__device__ __forceinline__ void merge(RowSum& a, RowSum b, float c) {
+  const float ref = nan_max(a.ref, b.ref);
+  rescale(a, ref, c);
+  rescale(b, ref, c);
+  a.s += b.s;
+  a.w += b.w;
 }
 
-// the order of the top tokens: larger value first (NaN above everything, -0 equal to 0), then the lower index
-__device__ __forceinline__ uint64_t order_key(float x, uint32_t index) {
-  uint32_t u = __float_as_uint(x + 0.f);
-  u = x != x ? 0xFFFFFFFFu : (u & 0x80000000u) ? ~u : u | 0x80000000u;
-  return (uint64_t)u << 32 | (uint32_t)~index;
+struct Running {
+  float ref, limit, slack;  // limit = ref + slack
+  float c;
+  Pair s, w;
+  __device__ __forceinline__ explicit Running(float c_) : ref(-3.402823466e38f), limit(-3.402823466e38f), slack(kSlack / c_), c(c_), s(0), w(0) {}
+  __device__ __forceinline__ void move(float top) {
+    RowSum lo, hi;
+    lo.ref = hi.ref = ref;
+    split(s, lo.s, hi.s);
+    split(w, lo.w, hi.w);
+    rescale(lo, top, c);
+    rescale(hi, top, c);
+    s = pair(lo.s, hi.s);
+    w = pair(lo.w, hi.w);
+    ref = top;
+    limit = top + slack;
+  }
+  __device__ __forceinline__ float push(const float (&v)[8]) {  // returns the largest
+    const float top = nan_max3(nan_max3(v[0], v[1], v[2]), nan_max3(v[3], v[4], v[5]), nan_max(v[6], v[7]));
+    if (!(top <= limit)) move(top);
+    const Pair minus = pair(-ref, -ref), cc = pair(c, c);
+#pragma unroll
+    for (int q = 0; q < 8; q += 2) {
+      float a0, a1;
+      split(mul2(add2(pair(v[q], v[q + 1]), minus), cc), a0, a1);
+      a0 = nan_max(a0, kFloor);
+      a1 = nan_max(a1, kFloor);
+      const Pair e = pair(exp2_fast(a0), exp2_fast(a1));
+      s = add2(s, e);
+      w = fma2(e, pair(a0, a1), w);
+    }
+    return top;
+  }
+  __device__ __forceinline__ void push1(float x) {
+    const float v[8] = {x, -INFINITY, -INFINITY, -INFINITY, -INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    push(v);
+  }
+  __device__ __forceinline__ RowSum sum() const {
+    float s0, s1, w0, w1;
+    split(s, s0, s1);
+    split(w, w0, w1);
+    return {ref, s0 + s1, w0 + w1};
+  }
+};
+
+__device__ __forceinline__ RowSum warp_merge(RowSum a, float c) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const RowSum b{__shfl_xor_sync(~0u, a.ref, o), __shfl_xor_sync(~0u, a.s, o), __shfl_xor_sync(~0u, a.w, o)};
+    // both lanes add in the same order, the lower lane's part first
+    RowSum lo = (threadIdx.x & o) ? b : a;
+    merge(lo, (threadIdx.x & o) ? a : b, c);
+    a = lo;
+  }
+  return a;
 }
+
+// ---- the top tokens -----------------------------------------------------------------------------------------------
+// One whole number per logit, larger for larger values (NaN above everything, -0 equal to 0) and, among equal ones, for
+// lower tokens: what is selected does not depend on the order in which candidates are met.
+__device__ __forceinline__ uint32_t value_key(float x) {
+  const uint32_t u = __float_as_uint(x + 0.f);
+  return x != x ? 0xFFFFFFFFu : (u & 0x80000000u) ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ uint64_t order_key(float x, uint32_t index) { return (uint64_t)value_key(x) << 32 | (uint32_t)~index; }
+__device__ __forceinline__ float key_value(uint64_t key) {
+  const uint32_t u = (uint32_t)(key >> 32);
+  return __uint_as_float((u & 0x80000000u) ? u ^ 0x80000000u : ~u);
+}
+
+// The k largest of keys[0 .. n), which are all different, in descending order to best[]; `lanes` threads work on it,
+// this one being the lane-th.  The caller synchronises before and after.
+__device__ __forceinline__ void select_top(const uint64_t* keys, int n, int k, uint64_t* best, int lane, int lanes) {
+  for (int i = lane; i < n; i += lanes) {
+    const uint64_t mine = keys[i];
+    int above = 0;
+    for (int j = 0; j < n; ++j) above += keys[j] > mine;
+    if (above < k) best[above] = mine;
+  }
+}
+
+struct RowOut {
+  float ref, scale, log_s;
+  bool empty;  // nothing but -inf: no token has any probability
+  __device__ __forceinline__ explicit RowOut(const RowSum& a, float scale_) : ref(a.ref), scale(scale_), log_s(logf(a.s)), empty(a.s == 0.f) {}
+  __device__ __forceinline__ float logprob(float x) const { return empty ? -INFINITY : fmaf(x - ref, scale, -log_s); }
+  __device__ __forceinline__ float lse() const { return empty ? -INFINITY : fmaf(ref, scale, log_s); }
+  __device__ __forceinline__ float entropy(const RowSum& a) const { return empty ? 0.f : fmaf(-kLn2, a.w / a.s, log_s); }
+};
 
 template <class T, class Id>
-__global__ void __launch_bounds__(kBlock) k_logprobs(const T* __restrict__ logits, const Id* __restrict__ ids, int64_t cols, int64_t ld, float scale, int top_k, LogProbsOut out) {
-  __shared__ RowSum part[kBlock];
-  __shared__ uint64_t best[kBlock];
-  const int64_t row = blockIdx.x;
-  const T* x = logits + row * ld;
-  RowSum a{-INFINITY, 0.f, 0.f};
-  for (int64_t c = threadIdx.x; c < cols; c += kBlock) merge(a, RowSum{widen(x[c]) * scale, 1.f, 0.f});
-  part[threadIdx.x] = a;
-  __syncthreads();
-  for (int o = kBlock / 2; o > 0; o /= 2) {
-    if (threadIdx.x < o) merge(part[threadIdx.x], part[threadIdx.x + o]);
-    __syncthreads();
+__device__ __forceinline__ void write_row(const RowSum& a, const RowOut& o, const T* x, const Id* ids, int64_t row, int64_t cols, const LogProbsOut& out) {
+  const int64_t id = (int64_t)__ldg(ids + row);
+  out.lse[row] = o.lse();
+  out.entropy[row] = o.entropy(a);
+  out.logprob[row] = id < 0 || id >= cols ? 0.f : o.logprob(widen(x[id]));
+}
+
+// A row as vectors of eight from its first element on a 16-byte boundary, and the few in front and behind.
+template <class T>
+struct Span {
+  const T* x;
+  int64_t head, vecs, cols;
+  __device__ __forceinline__ Span(const T* row, int64_t n) : x(row), cols(n) {
+    head = min((int64_t)((16 - (uintptr_t)row % 16) % 16 / sizeof(T)), n);
+    vecs = (n - head) >> 3;
   }
-  a = part[0];
-  const bool empty = a.m == -INFINITY;  // nothing but -inf: no token has any probability
-  const float lse = empty ? -INFINITY : a.m + logf(a.s);
-  if (threadIdx.x == 0) {
-    const int64_t id = ids[row];
-    out.lse[row] = lse;
-    out.entropy[row] = empty ? 0.f : logf(a.s) - a.w / a.s;
-    out.logprob[row] = id < 0 || id >= cols ? 0.f : empty ? -INFINITY : widen(x[id]) * scale - lse;
+  __device__ __forceinline__ int loose() const { return (int)(cols - (vecs << 3)); }                          // at most 14
+  __device__ __forceinline__ int64_t loose_at(int k) const { return k < head ? k : k + (vecs << 3); }          // where the k-th of them lies
+  __device__ __forceinline__ int64_t at(int64_t v) const { return head + (v << 3); }
+};
+
+constexpr int kMaxLoose = 14;
+
+// ---- one warp per row: short rows -----------------------------------------------------------------------------------
+// TOP (top_k <= 32): the k-th largest of the 32 lanes' largest keys bounds the k-th of the row from below, so a second
+// look at the row (it is in L1 by now) keeps little more than k candidates.
+constexpr int kWarpTop = 32;
+constexpr int kWarpCap = 256 + kWarpTop + kMaxLoose;
+
+__device__ __forceinline__ uint64_t warp_max(uint64_t k) {
+  const uint32_t hi = __reduce_max_sync(~0u, (uint32_t)(k >> 32));
+  const uint32_t lo = __reduce_max_sync(~0u, (uint32_t)(k >> 32) == hi ? (uint32_t)k : 0u);
+  return (uint64_t)hi << 32 | lo;
+}
+
+template <class T, class Id, bool TOP>
+__global__ void __launch_bounds__(kBlock) k_logprobs_warp(const T* __restrict__ logits, const Id* __restrict__ ids, int64_t rows, int64_t cols, int64_t ld, float scale, int top_k, LogProbsOut out) {
+  __shared__ uint64_t buf_[TOP ? kBlock / 32 : 1][kWarpCap], best_[TOP ? kBlock / 32 : 1][kWarpTop];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t row = (int64_t)blockIdx.x * (kBlock / 32) + warp;
+  if (row >= rows) return;
+  const Span<T> sp(logits + row * ld, cols);
+  const float c = scale * kLog2e;
+  Running run(c);
+  uint64_t mine = 0;
+  const int loose = sp.loose();
+  if (lane < loose) {
+    const int64_t at = sp.loose_at(lane);
+    const float v = widen(sp.x[at]);
+    run.push1(v);
+    if (TOP) mine = order_key(v, (uint32_t)at);
   }
-  uint64_t below = ~0ull;
-  for (int k = 0; k < top_k; ++k) {
-    uint64_t b = 0;
-    for (int64_t c = threadIdx.x; c < cols; c += kBlock) {
-      const uint64_t key = order_key(widen(x[c]), (uint32_t)c);
-      if ((k == 0 || key < below) && key > b) b = key;
+  constexpr int kFly = 4;
+  for (int64_t v0 = lane; v0 < sp.vecs; v0 += 32 * kFly) {
+    Raw8<T> raw[kFly];
+#pragma unroll
+    for (int k = 0; k < kFly; ++k)
+      if (v0 + k * 32 < sp.vecs) raw[k] = TOP ? load8_cached(sp.x + sp.at(v0 + k * 32)) : load8(sp.x + sp.at(v0 + k * 32));
+#pragma unroll
+    for (int k = 0; k < kFly; ++k) {
+      if (v0 + k * 32 >= sp.vecs) break;
+      float v[8];
+      widen8(raw[k], v);
+      const float top = run.push(v);
+      if (TOP && value_key(top) > (uint32_t)(mine >> 32)) {
+        int q = 0;
+#pragma unroll
+        for (int j = 7; j > 0; --j)
+          if (value_key(v[j]) == value_key(top)) q = j;
+        if (value_key(v[0]) == value_key(top)) q = 0;
+        mine = order_key(top, (uint32_t)(sp.at(v0 + k * 32) + q));
+      }
     }
-    best[threadIdx.x] = b;
+  }
+  const RowSum a = warp_merge(run.sum(), c);
+  const RowOut o(a, scale);
+  if (lane == 0) write_row(a, o, sp.x, ids, row, cols, out);
+  if (TOP) {
+    uint64_t *buf = buf_[warp], *best = best_[warp];
+    uint64_t floor_key = 0, left = mine;
+    for (int k = 0; k < top_k; ++k) {
+      floor_key = warp_max(left);
+      if (left == floor_key) left = 0;
+    }
+    int n = 0;
+    auto keep = [&](uint64_t key, bool have) {  // all lanes together
+      const uint32_t who = __ballot_sync(~0u, have && key >= floor_key);
+      if (have && key >= floor_key) buf[n + __popc(who & ((1u << lane) - 1))] = key;
+      n += __popc(who);
+    };
+    auto shrink = [&]() {
+      __syncwarp();
+      select_top(buf, n, top_k, best, lane, 32);
+      __syncwarp();
+      if (n > top_k) n = top_k;
+      for (int i = lane; i < n; i += 32) buf[i] = best[i];
+      if (n == top_k) floor_key = max(floor_key, best[top_k - 1]);
+      __syncwarp();
+    };
+    const int64_t at = lane < loose ? sp.loose_at(lane) : 0;
+    keep(lane < loose ? order_key(widen(sp.x[at]), (uint32_t)at) : 0, lane < loose);
+    for (int64_t v0 = 0; v0 < sp.vecs; v0 += 32) {
+      const bool have = v0 + lane < sp.vecs;
+      float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      if (have) widen8(load8_cached(sp.x + sp.at(v0 + lane)), v);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) keep(order_key(v[q], (uint32_t)(sp.at(v0 + lane) + q)), have);
+      if (n > kWarpTop) shrink();
+    }
+    shrink();
+    if (lane < top_k) {
+      out.top_value[row * top_k + lane] = o.logprob(key_value(best[lane]));
+      out.top_token[row * top_k + lane] = (int32_t)~(uint32_t)best[lane];
+    }
+  }
+}
+
+// ---- one block, or a cluster of blocks, per row: long rows ---------------------------------------------------------------
+// The blocks of a cluster take a row's vectors in equal runs and join their sums, and their top tokens, through
+// distributed shared memory, in the order of their ranks.
+//
+// TOP: while it streams, a thread notes the largest value of each of up to kSpells stretches of its vectors.  The k-th
+// largest of the block's 256 per-thread maxima bounds the k-th value of the row from below, so only the stretches that
+// reach it (about k of them, whatever the order of the values) are read a second time.  Their elements are taken 256
+// vectors at a time; the same bound among the threads' best keys of such a batch leaves at most 8 k of them.
+constexpr int kSpells = 8;
+constexpr int kBatchCap = 8 * kMaxTopK + kMaxTopK + 16;
+
+template <class T>
+struct Fly { static constexpr int n = sizeof(T) == 2 ? 4 : 2; };  // vectors in flight per thread: 64 bytes
+
+struct TopShared {
+  uint32_t spell[kSpells][kBlock];  // largest value key of a thread's stretch
+  uint64_t key[kBlock];
+  uint64_t buf[kBatchCap], best[kMaxTopK];
+  uint16_t item[kSpells * kBlock];
+  uint64_t bound;
+  int n, n_items;
+};
+
+// the k-th largest of the block's keys (ties by thread), to sh.bound
+__device__ __forceinline__ void kth_of_block(TopShared& sh, uint64_t key, int k) {
+  const int t = threadIdx.x;
+  sh.key[t] = key;
+  __syncthreads();
+  int above = 0;
+#pragma unroll 8
+  for (int j = 0; j < kBlock; ++j) {
+    const uint64_t other = sh.key[j];
+    above += other > key || (other == key && j < t);
+  }
+  if (above == k - 1) sh.bound = key;
+  __syncthreads();
+}
+
+template <class T, class Id, bool TOP>
+__global__ void __launch_bounds__(kBlock, 4) k_logprobs_block(const T* __restrict__ logits, const Id* __restrict__ ids, int64_t cols, int64_t ld, float scale, int top_k, LogProbsOut out) {
+  namespace cg = cooperative_groups;
+  constexpr int kFly = Fly<T>::n, kTile = kBlock * kFly;
+  __shared__ RowSum part[kBlock / 32], total;
+  __shared__ TopShared sh[1];
+  cg::cluster_group cluster = cg::this_cluster();
+  const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const int64_t row = blockIdx.x / ranks;
+  const Span<T> sp(logits + row * ld, cols);
+  const float c = scale * kLog2e;
+  const int64_t share = ((sp.vecs + ranks - 1) / ranks + kTile - 1) / kTile * kTile;  // whole tiles
+  const int64_t lo = min(sp.vecs, share * rank), hi = min(sp.vecs, lo + share);
+  const int tid = threadIdx.x, loose = rank == 0 ? sp.loose() : 0;
+  Running run(c);
+  if (tid < loose) run.push1(widen(sp.x[sp.loose_at(tid)]));
+  const int tiles = (int)((hi - lo + kTile - 1) / kTile), per = TOP ? max(1, (tiles + kSpells - 1) / kSpells) : max(1, tiles);
+  uint32_t thread_top = 0;
+  for (int g = 0, tile = 0; tile < tiles; ++g) {
+    float spell = -INFINITY;
+    for (const int end = min(tiles, tile + per); tile < end; ++tile) {
+      const int64_t v0 = lo + (int64_t)tile * kTile + tid;
+      Raw8<T> raw[kFly];
+#pragma unroll
+      for (int k = 0; k < kFly; ++k)
+        if (v0 + k * kBlock < hi) raw[k] = load8(sp.x + sp.at(v0 + k * kBlock));
+#pragma unroll
+      for (int k = 0; k < kFly; ++k) {
+        if (v0 + k * kBlock >= hi) break;
+        float v[8];
+        widen8(raw[k], v);
+        const float top = run.push(v);
+        if (TOP) spell = nan_max(spell, top);
+      }
+    }
+    if (TOP) {
+      const bool any = lo + (int64_t)g * per * kTile + tid < hi;
+      const uint32_t key = any ? value_key(spell) : 0u;
+      sh[0].spell[g][tid] = key;
+      thread_top = max(thread_top, key);
+    }
+  }
+  RowSum a = warp_merge(run.sum(), c);
+  if ((tid & 31) == 0) part[tid >> 5] = a;
+  __syncthreads();
+  if (tid == 0) {
+    for (int k = 1; k < kBlock / 32; ++k) merge(part[0], part[k], c);
+    total = part[0];
+  }
+  if (TOP) {
+    TopShared& t = sh[0];
+    if (tid == 0) t.n = t.n_items = 0;
+    kth_of_block(t, (uint64_t)thread_top << 32, top_k);
+    const uint32_t reach = (uint32_t)(t.bound >> 32);
+    for (int g = 0; g * per < tiles; ++g) {
+      const uint32_t key = t.spell[g][tid];
+      if (key >= reach && key != 0u) t.item[atomicAdd(&t.n_items, 1)] = (uint16_t)(g * kBlock + tid);
+    }
+    if (tid < loose) {
+      const int64_t at = sp.loose_at(tid);
+      t.buf[atomicAdd(&t.n, 1)] = order_key(widen(sp.x[at]), (uint32_t)at);
+    }
     __syncthreads();
-    for (int o = kBlock / 2; o > 0; o /= 2) {
-      if (threadIdx.x < o && best[threadIdx.x + o] > best[threadIdx.x]) best[threadIdx.x] = best[threadIdx.x + o];
+    const int slots = t.n_items * per * kFly;
+    uint64_t least = 0;  // a key has to be above this to be among the k best
+    for (int s0 = 0; s0 < slots; s0 += kBlock) {
+      uint64_t key[8], mine = 0;
+      bool have = s0 + tid < slots;
+      if (have) {
+        const int slot = s0 + tid, item = t.item[slot / (per * kFly)], k = slot % (per * kFly);
+        const int64_t v = lo + (int64_t)(item / kBlock * per + k / kFly) * kTile + k % kFly * kBlock + item % kBlock;
+        have = v < hi && item / kBlock * per + k / kFly < tiles;
+        if (have) {
+          float x[8];
+          widen8(load8_cached(sp.x + sp.at(v)), x);
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            key[q] = order_key(x[q], (uint32_t)(sp.at(v) + q));
+            if (key[q] > least) mine = max(mine, key[q]);
+          }
+        }
+      }
+      if (!__syncthreads_or(mine != 0)) continue;
+      kth_of_block(t, mine, top_k);
+      const uint64_t bound = t.bound;
+      if (have) {
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+          if (key[q] > least && key[q] >= bound) t.buf[atomicAdd(&t.n, 1)] = key[q];
+      }
+      __syncthreads();
+      const int n = t.n;
+      if (n > top_k) {
+        select_top(t.buf, n, top_k, t.best, tid, kBlock);
+        __syncthreads();
+        if (tid < top_k) t.buf[tid] = t.best[tid];
+        if (tid == 0) t.n = top_k;
+        least = t.best[top_k - 1];
+      }
       __syncthreads();
     }
-    below = best[0];
+    const int n = t.n;
     __syncthreads();
-    if (threadIdx.x == 0) {
-      const uint32_t index = ~(uint32_t)below;
-      out.top_value[row * top_k + k] = empty ? -INFINITY : widen(x[index]) * scale - lse;
-      out.top_token[row * top_k + k] = (int32_t)index;
+    if (ranks == 1) {
+      select_top(t.buf, n, top_k, t.best, tid, kBlock);
+    } else {  // this block's keys stay in buf, unordered; the first block collects them
+      if (tid == 0) t.n = min(n, top_k);
+      if (n > top_k) {
+        select_top(t.buf, n, top_k, t.best, tid, kBlock);
+        __syncthreads();
+        if (tid < top_k) t.buf[tid] = t.best[tid];
+      }
     }
+  }
+  if (ranks > 1) {
+    cluster.sync();
+    if (rank == 0) {
+      if (tid == 0)
+        for (int r = 1; r < ranks; ++r) merge(total, *cluster.map_shared_rank(&total, r), c);
+      if (TOP) {
+        TopShared& t = sh[0];
+        int n = t.n;
+        for (int r = 1; r < ranks; ++r) {
+          const TopShared& other = *cluster.map_shared_rank(&t, r);
+          const int m = other.n;
+          if (tid < m) t.buf[n + tid] = other.buf[tid];
+          n += m;
+        }
+        __syncthreads();
+        select_top(t.buf, n, top_k, t.best, tid, kBlock);
+      }
+    }
+    cluster.sync();  // shared memory of a block that has left must not be read
+    if (rank != 0) return;
+  }
+  __syncthreads();
+  a = total;
+  const RowOut o(a, scale);
+  if (tid == 0) write_row(a, o, sp.x, ids, row, cols, out);
+  if (TOP && tid < top_k) {
+    out.top_value[row * top_k + tid] = o.logprob(key_value(sh[0].best[tid]));
+    out.top_token[row * top_k + tid] = (int32_t)~(uint32_t)sh[0].best[tid];
   }
 }
 
@@ -89,12 +476,6 @@ __global__ void __launch_bounds__(kBlock) k_logprobs(const T* __restrict__ logit
 // element, with the few in front and behind taken one by one; VEC is false where the logits and the result do not
 // lie alike (a window of a wider array with another pitch).
 constexpr int kGradVecs = 4;  // vectors of a thread in flight
-
-__device__ __forceinline__ float exp2_fast(float x) {  // within two units of the last place; results below 2^-126 are 0
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
 
 struct GradRow {
   float c, lse, h, a, gh, hot;  // a = dlse - dlogprob; hot = what the token's own element gets on top
@@ -182,11 +563,34 @@ int64_t logprobs_workspace(const CallDesc&, int) { return 0; }
 
 cudaError_t launch_logprobs(const LaunchCtx& c, const CallDesc& d, const void* logits, const void* ids, const LogProbsOut& out, void*) {
   if (!d.rows) return cudaSuccess;
+  cudaError_t err = cudaSuccess;
   with_types(d.in_dt, d.ids_dt, [&](auto* i, auto* id) {
-    k_logprobs<<<(unsigned)d.rows, kBlock, 0, c.stream>>>((decltype(i))logits, (decltype(id))ids, d.cols, d.ld, (float)d.scale, d.top_k, out);
+    using T = std::remove_pointer_t<decltype(i)>;
+    using Id = std::remove_pointer_t<decltype(id)>;
+    if (d.cols <= kWarpRow && d.top_k <= kWarpTop) {
+      const unsigned blocks = (unsigned)((d.rows + kBlock / 32 - 1) / (kBlock / 32));
+      auto* f = d.top_k ? k_logprobs_warp<T, Id, true> : k_logprobs_warp<T, Id, false>;
+      f<<<blocks, kBlock, 0, c.stream>>>((const T*)logits, (const Id*)ids, d.rows, d.cols, d.ld, (float)d.scale, d.top_k, out);
+      return;
+    }
+    // few rows: the blocks of a cluster share each, as long as that leaves a block two tiles and the GPU is not full
+    int ranks = 1;
+    while (ranks < kMaxRanksPerRow && d.rows * ranks < (int64_t)c.sm_count * 4 && d.cols / (ranks * 2) >= 2 * kBlock * Fly<T>::n * 8) ranks *= 2;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(d.rows * ranks));
+    cfg.blockDim = dim3(kBlock);
+    cfg.stream = c.stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)ranks;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    auto* f = d.top_k ? k_logprobs_block<T, Id, true> : k_logprobs_block<T, Id, false>;
+    err = cudaLaunchKernelEx(&cfg, f, (const T*)logits, (const Id*)ids, d.cols, d.ld, (float)d.scale, d.top_k, out);
   });
   ++*c.launches;
-  return cudaGetLastError();
+  return err != cudaSuccess ? err : cudaGetLastError();
 }
 
 cudaError_t launch_logprobs_grad(const LaunchCtx& c, const CallDesc& d, const void* logits, const void* ids, const LogProbsGradIn& in, void* out) {

@@ -2785,7 +2785,7 @@ struct Planner {
         tokens.pop_back();
         call_shape(op, ids, tokens, "the ids operand");
         c.scale = 1.0 / positive("temperature", call_setting(op, "temperature", 1));
-        if (!(c.scale < INFINITY) || (float)c.scale <= 0.f || std::isinf((float)c.scale)) throw Error(RX_ERR_ARG, call_error(op, "temperature is out of the range of 32-bit floats"));
+        if (!(c.scale >= 1e-30 && c.scale <= 1e30)) throw Error(RX_ERR_ARG, call_error(op, "temperature has to lie between 1e-30 and 1e30"));
         std::vector<int> like = {logits, ids};
         for (size_t k = 2; k < op.in.size(); ++k) {
           static const char* names[] = {"lse", "entropy", "dlogprob", "dentropy", "dlse"};
