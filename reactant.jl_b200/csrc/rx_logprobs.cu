@@ -291,8 +291,8 @@ __global__ void __launch_bounds__(kBlock) k_logprobs_warp(const T* __restrict__ 
 //
 // TOP: while it streams, a thread notes the largest value of each of up to kSpells stretches of its vectors.  The k-th
 // largest of the block's 256 per-thread maxima bounds the k-th value of the row from below, so only the stretches that
-// reach it (about k of them, whatever the order of the values) are read a second time.  Their elements are taken 256
-// vectors at a time; the same bound among the threads' best keys of such a batch leaves at most 8 k of them.
+// reach it (about k of them, whatever the order of the values) are read a second time, 256 vectors at a time, and only
+// their elements that reach it are kept.
 constexpr int kSpells = 8;
 constexpr int kBatchCap = 8 * kMaxTopK + kMaxTopK + 16;
 
@@ -301,14 +301,39 @@ struct Fly { static constexpr int n = sizeof(T) == 2 ? 4 : 2; };  // vectors in 
 
 struct TopShared {
   uint32_t spell[kSpells][kBlock];  // largest value key of a thread's stretch
+  uint32_t top[kBlock];             // and of all of them
   uint64_t key[kBlock];
   uint64_t buf[kBatchCap], best[kMaxTopK];
   uint16_t item[kSpells * kBlock];
   uint64_t bound;
+  uint32_t reach;
   int n, n_items;
 };
 
-// the k-th largest of the block's keys (ties by thread), to sh.bound
+// The k-th largest of the block's 256 value keys, rounded down to its upper 20 bits, to sh.reach: the largest prefix
+// that at least k keys reach, bit by bit.  One warp does it with eight keys a lane (about 300 instructions; comparing
+// every key with every other took 16000 and doubled the time of a row).
+__device__ __forceinline__ void reach_of_block(TopShared& sh, uint32_t key, int k) {
+  sh.top[threadIdx.x] = key;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    uint32_t mine[kBlock / 32];
+#pragma unroll
+    for (int j = 0; j < kBlock / 32; ++j) mine[j] = sh.top[j * 32 + threadIdx.x];
+    uint32_t found = 0;
+    for (uint32_t bit = 1u << 31; bit >= 1u << 12; bit >>= 1) {
+      const uint32_t want = found | bit;
+      int n = 0;
+#pragma unroll
+      for (int j = 0; j < kBlock / 32; ++j) n += mine[j] >= want;
+      if (__reduce_add_sync(~0u, n) >= k) found = want;
+    }
+    if (threadIdx.x == 0) sh.reach = found;
+  }
+  __syncthreads();
+}
+
+// the k-th largest of the block's keys (ties by thread), to sh.bound; 0 is no key
 __device__ __forceinline__ void kth_of_block(TopShared& sh, uint64_t key, int k) {
   const int t = threadIdx.x;
   sh.key[t] = key;
@@ -375,8 +400,8 @@ __global__ void __launch_bounds__(kBlock, 4) k_logprobs_block(const T* __restric
   if (TOP) {
     TopShared& t = sh[0];
     if (tid == 0) t.n = t.n_items = 0;
-    kth_of_block(t, (uint64_t)thread_top << 32, top_k);
-    const uint32_t reach = (uint32_t)(t.bound >> 32);
+    reach_of_block(t, thread_top, top_k);
+    const uint32_t reach = t.reach;
     for (int g = 0; g * per < tiles; ++g) {
       const uint32_t key = t.spell[g][tid];
       if (key >= reach && key != 0u) t.item[atomicAdd(&t.n_items, 1)] = (uint16_t)(g * kBlock + tid);
@@ -387,7 +412,7 @@ __global__ void __launch_bounds__(kBlock, 4) k_logprobs_block(const T* __restric
     }
     __syncthreads();
     const int slots = t.n_items * per * kFly;
-    uint64_t least = 0;  // a key has to be above this to be among the k best
+    uint64_t least = reach ? ((uint64_t)reach << 32) - 1 : 0;  // a key has to be above this to be among the k best
     for (int s0 = 0; s0 < slots; s0 += kBlock) {
       uint64_t key[8], mine = 0;
       bool have = s0 + tid < slots;
@@ -405,13 +430,30 @@ __global__ void __launch_bounds__(kBlock, 4) k_logprobs_block(const T* __restric
           }
         }
       }
-      if (!__syncthreads_or(mine != 0)) continue;
-      kth_of_block(t, mine, top_k);
-      const uint64_t bound = t.bound;
+      const int before = t.n;
+      int wants = 0;
+      if (have) {
+#pragma unroll
+        for (int q = 0; q < 8; ++q) wants += key[q] > least;
+      }
+      if (!__syncthreads_or(wants)) continue;
+      // as a rule the bound leaves few keys and all of them fit; where most of a row is equal they may not, and then
+      // only those that reach the k-th of the threads' best are taken: at most 8 k
+      int at = wants ? atomicAdd(&t.n, wants) : 0;
+      const bool fits = !__syncthreads_or(wants && at + wants > kBatchCap);
+      uint64_t bound = 0;
+      if (!fits) {
+        if (tid == 0) t.n = before;
+        kth_of_block(t, mine, top_k);
+        bound = t.bound;
+      }
       if (have) {
 #pragma unroll
         for (int q = 0; q < 8; ++q)
-          if (key[q] > least && key[q] >= bound) t.buf[atomicAdd(&t.n, 1)] = key[q];
+          if (key[q] > least && key[q] >= bound) {
+            if (!fits) at = atomicAdd(&t.n, 1);
+            t.buf[at++] = key[q];
+          }
       }
       __syncthreads();
       const int n = t.n;
