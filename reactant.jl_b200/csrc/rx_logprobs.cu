@@ -122,14 +122,18 @@ struct Running {
   }
 };
 
-__device__ __forceinline__ RowSum warp_merge(RowSum a, float c) {
+// The sums of W neighbouring lanes together, in all of them: one common reference, one rescaling per lane, and sums in
+// the order of a butterfly (the same in every lane: a + b is b + a).
+template <int W>
+__device__ __forceinline__ RowSum lanes_sum(RowSum a, float c) {
+  float ref = a.ref;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const RowSum b{__shfl_xor_sync(~0u, a.ref, o), __shfl_xor_sync(~0u, a.s, o), __shfl_xor_sync(~0u, a.w, o)};
-    // both lanes add in the same order, the lower lane's part first
-    RowSum lo = (threadIdx.x & o) ? b : a;
-    merge(lo, (threadIdx.x & o) ? a : b, c);
-    a = lo;
+  for (int o = W / 2; o > 0; o >>= 1) ref = nan_max(ref, __shfl_xor_sync(~0u, ref, o));
+  rescale(a, ref, c);
+#pragma unroll
+  for (int o = W / 2; o > 0; o >>= 1) {
+    a.s += __shfl_xor_sync(~0u, a.s, o);
+    a.w += __shfl_xor_sync(~0u, a.w, o);
   }
   return a;
 }
@@ -147,15 +151,19 @@ __device__ __forceinline__ float key_value(uint64_t key) {
   return __uint_as_float((u & 0x80000000u) ? u ^ 0x80000000u : ~u);
 }
 
-// The k largest of keys[0 .. n), which are all different, in descending order to best[]; `lanes` threads work on it,
-// this one being the lane-th.  The caller synchronises before and after.
-__device__ __forceinline__ void select_top(const uint64_t* keys, int n, int k, uint64_t* best, int lane, int lanes) {
+// The k largest of keys[0 .. n), which are all different: put(place, key) for each, by one of the `lanes` threads that
+// work on it, this one being the lane-th.  The caller synchronises before and after.
+template <class Put>
+__device__ __forceinline__ void select_top(const uint64_t* keys, int n, int k, int lane, int lanes, Put put) {
   for (int i = lane; i < n; i += lanes) {
     const uint64_t mine = keys[i];
     int above = 0;
     for (int j = 0; j < n; ++j) above += keys[j] > mine;
-    if (above < k) best[above] = mine;
+    if (above < k) put(above, mine);
   }
+}
+__device__ __forceinline__ void select_top(const uint64_t* keys, int n, int k, uint64_t* best, int lane, int lanes) {
+  select_top(keys, n, k, lane, lanes, [&](int place, uint64_t key) { best[place] = key; });
 }
 
 struct RowOut {
@@ -191,17 +199,111 @@ struct Span {
 
 constexpr int kMaxLoose = 14;
 
+// ---- eight lanes per row: rows of up to 256 --------------------------------------------------------------------------
+// Four rows a warp, a row's elements in its lanes' registers, read one by one (a warp's four rows lie next to each
+// other).  TOP: the k-th largest value is searched for bit by bit over all elements, its upper 20 bits first; where
+// that leaves too many (most of the row is equal), to the last bit, and then the last index that is still wanted among
+// the elements equal to it.  What is left, little more than k, is ordered by counting.
+constexpr int kLanes = 8, kGroupRow = 256, kGroupCap = 2 * kMaxTopK + 8;
+
+template <int W>
+__device__ __forceinline__ int lanes_count(int n) {
+#pragma unroll
+  for (int o = W / 2; o > 0; o >>= 1) n += __shfl_xor_sync(~0u, n, o);
+  return n;
+}
+
+template <class T, class Id, bool TOP, int NE>
+__global__ void __launch_bounds__(kBlock) k_logprobs_group(const T* __restrict__ logits, const Id* __restrict__ ids, int64_t rows, int64_t cols_, int64_t ld, float scale, int top_k, LogProbsOut out) {
+  constexpr int kRows = kBlock / kLanes;
+  __shared__ uint64_t buf_[TOP ? kRows : 1][kGroupCap];
+  const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes, cols = (int)cols_;
+  const int64_t row = (int64_t)blockIdx.x * kRows + group;
+  const bool live = row < rows;
+  const T* x = logits + (live ? row : 0) * ld;
+  const float c = scale * kLog2e;
+  float v[NE];
+#pragma unroll
+  for (int j = 0; j < NE; ++j) v[j] = lane + j * kLanes < cols ? widen(__ldcs(x + lane + j * kLanes)) : -INFINITY;
+  float top = v[0];
+#pragma unroll
+  for (int j = 1; j + 1 < NE; j += 2) top = nan_max3(top, v[j], v[j + 1]);
+  top = nan_max(top, v[NE - 1]);
+#pragma unroll
+  for (int o = kLanes / 2; o > 0; o >>= 1) top = nan_max(top, __shfl_xor_sync(~0u, top, o));
+  RowSum a{nan_max(top, -3.402823466e38f), 0.f, 0.f};
+#pragma unroll
+  for (int j = 0; j < NE; ++j) {
+    const float t = nan_max((v[j] - a.ref) * c, kFloor), e = exp2_fast(t);
+    a.s += e;
+    a.w = fmaf(e, t, a.w);
+  }
+#pragma unroll
+  for (int o = kLanes / 2; o > 0; o >>= 1) {
+    a.s += __shfl_xor_sync(~0u, a.s, o);
+    a.w += __shfl_xor_sync(~0u, a.w, o);
+  }
+  const RowOut o(a, scale);
+  if (live && lane == 0) write_row(a, o, x, ids, row, cols_, out);
+  if (TOP) {
+    uint32_t key[NE];
+#pragma unroll
+    for (int j = 0; j < NE; ++j) key[j] = lane + j * kLanes < cols ? value_key(v[j]) : 0u;
+    uint32_t reach = 0;
+    int reached = cols;
+    auto search = [&](uint32_t from, uint32_t to) {
+      for (uint32_t bit = from; bit >= to && bit; bit >>= 1) {
+        int n = 0;
+#pragma unroll
+        for (int j = 0; j < NE; ++j) n += key[j] >= (reach | bit);
+        n = lanes_count<kLanes>(n);
+        if (n >= top_k) {
+          reach |= bit;
+          reached = n;
+        }
+      }
+    };
+    search(1u << 31, 1u << 12);
+    int last = cols;  // of the elements equal to `reach`, those with an index up to this one count
+    if (__any_sync(~0u, reached > 2 * top_k + 8)) {
+      search(1u << 11, 1u);
+      int above = 0;
+#pragma unroll
+      for (int j = 0; j < NE; ++j) above += key[j] > reach;
+      const int wanted = top_k - lanes_count<kLanes>(above);
+      last = 0;
+      for (int bit = kGroupRow / 2; bit > 0; bit >>= 1) {  // the largest index with fewer than `wanted` equal ones below it
+        int n = 0;
+#pragma unroll
+        for (int j = 0; j < NE; ++j) n += key[j] == reach && lane + j * kLanes < (last | bit);
+        if (lanes_count<kLanes>(n) < wanted) last |= bit;
+      }
+    }
+    uint64_t* buf = buf_[group];
+    const uint32_t mates = ((1u << kLanes) - 1) << (threadIdx.x % 32 / kLanes * kLanes), before = mates & ((1u << (threadIdx.x % 32)) - 1);
+    int n = 0;
+#pragma unroll
+    for (int j = 0; j < NE; ++j) {
+      const int at = lane + j * kLanes;
+      const bool take = key[j] != 0u && (key[j] > reach || (key[j] == reach && at <= last) || (last == cols && key[j] >= reach));
+      const uint32_t who = __ballot_sync(~0u, take);
+      if (take) buf[n + __popc(who & before)] = (uint64_t)key[j] << 32 | (uint32_t)~at;
+      n += __popc(who & mates);
+    }
+    __syncwarp();
+    if (live)
+      select_top(buf, n, top_k, lane, kLanes, [&](int place, uint64_t k) {
+        out.top_value[row * top_k + place] = o.logprob(key_value(k));
+        out.top_token[row * top_k + place] = (int32_t)~(uint32_t)k;
+      });
+  }
+}
+
 // ---- one warp per row: short rows -----------------------------------------------------------------------------------
-// TOP (top_k <= 32): the k-th largest of the 32 lanes' largest keys bounds the k-th of the row from below, so a second
-// look at the row (it is in L1 by now) keeps little more than k candidates.
+// TOP (top_k <= 32): the k-th largest of the 32 lanes' largest values bounds the k-th of the row from below, so a
+// second look at the row (it is in L1 by now) keeps little more than k candidates.
 constexpr int kWarpTop = 32;
 constexpr int kWarpCap = 256 + kWarpTop + kMaxLoose;
-
-__device__ __forceinline__ uint64_t warp_max(uint64_t k) {
-  const uint32_t hi = __reduce_max_sync(~0u, (uint32_t)(k >> 32));
-  const uint32_t lo = __reduce_max_sync(~0u, (uint32_t)(k >> 32) == hi ? (uint32_t)k : 0u);
-  return (uint64_t)hi << 32 | lo;
-}
 
 template <class T, class Id, bool TOP>
 __global__ void __launch_bounds__(kBlock) k_logprobs_warp(const T* __restrict__ logits, const Id* __restrict__ ids, int64_t rows, int64_t cols, int64_t ld, float scale, int top_k, LogProbsOut out) {
@@ -212,50 +314,48 @@ __global__ void __launch_bounds__(kBlock) k_logprobs_warp(const T* __restrict__ 
   const Span<T> sp(logits + row * ld, cols);
   const float c = scale * kLog2e;
   Running run(c);
-  uint64_t mine = 0;
+  float mine = -INFINITY;
   const int loose = sp.loose();
+  float extra = -INFINITY;
   if (lane < loose) {
-    const int64_t at = sp.loose_at(lane);
-    const float v = widen(sp.x[at]);
-    run.push1(v);
-    if (TOP) mine = order_key(v, (uint32_t)at);
+    extra = widen(sp.x[sp.loose_at(lane)]);
+    run.push1(extra);
   }
   constexpr int kFly = 4;
-  for (int64_t v0 = lane; v0 < sp.vecs; v0 += 32 * kFly) {
+  const int vecs = (int)sp.vecs;
+  const T* body = sp.x + sp.head;
+  for (int v0 = lane; v0 < vecs; v0 += 32 * kFly) {
     Raw8<T> raw[kFly];
 #pragma unroll
     for (int k = 0; k < kFly; ++k)
-      if (v0 + k * 32 < sp.vecs) raw[k] = TOP ? load8_cached(sp.x + sp.at(v0 + k * 32)) : load8(sp.x + sp.at(v0 + k * 32));
+      if (v0 + k * 32 < vecs) raw[k] = TOP ? load8_cached(body + (v0 + k * 32) * 8) : load8(body + (v0 + k * 32) * 8);
 #pragma unroll
     for (int k = 0; k < kFly; ++k) {
-      if (v0 + k * 32 >= sp.vecs) break;
+      if (v0 + k * 32 >= vecs) break;
       float v[8];
       widen8(raw[k], v);
       const float top = run.push(v);
-      if (TOP && value_key(top) > (uint32_t)(mine >> 32)) {
-        int q = 0;
-#pragma unroll
-        for (int j = 7; j > 0; --j)
-          if (value_key(v[j]) == value_key(top)) q = j;
-        if (value_key(v[0]) == value_key(top)) q = 0;
-        mine = order_key(top, (uint32_t)(sp.at(v0 + k * 32) + q));
-      }
+      if (TOP) mine = nan_max(mine, top);
     }
   }
-  const RowSum a = warp_merge(run.sum(), c);
+  const RowSum a = lanes_sum<32>(run.sum(), c);
   const RowOut o(a, scale);
   if (lane == 0) write_row(a, o, sp.x, ids, row, cols, out);
   if (TOP) {
     uint64_t *buf = buf_[warp], *best = best_[warp];
-    uint64_t floor_key = 0, left = mine;
-    for (int k = 0; k < top_k; ++k) {
-      floor_key = warp_max(left);
-      if (left == floor_key) left = 0;
-    }
+    const uint32_t top_key = lane < vecs ? value_key(mine) : 0u;
+    uint32_t reach = 0;
+    for (uint32_t bit = 1u << 31; bit >= 1u << 12; bit >>= 1)
+      if (__popc(__ballot_sync(~0u, top_key >= (reach | bit))) >= top_k) reach |= bit;
+    // the same bound as a float: what is not below it is a candidate (NaN included; everything, where there is no bound)
+    const float least_value = key_value((uint64_t)reach << 32);
+    uint64_t least = 0;
     int n = 0;
-    auto keep = [&](uint64_t key, bool have) {  // all lanes together
-      const uint32_t who = __ballot_sync(~0u, have && key >= floor_key);
-      if (have && key >= floor_key) buf[n + __popc(who & ((1u << lane) - 1))] = key;
+    auto keep = [&](bool take, float v, int at) {  // all lanes together
+      const uint32_t who = __ballot_sync(~0u, take);
+      if (!who) return;
+      const uint64_t key = order_key(v, (uint32_t)at);
+      if (take) buf[n + __popc(who & ((1u << lane) - 1))] = key;
       n += __popc(who);
     };
     auto shrink = [&]() {
@@ -264,24 +364,26 @@ __global__ void __launch_bounds__(kBlock) k_logprobs_warp(const T* __restrict__ 
       __syncwarp();
       if (n > top_k) n = top_k;
       for (int i = lane; i < n; i += 32) buf[i] = best[i];
-      if (n == top_k) floor_key = max(floor_key, best[top_k - 1]);
+      if (n == top_k) least = best[top_k - 1];
       __syncwarp();
     };
-    const int64_t at = lane < loose ? sp.loose_at(lane) : 0;
-    keep(lane < loose ? order_key(widen(sp.x[at]), (uint32_t)at) : 0, lane < loose);
-    for (int64_t v0 = 0; v0 < sp.vecs; v0 += 32) {
-      const bool have = v0 + lane < sp.vecs;
+    keep(lane < loose && !(extra < least_value), extra, lane < loose ? (int)sp.loose_at(lane) : 0);
+    for (int v0 = 0; v0 < vecs; v0 += 32) {
+      const bool have = v0 + lane < vecs;
       float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      if (have) widen8(load8_cached(sp.x + sp.at(v0 + lane)), v);
+      if (have) widen8(load8_cached(body + (v0 + lane) * 8), v);
+      const float top = nan_max3(nan_max3(v[0], v[1], v[2]), nan_max3(v[3], v[4], v[5]), nan_max(v[6], v[7]));
+      if (!__any_sync(~0u, have && !(top < least_value))) continue;
+      const int at = (int)sp.head + (v0 + lane) * 8;
 #pragma unroll
-      for (int q = 0; q < 8; ++q) keep(order_key(v[q], (uint32_t)(sp.at(v0 + lane) + q)), have);
+      for (int q = 0; q < 8; ++q) keep(have && !(v[q] < least_value) && order_key(v[q], (uint32_t)(at + q)) > least, v[q], at + q);
       if (n > kWarpTop) shrink();
     }
-    shrink();
-    if (lane < top_k) {
-      out.top_value[row * top_k + lane] = o.logprob(key_value(best[lane]));
-      out.top_token[row * top_k + lane] = (int32_t)~(uint32_t)best[lane];
-    }
+    __syncwarp();
+    select_top(buf, n, top_k, lane, 32, [&](int place, uint64_t key) {
+      out.top_value[row * top_k + place] = o.logprob(key_value(key));
+      out.top_token[row * top_k + place] = (int32_t)~(uint32_t)key;
+    });
   }
 }
 
@@ -390,12 +492,12 @@ __global__ void __launch_bounds__(kBlock, 4) k_logprobs_block(const T* __restric
       thread_top = max(thread_top, key);
     }
   }
-  RowSum a = warp_merge(run.sum(), c);
+  RowSum a = lanes_sum<32>(run.sum(), c);
   if ((tid & 31) == 0) part[tid >> 5] = a;
   __syncthreads();
-  if (tid == 0) {
-    for (int k = 1; k < kBlock / 32; ++k) merge(part[0], part[k], c);
-    total = part[0];
+  if (tid < 32) {
+    a = lanes_sum<kBlock / 32>(part[tid % (kBlock / 32)], c);
+    if (tid == 0) total = a;
   }
   if (TOP) {
     TopShared& t = sh[0];
@@ -609,6 +711,14 @@ cudaError_t launch_logprobs(const LaunchCtx& c, const CallDesc& d, const void* l
   with_types(d.in_dt, d.ids_dt, [&](auto* i, auto* id) {
     using T = std::remove_pointer_t<decltype(i)>;
     using Id = std::remove_pointer_t<decltype(id)>;
+    if (d.cols <= kGroupRow) {
+      const unsigned blocks = (unsigned)((d.rows + kBlock / kLanes - 1) / (kBlock / kLanes));
+      auto go = [&](auto* f) { f<<<blocks, kBlock, 0, c.stream>>>((const T*)logits, (const Id*)ids, d.rows, d.cols, d.ld, (float)d.scale, d.top_k, out); };
+      if (d.cols <= 64) go(d.top_k ? k_logprobs_group<T, Id, true, 8> : k_logprobs_group<T, Id, false, 8>);
+      else if (d.cols <= 128) go(d.top_k ? k_logprobs_group<T, Id, true, 16> : k_logprobs_group<T, Id, false, 16>);
+      else go(d.top_k ? k_logprobs_group<T, Id, true, 32> : k_logprobs_group<T, Id, false, 32>);
+      return;
+    }
     if (d.cols <= kWarpRow && d.top_k <= kWarpTop) {
       const unsigned blocks = (unsigned)((d.rows + kBlock / 32 - 1) / (kBlock / 32));
       auto* f = d.top_k ? k_logprobs_warp<T, Id, true> : k_logprobs_warp<T, Id, false>;

@@ -295,7 +295,8 @@ def masked_logits(rx, rng, shape, et, scale=3.0):
     return x.astype(np_et(rx, et))
 
 
-LOGPROB_SIZES = [(1, 1, 1), (1, 8, 3), ((2, 3), 33, 5), (5, 1000, 64), (3, 1025, 20), (2, 50021, 7), (64, 259, 0), (0, 16, 2), (1, 131072, 32), (300, 64, 1)]
+LOGPROB_SIZES = [(1, 1, 1), (1, 8, 3), ((2, 3), 33, 5), (5, 1000, 64), (3, 1025, 20), (2, 50021, 7), (64, 259, 0), (0, 16, 2), (1, 131072, 32), (300, 64, 1),
+                 (37, 64, 64), (35, 128, 33), (33, 256, 20), (9, 257, 32), (5, 4096, 32), (2, 4097, 33)]
 
 
 @pytest.mark.gpu
@@ -324,7 +325,7 @@ def check_logprobs(got, want, x, temperature, top_k):
 @pytest.mark.gpu
 @pytest.mark.parametrize("et", ["f32", "bf16"])
 @pytest.mark.parametrize("pattern", ["equal", "rising", "falling", "two values", "zeros of both signs", "one finite", "nothing", "huge", "far apart", "lowest"])
-@pytest.mark.parametrize("vocab", [37, 9001])
+@pytest.mark.parametrize("vocab", [37, 250, 3001, 9001])
 def test_token_logprobs_patterns(rx, ref, client, pattern, vocab, et):
     """Ties, orders that defeat a running threshold, rows that a mask empties, values at the ends of the range."""
     t, lowest = 3, -3.3895313892515355e38  # the largest finite bf16
