@@ -12,7 +12,9 @@ namespace rx {
 namespace {
 
 constexpr int kBlock = 256;
-constexpr int kWarpRow = 4096;       // rows up to this long are one warp's
+// Rows up to this long are one warp's, where there are enough of them (times with a block of 128 a row in brackets, f32:
+// 25000 x 4100 65.7 [87] us, 12500 x 8200 65.4 [71], 6000 x 16500 75 [72]; with twenty top tokens 126 [188], 147 [118]).
+constexpr int kWarpRow = 8192, kWarpRowTop = 6144;
 constexpr int kMaxRanksPerRow = 8;   // blocks of a cluster that share a row
 
 __device__ __forceinline__ float exp2_fast(float x) {  // within two units of the last place; results below 2^-126 are 0
@@ -111,8 +113,10 @@ struct Running {
     return top;
   }
   __device__ __forceinline__ void push1(float x) {
-    const float v[8] = {x, -INFINITY, -INFINITY, -INFINITY, -INFINITY, -INFINITY, -INFINITY, -INFINITY};
-    push(v);
+    if (!(x <= limit)) move(x);
+    const float a = nan_max((x - ref) * c, kFloor), e = exp2_fast(a);
+    s = add2(s, pair(e, 0.f));
+    w = add2(w, pair(e * a, 0.f));
   }
   __device__ __forceinline__ RowSum sum() const {
     float s0, s1, w0, w1;
@@ -199,12 +203,15 @@ struct Span {
 
 constexpr int kMaxLoose = 14;
 
-// ---- eight lanes per row: rows of up to 256 --------------------------------------------------------------------------
-// Four rows a warp, a row's elements in its lanes' registers, read one by one (a warp's four rows lie next to each
-// other).  TOP: the k-th largest value is searched for bit by bit over all elements, its upper 20 bits first; where
-// that leaves too many (most of the row is equal), to the last bit, and then the last index that is still wanted among
-// the elements equal to it.  What is left, little more than k, is ordered by counting.
-constexpr int kLanes = 8, kGroupRow = 256, kGroupCap = 2 * kMaxTopK + 8;
+// ---- W = 8 or 32 lanes per row: rows of up to 1024 -----------------------------------------------------------------
+// A row's elements sit in its lanes' registers, NE each, read one by one (eight lanes: a warp's four rows lie next to
+// each other).  TOP: the k-th largest value is bounded bit by bit, its upper 16 bits first -- among all elements, or, with
+// 32 lanes and k <= 32, among the lanes' largest, which is one vote a bit.  Where that leaves too many (most of the row
+// is equal), it is searched for to the last bit, and then the last index that is still wanted among the elements equal
+// to it.  What is left, little more than k, is ordered by counting.
+constexpr int kGroupRow = 1024, kNarrowRow = 256;
+template <int W>
+struct GroupCap { static constexpr int n = W == 8 ? 2 * kMaxTopK + 8 : 4 * kMaxTopK; };
 
 template <int W>
 __device__ __forceinline__ int lanes_count(int n) {
@@ -213,24 +220,25 @@ __device__ __forceinline__ int lanes_count(int n) {
   return n;
 }
 
-template <class T, class Id, bool TOP, int NE>
-__global__ void __launch_bounds__(kBlock) k_logprobs_group(const T* __restrict__ logits, const Id* __restrict__ ids, int64_t rows, int64_t cols_, int64_t ld, float scale, int top_k, LogProbsOut out) {
-  constexpr int kRows = kBlock / kLanes;
-  __shared__ uint64_t buf_[TOP ? kRows : 1][kGroupCap];
-  const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes, cols = (int)cols_;
+template <class T, class Id, bool TOP, int W, int NE>
+__global__ void __launch_bounds__(kBlock, NE == 32 ? (W == 8 ? 2 : 3) : 4) k_logprobs_group(const T* __restrict__ logits, const Id* __restrict__ ids, int64_t rows, int64_t cols_, int64_t ld, float scale, int top_k, LogProbsOut out) {
+  constexpr int kRows = kBlock / W, kCap = GroupCap<W>::n;
+  __shared__ uint64_t buf_[TOP ? kRows : 1][kCap];
+  const int lane = threadIdx.x % W, group = threadIdx.x / W, cols = (int)cols_;
   const int64_t row = (int64_t)blockIdx.x * kRows + group;
   const bool live = row < rows;
   const T* x = logits + (live ? row : 0) * ld;
   const float c = scale * kLog2e;
   float v[NE];
 #pragma unroll
-  for (int j = 0; j < NE; ++j) v[j] = lane + j * kLanes < cols ? widen(__ldcs(x + lane + j * kLanes)) : -INFINITY;
+  for (int j = 0; j < NE; ++j) v[j] = lane + j * W < cols ? widen(__ldcs(x + lane + j * W)) : -INFINITY;
   float top = v[0];
 #pragma unroll
   for (int j = 1; j + 1 < NE; j += 2) top = nan_max3(top, v[j], v[j + 1]);
   top = nan_max(top, v[NE - 1]);
+  const float lane_top = top;
 #pragma unroll
-  for (int o = kLanes / 2; o > 0; o >>= 1) top = nan_max(top, __shfl_xor_sync(~0u, top, o));
+  for (int o = W / 2; o > 0; o >>= 1) top = nan_max(top, __shfl_xor_sync(~0u, top, o));
   RowSum a{nan_max(top, -3.402823466e38f), 0.f, 0.f};
 #pragma unroll
   for (int j = 0; j < NE; ++j) {
@@ -239,60 +247,86 @@ __global__ void __launch_bounds__(kBlock) k_logprobs_group(const T* __restrict__
     a.w = fmaf(e, t, a.w);
   }
 #pragma unroll
-  for (int o = kLanes / 2; o > 0; o >>= 1) {
+  for (int o = W / 2; o > 0; o >>= 1) {
     a.s += __shfl_xor_sync(~0u, a.s, o);
     a.w += __shfl_xor_sync(~0u, a.w, o);
   }
   const RowOut o(a, scale);
   if (live && lane == 0) write_row(a, o, x, ids, row, cols_, out);
   if (TOP) {
-    uint32_t key[NE];
+    uint64_t* buf = buf_[group];
+    const uint32_t mates = (W == 32 ? ~0u : (1u << W % 32) - 1) << (threadIdx.x % 32 / W * W), before = mates & ((1u << (threadIdx.x % 32)) - 1);
+    int n = 0;
+    bool done = false;
+    if (W == 32 && top_k <= 32) {
+      const uint32_t best = lane < cols ? value_key(lane_top) : 0u;
+      uint32_t reach = 0;
+      for (uint32_t bit = 1u << 31; bit >= 1u << 16; bit >>= 1)
+        if (__popc(__ballot_sync(~0u, best >= (reach | bit))) >= top_k) reach |= bit;
+      const float least = key_value((uint64_t)reach << 32);  // NaN, where there is no bound: nothing is below it
+      done = true;
 #pragma unroll
-    for (int j = 0; j < NE; ++j) key[j] = lane + j * kLanes < cols ? value_key(v[j]) : 0u;
-    uint32_t reach = 0;
-    int reached = cols;
-    auto search = [&](uint32_t from, uint32_t to) {
-      for (uint32_t bit = from; bit >= to && bit; bit >>= 1) {
-        int n = 0;
-#pragma unroll
-        for (int j = 0; j < NE; ++j) n += key[j] >= (reach | bit);
-        n = lanes_count<kLanes>(n);
-        if (n >= top_k) {
-          reach |= bit;
-          reached = n;
+      for (int j = 0; j < NE; ++j) {
+        const int at = lane + j * W;
+        const bool take = at < cols && !(v[j] < least);
+        const uint32_t who = __ballot_sync(~0u, take);
+        if (!who) continue;
+        if (n + __popc(who) > kCap) {
+          done = false;
+          break;
         }
-      }
-    };
-    search(1u << 31, 1u << 12);
-    int last = cols;  // of the elements equal to `reach`, those with an index up to this one count
-    if (__any_sync(~0u, reached > 2 * top_k + 8)) {
-      search(1u << 11, 1u);
-      int above = 0;
-#pragma unroll
-      for (int j = 0; j < NE; ++j) above += key[j] > reach;
-      const int wanted = top_k - lanes_count<kLanes>(above);
-      last = 0;
-      for (int bit = kGroupRow / 2; bit > 0; bit >>= 1) {  // the largest index with fewer than `wanted` equal ones below it
-        int n = 0;
-#pragma unroll
-        for (int j = 0; j < NE; ++j) n += key[j] == reach && lane + j * kLanes < (last | bit);
-        if (lanes_count<kLanes>(n) < wanted) last |= bit;
+        if (take) buf[n + __popc(who & before)] = order_key(v[j], (uint32_t)at);
+        n += __popc(who);
       }
     }
-    uint64_t* buf = buf_[group];
-    const uint32_t mates = ((1u << kLanes) - 1) << (threadIdx.x % 32 / kLanes * kLanes), before = mates & ((1u << (threadIdx.x % 32)) - 1);
-    int n = 0;
+    if (!done) {
+      __syncwarp();
+      uint32_t reach = 0;
+      int reached = cols, last = cols;  // of the elements equal to `reach`, those with an index up to `last` count
+      uint32_t key[NE];
 #pragma unroll
-    for (int j = 0; j < NE; ++j) {
-      const int at = lane + j * kLanes;
-      const bool take = key[j] != 0u && (key[j] > reach || (key[j] == reach && at <= last) || (last == cols && key[j] >= reach));
-      const uint32_t who = __ballot_sync(~0u, take);
-      if (take) buf[n + __popc(who & before)] = (uint64_t)key[j] << 32 | (uint32_t)~at;
-      n += __popc(who & mates);
+      for (int j = 0; j < NE; ++j) key[j] = lane + j * W < cols ? value_key(v[j]) : 0u;
+      auto search = [&](uint32_t from, uint32_t to) {
+        for (uint32_t bit = from; bit >= to && bit; bit >>= 1) {
+          int m = 0;
+#pragma unroll
+          for (int j = 0; j < NE; ++j) m += key[j] >= (reach | bit);
+          m = lanes_count<W>(m);
+          if (m >= top_k) {
+            reach |= bit;
+            reached = m;
+          }
+        }
+      };
+      search(1u << 31, 1u << 16);
+      if (__any_sync(~0u, reached > 2 * top_k + 8)) {
+        search(1u << 15, 1u);
+        int above = 0;
+#pragma unroll
+        for (int j = 0; j < NE; ++j) above += key[j] > reach;
+        const int wanted = top_k - lanes_count<W>(above);
+        last = 0;
+        for (int bit = W * NE / 2; bit > 0; bit >>= 1) {  // the largest index with fewer than `wanted` equal ones below it
+          int m = 0;
+#pragma unroll
+          for (int j = 0; j < NE; ++j) m += key[j] == reach && lane + j * W < (last | bit);
+          if (lanes_count<W>(m) < wanted) last |= bit;
+        }
+      }
+      n = 0;
+#pragma unroll
+      for (int j = 0; j < NE; ++j) {
+        const int at = lane + j * W;
+        const uint32_t k = key[j];
+        const bool take = k != 0u && (k > reach || (k == reach && at <= last));
+        const uint32_t who = __ballot_sync(~0u, take);
+        if (take) buf[n + __popc(who & before)] = (uint64_t)k << 32 | (uint32_t)~at;
+        n += __popc(who & mates);
+      }
     }
     __syncwarp();
     if (live)
-      select_top(buf, n, top_k, lane, kLanes, [&](int place, uint64_t k) {
+      select_top(buf, n, top_k, lane, W, [&](int place, uint64_t k) {
         out.top_value[row * top_k + place] = o.logprob(key_value(k));
         out.top_token[row * top_k + place] = (int32_t)~(uint32_t)k;
       });
@@ -348,13 +382,15 @@ __global__ void __launch_bounds__(kBlock) k_logprobs_warp(const T* __restrict__ 
     for (uint32_t bit = 1u << 31; bit >= 1u << 12; bit >>= 1)
       if (__popc(__ballot_sync(~0u, top_key >= (reach | bit))) >= top_k) reach |= bit;
     // the same bound as a float: what is not below it is a candidate (NaN included; everything, where there is no bound)
-    const float least_value = key_value((uint64_t)reach << 32);
+    float least_value = key_value((uint64_t)reach << 32);
     uint64_t least = 0;
     int n = 0;
     auto keep = [&](bool take, float v, int at) {  // all lanes together
-      const uint32_t who = __ballot_sync(~0u, take);
+      uint32_t who = __ballot_sync(~0u, take);
       if (!who) return;
       const uint64_t key = order_key(v, (uint32_t)at);
+      take = take && key > least;
+      who = __ballot_sync(~0u, take);
       if (take) buf[n + __popc(who & ((1u << lane) - 1))] = key;
       n += __popc(who);
     };
@@ -364,7 +400,10 @@ __global__ void __launch_bounds__(kBlock) k_logprobs_warp(const T* __restrict__ 
       __syncwarp();
       if (n > top_k) n = top_k;
       for (int i = lane; i < n; i += 32) buf[i] = best[i];
-      if (n == top_k) least = best[top_k - 1];
+      if (n == top_k) {
+        least = best[top_k - 1];
+        least_value = key_value(least);
+      }
       __syncwarp();
     };
     keep(lane < loose && !(extra < least_value), extra, lane < loose ? (int)sp.loose_at(lane) : 0);
@@ -376,7 +415,7 @@ __global__ void __launch_bounds__(kBlock) k_logprobs_warp(const T* __restrict__ 
       if (!__any_sync(~0u, have && !(top < least_value))) continue;
       const int at = (int)sp.head + (v0 + lane) * 8;
 #pragma unroll
-      for (int q = 0; q < 8; ++q) keep(have && !(v[q] < least_value) && order_key(v[q], (uint32_t)(at + q)) > least, v[q], at + q);
+      for (int q = 0; q < 8; ++q) keep(have && !(v[q] < least_value), v[q], at + q);
       if (n > kWarpTop) shrink();
     }
     __syncwarp();
@@ -392,8 +431,8 @@ __global__ void __launch_bounds__(kBlock) k_logprobs_warp(const T* __restrict__ 
 // distributed shared memory, in the order of their ranks.
 //
 // TOP: while it streams, a thread notes the largest value of each of up to kSpells stretches of its vectors.  The k-th
-// largest of the block's 256 per-thread maxima bounds the k-th value of the row from below, so only the stretches that
-// reach it (about k of them, whatever the order of the values) are read a second time, 256 vectors at a time, and only
+// largest of the block's per-thread maxima bounds the k-th value of the row from below, so only the stretches that
+// reach it (about k of them, whatever the order of the values) are read a second time, a vector a thread at a time, and only
 // their elements that reach it are kept.
 constexpr int kSpells = 8;
 constexpr int kBatchCap = 8 * kMaxTopK + kMaxTopK + 16;
@@ -401,33 +440,35 @@ constexpr int kBatchCap = 8 * kMaxTopK + kMaxTopK + 16;
 template <class T>
 struct Fly { static constexpr int n = sizeof(T) == 2 ? 4 : 2; };  // vectors in flight per thread: 64 bytes
 
+template <int kLong>
 struct TopShared {
-  uint32_t spell[kSpells][kBlock];  // largest value key of a thread's stretch
-  uint32_t top[kBlock];             // and of all of them
-  uint64_t key[kBlock];
+  uint32_t spell[kSpells][kLong];  // largest value key of a thread's stretch
+  uint32_t top[kLong];             // and of all of them
+  uint64_t key[kLong];
   uint64_t buf[kBatchCap], best[kMaxTopK];
-  uint16_t item[kSpells * kBlock];
+  uint16_t item[kSpells * kLong];
   uint64_t bound;
   uint32_t reach;
   int n, n_items;
 };
 
-// The k-th largest of the block's 256 value keys, rounded down to its upper 20 bits, to sh.reach: the largest prefix
-// that at least k keys reach, bit by bit.  One warp does it with eight keys a lane (about 300 instructions; comparing
+// The k-th largest of the block's value keys, rounded down to its upper 20 bits, to sh.reach: the largest prefix
+// that at least k keys reach, bit by bit.  One warp does it with four keys a lane (about 200 instructions; comparing
 // every key with every other took 16000 and doubled the time of a row).
-__device__ __forceinline__ void reach_of_block(TopShared& sh, uint32_t key, int k) {
+template <int kLong>
+__device__ __forceinline__ void reach_of_block(TopShared<kLong>& sh, uint32_t key, int k) {
   sh.top[threadIdx.x] = key;
   __syncthreads();
   if (threadIdx.x < 32) {
-    uint32_t mine[kBlock / 32];
+    uint32_t mine[kLong / 32];
 #pragma unroll
-    for (int j = 0; j < kBlock / 32; ++j) mine[j] = sh.top[j * 32 + threadIdx.x];
+    for (int j = 0; j < kLong / 32; ++j) mine[j] = sh.top[j * 32 + threadIdx.x];
     uint32_t found = 0;
     for (uint32_t bit = 1u << 31; bit >= 1u << 12; bit >>= 1) {
       const uint32_t want = found | bit;
       int n = 0;
 #pragma unroll
-      for (int j = 0; j < kBlock / 32; ++j) n += mine[j] >= want;
+      for (int j = 0; j < kLong / 32; ++j) n += mine[j] >= want;
       if (__reduce_add_sync(~0u, n) >= k) found = want;
     }
     if (threadIdx.x == 0) sh.reach = found;
@@ -436,13 +477,14 @@ __device__ __forceinline__ void reach_of_block(TopShared& sh, uint32_t key, int 
 }
 
 // the k-th largest of the block's keys (ties by thread), to sh.bound; 0 is no key
-__device__ __forceinline__ void kth_of_block(TopShared& sh, uint64_t key, int k) {
+template <int kLong>
+__device__ __forceinline__ void kth_of_block(TopShared<kLong>& sh, uint64_t key, int k) {
   const int t = threadIdx.x;
   sh.key[t] = key;
   __syncthreads();
   int above = 0;
 #pragma unroll 8
-  for (int j = 0; j < kBlock; ++j) {
+  for (int j = 0; j < kLong; ++j) {
     const uint64_t other = sh.key[j];
     above += other > key || (other == key && j < t);
   }
@@ -450,12 +492,12 @@ __device__ __forceinline__ void kth_of_block(TopShared& sh, uint64_t key, int k)
   __syncthreads();
 }
 
-template <class T, class Id, bool TOP>
-__global__ void __launch_bounds__(kBlock, 4) k_logprobs_block(const T* __restrict__ logits, const Id* __restrict__ ids, int64_t cols, int64_t ld, float scale, int top_k, LogProbsOut out) {
+template <class T, class Id, bool TOP, int kLong>
+__global__ void __launch_bounds__(kLong, kLong == 128 ? 6 : 1) k_logprobs_block(const T* __restrict__ logits, const Id* __restrict__ ids, int64_t cols, int64_t ld, float scale, int top_k, LogProbsOut out) {
   namespace cg = cooperative_groups;
-  constexpr int kFly = Fly<T>::n, kTile = kBlock * kFly;
-  __shared__ RowSum part[kBlock / 32], total;
-  __shared__ TopShared sh[1];
+  constexpr int kFly = Fly<T>::n, kTile = kLong * kFly;
+  __shared__ RowSum part[kLong / 32], total;
+  __shared__ TopShared<kLong> sh[1];
   cg::cluster_group cluster = cg::this_cluster();
   const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int64_t row = blockIdx.x / ranks;
@@ -468,17 +510,25 @@ __global__ void __launch_bounds__(kBlock, 4) k_logprobs_block(const T* __restric
   if (tid < loose) run.push1(widen(sp.x[sp.loose_at(tid)]));
   const int tiles = (int)((hi - lo + kTile - 1) / kTile), per = TOP ? max(1, (tiles + kSpells - 1) / kSpells) : max(1, tiles);
   uint32_t thread_top = 0;
+  const int mine = (int)(hi - lo) - tid;  // vectors from this thread's first one to the end of the block's run
+  const T* body = sp.x + sp.at(lo + tid);
+  Raw8<T> next[kFly];
+#pragma unroll
+  for (int k = 0; k < kFly; ++k)
+    if (k * kLong < mine) next[k] = load8(body + k * kLong * 8);
   for (int g = 0, tile = 0; tile < tiles; ++g) {
     float spell = -INFINITY;
     for (const int end = min(tiles, tile + per); tile < end; ++tile) {
-      const int64_t v0 = lo + (int64_t)tile * kTile + tid;
       Raw8<T> raw[kFly];
 #pragma unroll
+      for (int k = 0; k < kFly; ++k) raw[k] = next[k];
+      const int at = (tile + 1) * kTile;
+#pragma unroll
       for (int k = 0; k < kFly; ++k)
-        if (v0 + k * kBlock < hi) raw[k] = load8(sp.x + sp.at(v0 + k * kBlock));
+        if (at + k * kLong < mine) next[k] = load8(body + (int64_t)(at + k * kLong) * 8);
 #pragma unroll
       for (int k = 0; k < kFly; ++k) {
-        if (v0 + k * kBlock >= hi) break;
+        if (at - kTile + k * kLong >= mine) break;
         float v[8];
         widen8(raw[k], v);
         const float top = run.push(v);
@@ -496,17 +546,17 @@ __global__ void __launch_bounds__(kBlock, 4) k_logprobs_block(const T* __restric
   if ((tid & 31) == 0) part[tid >> 5] = a;
   __syncthreads();
   if (tid < 32) {
-    a = lanes_sum<kBlock / 32>(part[tid % (kBlock / 32)], c);
+    a = lanes_sum<kLong / 32>(part[tid % (kLong / 32)], c);
     if (tid == 0) total = a;
   }
   if (TOP) {
-    TopShared& t = sh[0];
+    TopShared<kLong>& t = sh[0];
     if (tid == 0) t.n = t.n_items = 0;
     reach_of_block(t, thread_top, top_k);
     const uint32_t reach = t.reach;
     for (int g = 0; g * per < tiles; ++g) {
       const uint32_t key = t.spell[g][tid];
-      if (key >= reach && key != 0u) t.item[atomicAdd(&t.n_items, 1)] = (uint16_t)(g * kBlock + tid);
+      if (key >= reach && key != 0u) t.item[atomicAdd(&t.n_items, 1)] = (uint16_t)(g * kLong + tid);
     }
     if (tid < loose) {
       const int64_t at = sp.loose_at(tid);
@@ -515,13 +565,13 @@ __global__ void __launch_bounds__(kBlock, 4) k_logprobs_block(const T* __restric
     __syncthreads();
     const int slots = t.n_items * per * kFly;
     uint64_t least = reach ? ((uint64_t)reach << 32) - 1 : 0;  // a key has to be above this to be among the k best
-    for (int s0 = 0; s0 < slots; s0 += kBlock) {
+    for (int s0 = 0; s0 < slots; s0 += kLong) {
       uint64_t key[8], mine = 0;
       bool have = s0 + tid < slots;
       if (have) {
         const int slot = s0 + tid, item = t.item[slot / (per * kFly)], k = slot % (per * kFly);
-        const int64_t v = lo + (int64_t)(item / kBlock * per + k / kFly) * kTile + k % kFly * kBlock + item % kBlock;
-        have = v < hi && item / kBlock * per + k / kFly < tiles;
+        const int64_t v = lo + (int64_t)(item / kLong * per + k / kFly) * kTile + k % kFly * kLong + item % kLong;
+        have = v < hi && item / kLong * per + k / kFly < tiles;
         if (have) {
           float x[8];
           widen8(load8_cached(sp.x + sp.at(v)), x);
@@ -560,7 +610,7 @@ __global__ void __launch_bounds__(kBlock, 4) k_logprobs_block(const T* __restric
       __syncthreads();
       const int n = t.n;
       if (n > top_k) {
-        select_top(t.buf, n, top_k, t.best, tid, kBlock);
+        select_top(t.buf, n, top_k, t.best, tid, kLong);
         __syncthreads();
         if (tid < top_k) t.buf[tid] = t.best[tid];
         if (tid == 0) t.n = top_k;
@@ -571,11 +621,11 @@ __global__ void __launch_bounds__(kBlock, 4) k_logprobs_block(const T* __restric
     const int n = t.n;
     __syncthreads();
     if (ranks == 1) {
-      select_top(t.buf, n, top_k, t.best, tid, kBlock);
+      select_top(t.buf, n, top_k, t.best, tid, kLong);
     } else {  // this block's keys stay in buf, unordered; the first block collects them
       if (tid == 0) t.n = min(n, top_k);
       if (n > top_k) {
-        select_top(t.buf, n, top_k, t.best, tid, kBlock);
+        select_top(t.buf, n, top_k, t.best, tid, kLong);
         __syncthreads();
         if (tid < top_k) t.buf[tid] = t.best[tid];
       }
@@ -587,16 +637,16 @@ __global__ void __launch_bounds__(kBlock, 4) k_logprobs_block(const T* __restric
       if (tid == 0)
         for (int r = 1; r < ranks; ++r) merge(total, *cluster.map_shared_rank(&total, r), c);
       if (TOP) {
-        TopShared& t = sh[0];
+        TopShared<kLong>& t = sh[0];
         int n = t.n;
         for (int r = 1; r < ranks; ++r) {
-          const TopShared& other = *cluster.map_shared_rank(&t, r);
+          const TopShared<kLong>& other = *cluster.map_shared_rank(&t, r);
           const int m = other.n;
           if (tid < m) t.buf[n + tid] = other.buf[tid];
           n += m;
         }
         __syncthreads();
-        select_top(t.buf, n, top_k, t.best, tid, kBlock);
+        select_top(t.buf, n, top_k, t.best, tid, kLong);
       }
     }
     cluster.sync();  // shared memory of a block that has left must not be read
@@ -712,34 +762,44 @@ cudaError_t launch_logprobs(const LaunchCtx& c, const CallDesc& d, const void* l
     using T = std::remove_pointer_t<decltype(i)>;
     using Id = std::remove_pointer_t<decltype(id)>;
     if (d.cols <= kGroupRow) {
-      const unsigned blocks = (unsigned)((d.rows + kBlock / kLanes - 1) / (kBlock / kLanes));
+      const int rows = kBlock / (d.cols <= kNarrowRow ? 8 : 32);
+      const unsigned blocks = (unsigned)((d.rows + rows - 1) / rows);
       auto go = [&](auto* f) { f<<<blocks, kBlock, 0, c.stream>>>((const T*)logits, (const Id*)ids, d.rows, d.cols, d.ld, (float)d.scale, d.top_k, out); };
-      if (d.cols <= 64) go(d.top_k ? k_logprobs_group<T, Id, true, 8> : k_logprobs_group<T, Id, false, 8>);
-      else if (d.cols <= 128) go(d.top_k ? k_logprobs_group<T, Id, true, 16> : k_logprobs_group<T, Id, false, 16>);
-      else go(d.top_k ? k_logprobs_group<T, Id, true, 32> : k_logprobs_group<T, Id, false, 32>);
+      if (d.cols <= 64) go(d.top_k ? k_logprobs_group<T, Id, true, 8, 8> : k_logprobs_group<T, Id, false, 8, 8>);
+      else if (d.cols <= 128) go(d.top_k ? k_logprobs_group<T, Id, true, 8, 16> : k_logprobs_group<T, Id, false, 8, 16>);
+      else if (d.cols <= kNarrowRow) go(d.top_k ? k_logprobs_group<T, Id, true, 8, 32> : k_logprobs_group<T, Id, false, 8, 32>);
+      else if (d.cols <= 512) go(d.top_k ? k_logprobs_group<T, Id, true, 32, 16> : k_logprobs_group<T, Id, false, 32, 16>);
+      else go(d.top_k ? k_logprobs_group<T, Id, true, 32, 32> : k_logprobs_group<T, Id, false, 32, 32>);
       return;
     }
-    if (d.cols <= kWarpRow && d.top_k <= kWarpTop) {
+    if (d.cols <= (d.top_k ? kWarpRowTop : kWarpRow) && d.top_k <= kWarpTop && d.rows >= (int64_t)c.sm_count * 16) {
       const unsigned blocks = (unsigned)((d.rows + kBlock / 32 - 1) / (kBlock / 32));
       auto* f = d.top_k ? k_logprobs_warp<T, Id, true> : k_logprobs_warp<T, Id, false>;
       f<<<blocks, kBlock, 0, c.stream>>>((const T*)logits, (const Id*)ids, d.rows, d.cols, d.ld, (float)d.scale, d.top_k, out);
       return;
     }
-    // few rows: the blocks of a cluster share each, as long as that leaves a block two tiles and the GPU is not full
-    int ranks = 1;
-    while (ranks < kMaxRanksPerRow && d.rows * ranks < (int64_t)c.sm_count * 4 && d.cols / (ranks * 2) >= 2 * kBlock * Fly<T>::n * 8) ranks *= 2;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(d.rows * ranks));
-    cfg.blockDim = dim3(kBlock);
-    cfg.stream = c.stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)ranks;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    auto* f = d.top_k ? k_logprobs_block<T, Id, true> : k_logprobs_block<T, Id, false>;
-    err = cudaLaunchKernelEx(&cfg, f, (const T*)logits, (const Id*)ids, d.cols, d.ld, (float)d.scale, d.top_k, out);
+    // few rows: the blocks of a cluster share each, as long as that leaves a block two tiles, and blocks are large while
+    // there are fewer of them than SMs (4 x 131072 bf16: 9.9 us with blocks of 512, 12.6 with
+    // 128, between two events)
+    auto go = [&](auto size) {
+      constexpr int kLong = decltype(size)::value;
+      int ranks = 1;
+      while (ranks < kMaxRanksPerRow && d.rows * ranks < (int64_t)c.sm_count * 8 && d.cols / (ranks * 2) >= (kLong == 128 ? 2 : 1) * kLong * Fly<T>::n * 8) ranks *= 2;
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3((unsigned)(d.rows * ranks));
+      cfg.blockDim = dim3(kLong);
+      cfg.stream = c.stream;
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = (unsigned)ranks;
+      attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      auto* f = d.top_k ? k_logprobs_block<T, Id, true, kLong> : k_logprobs_block<T, Id, false, kLong>;
+      err = cudaLaunchKernelEx(&cfg, f, (const T*)logits, (const Id*)ids, d.cols, d.ld, (float)d.scale, d.top_k, out);
+    };
+    if (d.rows * kMaxRanksPerRow <= c.sm_count) go(std::integral_constant<int, 512>());
+    else go(std::integral_constant<int, 128>());
   });
   ++*c.launches;
   return err != cudaSuccess ? err : cudaGetLastError();
