@@ -2,6 +2,8 @@
 #include "rx_token.cuh"
 #include "rx_token.h"
 
+#include <cooperative_groups.h>
+
 #include <algorithm>
 
 namespace rx {
@@ -86,75 +88,338 @@ __global__ void __launch_bounds__(kBlock) k_embedding(const In* __restrict__ tab
   }
 }
 
-// Stable counting of the tokens by id, 8 bits at a time: one CTA, each thread a contiguous piece of the tokens.
-// keys/pos: two buffers of `rows` each; a token outside the table gets the key `vocab`.
+// ---- the gradient ----------------------------------------------------------------------------------------------------
+// dtable[v] = scale * sum of dy[t] over the tokens with id v, added in the order of the tokens and so the same from run
+// to run, in four parts:
+//   k_sort_tokens   the tokens' places sorted by id (stably), and which rows have a token at all
+//   k_sum_runs      chunks of kChunk places: a run of one id inside a chunk is summed and written to its row; a run that
+//                   crosses a border of chunks leaves its part of the sum in the workspace
+//   (same launch)   rows without a token are filled with zeros
+//   k_join_runs     the parts of every run that crosses borders, added in the order of the chunks
+// No atomic touches a sum.  The work is bound by memory: the gradients are read once, the table's written once; cutting
+// at fixed places rather than by id keeps the blocks even when few ids hold most of the tokens.
+
+// Sort: least significant digits first, up to 9 bits a pass, by one cluster of up to eight blocks.  Each warp owns a run
+// of consecutive tokens: it counts their digits in its own row of shared memory (equal digits among 32 tokens meet
+// through a vote, the lowest lane adds), the counts become places through sums over warps, blocks (distributed shared
+// memory) and digits, and a second walk writes key and place.
+constexpr int kSortBlock = 1024, kSortWarps = kSortBlock / 32, kBins = 512, kSortRanks = 8;
+
+struct SortShared {
+  uint32_t count[kSortWarps][kBins];
+  uint32_t total[kBins], base[kBins];
+  uint32_t warp_sum[kSortWarps];
+};
+
 template <class Id>
-__global__ void __launch_bounds__(kBlock) k_sort_tokens(const Id* __restrict__ ids, int64_t rows, int64_t vocab, int passes, int32_t* keys0, int32_t* pos0, int32_t* keys1, int32_t* pos1) {
-  __shared__ int32_t start[256];
-  const int64_t per = (rows + kBlock - 1) / kBlock, lo = min(rows, per * threadIdx.x), hi = min(rows, lo + per);
-  for (int64_t t = lo; t < hi; ++t) {
-    const int64_t id = ids[t];
-    keys0[t] = id >= 0 && id < vocab ? (int32_t)id : (int32_t)vocab;
-    pos0[t] = (int32_t)t;
+__global__ void __launch_bounds__(kSortBlock) k_sort_tokens(const Id* __restrict__ ids, int64_t rows, int64_t vocab, int passes, int digit, int32_t* a, int32_t* b, uint8_t* touched, int32_t* crossing) {
+  namespace cg = cooperative_groups;
+  extern __shared__ __align__(16) uint8_t raw[];
+  SortShared& sh = *(SortShared*)raw;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  {
+    const int64_t words = (vocab + 15) / 16;
+    for (int64_t i = (int64_t)rank * kSortBlock + tid; i < words; i += (int64_t)ranks * kSortBlock) ((uint4*)touched)[i] = make_uint4(0, 0, 0, 0);
+    if (rank == 0 && tid == 0) *crossing = 0;
   }
-  __syncthreads();
-  int32_t *k0 = keys0, *p0 = pos0, *k1 = keys1, *p1 = pos1;
+  const int64_t per = ((rows + ranks * kSortWarps - 1) / (ranks * kSortWarps) + 31) / 32 * 32;
+  const int64_t lo = min(rows, per * (rank * kSortWarps + warp)), hi = min(rows, lo + per);
+  const uint32_t below = (1u << lane) - 1;
   for (int pass = 0; pass < passes; ++pass) {
-    const int shift = 8 * pass;
-    start[threadIdx.x] = 0;
+    const int32_t* from = pass % 2 ? a : b;  // the first pass reads the ids
+    int32_t* to = pass % 2 ? b : a;
+    const int shift = pass * digit;
+    const uint32_t mask = (1u << digit) - 1;
+    auto key_at = [&](int64_t t) -> int32_t {
+      if (pass) return __ldcg(from + t);
+      const int64_t id = (int64_t)__ldg(ids + t);
+      return id >= 0 && id < vocab ? (int32_t)id : (int32_t)vocab;  // a token outside the table comes last
+    };
+    for (int k = lane; k < kBins; k += 32) sh.count[warp][k] = 0;
+    __syncwarp();
+    for (int64_t t0 = lo; t0 < hi; t0 += 32) {
+      const bool have = t0 + lane < hi;
+      const uint32_t d = have ? (uint32_t)key_at(t0 + lane) >> shift & mask : ~0u;
+      const uint32_t same = __match_any_sync(~0u, d);
+      if (have && !(same & below)) sh.count[warp][d] += __popc(same);
+      __syncwarp();
+    }
     __syncthreads();
-    for (int64_t t = lo; t < hi; ++t) atomicAdd(&start[(k0[t] >> shift) & 255], 1);
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      int32_t sum = 0;
-      for (int b = 0; b < 256; ++b) {
-        const int32_t n = start[b];
-        start[b] = sum;
+    if (tid < kBins) {
+      uint32_t sum = 0;
+#pragma unroll 8
+      for (int w = 0; w < kSortWarps; ++w) {
+        const uint32_t n = sh.count[w][tid];
+        sh.count[w][tid] = sum;
         sum += n;
       }
+      sh.total[tid] = sum;
+    }
+    cluster.sync();
+    uint32_t before = 0, all = 0;
+    if (tid < kBins)
+      for (int r = 0; r < ranks; ++r) {
+        const uint32_t n = *cluster.map_shared_rank(&sh.total[tid], r);
+        if (r < rank) before += n;
+        all += n;
+      }
+    uint32_t scan = all;  // over the digits
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t n = __shfl_up_sync(~0u, scan, o);
+      if (lane >= o) scan += n;
+    }
+    if (lane == 31) sh.warp_sum[warp] = scan;
+    __syncthreads();
+    if (tid < kBins) {
+      uint32_t front = 0;
+      for (int w = 0; w < warp; ++w) front += sh.warp_sum[w];
+      sh.base[tid] = front + scan - all + before;
     }
     __syncthreads();
-    for (int who = 0; who < kBlock; ++who) {  // in the order of the tokens
-      if (threadIdx.x == who)
-        for (int64_t t = lo; t < hi; ++t) {
-          const int32_t at = start[(k0[t] >> shift) & 255]++;
-          k1[at] = k0[t];
-          p1[at] = p0[t];
+    for (int64_t t0 = lo; t0 < hi; t0 += 32) {
+      const bool have = t0 + lane < hi;
+      const int32_t key = have ? key_at(t0 + lane) : 0;
+      const uint32_t d = have ? (uint32_t)key >> shift & mask : ~0u;
+      const uint32_t same = __match_any_sync(~0u, d);
+      const uint32_t at = have ? sh.base[d] + sh.count[warp][d] + __popc(same & below) : 0;
+      __syncwarp();
+      if (have) {
+        if (!(same & below)) sh.count[warp][d] += __popc(same);
+        to[at] = key;
+        to[rows + at] = pass ? __ldcg(from + rows + t0 + lane) : (int32_t)(t0 + lane);
+        if (!pass && key < vocab) touched[key] = 1;
+      }
+      __syncwarp();
+    }
+    cluster.sync();
+  }
+}
+
+struct GradArgs {
+  const int32_t *key, *pos;  // sorted
+  const uint8_t* touched;    // null: no row has a token
+  float* part;               // [chunks][2][cols]: what a chunk adds to the run that enters it, and to the one that leaves it
+  int32_t *crossing, *list;  // chunks in which a run starts that leaves them
+  int64_t rows, cols, ld, vocab;
+  float scale;
+  int chunk, lanes, log_lanes;  // places in a chunk; threads that share one
+  int64_t chunks, chunk_blocks, slices;
+  Divisor by_row;
+  bool small;
+};
+
+constexpr int kMaxChunk = 32, kFillUnits = 8;
+
+// Zeros for the rows that no token has: units of eight consecutive elements of the result, kFillUnits a thread.
+template <class Out, bool VEC>
+__device__ __forceinline__ void fill_rows(const GradArgs& g, Out* out, int64_t block) {
+  const float zero[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  const int64_t n = g.vocab * g.cols, units = (n + 7) >> 3, per_row = g.cols >> 3;
+  const int64_t base = block * (kBlock * kFillUnits) + threadIdx.x;
+#pragma unroll
+  for (int k = 0; k < kFillUnits; ++k) {
+    const int64_t u = base + k * kBlock;
+    if (u >= units) return;
+    if (VEC) {
+      const int64_t t = g.small ? g.by_row.quotient((uint32_t)u) : u / per_row;
+      if (!g.touched || !__ldg(g.touched + t)) store8(out + u * 8, zero);
+    } else {
+      int64_t t = g.small ? g.by_row.quotient((uint32_t)(u * 8)) : u * 8 / g.cols;
+      const int64_t last = min(u * 8 + 7, n - 1);
+      bool free = !g.touched || !__ldg(g.touched + t);
+      if (free && last == u * 8 + 7 && last < (t + 1) * g.cols) {
+        store8(out + u * 8, zero);
+        continue;
+      }
+      for (int64_t i = u * 8; i <= last; ++i) {
+        if (i == (t + 1) * g.cols) {
+          ++t;
+          free = !g.touched || !__ldg(g.touched + t);
         }
-      __syncthreads();
+        if (free) put(out + i, 0.f);
+      }
     }
-    int32_t* x = k0; k0 = k1; k1 = x;
-    x = p0; p0 = p1; p1 = x;
   }
 }
 
-// One CTA per row of the table: its tokens by bisection, their gradients added in the order of the tokens.
-template <class In, class Out>
-__global__ void __launch_bounds__(kBlock) k_embedding_grad(const In* __restrict__ dy, const int32_t* __restrict__ keys, const int32_t* __restrict__ pos, Out* __restrict__ out, int64_t rows, int64_t cols,
-                                                           int64_t ld, float scale) {
-  const int32_t v = blockIdx.x;
-  auto first = [&](int32_t key) {
-    int64_t lo = 0, hi = rows;
-    while (lo < hi) {
-      const int64_t mid = (lo + hi) / 2;
-      if (keys[mid] < key) lo = mid + 1;
-      else hi = mid;
+// Columns of a thread: eight consecutive ones (VEC), or eight that lie `lanes` apart (rows that do not start on 16 bytes).
+template <class In, class Out, bool VEC>
+__global__ void __launch_bounds__(kBlock) k_sum_runs(const In* __restrict__ dy, Out* __restrict__ out, const __grid_constant__ GradArgs g) {
+  __shared__ int32_t skey[kMaxChunk * kBlock / 8 + 2], spos[kMaxChunk * kBlock / 8];
+  if (blockIdx.x >= g.chunk_blocks * g.slices) {
+    fill_rows<Out, VEC>(g, out, blockIdx.x - g.chunk_blocks * g.slices);
+    return;
+  }
+  const int64_t block = blockIdx.x / g.slices, slice = blockIdx.x - block * g.slices;
+  const int groups = kBlock >> g.log_lanes, places = groups * g.chunk;
+  const int64_t first = block * places;
+  for (int i = threadIdx.x; i < places; i += kBlock) {
+    const int64_t q = first + i;
+    skey[i + 1] = q < g.rows ? __ldg(g.key + q) : INT32_MAX;
+    spos[i] = q < g.rows ? __ldg(g.pos + q) : 0;
+  }
+  if (threadIdx.x == 0) skey[0] = first > 0 ? __ldg(g.key + first - 1) : -1;
+  if (threadIdx.x == 1) skey[places + 1] = first + places < g.rows ? __ldg(g.key + first + places) : INT32_MAX;
+  __syncthreads();
+  const int lane = threadIdx.x & (g.lanes - 1), group = threadIdx.x >> g.log_lanes;
+  const int64_t chunk = block * groups + group;
+  if (chunk >= g.chunks) return;
+  const int32_t *key = skey + 1 + group * g.chunk, *pos = spos + group * g.chunk;
+  const int64_t c0 = slice * (8 * g.lanes) + (VEC ? lane * 8 : lane);
+  auto col = [&](int j) { return c0 + (VEC ? j : j * g.lanes); };
+  if (c0 >= g.cols && !(lane == 0 && slice == 0)) return;
+  const bool mine = c0 < g.cols;
+  float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  int32_t now = key[0];
+  bool enters = now == key[-1];
+  auto flush = [&](bool leaves) {
+    if (!mine) return;
+    if (enters || leaves) {
+      float* p = g.part + (chunk * 2 + (enters ? 0 : 1)) * g.cols;
+      if (VEC) {
+        *(float4*)(p + c0) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+        *(float4*)(p + c0 + 4) = make_float4(acc[4], acc[5], acc[6], acc[7]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (col(j) < g.cols) p[col(j)] = acc[j];
+      }
+    } else {
+      Out* p = out + (int64_t)now * g.cols;
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = g.scale * acc[j];
+      if (VEC) store8(p + c0, v);
+      else
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (col(j) < g.cols) put(p + col(j), v[j]);
     }
-    return lo;
   };
-  const int64_t b = first(v), e = first(v + 1);
-  for (int64_t c = threadIdx.x; c < cols; c += kBlock) {
-    float sum = 0;
-    for (int64_t q = b; q < e; ++q) sum += widen(dy[(int64_t)pos[q] * ld + c]);
-    put(out + (int64_t)v * cols + c, scale * sum);
+  constexpr int kFly = 4;
+  int i = 0;
+  for (; i < g.chunk && key[i] < g.vocab; i += kFly) {
+    float v[kFly][8];
+    Raw8<In> raw[kFly];
+#pragma unroll
+    for (int k = 0; k < kFly; ++k) {
+      if (i + k >= g.chunk || key[i + k] >= g.vocab || !mine) continue;
+      const In* p = dy + (int64_t)pos[i + k] * g.ld;
+      if (VEC) raw[k] = load8(p + c0);
+      else
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[k][j] = col(j) < g.cols ? widen(__ldcs(p + col(j))) : 0.f;
+    }
+#pragma unroll
+    for (int k = 0; k < kFly; ++k) {
+      if (i + k >= g.chunk || key[i + k] >= g.vocab) break;
+      if (key[i + k] != now) {
+        flush(false);
+        enters = false;
+        now = key[i + k];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[j] = 0.f;
+      }
+      if (VEC && mine) widen8(raw[k], v[k]);
+      if (mine) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[j] += v[k][j];
+      }
+    }
+  }
+  if (now >= g.vocab) return;  // nothing but tokens outside the table
+  const bool leaves = key[g.chunk - 1] == now && key[g.chunk] == now;
+  flush(leaves);
+  if (leaves && !enters && lane == 0 && slice == 0) g.list[atomicAdd(g.crossing, 1)] = (int32_t)chunk;
+}
+
+// The runs that cross borders of chunks.  A block adds the parts of one run for 256 columns: its eight warps take equal
+// stretches of the run's chunks, their sums are added in the order of the warps.
+template <class Out>
+__global__ void __launch_bounds__(kBlock) k_join_runs(Out* __restrict__ out, const __grid_constant__ GradArgs g) {
+  __shared__ float sum[kBlock / 32][kBlock];
+  const int n = *g.crossing, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t slices = (g.cols + kBlock - 1) / kBlock, work = n * slices;
+  for (int64_t w = blockIdx.x; w < work; w += gridDim.x) {
+    const int64_t item = w / slices, c0 = (w - item * slices) * kBlock;
+    const int64_t chunk = g.list[item];
+    const int32_t key = __ldg(g.key + (chunk + 1) * g.chunk - 1);
+    int64_t m = 0;  // chunks behind this one that begin inside the run
+    for (;;) {
+      const int64_t c = chunk + 1 + m + threadIdx.x;
+      const int same = __syncthreads_count(c < g.chunks && __ldg(g.key + c * g.chunk) == key);
+      m += same;
+      if (same < kBlock) break;
+    }
+    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    const int64_t lo = chunk + 1 + m * warp / (kBlock / 32), hi = chunk + 1 + m * (warp + 1) / (kBlock / 32);
+#pragma unroll 4
+    for (int64_t c = lo; c < hi; ++c) {
+      const float* p = g.part + c * 2 * g.cols + c0 + lane;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (c0 + lane + j * 32 < g.cols) acc[j] += __ldg(p + j * 32);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sum[warp][lane + j * 32] = acc[j];
+    __syncthreads();
+    const int64_t c = c0 + threadIdx.x;
+    if (c < g.cols) {
+      float total = __ldg(g.part + (chunk * 2 + 1) * g.cols + c);
+#pragma unroll
+      for (int k = 0; k < kBlock / 32; ++k) total += sum[k][threadIdx.x];
+      put(out + (int64_t)key * g.cols + c, g.scale * total);
+    }
+    __syncthreads();
   }
 }
 
-int sort_passes(int64_t vocab) {
-  int passes = 1;
-  while (passes < 4 && (vocab >> (8 * passes))) ++passes;
-  return passes;
-}
+// How the gradient is cut, and where its parts lie in the workspace.
+struct GradPlan {
+  int passes, digit, ranks;
+  GradArgs g;
+  int64_t keys_a, keys_b, touched, crossing, list, part, bytes;  // byte offsets
+  GradPlan(const CallDesc& d, int sm_count) : g{} {
+    int bits = 1;
+    while (bits < 31 && (d.vocab >> bits)) ++bits;
+    passes = (bits + 8) / 9;
+    digit = (bits + passes - 1) / passes;
+    ranks = 1;
+    while (ranks < kSortRanks && (int64_t)ranks * kSortBlock < d.rows) ranks *= 2;
+    g.rows = d.rows;
+    g.cols = d.cols;
+    g.ld = d.ld;
+    g.vocab = d.vocab;
+    g.scale = (float)d.scale;
+    g.lanes = 8;
+    g.log_lanes = 3;
+    while (g.lanes < kBlock && g.lanes * 8 < d.cols) {
+      g.lanes *= 2;
+      ++g.log_lanes;
+    }
+    const int groups = kBlock / g.lanes;
+    g.slices = std::max<int64_t>(1, (d.cols + 8 * g.lanes - 1) / (8 * g.lanes));
+    // chunks as long as they still give every SM two blocks
+    g.chunk = kMaxChunk;
+    while (g.chunk > 8 && (d.rows + (int64_t)g.chunk * groups - 1) / ((int64_t)g.chunk * groups) * g.slices < sm_count * 2) g.chunk /= 2;
+    g.chunks = (d.rows + g.chunk - 1) / g.chunk;
+    g.chunk_blocks = (g.chunks + groups - 1) / groups;
+    auto take = [&](int64_t n) {
+      const int64_t at = bytes;
+      bytes += (n + 255) / 256 * 256;
+      return at;
+    };
+    bytes = 0;
+    keys_a = take(2 * d.rows * 4);
+    keys_b = take(2 * d.rows * 4);
+    touched = take(d.vocab + 16);
+    crossing = take(4);
+    list = take(g.chunks * 4);
+    part = take(g.chunks * 2 * d.cols * 4);
+  }
+};
 
 // calls f with null pointers of the types that the three element types stand for
 template <class F>
@@ -192,22 +457,62 @@ cudaError_t launch_embedding(const LaunchCtx& c, const CallDesc& d, const void* 
   return cudaGetLastError();
 }
 
-int64_t embedding_grad_workspace(const CallDesc& d, int) { return 4 * d.rows * (int64_t)sizeof(int32_t); }
+int64_t embedding_grad_workspace(const CallDesc& d, int sm_count) { return d.rows && d.vocab * d.cols ? GradPlan(d, sm_count).bytes : 0; }
 
 cudaError_t launch_embedding_grad(const LaunchCtx& c, const CallDesc& d, const void* dy, const void* ids, void* out, void* workspace) {
   if (d.vocab * d.cols == 0) return cudaSuccess;
-  int32_t* w = (int32_t*)workspace;
-  int32_t *k0 = w, *p0 = w + d.rows, *k1 = w + 2 * d.rows, *p1 = w + 3 * d.rows;
-  const int passes = sort_passes(d.vocab);
+  GradPlan p(d, c.sm_count);
+  GradArgs& g = p.g;
+  char* w = (char*)workspace;
+  const int64_t n = d.vocab * d.cols;
+  const bool vec_out = d.cols % 8 == 0;
+  const bool vec = vec_out && aligned16(dy) && d.ld * (int64_t)dt_size(d.in_dt) % 16 == 0;
+  g.by_row = Divisor(vec ? d.cols / 8 : d.cols);
+  g.small = n < (int64_t)1 << 31;
+  const int64_t fill_blocks = ((n + 7) / 8 + kBlock * kFillUnits - 1) / (kBlock * kFillUnits);
+  cudaError_t err = cudaSuccess;
   with_types(d.in_dt, d.out_dt, d.ids_dt, [&](auto* i, auto* o, auto* id) {
+    using In = std::remove_pointer_t<decltype(i)>;
+    using Out = std::remove_pointer_t<decltype(o)>;
+    using Id = std::remove_pointer_t<decltype(id)>;
     if (d.rows) {
-      k_sort_tokens<<<1, kBlock, 0, c.stream>>>((decltype(id))ids, d.rows, d.vocab, passes, k0, p0, k1, p1);
+      int32_t *a = (int32_t*)(w + p.keys_a), *b = (int32_t*)(w + p.keys_b);
+      g.key = p.passes % 2 ? a : b;
+      g.pos = g.key + d.rows;
+      g.touched = (const uint8_t*)(w + p.touched);
+      g.crossing = (int32_t*)(w + p.crossing);
+      g.list = (int32_t*)(w + p.list);
+      g.part = (float*)(w + p.part);
+      auto* sort = k_sort_tokens<Id>;
+      err = cudaFuncSetAttribute(sort, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(SortShared));  // of the current device
+      if (err != cudaSuccess) return;
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3((unsigned)p.ranks);
+      cfg.blockDim = dim3(kSortBlock);
+      cfg.dynamicSmemBytes = sizeof(SortShared);
+      cfg.stream = c.stream;
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = (unsigned)p.ranks;
+      attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      err = cudaLaunchKernelEx(&cfg, sort, (const Id*)ids, d.rows, d.vocab, p.passes, p.digit, a, b, (uint8_t*)(w + p.touched), g.crossing);
+      if (err != cudaSuccess) return;
+      ++*c.launches;
+    } else {
+      g.chunk_blocks = 0;
+    }
+    auto* sum = vec ? k_sum_runs<In, Out, true> : k_sum_runs<In, Out, false>;
+    sum<<<(unsigned)(g.chunk_blocks * g.slices + fill_blocks), kBlock, 0, c.stream>>>((const In*)dy, (Out*)out, g);
+    ++*c.launches;
+    if (g.chunks > 1) {
+      const int64_t most = g.chunks * ((d.cols + kBlock - 1) / kBlock);
+      k_join_runs<Out><<<(unsigned)std::min<int64_t>(most, (int64_t)c.sm_count * 4), kBlock, 0, c.stream>>>((Out*)out, g);
       ++*c.launches;
     }
-    k_embedding_grad<<<(unsigned)d.vocab, kBlock, 0, c.stream>>>((decltype(i))dy, passes % 2 ? k1 : k0, passes % 2 ? p1 : p0, (decltype(o))out, d.rows, d.cols, d.ld, (float)d.scale);
   });
-  ++*c.launches;
-  return cudaGetLastError();
+  return err != cudaSuccess ? err : cudaGetLastError();
 }
 
 }  // namespace rx

@@ -52,8 +52,9 @@ __device__ __forceinline__ void store8(uint16_t* p, const float (&v)[8]) {
 // invariant integers using multiplication", 1994): with l = ceil(log2 d) and m = ceil(2^(31 + l) / d), which is below
 // 2^32, n / d = (n m) >> (31 + l) for every n < 2^31.
 struct Divisor {
-  uint32_t d, m;
-  int shift;
+  uint32_t d = 0, m = 0;
+  int shift = 0;
+  Divisor() = default;
   explicit Divisor(int64_t divisor) : d((uint32_t)divisor), m(0), shift(0) {
     if (divisor <= 0 || divisor >= (int64_t)1 << 31) return;  // not used
     int l = 0;

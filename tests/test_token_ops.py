@@ -450,3 +450,19 @@ def test_step_repeats_itself_and_follows_its_key(rx, client):
     assert all(np.array_equal(f64(x), f64(y)) for x, y in zip(a, b))
     c = run(rx, client, text, p + [ids, np.roll(ids, -1), np.array([1, 3], np.int32)])
     assert not np.array_equal(f64(a[0]), f64(c[0]))  # another key, another mask
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("pattern", ["one", "two", "all different", "padding only", "runs of 33", "falling", "first and last"])
+@pytest.mark.parametrize("tokens,features", [(31, 8), (1024, 40), (8193, 8), (4000, 2056)])
+def test_embedding_grad_patterns(rx, ref, client, pattern, tokens, features):
+    """Runs that fill, cross and end at the borders of the pieces the work is cut into."""
+    vocab = 9000
+    i = np.arange(tokens)
+    ids = {"one": np.full(tokens, 77), "two": np.where(i % 2, 8999, 0), "all different": i % vocab, "padding only": np.where(i % 2, -1, vocab), "runs of 33": i // 33, "falling": (vocab - 1 - i // 8) % vocab,
+           "first and last": np.where(i < tokens // 2, 0, vocab - 1)}[pattern].astype(np.int32)
+    rng = np.random.default_rng(12)
+    dy = rng.integers(-8, 9, (tokens, features)).astype(np.float32)  # whole numbers: every sum is exact
+    text = rx.programs.embedding_grad(vocab, features, tokens, et="f32")
+    got, = run(rx, client, text, [dy, ids])
+    assert np.array_equal(got, ref.run_module(text, [dy, ids])[0])
