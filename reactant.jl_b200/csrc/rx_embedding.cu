@@ -58,7 +58,7 @@ __global__ void __launch_bounds__(kBlock) k_embedding(const In* __restrict__ tab
 #pragma unroll
         for (int q = 0; q < 8; ++q) v[q] *= scale;
       }
-      store8(out + (base + k * kBlock) * 8, v);
+      store8_whole(out + (base + k * kBlock) * 8, v);
     }
   } else {
 #pragma unroll 1
@@ -81,7 +81,7 @@ __global__ void __launch_bounds__(kBlock) k_embedding(const In* __restrict__ tab
           }
         }
       }
-      if (m == 8) store8(out + u * 8, v);
+      if (m == 8) store8_whole(out + u * 8, v);
       else
         for (int q = 0; q < m; ++q) put(out + u * 8 + q, v[q]);
     }
@@ -104,12 +104,23 @@ __global__ void __launch_bounds__(kBlock) k_embedding(const In* __restrict__ tab
 // through a vote, the lowest lane adds), the counts become places through sums over warps, blocks (distributed shared
 // memory) and digits, and a second walk writes key and place.
 constexpr int kSortBlock = 1024, kSortWarps = kSortBlock / 32, kBins = 512, kSortRanks = 8;
+constexpr int kHold = 8;  // groups of 32 tokens whose keys a warp asks for at once
 
 struct SortShared {
   uint32_t count[kSortWarps][kBins];
   uint32_t total[kBins], base[kBins];
   uint32_t warp_sum[kSortWarps];
 };
+
+// the lanes that have this lane's digit (of `digit` bits; digit + 1 where some lanes have none), by one vote a bit
+__device__ __forceinline__ uint32_t lanes_with(uint32_t d, int bits) {
+  uint32_t same = ~0u;
+  for (int b = 0; b < bits; ++b) {
+    const uint32_t set = __ballot_sync(~0u, d >> b & 1);
+    same &= d >> b & 1 ? set : ~set;
+  }
+  return same;
+}
 
 template <class Id>
 __global__ void __launch_bounds__(kSortBlock) k_sort_tokens(const Id* __restrict__ ids, int64_t rows, int64_t vocab, int passes, int digit, int32_t* a, int32_t* b, uint8_t* touched, int32_t* crossing) {
@@ -138,12 +149,23 @@ __global__ void __launch_bounds__(kSortBlock) k_sort_tokens(const Id* __restrict
     };
     for (int k = lane; k < kBins; k += 32) sh.count[warp][k] = 0;
     __syncwarp();
-    for (int64_t t0 = lo; t0 < hi; t0 += 32) {
-      const bool have = t0 + lane < hi;
-      const uint32_t d = have ? (uint32_t)key_at(t0 + lane) >> shift & mask : ~0u;
-      const uint32_t same = __match_any_sync(~0u, d);
-      if (have && !(same & below)) sh.count[warp][d] += __popc(same);
-      __syncwarp();
+    int32_t key[kHold];
+    auto fetch = [&](int64_t t0) {
+#pragma unroll
+      for (int k = 0; k < kHold; ++k)
+        if (t0 + k * 32 + lane < hi) key[k] = key_at(t0 + k * 32 + lane);
+    };
+    for (int64_t t0 = lo; t0 < hi; t0 += 32 * kHold) {
+      fetch(t0);
+#pragma unroll
+      for (int k = 0; k < kHold; ++k) {
+        if (t0 + k * 32 >= hi) break;
+        const bool have = t0 + k * 32 + lane < hi;
+        const uint32_t d = have ? (uint32_t)key[k] >> shift & mask : ~0u;
+        const uint32_t same = lanes_with(d, digit + 1);
+        if (have && !(same & below)) sh.count[warp][d] += __popc(same);
+        __syncwarp();
+      }
     }
     __syncthreads();
     if (tid < kBins) {
@@ -178,20 +200,30 @@ __global__ void __launch_bounds__(kSortBlock) k_sort_tokens(const Id* __restrict
       sh.base[tid] = front + scan - all + before;
     }
     __syncthreads();
-    for (int64_t t0 = lo; t0 < hi; t0 += 32) {
-      const bool have = t0 + lane < hi;
-      const int32_t key = have ? key_at(t0 + lane) : 0;
-      const uint32_t d = have ? (uint32_t)key >> shift & mask : ~0u;
-      const uint32_t same = __match_any_sync(~0u, d);
-      const uint32_t at = have ? sh.base[d] + sh.count[warp][d] + __popc(same & below) : 0;
-      __syncwarp();
-      if (have) {
-        if (!(same & below)) sh.count[warp][d] += __popc(same);
-        to[at] = key;
-        to[rows + at] = pass ? __ldcg(from + rows + t0 + lane) : (int32_t)(t0 + lane);
-        if (!pass && key < vocab) touched[key] = 1;
+    for (int64_t t0 = lo; t0 < hi; t0 += 32 * kHold) {
+      if (hi - lo > 32 * kHold) fetch(t0);  // a short run still has its keys
+      int32_t pos[kHold];
+#pragma unroll
+      for (int k = 0; k < kHold; ++k) {
+        const int64_t t = t0 + k * 32 + lane;
+        if (t < hi) pos[k] = pass ? __ldcg(from + rows + t) : (int32_t)t;
       }
-      __syncwarp();
+#pragma unroll
+      for (int k = 0; k < kHold; ++k) {
+        if (t0 + k * 32 >= hi) break;
+        const bool have = t0 + k * 32 + lane < hi;
+        const uint32_t d = have ? (uint32_t)key[k] >> shift & mask : ~0u;
+        const uint32_t same = lanes_with(d, digit + 1);
+        const uint32_t at = have ? sh.base[d] + sh.count[warp][d] + __popc(same & below) : 0;
+        __syncwarp();
+        if (have) {
+          if (!(same & below)) sh.count[warp][d] += __popc(same);
+          to[at] = key[k];
+          to[rows + at] = pos[k];
+          if (!pass && key[k] < vocab) touched[key[k]] = 1;
+        }
+        __syncwarp();
+      }
     }
     cluster.sync();
   }
@@ -210,7 +242,7 @@ struct GradArgs {
   bool small;
 };
 
-constexpr int kMaxChunk = 32, kFillUnits = 8;
+constexpr int kMaxChunk = 128, kMaxPlaces = 1024, kFillUnits = 8;
 
 // Zeros for the rows that no token has: units of eight consecutive elements of the result, kFillUnits a thread.
 template <class Out, bool VEC>
@@ -224,13 +256,13 @@ __device__ __forceinline__ void fill_rows(const GradArgs& g, Out* out, int64_t b
     if (u >= units) return;
     if (VEC) {
       const int64_t t = g.small ? g.by_row.quotient((uint32_t)u) : u / per_row;
-      if (!g.touched || !__ldg(g.touched + t)) store8(out + u * 8, zero);
+      if (!g.touched || !__ldg(g.touched + t)) store8_whole(out + u * 8, zero);
     } else {
       int64_t t = g.small ? g.by_row.quotient((uint32_t)(u * 8)) : u * 8 / g.cols;
       const int64_t last = min(u * 8 + 7, n - 1);
       bool free = !g.touched || !__ldg(g.touched + t);
       if (free && last == u * 8 + 7 && last < (t + 1) * g.cols) {
-        store8(out + u * 8, zero);
+        store8_whole(out + u * 8, zero);
         continue;
       }
       for (int64_t i = u * 8; i <= last; ++i) {
@@ -247,7 +279,7 @@ __device__ __forceinline__ void fill_rows(const GradArgs& g, Out* out, int64_t b
 // Columns of a thread: eight consecutive ones (VEC), or eight that lie `lanes` apart (rows that do not start on 16 bytes).
 template <class In, class Out, bool VEC>
 __global__ void __launch_bounds__(kBlock) k_sum_runs(const In* __restrict__ dy, Out* __restrict__ out, const __grid_constant__ GradArgs g) {
-  __shared__ int32_t skey[kMaxChunk * kBlock / 8 + 2], spos[kMaxChunk * kBlock / 8];
+  __shared__ int32_t skey[kMaxPlaces + 2], spos[kMaxPlaces];
   if (blockIdx.x >= g.chunk_blocks * g.slices) {
     fill_rows<Out, VEC>(g, out, blockIdx.x - g.chunk_blocks * g.slices);
     return;
@@ -291,7 +323,7 @@ __global__ void __launch_bounds__(kBlock) k_sum_runs(const In* __restrict__ dy, 
       float v[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = g.scale * acc[j];
-      if (VEC) store8(p + c0, v);
+      if (VEC) store8_whole(p + c0, v);
       else
 #pragma unroll
         for (int j = 0; j < 8; ++j)
@@ -402,7 +434,7 @@ struct GradPlan {
     const int groups = kBlock / g.lanes;
     g.slices = std::max<int64_t>(1, (d.cols + 8 * g.lanes - 1) / (8 * g.lanes));
     // chunks as long as they still give every SM two blocks
-    g.chunk = kMaxChunk;
+    g.chunk = std::min(kMaxChunk, kMaxPlaces / groups);
     while (g.chunk > 8 && (d.rows + (int64_t)g.chunk * groups - 1) / ((int64_t)g.chunk * groups) * g.slices < sm_count * 2) g.chunk /= 2;
     g.chunks = (d.rows + g.chunk - 1) / g.chunk;
     g.chunk_blocks = (g.chunks + groups - 1) / groups;
@@ -508,7 +540,7 @@ cudaError_t launch_embedding_grad(const LaunchCtx& c, const CallDesc& d, const v
     ++*c.launches;
     if (g.chunks > 1) {
       const int64_t most = g.chunks * ((d.cols + kBlock - 1) / kBlock);
-      k_join_runs<Out><<<(unsigned)std::min<int64_t>(most, (int64_t)c.sm_count * 4), kBlock, 0, c.stream>>>((Out*)out, g);
+      k_join_runs<Out><<<(unsigned)std::min<int64_t>(most, (int64_t)c.sm_count * 8), kBlock, 0, c.stream>>>((Out*)out, g);
       ++*c.launches;
     }
   });

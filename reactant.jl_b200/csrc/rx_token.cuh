@@ -48,6 +48,12 @@ __device__ __forceinline__ void store8(uint16_t* p, const float (&v)[8]) {
   __stcs((uint4*)p, make_uint4(bf16x2_bits(v[0], v[1]), bf16x2_bits(v[2], v[3]), bf16x2_bits(v[4], v[5]), bf16x2_bits(v[6], v[7])));
 }
 
+// The same where the eight elements start on their own size (32 bytes for floats): one store a lane, whole sectors.
+__device__ __forceinline__ void store8_whole(float* p, const float (&v)[8]) {
+  asm volatile("st.global.cs.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]) : "memory");
+}
+__device__ __forceinline__ void store8_whole(uint16_t* p, const float (&v)[8]) { store8(p, v); }
+
 // Quotients of numbers below 2^31 by a fixed divisor with one multiplication (Granlund and Montgomery, "Division by
 // invariant integers using multiplication", 1994): with l = ceil(log2 d) and m = ceil(2^(31 + l) / d), which is below
 // 2^32, n / d = (n m) >> (31 + l) for every n < 2^31.
