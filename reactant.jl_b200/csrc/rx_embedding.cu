@@ -91,28 +91,36 @@ __global__ void __launch_bounds__(kBlock) k_embedding(const In* __restrict__ tab
 // ---- the gradient ----------------------------------------------------------------------------------------------------
 // dtable[v] = scale * sum of dy[t] over the tokens with id v, added in the order of the tokens and so the same from run
 // to run, in four parts:
-//   k_sort_tokens   the tokens' places sorted by id (stably), and which rows have a token at all
-//   k_sum_runs      chunks of kChunk places: a run of one id inside a chunk is summed and written to its row; a run that
-//                   crosses a border of chunks leaves its part of the sum in the workspace
+//   sort            the tokens' places sorted by id (stably), and which rows have a token at all
+//   k_sum_runs      chunks of the sorted places: a run of one id inside a chunk is summed and written to its row; a run
+//                   that crosses a border of chunks leaves its part of the sum in the workspace
 //   (same launch)   rows without a token are filled with zeros
 //   k_join_runs     the parts of every run that crosses borders, added in the order of the chunks
 // No atomic touches a sum.  The work is bound by memory: the gradients are read once, the table's written once; cutting
 // at fixed places rather than by id keeps the blocks even when few ids hold most of the tokens.
 
-// Sort: least significant digits first, up to 9 bits a pass, by one cluster of up to eight blocks.  Each warp owns a run
-// of consecutive tokens: it counts their digits in its own row of shared memory (equal digits among 32 tokens meet
-// through a vote, the lowest lane adds), the counts become places through sums over warps, blocks (distributed shared
-// memory) and digits, and a second walk writes key and place.
+// Sort: least significant digits first, up to 9 bits a pass.  Each warp owns a run of consecutive tokens: it counts their
+// digits in its own row of shared memory (equal digits among 32 tokens are found by votes, the lowest lane adds), the
+// counts become places through sums over warps, blocks and digits, and a second walk writes key and place.
+//
+// Up to kClusterTokens one cluster of up to eight blocks does all passes in one launch, the blocks' counts meeting in
+// distributed shared memory.  More tokens are spread over up to kPlaceBlocks blocks, two launches a pass: what bounds a
+// pass is the scattered stores, one sector a cycle and SM (65536 tokens: 51 us on the cluster's eight SMs).  (Writing
+// the zeros of the untouched rows from further blocks of these launches made the whole slower, 251 -> 280 us at 65536
+// tokens and 131072 x 2048: the sort's loads and stores then wait behind the fill's.)
 constexpr int kSortBlock = 1024, kSortWarps = kSortBlock / 32, kBins = 512, kSortRanks = 8;
 constexpr int kHold = 8;  // groups of 32 tokens whose keys a warp asks for at once
+constexpr int64_t kClusterTokens = kSortRanks * kSortBlock;
+constexpr int kPlaceBlocks = 128;
 
 struct SortShared {
   uint32_t count[kSortWarps][kBins];
   uint32_t total[kBins], base[kBins];
   uint32_t warp_sum[kSortWarps];
+  uint32_t half_all[kBins], half_before[kBins];
 };
 
-// the lanes that have this lane's digit (of `digit` bits; digit + 1 where some lanes have none), by one vote a bit
+// the lanes that have this lane's digit, by one vote a bit (one bit more than the digit where some lanes have none)
 __device__ __forceinline__ uint32_t lanes_with(uint32_t d, int bits) {
   uint32_t same = ~0u;
   for (int b = 0; b < bits; ++b) {
@@ -123,40 +131,39 @@ __device__ __forceinline__ uint32_t lanes_with(uint32_t d, int bits) {
 }
 
 template <class Id>
-__global__ void __launch_bounds__(kSortBlock) k_sort_tokens(const Id* __restrict__ ids, int64_t rows, int64_t vocab, int passes, int digit, int32_t* a, int32_t* b, uint8_t* touched, int32_t* crossing) {
-  namespace cg = cooperative_groups;
-  extern __shared__ __align__(16) uint8_t raw[];
-  SortShared& sh = *(SortShared*)raw;
-  cg::cluster_group cluster = cg::this_cluster();
-  const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  {
-    const int64_t words = (vocab + 15) / 16;
-    for (int64_t i = (int64_t)rank * kSortBlock + tid; i < words; i += (int64_t)ranks * kSortBlock) ((uint4*)touched)[i] = make_uint4(0, 0, 0, 0);
-    if (rank == 0 && tid == 0) *crossing = 0;
+struct SortPass {
+  const Id* ids;
+  const int32_t* from;  // keys and, `rows` behind them, places; null: the first pass, which reads the ids
+  int32_t* to;
+  uint8_t* touched;     // rows with a token, marked by the first pass
+  int64_t rows, vocab, lo, hi;  // this warp's run
+  int shift, digit, lane, warp;
+
+  __device__ __forceinline__ void own(int rank, int ranks) {
+    lane = threadIdx.x & 31;
+    warp = threadIdx.x >> 5;
+    const int64_t per = ((rows + ranks * kSortWarps - 1) / (ranks * kSortWarps) + 31) / 32 * 32;
+    lo = min(rows, per * (rank * kSortWarps + warp));
+    hi = min(rows, lo + per);
   }
-  const int64_t per = ((rows + ranks * kSortWarps - 1) / (ranks * kSortWarps) + 31) / 32 * 32;
-  const int64_t lo = min(rows, per * (rank * kSortWarps + warp)), hi = min(rows, lo + per);
-  const uint32_t below = (1u << lane) - 1;
-  for (int pass = 0; pass < passes; ++pass) {
-    const int32_t* from = pass % 2 ? a : b;  // the first pass reads the ids
-    int32_t* to = pass % 2 ? b : a;
-    const int shift = pass * digit;
-    const uint32_t mask = (1u << digit) - 1;
-    auto key_at = [&](int64_t t) -> int32_t {
-      if (pass) return __ldcg(from + t);
-      const int64_t id = (int64_t)__ldg(ids + t);
-      return id >= 0 && id < vocab ? (int32_t)id : (int32_t)vocab;  // a token outside the table comes last
-    };
+  __device__ __forceinline__ int32_t key_at(int64_t t) const {
+    if (from) return __ldcg(from + t);
+    const int64_t id = (int64_t)__ldg(ids + t);
+    return id >= 0 && id < vocab ? (int32_t)id : (int32_t)vocab;  // a token outside the table comes last
+  }
+  __device__ __forceinline__ void fetch(int64_t t0, int32_t (&key)[kHold]) const {
+#pragma unroll
+    for (int k = 0; k < kHold; ++k)
+      if (t0 + k * 32 + lane < hi) key[k] = key_at(t0 + k * 32 + lane);
+  }
+  // First walk: counts of this block's digits, as sums over the warps in front, and their totals.  `key` keeps the keys
+  // of a short run.
+  __device__ __forceinline__ void count(SortShared& sh, int32_t (&key)[kHold]) const {
     for (int k = lane; k < kBins; k += 32) sh.count[warp][k] = 0;
     __syncwarp();
-    int32_t key[kHold];
-    auto fetch = [&](int64_t t0) {
-#pragma unroll
-      for (int k = 0; k < kHold; ++k)
-        if (t0 + k * 32 + lane < hi) key[k] = key_at(t0 + k * 32 + lane);
-    };
+    const uint32_t below = (1u << lane) - 1, mask = (1u << digit) - 1;
     for (int64_t t0 = lo; t0 < hi; t0 += 32 * kHold) {
-      fetch(t0);
+      fetch(t0, key);
 #pragma unroll
       for (int k = 0; k < kHold; ++k) {
         if (t0 + k * 32 >= hi) break;
@@ -168,25 +175,20 @@ __global__ void __launch_bounds__(kSortBlock) k_sort_tokens(const Id* __restrict
       }
     }
     __syncthreads();
-    if (tid < kBins) {
+    if (threadIdx.x < kBins) {
       uint32_t sum = 0;
 #pragma unroll 8
       for (int w = 0; w < kSortWarps; ++w) {
-        const uint32_t n = sh.count[w][tid];
-        sh.count[w][tid] = sum;
+        const uint32_t n = sh.count[w][threadIdx.x];
+        sh.count[w][threadIdx.x] = sum;
         sum += n;
       }
-      sh.total[tid] = sum;
+      sh.total[threadIdx.x] = sum;
     }
-    cluster.sync();
-    uint32_t before = 0, all = 0;
-    if (tid < kBins)
-      for (int r = 0; r < ranks; ++r) {
-        const uint32_t n = *cluster.map_shared_rank(&sh.total[tid], r);
-        if (r < rank) before += n;
-        all += n;
-      }
-    uint32_t scan = all;  // over the digits
+  }
+  // all: tokens of all blocks with digit threadIdx.x; before: those of the blocks in front
+  __device__ __forceinline__ void bases(SortShared& sh, uint32_t all, uint32_t before) const {
+    uint32_t scan = all;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const uint32_t n = __shfl_up_sync(~0u, scan, o);
@@ -194,19 +196,22 @@ __global__ void __launch_bounds__(kSortBlock) k_sort_tokens(const Id* __restrict
     }
     if (lane == 31) sh.warp_sum[warp] = scan;
     __syncthreads();
-    if (tid < kBins) {
-      uint32_t front = 0;
-      for (int w = 0; w < warp; ++w) front += sh.warp_sum[w];
-      sh.base[tid] = front + scan - all + before;
+    if (threadIdx.x < kBins) {
+      uint32_t front = lane < warp ? sh.warp_sum[lane] : 0;  // (at most 16 warps are in front of a digit's)
+      front = __reduce_add_sync(~0u, front);
+      sh.base[threadIdx.x] = front + scan - all + before;
     }
     __syncthreads();
+  }
+  __device__ __forceinline__ void place(SortShared& sh, int32_t (&key)[kHold]) const {
+    const uint32_t below = (1u << lane) - 1, mask = (1u << digit) - 1;
     for (int64_t t0 = lo; t0 < hi; t0 += 32 * kHold) {
-      if (hi - lo > 32 * kHold) fetch(t0);  // a short run still has its keys
+      if (hi - lo > 32 * kHold) fetch(t0, key);
       int32_t pos[kHold];
 #pragma unroll
       for (int k = 0; k < kHold; ++k) {
         const int64_t t = t0 + k * 32 + lane;
-        if (t < hi) pos[k] = pass ? __ldcg(from + rows + t) : (int32_t)t;
+        if (t < hi) pos[k] = from ? __ldcg(from + rows + t) : (int32_t)t;
       }
 #pragma unroll
       for (int k = 0; k < kHold; ++k) {
@@ -220,13 +225,121 @@ __global__ void __launch_bounds__(kSortBlock) k_sort_tokens(const Id* __restrict
           if (!(same & below)) sh.count[warp][d] += __popc(same);
           to[at] = key[k];
           to[rows + at] = pos[k];
-          if (!pass && key[k] < vocab) touched[key[k]] = 1;
+          if (!from && key[k] < vocab) touched[key[k]] = 1;
         }
         __syncwarp();
       }
     }
-    cluster.sync();
   }
+};
+
+__device__ __forceinline__ void clear_touched(uint8_t* touched, int64_t vocab, int32_t* crossing, int rank, int ranks) {
+  const int64_t words = (vocab + 15) / 16;
+  for (int64_t i = (int64_t)rank * kSortBlock + threadIdx.x; i < words; i += (int64_t)ranks * kSortBlock) ((uint4*)touched)[i] = make_uint4(0, 0, 0, 0);
+  if (rank == 0 && threadIdx.x == 0) *crossing = 0;
+}
+
+template <class Id>
+__global__ void __launch_bounds__(kSortBlock) k_sort_tokens(SortPass<Id> s, int passes, int32_t* a, int32_t* b, int32_t* crossing) {
+  namespace cg = cooperative_groups;
+  extern __shared__ __align__(16) uint8_t raw[];
+  SortShared& sh = *(SortShared*)raw;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  clear_touched(s.touched, s.vocab, crossing, rank, ranks);
+  s.own(rank, ranks);
+  for (int pass = 0; pass < passes; ++pass) {
+    s.from = pass == 0 ? nullptr : pass % 2 ? a : b;
+    s.to = pass % 2 ? b : a;
+    s.shift = pass * s.digit;
+    int32_t key[kHold];
+    s.count(sh, key);
+    cluster.sync();
+    uint32_t before = 0, all = 0;
+    if (threadIdx.x < kBins)
+      for (int r = 0; r < ranks; ++r) {
+        const uint32_t n = *cluster.map_shared_rank(&sh.total[threadIdx.x], r);
+        if (r < rank) before += n;
+        all += n;
+      }
+    s.bases(sh, all, before);
+    s.place(sh, key);
+    cluster.sync();  // what was written is visible, and nobody reads this block's totals any more
+  }
+}
+
+// Up to 1024 tokens: one block, a token a thread, sorted as (id, place) by Batcher's bitonic network; exchanges within a
+// warp are shuffles (700 tokens: 4 us against 11 for two passes over digits).
+template <class Id>
+__global__ void __launch_bounds__(kSortBlock) k_sort_few_tokens(const Id* __restrict__ ids, int rows, int64_t vocab, int32_t* key, int32_t* pos, uint8_t* touched, int32_t* crossing) {
+  __shared__ uint64_t sh[kSortBlock];
+  const int t = threadIdx.x;
+  uint64_t mine = ~0ull;
+  int32_t k = INT32_MAX;
+  if (t < rows) {
+    const int64_t id = (int64_t)__ldg(ids + t);
+    k = id >= 0 && id < vocab ? (int32_t)id : (int32_t)vocab;
+    mine = (uint64_t)(uint32_t)k << 32 | (uint32_t)t;
+  }
+  clear_touched(touched, vocab, crossing, 0, 1);
+  for (int size = 2; size <= kSortBlock; size *= 2)
+    for (int apart = size / 2; apart > 0; apart /= 2) {
+      uint64_t other;
+      if (apart >= 32) {
+        __syncthreads();
+        sh[t] = mine;
+        __syncthreads();
+        other = sh[t ^ apart];
+      } else {
+        other = __shfl_xor_sync(~0u, mine, apart);
+      }
+      const bool low = ((t & apart) == 0) == ((t & size) == 0);  // this thread keeps the smaller of the two
+      mine = low == (other < mine) ? other : mine;
+    }
+  if (t < rows) {
+    key[t] = (int32_t)(mine >> 32);
+    pos[t] = (int32_t)(uint32_t)mine;
+  }
+  if (k < vocab) touched[k] = 1;  // (every store of zeros is behind one of the barriers above)
+}
+
+// one pass in two launches: totals[block][digit], then the places
+template <class Id>
+__global__ void __launch_bounds__(kSortBlock) k_count_tokens(SortPass<Id> s, uint32_t* totals, int32_t* crossing) {
+  extern __shared__ __align__(16) uint8_t raw[];
+  SortShared& sh = *(SortShared*)raw;
+  if (!s.from) clear_touched(s.touched, s.vocab, crossing, blockIdx.x, gridDim.x);
+  s.own(blockIdx.x, gridDim.x);
+  int32_t key[kHold];
+  s.count(sh, key);
+  if (threadIdx.x < kBins) totals[blockIdx.x * kBins + threadIdx.x] = sh.total[threadIdx.x];
+}
+template <class Id>
+__global__ void __launch_bounds__(kSortBlock) k_place_tokens(SortPass<Id> s, const uint32_t* __restrict__ totals) {
+  extern __shared__ __align__(16) uint8_t raw[];
+  SortShared& sh = *(SortShared*)raw;
+  s.own(blockIdx.x, gridDim.x);
+  // the totals of all blocks, two threads a digit: every second block each
+  const int bin = threadIdx.x % kBins, half = threadIdx.x / kBins, ranks = gridDim.x;
+  uint32_t before = 0, all = 0;
+#pragma unroll 16
+  for (int r = half; r < ranks; r += 2) {
+    const uint32_t n = __ldg(totals + r * kBins + bin);
+    if (r < (int)blockIdx.x) before += n;
+    all += n;
+  }
+  if (half) {
+    sh.half_all[bin] = all;
+    sh.half_before[bin] = before;
+  }
+  int32_t key[kHold];
+  s.count(sh, key);
+  if (!half) {
+    all += sh.half_all[bin];
+    before += sh.half_before[bin];
+  }
+  s.bases(sh, half ? 0 : all, before);
+  s.place(sh, key);
 }
 
 struct GradArgs {
@@ -244,41 +357,46 @@ struct GradArgs {
 
 constexpr int kMaxChunk = 128, kMaxPlaces = 1024, kFillUnits = 8;
 
-// Zeros for the rows that no token has: units of eight consecutive elements of the result, kFillUnits a thread.
+// Zeros for the rows that no token has: units of eight consecutive elements of the result, kFillUnits a thread, whose
+// rows are all looked up before the first is written.  
 template <class Out, bool VEC>
 __device__ __forceinline__ void fill_rows(const GradArgs& g, Out* out, int64_t block) {
   const float zero[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   const int64_t n = g.vocab * g.cols, units = (n + 7) >> 3, per_row = g.cols >> 3;
   const int64_t base = block * (kBlock * kFillUnits) + threadIdx.x;
+  auto row = [&](int64_t i) -> int64_t {  // of element i
+    if (VEC) return g.small ? g.by_row.quotient((uint32_t)(i >> 3)) : (i >> 3) / per_row;
+    return g.small ? g.by_row.quotient((uint32_t)i) : i / g.cols;
+  };
+  bool free[kFillUnits];
 #pragma unroll
   for (int k = 0; k < kFillUnits; ++k) {
     const int64_t u = base + k * kBlock;
-    if (u >= units) return;
+    free[k] = u < units;
+    if (!free[k] || !g.touched) continue;
+    const int64_t t = row(u * 8);
+    uint32_t any = __ldg(g.touched + t);
+    if (!VEC) any |= __ldg(g.touched + row(min(u * 8 + 7, n - 1)));
+    free[k] = !any;
+  }
+#pragma unroll
+  for (int k = 0; k < kFillUnits; ++k) {
+    const int64_t u = base + k * kBlock;
     if (VEC) {
-      const int64_t t = g.small ? g.by_row.quotient((uint32_t)u) : u / per_row;
-      if (!g.touched || !__ldg(g.touched + t)) store8_whole(out + u * 8, zero);
-    } else {
-      int64_t t = g.small ? g.by_row.quotient((uint32_t)(u * 8)) : u * 8 / g.cols;
-      const int64_t last = min(u * 8 + 7, n - 1);
-      bool free = !g.touched || !__ldg(g.touched + t);
-      if (free && last == u * 8 + 7 && last < (t + 1) * g.cols) {
-        store8_whole(out + u * 8, zero);
-        continue;
-      }
-      for (int64_t i = u * 8; i <= last; ++i) {
-        if (i == (t + 1) * g.cols) {
-          ++t;
-          free = !g.touched || !__ldg(g.touched + t);
-        }
-        if (free) put(out + i, 0.f);
-      }
+      if (free[k]) store8_whole(out + u * 8, zero);
+    } else if (u < units) {
+      // a unit whose ends lie in rows without a token: so do its middle's, where a row is eight elements or longer
+      if (free[k] && u * 8 + 8 <= n && g.cols >= 8) store8_whole(out + u * 8, zero);
+      else
+        for (int64_t i = u * 8; i < min(u * 8 + 8, n); ++i)
+          if (!g.touched || !__ldg(g.touched + row(i))) put(out + i, 0.f);
     }
   }
 }
 
 // Columns of a thread: eight consecutive ones (VEC), or eight that lie `lanes` apart (rows that do not start on 16 bytes).
 template <class In, class Out, bool VEC>
-__global__ void __launch_bounds__(kBlock) k_sum_runs(const In* __restrict__ dy, Out* __restrict__ out, const __grid_constant__ GradArgs g) {
+__global__ void __launch_bounds__(kBlock, VEC ? 1 : 3) k_sum_runs(const In* __restrict__ dy, Out* __restrict__ out, const __grid_constant__ GradArgs g) {
   __shared__ int32_t skey[kMaxPlaces + 2], spos[kMaxPlaces];
   if (blockIdx.x >= g.chunk_blocks * g.slices) {
     fill_rows<Out, VEC>(g, out, blockIdx.x - g.chunk_blocks * g.slices);
@@ -411,15 +529,18 @@ __global__ void __launch_bounds__(kBlock) k_join_runs(Out* __restrict__ out, con
 // How the gradient is cut, and where its parts lie in the workspace.
 struct GradPlan {
   int passes, digit, ranks;
+  bool spread;  // the sort in launches of its own passes, over many SMs
   GradArgs g;
-  int64_t keys_a, keys_b, touched, crossing, list, part, bytes;  // byte offsets
+  int64_t keys_a, keys_b, touched, crossing, list, totals, part, bytes;  // byte offsets
   GradPlan(const CallDesc& d, int sm_count) : g{} {
     int bits = 1;
     while (bits < 31 && (d.vocab >> bits)) ++bits;
     passes = (bits + 8) / 9;
     digit = (bits + passes - 1) / passes;
-    ranks = 1;
+    ranks = 2;
     while (ranks < kSortRanks && (int64_t)ranks * kSortBlock < d.rows) ranks *= 2;
+    spread = d.rows > kClusterTokens;
+    if (spread) ranks = (int)std::min<int64_t>(kPlaceBlocks, (d.rows + kSortBlock - 1) / kSortBlock);
     g.rows = d.rows;
     g.cols = d.cols;
     g.ld = d.ld;
@@ -449,6 +570,7 @@ struct GradPlan {
     touched = take(d.vocab + 16);
     crossing = take(4);
     list = take(g.chunks * 4);
+    totals = take((int64_t)kPlaceBlocks * kBins * 4);
     part = take(g.chunks * 2 * d.cols * 4);
   }
 };
@@ -501,7 +623,8 @@ cudaError_t launch_embedding_grad(const LaunchCtx& c, const CallDesc& d, const v
   const bool vec = vec_out && aligned16(dy) && d.ld * (int64_t)dt_size(d.in_dt) % 16 == 0;
   g.by_row = Divisor(vec ? d.cols / 8 : d.cols);
   g.small = n < (int64_t)1 << 31;
-  const int64_t fill_blocks = ((n + 7) / 8 + kBlock * kFillUnits - 1) / (kBlock * kFillUnits);
+  const int64_t units = (n + 7) / 8;
+  const int64_t fill_blocks = (units + kBlock * kFillUnits - 1) / (kBlock * kFillUnits);
   cudaError_t err = cudaSuccess;
   with_types(d.in_dt, d.out_dt, d.ids_dt, [&](auto* i, auto* o, auto* id) {
     using In = std::remove_pointer_t<decltype(i)>;
@@ -515,23 +638,50 @@ cudaError_t launch_embedding_grad(const LaunchCtx& c, const CallDesc& d, const v
       g.crossing = (int32_t*)(w + p.crossing);
       g.list = (int32_t*)(w + p.list);
       g.part = (float*)(w + p.part);
-      auto* sort = k_sort_tokens<Id>;
-      err = cudaFuncSetAttribute(sort, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(SortShared));  // of the current device
-      if (err != cudaSuccess) return;
-      cudaLaunchConfig_t cfg = {};
-      cfg.gridDim = dim3((unsigned)p.ranks);
-      cfg.blockDim = dim3(kSortBlock);
-      cfg.dynamicSmemBytes = sizeof(SortShared);
-      cfg.stream = c.stream;
-      cudaLaunchAttribute attr[1];
-      attr[0].id = cudaLaunchAttributeClusterDimension;
-      attr[0].val.clusterDim.x = (unsigned)p.ranks;
-      attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-      cfg.attrs = attr;
-      cfg.numAttrs = 1;
-      err = cudaLaunchKernelEx(&cfg, sort, (const Id*)ids, d.rows, d.vocab, p.passes, p.digit, a, b, (uint8_t*)(w + p.touched), g.crossing);
-      if (err != cudaSuccess) return;
-      ++*c.launches;
+      SortPass<Id> pass{};
+      pass.ids = (const Id*)ids;
+      pass.touched = (uint8_t*)(w + p.touched);
+      pass.rows = d.rows;
+      pass.vocab = d.vocab;
+      pass.digit = p.digit;
+      auto allow = [&](auto* f) { return cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(SortShared)); };  // of the current device
+      if (d.rows <= kSortBlock) {
+        k_sort_few_tokens<Id><<<1, kSortBlock, 0, c.stream>>>((const Id*)ids, (int)d.rows, d.vocab, (int32_t*)g.key, (int32_t*)g.pos, pass.touched, g.crossing);
+        ++*c.launches;
+      } else if (!p.spread) {
+        auto* sort = k_sort_tokens<Id>;
+        err = allow(sort);
+        if (err != cudaSuccess) return;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)p.ranks);
+        cfg.blockDim = dim3(kSortBlock);
+        cfg.dynamicSmemBytes = sizeof(SortShared);
+        cfg.stream = c.stream;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = (unsigned)p.ranks;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        err = cudaLaunchKernelEx(&cfg, sort, pass, p.passes, a, b, g.crossing);
+        if (err != cudaSuccess) return;
+        ++*c.launches;
+      } else {
+        auto* count = k_count_tokens<Id>;
+        auto* place = k_place_tokens<Id>;
+        err = allow(count);
+        if (err == cudaSuccess) err = allow(place);
+        if (err != cudaSuccess) return;
+        uint32_t* totals = (uint32_t*)(w + p.totals);
+        for (int k = 0; k < p.passes; ++k) {
+          pass.from = k == 0 ? nullptr : k % 2 ? a : b;
+          pass.to = k % 2 ? b : a;
+          pass.shift = k * p.digit;
+          count<<<p.ranks, kSortBlock, sizeof(SortShared), c.stream>>>(pass, totals, g.crossing);
+          place<<<p.ranks, kSortBlock, sizeof(SortShared), c.stream>>>(pass, totals);
+          *c.launches += 2;
+        }
+      }
     } else {
       g.chunk_blocks = 0;
     }
