@@ -241,9 +241,14 @@ class NamedSharding:
 # buffers and arrays  (src/Types.jl:155-263, src/ConcreteRArray.jl)
 # ----------------------------------------------------------------------------
 class _Buffer:
+    __slots__ = ("handle", "device", "_free", "__weakref__")
+
     def __init__(self, handle, device: Device):
-        self.handle, self.device = handle, device
-        self._fin = weakref.finalize(self, lib().PjRtBufferFree, handle)
+        self.handle, self.device, self._free = handle, device, lib().PjRtBufferFree
+
+    def __del__(self):
+        # (a weakref.finalize would do the same at several times the cost, on every result of every call)
+        self._free(self.handle)
 
     @property
     def dims(self):
@@ -282,6 +287,13 @@ class ConcreteRArray:
         self.dtype = np.dtype(dtype)
         self.sharding = sharding
         self.replicated = replicated
+
+    @classmethod
+    def _of(cls, data, shape, dtype):
+        """An unsharded array from what is known to be in order already."""
+        a = cls.__new__(cls)
+        a.data, a.shape, a.dtype, a.sharding, a.replicated = data, shape, dtype, None, False
+        return a
 
     @property
     def ndim(self):
@@ -451,6 +463,28 @@ class Thunk:
         self.param_sharded_dim = [l.RxExecutableParameterShardedDim(handle, i) for i in range(self.num_parameters)]
         self.result_sharded_dim = [l.RxExecutableResultShardedDim(handle, i) for i in range(self.num_results)]
         self.param_alias = [l.RxExecutableParameterAlias(handle, i) for i in range(self.num_parameters)]
+        self._execute = l.XLAExecuteSharded
+        self._args_t = C.c_void_p * max(1, self.num_parameters)
+        self._outs_t = C.c_void_p * max(1, self.num_results)
+        mask_t = C.c_uint8 * max(1, self.num_parameters)
+        self._masks = (mask_t(), mask_t(*[int(a >= 0) for a in self.param_alias]))
+        self._result_info = None  # (class, shape, dtype) of each result, known from the first call on
+
+    def _call_single(self, args, donate):
+        """The call on one device without waiting: no futures, and the results' shapes are looked up once."""
+        dev = args[0].data[0].device if args else self.client.addressable_devices[0]
+        out = self._outs_t()
+        self._execute(self.handle, len(args), self._args_t(*[a.data[0].handle for a in args]), dev.handle, self._masks[1 if donate else 0], self.num_results, out, None, None)
+        check()
+        bufs = [_Buffer(h, dev) for h in out[:self.num_results]]
+        if self._result_info is None:
+            self._result_info = [(ConcreteRArray if b.dims else ConcreteRNumber, tuple(reversed(b.dims)), b.dtype) for b in bufs]
+        results = tuple(cls._of([b], shape, dtype) for b, (cls, shape, dtype) in zip(bufs, self._result_info))
+        if donate:
+            for a, k in zip(args, self.param_alias):
+                if 0 <= k < len(results):
+                    a.data = results[k].data
+        return results[0] if len(results) == 1 else results
 
     def describe(self) -> dict:
         return json.loads(take_string(lib().RxExecutableDescribe(self.handle)))
@@ -464,6 +498,8 @@ class Thunk:
         if len(args) != self.num_parameters:
             raise ReactantError(12, f"thunk takes {self.num_parameters} arguments, got {len(args)}")
         sharded = self.num_partitions > 1
+        if not sharded and not self.sync and all(len(a.data) == 1 for a in args):
+            return self._call_single(args, donate)
         ndev = len(self.client.addressable_devices) if sharded else 1
         for a in args:
             if len(a.data) != ndev:

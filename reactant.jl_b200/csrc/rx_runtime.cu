@@ -74,6 +74,8 @@ char* dup_cstr(const std::string& s) {
   return p;
 }
 
+constexpr size_t kMaxBusyBlocks = 4;  // blocks of one size that wait for another stream before an allocation waits with them
+
 size_t round_up(size_t b) { return b == 0 ? 256 : (b + 255) & ~(size_t)255; }
 
 }  // namespace
@@ -94,14 +96,28 @@ void* RxDevice::alloc(size_t bytes) {
     std::lock_guard<std::mutex> lk(mu);
     auto it = pool.find(rb);
     if (it != pool.end() && !it->second.empty()) {
-      void* p = it->second.back();
-      it->second.pop_back();
+      std::vector<Block>& blocks = it->second;
+      size_t take = blocks.size(), k = blocks.size();
+      while (k > 0 && blocks[k - 1].busy) --k;
+      if (k > 0) take = k - 1;  // the latest that only this device's stream has used
+      for (k = 0; take == blocks.size() && k < blocks.size(); ++k)
+        if (cudaEventQuery(blocks[k].busy) == cudaSuccess) take = k;
+      cudaGetLastError();  // "not ready" is no error
+      if (take == blocks.size() && (blocks.size() >= kMaxBusyBlocks || (bytes_limit > 0 && bytes_in_use + pool_bytes + (int64_t)rb > bytes_limit))) take = 0;
+      if (take == blocks.size()) goto fresh;
+      void* p = blocks[take].p;
+      if (blocks[take].busy) {
+        cudaStreamWaitEvent(stream, blocks[take].busy, 0);  // at once, where it has passed already
+        cudaEventDestroy(blocks[take].busy);
+      }
+      blocks.erase(blocks.begin() + take);
       pool_bytes -= (int64_t)rb;
       bytes_in_use += (int64_t)rb;
       peak_bytes_in_use = std::max(peak_bytes_in_use, bytes_in_use);
       return p;
     }
   }
+fresh:
   if (bytes_limit > 0 && bytes_in_use + pool_bytes + (int64_t)rb > bytes_limit) trim();
   void* p = nullptr;
   CK(cudaSetDevice(ordinal));
@@ -123,24 +139,25 @@ void* RxDevice::alloc(size_t bytes) {
   return p;
 }
 
-void RxDevice::release(void* p, size_t bytes) {
+void RxDevice::release(void* p, size_t bytes, cudaEvent_t busy) {
   if (!p) return;
   if (closed.load()) {  // pool and stream are gone: hand the block back to the driver
     cudaSetDevice(ordinal);
+    if (busy) cudaEventDestroy(busy);
     cudaFree(p);
     cudaGetLastError();
     return;
   }
   size_t rb = round_up(bytes);
   std::lock_guard<std::mutex> lk(mu);
-  pool[rb].push_back(p);
+  pool[rb].push_back({p, busy});
   bytes_in_use -= (int64_t)rb;
   pool_bytes += (int64_t)rb;
   peak_pool_bytes = std::max(peak_pool_bytes, pool_bytes);
 }
 
 void RxDevice::trim() {
-  std::map<size_t, std::vector<void*>> old;
+  std::map<size_t, std::vector<Block>> old;
   {
     std::lock_guard<std::mutex> lk(mu);
     old.swap(pool);
@@ -150,7 +167,13 @@ void RxDevice::trim() {
   cudaSetDevice(ordinal);
   cudaStreamSynchronize(stream);  // cached blocks may still be read by queued work
   for (auto& kv : old)
-    for (void* p : kv.second) cudaFree(p);
+    for (Block& b : kv.second) {
+      if (b.busy) {
+        cudaEventSynchronize(b.busy);
+        cudaEventDestroy(b.busy);
+      }
+      cudaFree(b.p);
+    }
 }
 
 void RxDevice::hand_back(void* tensor) {
@@ -1321,10 +1344,10 @@ void handed_out_deleter(rx::DLManagedTensor* t) {
     if (ev) cudaEventDestroy(ev);
     cudaDeviceSynchronize();
   } else {
-    h->st->make_ready();
     std::lock_guard<std::mutex> g(h->st->pending_mu);
-    if (h->st->pending) {
-      cudaStreamWaitEvent(d->stream, h->st->pending, 0);
+    if (h->st->pending) {  // another consumer's, or an all-reduce's: the new event stands for both
+      cudaStreamWaitEvent(h->consumer, h->st->pending, 0);
+      cudaEventRecord(ev, h->consumer);
       cudaEventDestroy(h->st->pending);
     }
     h->st->pending = ev;

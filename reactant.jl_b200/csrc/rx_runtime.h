@@ -51,7 +51,10 @@ struct RxDevice : std::enable_shared_from_this<RxDevice> {
   std::mutex exec_mu;
   // memory pool (exact-size free lists, stream ordered on `stream`)
   std::mutex mu;
-  std::map<size_t, std::vector<void*>> pool;
+  // A block that another stream may still be using carries that stream's event: it is handed out again once the event
+  // has passed, and only behind a wait for it when several such blocks of its size are waiting already.
+  struct Block { void* p; cudaEvent_t busy; };
+  std::map<size_t, std::vector<Block>> pool;
   int64_t num_allocs = 0, bytes_in_use = 0, peak_bytes_in_use = 0, largest_alloc = 0, bytes_limit = 0, pool_bytes = 0, peak_pool_bytes = 0;
   uint32_t* scratch = nullptr;
   size_t scratch_words = 0;
@@ -89,7 +92,7 @@ struct RxDevice : std::enable_shared_from_this<RxDevice> {
   void reap(bool all);                     // owners whose memory is free now get it back
 
   void* alloc(size_t bytes);
-  void release(void* p, size_t bytes);
+  void release(void* p, size_t bytes, cudaEvent_t busy = nullptr);  // takes the event over
   void trim();
   rx::LaunchCtx ctx() {
     rx::LaunchCtx c;
@@ -112,7 +115,8 @@ struct Storage {
   size_t bytes;
   // Set when the last writer of this block ran on the device's communication stream (an all-reduce that was still
   // in flight when the execution that produced it returned): whoever touches the block next on the compute stream
-  // -- the next execution, a copy to the host, or the release of the memory -- waits for this event first.
+  // -- the next execution, a copy to the host, or whoever is given the memory after its release -- waits for this
+  // event first.  A consumer that was handed the block (DLPack) leaves its stream's event here in the same way.
   std::mutex pending_mu;
   cudaEvent_t pending = nullptr;
   void* foreign = nullptr;  // the DLPack tensor that owns this memory, when it was taken over from another library
@@ -125,15 +129,15 @@ struct Storage {
     pending = nullptr;
   }
   ~Storage() {
-    if (pending) {
+    if (pending && foreign) {
       int cur = 0;
       cudaGetDevice(&cur);
       cudaSetDevice(dev->ordinal);
-      make_ready();  // the pool hands the block out again in compute-stream order
+      make_ready();  // the owner gets it back behind what is queued here
       cudaSetDevice(cur);
     }
     if (foreign) dev->hand_back(foreign);
-    else dev->release(ptr, bytes);
+    else dev->release(ptr, bytes, pending);
   }
 };
 
