@@ -2,8 +2,6 @@
 #include "rx_token.cuh"
 #include "rx_token.h"
 
-#include <cooperative_groups.h>
-
 #include <algorithm>
 
 namespace rx {
@@ -16,9 +14,7 @@ constexpr int kBlock = 256;
 //
 // Bound by memory: every distinct row is read, every row of the result written once.  The result is cut into units of
 // eight consecutive elements; a thread takes kUnits of them, a block apart, and asks for the ids and then the rows of
-// all of them before it stores.  VEC: rows of the table and of the result start on 16 bytes, so a unit is a vector of
-// one row.  Otherwise (an odd row length) the elements of a unit are read one by one, from up to eight rows, and still
-// leave as one vector.  65536 tokens of 2048 bf16 features: 72.9 us (one element a thread and a 64-bit division each: 361).
+// all of them before it stores.  Rows of the table and of the result start on 16 bytes, so a unit is a vector of one row.  65536 tokens of 2048 bf16 features: 72.9 us (one element a thread and a 64-bit division each: 361).
 constexpr int kUnits = 4;
 
 template <class Id>
@@ -27,64 +23,79 @@ __device__ __forceinline__ int64_t row_of(const Id* ids, int64_t t, int64_t voca
   return id >= 0 && id < vocab ? id : -1;
 }
 
-template <class In, class Out, class Id, bool VEC>
+template <class In, class Out, class Id>
 __global__ void __launch_bounds__(kBlock) k_embedding(const In* __restrict__ table, const Id* __restrict__ ids, Out* __restrict__ out, int64_t n, int64_t cols, Divisor by_row, bool small, int64_t ld,
                                                       int64_t vocab, float scale) {
-  const int64_t units = (n + 7) >> 3;
+  const int64_t units = n >> 3, per_row = cols >> 3;
   const int64_t base = (int64_t)blockIdx.x * (kBlock * kUnits) + threadIdx.x;
-  if (VEC) {
-    const int64_t per_row = cols >> 3;
-    int64_t row[kUnits], col[kUnits];
+  int64_t row[kUnits], col[kUnits];
 #pragma unroll
-    for (int k = 0; k < kUnits; ++k) {
-      const int64_t u = base + k * kBlock;
-      row[k] = -2;
-      if (u < units) {
-        const int64_t t = small ? by_row.quotient((uint32_t)u) : u / per_row;
-        col[k] = (u - t * per_row) << 3;
-        row[k] = row_of(ids, t, vocab);
-      }
+  for (int k = 0; k < kUnits; ++k) {
+    const int64_t u = base + k * kBlock;
+    row[k] = -2;
+    if (u < units) {
+      const int64_t t = small ? by_row.quotient((uint32_t)u) : u / per_row;
+      col[k] = (u - t * per_row) << 3;
+      row[k] = row_of(ids, t, vocab);
     }
-    Raw8<In> r[kUnits];
+  }
+  Raw8<In> r[kUnits];
 #pragma unroll
-    for (int k = 0; k < kUnits; ++k)
-      if (row[k] >= 0) r[k] = load8_cached(table + row[k] * ld + col[k]);
+  for (int k = 0; k < kUnits; ++k)
+    if (row[k] >= 0) r[k] = load8_cached(table + row[k] * ld + col[k]);
 #pragma unroll
-    for (int k = 0; k < kUnits; ++k) {
-      if (row[k] == -2) break;
-      float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      if (row[k] >= 0) {
-        widen8(r[k], v);
+  for (int k = 0; k < kUnits; ++k) {
+    if (row[k] == -2) break;
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (row[k] >= 0) {
+      widen8(r[k], v);
 #pragma unroll
-        for (int q = 0; q < 8; ++q) v[q] *= scale;
-      }
-      store8_whole(out + (base + k * kBlock) * 8, v);
+      for (int q = 0; q < 8; ++q) v[q] *= scale;
     }
-  } else {
-#pragma unroll 1
-    for (int k = 0; k < kUnits; ++k) {
-      const int64_t u = base + k * kBlock;
-      if (u >= units) break;
-      int64_t t = small ? by_row.quotient((uint32_t)(u * 8)) : u * 8 / cols;
-      int64_t c = u * 8 - t * cols;
-      int64_t row = row_of(ids, t, vocab);
-      const int m = (int)min((int64_t)8, n - u * 8);
-      float v[8];
+    store8_whole(out + (base + k * kBlock) * 8, v);
+  }
+}
+
+// Rows that do not start on 16 bytes (an odd length, a window of a wider table): a warp takes kRowVecs vectors of a row of
+// the result, cut at the result's vectors, and reads the 16-byte lines that hold the elements; the few in front of the
+// first vector and behind the last go one by one.  (65536 x 2047 bf16: 87 us, 2048 73; units across rows, each with its own
+// shift, took 184.)
+constexpr int kRowVecs = 128;
+
+template <class In, class Out, class Id>
+__global__ void __launch_bounds__(kBlock) k_embedding_rows(const In* __restrict__ table, const In* end, const Id* __restrict__ ids, Out* __restrict__ out, int64_t rows, int64_t cols, int parts,
+                                                           Divisor by_part, int64_t ld, int64_t vocab, float scale) {
+  const int lane = threadIdx.x & 31;
+  const int64_t w = (int64_t)blockIdx.x * (kBlock / 32) + threadIdx.x / 32;
+  const int64_t t = w < (int64_t)1 << 31 ? by_part.quotient((uint32_t)w) : w / parts;
+  if (t >= rows) return;
+  const int part = (int)(w - t * parts);
+  const int64_t row = row_of(ids, t, vocab);
+  const In* x = table + (row < 0 ? 0 : row) * ld;
+  Out* y = out + t * cols;
+  constexpr int kWhole = 8 * sizeof(Out);
+  const int head = (int)min((int64_t)((kWhole - (uintptr_t)y % kWhole) % kWhole / sizeof(Out)), cols), vecs = (int)((cols - head) >> 3), rest = head + 8 * vecs;
+  if (part == 0 && lane < head) put(y + lane, row < 0 ? 0.f : scale * widen(__ldg(x + lane)));
+  if (part == parts - 1 && rest + lane < cols) put(y + rest + lane, row < 0 ? 0.f : scale * widen(__ldg(x + rest + lane)));
+  const int last = min(vecs, (part + 1) * kRowVecs);
+  constexpr int kFly = kRowVecs / 32;
+  const int v0 = part * kRowVecs + lane;
+  Lines<In> lines[kFly];
+  if (row >= 0) {
 #pragma unroll
-      for (int q = 0; q < 8; ++q) {
-        v[q] = 0.f;
-        if (q < m) {
-          if (row >= 0) v[q] = scale * widen(__ldg(table + row * ld + c));
-          if (++c == cols && q + 1 < m) {
-            c = 0;
-            row = row_of(ids, ++t, vocab);
-          }
-        }
-      }
-      if (m == 8) store8_whole(out + u * 8, v);
-      else
-        for (int q = 0; q < m; ++q) put(out + u * 8 + q, v[q]);
+    for (int k = 0; k < kFly; ++k)
+      if (v0 + k * 32 < last) lines[k].fetch(x + head + (v0 + k * 32) * 8, end);
+  }
+#pragma unroll
+  for (int k = 0; k < kFly; ++k) {
+    if (v0 + k * 32 >= last) break;
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (row >= 0) {
+      lines[k].get(v);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v[q] *= scale;
     }
+    store8_whole(y + head + (v0 + k * 32) * 8, v);
   }
 }
 
@@ -92,32 +103,29 @@ __global__ void __launch_bounds__(kBlock) k_embedding(const In* __restrict__ tab
 // dtable[v] = scale * sum of dy[t] over the tokens with id v, added in the order of the tokens and so the same from run
 // to run, in four parts:
 //   sort            the tokens' places sorted by id (stably), and which rows have a token at all
-//   k_sum_runs      chunks of the sorted places: a run of one id inside a chunk is summed and written to its row; a run
-//                   that crosses a border of chunks leaves its part of the sum in the workspace
+//   k_sum_runs      chunks of the sorted places: a run of one id is summed and written to its row by the chunk it begins
+//                   in, if it ends no later than the next one; chunks that a longer run touches leave their parts of
+//                   its sum in the workspace
 //   (same launch)   rows without a token are filled with zeros
-//   k_join_runs     the parts of every run that crosses borders, added in the order of the chunks
+//   k_join_runs     the parts of the long runs, added in the order of the chunks
 // No atomic touches a sum.  The work is bound by memory: the gradients are read once, the table's written once; cutting
 // at fixed places rather than by id keeps the blocks even when few ids hold most of the tokens.
 
-// Sort: least significant digits first, up to 9 bits a pass.  Each warp owns a run of consecutive tokens: it counts their
-// digits in its own row of shared memory (equal digits among 32 tokens are found by votes, the lowest lane adds), the
-// counts become places through sums over warps, blocks and digits, and a second walk writes key and place.
-//
-// Up to kClusterTokens one cluster of up to eight blocks does all passes in one launch, the blocks' counts meeting in
-// distributed shared memory.  More tokens are spread over up to kPlaceBlocks blocks, two launches a pass: what bounds a
-// pass is the scattered stores, one sector a cycle and SM (65536 tokens: 51 us on the cluster's eight SMs).  (Writing
-// the zeros of the untouched rows from further blocks of these launches made the whole slower, 251 -> 280 us at 65536
-// tokens and 131072 x 2048: the sort's loads and stores then wait behind the fill's.)
-constexpr int kSortBlock = 1024, kSortWarps = kSortBlock / 32, kBins = 512, kSortRanks = 8;
+// Sort of many tokens: least significant digits first, up to 9 bits a pass, two launches of up to kPlaceBlocks blocks a
+// pass.  Each warp owns a run of consecutive tokens: it counts their digits in its own row of shared memory (equal digits
+// among 32 tokens are found by votes, the lowest lane adds), the counts become places through sums over warps, blocks and
+// digits, and a second walk writes key and place.  What bounds a pass is latency, and on few SMs the scattered stores, one
+// sector a cycle each (65536 tokens on one cluster of eight blocks: 51 us, spread over 64 blocks 22).  Writing the zeros
+// of the untouched rows from further blocks of these launches made the whole slower, 251 -> 280 us at 65536 tokens and
+// 131072 x 2048: the sort's loads and stores then wait behind the fill's.
+constexpr int kBins = 512, kSortBlock = kBins, kSortWarps = kSortBlock / 32;  // a thread a digit
 constexpr int kHold = 8;  // groups of 32 tokens whose keys a warp asks for at once
-constexpr int64_t kClusterTokens = kSortRanks * kSortBlock;
-constexpr int kPlaceBlocks = 128;
+constexpr int kPlaceBlocks = 64;
 
 struct SortShared {
   uint32_t count[kSortWarps][kBins];
-  uint32_t total[kBins], base[kBins];
+  uint32_t base[kBins];
   uint32_t warp_sum[kSortWarps];
-  uint32_t half_all[kBins], half_before[kBins];
 };
 
 // the lanes that have this lane's digit, by one vote a bit (one bit more than the digit where some lanes have none)
@@ -156,14 +164,21 @@ struct SortPass {
     for (int k = 0; k < kHold; ++k)
       if (t0 + k * 32 + lane < hi) key[k] = key_at(t0 + k * 32 + lane);
   }
-  // First walk: counts of this block's digits, as sums over the warps in front, and their totals.  `key` keeps the keys
-  // of a short run.
-  __device__ __forceinline__ void count(SortShared& sh, int32_t (&key)[kHold]) const {
+  __device__ __forceinline__ bool held() const { return hi - lo <= 32 * kHold; }
+  __device__ __forceinline__ void fetch_places(int64_t t0, int32_t (&pos)[kHold]) const {
+#pragma unroll
+    for (int k = 0; k < kHold; ++k) {
+      const int64_t t = t0 + k * 32 + lane;
+      if (t < hi) pos[k] = from ? __ldcg(from + rows + t) : (int32_t)t;
+    }
+  }
+  // First walk: counts of this block's digits, as sums over the warps in front; returns the total of digit threadIdx.x.
+  __device__ __forceinline__ uint32_t count(SortShared& sh, int32_t (&key)[kHold], bool fetched = false) const {
     for (int k = lane; k < kBins; k += 32) sh.count[warp][k] = 0;
     __syncwarp();
     const uint32_t below = (1u << lane) - 1, mask = (1u << digit) - 1;
     for (int64_t t0 = lo; t0 < hi; t0 += 32 * kHold) {
-      fetch(t0, key);
+      if (!fetched || !held()) fetch(t0, key);
 #pragma unroll
       for (int k = 0; k < kHold; ++k) {
         if (t0 + k * 32 >= hi) break;
@@ -175,16 +190,14 @@ struct SortPass {
       }
     }
     __syncthreads();
-    if (threadIdx.x < kBins) {
-      uint32_t sum = 0;
-#pragma unroll 8
-      for (int w = 0; w < kSortWarps; ++w) {
-        const uint32_t n = sh.count[w][threadIdx.x];
-        sh.count[w][threadIdx.x] = sum;
-        sum += n;
-      }
-      sh.total[threadIdx.x] = sum;
+    uint32_t sum = 0;
+#pragma unroll
+    for (int w = 0; w < kSortWarps; ++w) {
+      const uint32_t n = sh.count[w][threadIdx.x];
+      sh.count[w][threadIdx.x] = sum;
+      sum += n;
     }
+    return sum;
   }
   // all: tokens of all blocks with digit threadIdx.x; before: those of the blocks in front
   __device__ __forceinline__ void bases(SortShared& sh, uint32_t all, uint32_t before) const {
@@ -196,22 +209,16 @@ struct SortPass {
     }
     if (lane == 31) sh.warp_sum[warp] = scan;
     __syncthreads();
-    if (threadIdx.x < kBins) {
-      uint32_t front = lane < warp ? sh.warp_sum[lane] : 0;  // (at most 16 warps are in front of a digit's)
-      front = __reduce_add_sync(~0u, front);
-      sh.base[threadIdx.x] = front + scan - all + before;
-    }
+    const uint32_t front = __reduce_add_sync(~0u, lane < warp ? sh.warp_sum[lane] : 0);
+    sh.base[threadIdx.x] = front + scan - all + before;
     __syncthreads();
   }
-  __device__ __forceinline__ void place(SortShared& sh, int32_t (&key)[kHold]) const {
+  __device__ __forceinline__ void place(SortShared& sh, int32_t (&key)[kHold], int32_t (&pos)[kHold]) const {
     const uint32_t below = (1u << lane) - 1, mask = (1u << digit) - 1;
     for (int64_t t0 = lo; t0 < hi; t0 += 32 * kHold) {
-      if (hi - lo > 32 * kHold) fetch(t0, key);
-      int32_t pos[kHold];
-#pragma unroll
-      for (int k = 0; k < kHold; ++k) {
-        const int64_t t = t0 + k * 32 + lane;
-        if (t < hi) pos[k] = from ? __ldcg(from + rows + t) : (int32_t)t;
+      if (!held()) {
+        fetch(t0, key);
+        fetch_places(t0, pos);
       }
 #pragma unroll
       for (int k = 0; k < kHold; ++k) {
@@ -225,7 +232,7 @@ struct SortPass {
           if (!(same & below)) sh.count[warp][d] += __popc(same);
           to[at] = key[k];
           to[rows + at] = pos[k];
-          if (!from && key[k] < vocab) touched[key[k]] = 1;
+          if (!from && key[k] < vocab && !touched[key[k]]) touched[key[k]] = 1;  // few lines take the marks of frequent ids: look first
         }
         __syncwarp();
       }
@@ -239,115 +246,89 @@ __device__ __forceinline__ void clear_touched(uint8_t* touched, int64_t vocab, i
   if (rank == 0 && threadIdx.x == 0) *crossing = 0;
 }
 
-template <class Id>
-__global__ void __launch_bounds__(kSortBlock) k_sort_tokens(SortPass<Id> s, int passes, int32_t* a, int32_t* b, int32_t* crossing) {
-  namespace cg = cooperative_groups;
-  extern __shared__ __align__(16) uint8_t raw[];
-  SortShared& sh = *(SortShared*)raw;
-  cg::cluster_group cluster = cg::this_cluster();
-  const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-  clear_touched(s.touched, s.vocab, crossing, rank, ranks);
-  s.own(rank, ranks);
-  for (int pass = 0; pass < passes; ++pass) {
-    s.from = pass == 0 ? nullptr : pass % 2 ? a : b;
-    s.to = pass % 2 ? b : a;
-    s.shift = pass * s.digit;
-    int32_t key[kHold];
-    s.count(sh, key);
-    cluster.sync();
-    uint32_t before = 0, all = 0;
-    if (threadIdx.x < kBins)
-      for (int r = 0; r < ranks; ++r) {
-        const uint32_t n = *cluster.map_shared_rank(&sh.total[threadIdx.x], r);
-        if (r < rank) before += n;
-        all += n;
-      }
-    s.bases(sh, all, before);
-    s.place(sh, key);
-    cluster.sync();  // what was written is visible, and nobody reads this block's totals any more
-  }
-}
+// Up to kRankTokens: every token's place is the number of tokens that come before it, counted outright.  A warp takes four
+// tokens and compares them with four keys a lane at a time; 8192 x 8192 comparisons are about 5 us of what the SMs issue,
+// 1024 x 1024 nothing, and one launch without any exchange between blocks replaces four.
+constexpr int kRankTokens = 8192, kRankBlock = 512, kRankPerBlock = 4 * kRankBlock / 32;
 
-// Up to 1024 tokens: one block, a token a thread, sorted as (id, place) by Batcher's bitonic network; exchanges within a
-// warp are shuffles (700 tokens: 4 us against 11 for two passes over digits).
 template <class Id>
-__global__ void __launch_bounds__(kSortBlock) k_sort_few_tokens(const Id* __restrict__ ids, int rows, int64_t vocab, int32_t* key, int32_t* pos, uint8_t* touched, int32_t* crossing) {
-  __shared__ uint64_t sh[kSortBlock];
-  const int t = threadIdx.x;
-  uint64_t mine = ~0ull;
-  int32_t k = INT32_MAX;
-  if (t < rows) {
-    const int64_t id = (int64_t)__ldg(ids + t);
-    k = id >= 0 && id < vocab ? (int32_t)id : (int32_t)vocab;
-    mine = (uint64_t)(uint32_t)k << 32 | (uint32_t)t;
-  }
-  clear_touched(touched, vocab, crossing, 0, 1);
-  for (int size = 2; size <= kSortBlock; size *= 2)
-    for (int apart = size / 2; apart > 0; apart /= 2) {
-      uint64_t other;
-      if (apart >= 32) {
-        __syncthreads();
-        sh[t] = mine;
-        __syncthreads();
-        other = sh[t ^ apart];
-      } else {
-        other = __shfl_xor_sync(~0u, mine, apart);
-      }
-      const bool low = ((t & apart) == 0) == ((t & size) == 0);  // this thread keeps the smaller of the two
-      mine = low == (other < mine) ? other : mine;
+__global__ void __launch_bounds__(kRankBlock) k_rank_tokens(const Id* __restrict__ ids, int rows, int64_t vocab, int32_t* __restrict__ key, int32_t* __restrict__ pos, uint8_t* touched) {
+  __shared__ __align__(16) uint32_t sh[kRankTokens];
+  const int vecs = (rows + 3) / 4, lane = threadIdx.x & 31;
+#pragma unroll 8
+  for (int t = threadIdx.x; t < vecs * 4; t += kRankBlock) {
+    uint32_t k = ~0u;
+    if (t < rows) {
+      const int64_t id = (int64_t)__ldg(ids + t);
+      k = id >= 0 && id < vocab ? (uint32_t)id : (uint32_t)vocab;  // a token outside the table comes last
     }
-  if (t < rows) {
-    key[t] = (int32_t)(mine >> 32);
-    pos[t] = (int32_t)(uint32_t)mine;
+    sh[t] = k;
   }
-  if (k < vocab) touched[k] = 1;  // (every store of zeros is behind one of the barriers above)
+  __syncthreads();
+  const int own = blockIdx.x * (kRankPerBlock / 4) + threadIdx.x / 32;
+  if (own >= vecs) return;
+  const uint4 m4 = ((const uint4*)sh)[own];
+  const uint32_t mine[4] = {m4.x, m4.y, m4.z, m4.w};
+  int before[4] = {0, 0, 0, 0};
+#pragma unroll 2
+  for (int v = lane; v < vecs; v += 32) {
+    const uint4 k = ((const uint4*)sh)[v];
+    const uint32_t front = v < own;  // equal ids in front count, those behind do not
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t limit = mine[i] + front;
+      before[i] += (k.x < limit) + (k.y < limit) + (k.z < limit) + (k.w < limit);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    before[i] = __reduce_add_sync(~0u, before[i]);
+#pragma unroll
+    for (int j = 0; j < i; ++j) before[i] += mine[j] == mine[i];
+    const int t = own * 4 + i;
+    if (lane == i && t < rows) {
+      key[before[i]] = (int32_t)mine[i];
+      pos[before[i]] = t;
+      if (mine[i] < (uint32_t)vocab && !touched[mine[i]]) touched[mine[i]] = 1;
+    }
+  }
 }
 
 // one pass in two launches: totals[block][digit], then the places
 template <class Id>
 __global__ void __launch_bounds__(kSortBlock) k_count_tokens(SortPass<Id> s, uint32_t* totals, int32_t* crossing) {
-  extern __shared__ __align__(16) uint8_t raw[];
-  SortShared& sh = *(SortShared*)raw;
+  __shared__ SortShared sh;
   if (!s.from) clear_touched(s.touched, s.vocab, crossing, blockIdx.x, gridDim.x);
   s.own(blockIdx.x, gridDim.x);
   int32_t key[kHold];
-  s.count(sh, key);
-  if (threadIdx.x < kBins) totals[blockIdx.x * kBins + threadIdx.x] = sh.total[threadIdx.x];
+  totals[blockIdx.x * kBins + threadIdx.x] = s.count(sh, key);
 }
 template <class Id>
 __global__ void __launch_bounds__(kSortBlock) k_place_tokens(SortPass<Id> s, const uint32_t* __restrict__ totals) {
-  extern __shared__ __align__(16) uint8_t raw[];
-  SortShared& sh = *(SortShared*)raw;
+  __shared__ SortShared sh;
   s.own(blockIdx.x, gridDim.x);
-  // the totals of all blocks, two threads a digit: every second block each
-  const int bin = threadIdx.x % kBins, half = threadIdx.x / kBins, ranks = gridDim.x;
+  int32_t key[kHold], pos[kHold];
+  s.fetch(s.lo, key);  // asked for ahead of the totals
+  s.fetch_places(s.lo, pos);
   uint32_t before = 0, all = 0;
-#pragma unroll 16
-  for (int r = half; r < ranks; r += 2) {
-    const uint32_t n = __ldg(totals + r * kBins + bin);
+  const int ranks = gridDim.x;
+#pragma unroll
+  for (int r = 0; r < kPlaceBlocks; ++r) {
+    const uint32_t n = r < ranks ? __ldg(totals + r * kBins + threadIdx.x) : 0;
     if (r < (int)blockIdx.x) before += n;
     all += n;
   }
-  if (half) {
-    sh.half_all[bin] = all;
-    sh.half_before[bin] = before;
-  }
-  int32_t key[kHold];
-  s.count(sh, key);
-  if (!half) {
-    all += sh.half_all[bin];
-    before += sh.half_before[bin];
-  }
-  s.bases(sh, half ? 0 : all, before);
-  s.place(sh, key);
+  s.count(sh, key, true);
+  s.bases(sh, all, before);
+  s.place(sh, key, pos);
 }
 
 struct GradArgs {
   const int32_t *key, *pos;  // sorted
   const uint8_t* touched;    // null: no row has a token
-  float* part;               // [chunks][2][cols]: what a chunk adds to the run that enters it, and to the one that leaves it
-  int32_t *crossing, *list;  // chunks in which a run starts that leaves them
-  int64_t rows, cols, ld, vocab;
+  float* part;               // [chunks][2][pitch]: what a chunk adds to the long run that enters it, and to the one that leaves it
+  int32_t *crossing, *list;  // chunks in which a long run begins, how many and which
+  int64_t rows, cols, ld, vocab, pitch;
   float scale;
   int chunk, lanes, log_lanes;  // places in a chunk; threads that share one
   int64_t chunks, chunk_blocks, slices;
@@ -357,11 +338,32 @@ struct GradArgs {
 
 constexpr int kMaxChunk = 128, kMaxPlaces = 1024, kFillUnits = 8;
 
-// Zeros for the rows that no token has: units of eight consecutive elements of the result, kFillUnits a thread, whose
-// rows are all looked up before the first is written.  
+// Zeros for the rows that no token has.  Rows that are whole vectors, and short ones, go by units of eight consecutive
+// elements of the result, kFillUnits a thread, whose rows are all looked up before the first is written; long rows of an
+// odd length go by warps, a row at a time from its first element on a whole vector's boundary.
+constexpr int kFillRow = 256, kFillRows = 4;  // elements from which a row is a warp's; rows a warp
+
 template <class Out, bool VEC>
 __device__ __forceinline__ void fill_rows(const GradArgs& g, Out* out, int64_t block) {
   const float zero[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (!VEC && g.cols >= kFillRow) {
+    const int lane = threadIdx.x & 31;
+    const int64_t first = (block * (kBlock / 32) + threadIdx.x / 32) * kFillRows;
+    uint32_t busy[kFillRows];
+#pragma unroll
+    for (int k = 0; k < kFillRows; ++k) busy[k] = first + k >= g.vocab || (g.touched && __ldg(g.touched + first + k));
+#pragma unroll
+    for (int k = 0; k < kFillRows; ++k) {
+      if (busy[k]) continue;
+      Out* row = out + (first + k) * g.cols;
+      constexpr int kWhole = 8 * sizeof(Out);
+      const int head = (int)((kWhole - (uintptr_t)row % kWhole) % kWhole / sizeof(Out)), vecs = (int)((g.cols - head) >> 3), rest = head + 8 * vecs;
+      if (lane < head) put(row + lane, 0.f);
+      for (int v = lane; v < vecs; v += 32) store8_whole(row + head + 8 * v, zero);
+      if (rest + lane < g.cols) put(row + rest + lane, 0.f);
+    }
+    return;
+  }
   const int64_t n = g.vocab * g.cols, units = (n + 7) >> 3, per_row = g.cols >> 3;
   const int64_t base = block * (kBlock * kFillUnits) + threadIdx.x;
   auto row = [&](int64_t i) -> int64_t {  // of element i
@@ -394,10 +396,13 @@ __device__ __forceinline__ void fill_rows(const GradArgs& g, Out* out, int64_t b
   }
 }
 
-// Columns of a thread: eight consecutive ones (VEC), or eight that lie `lanes` apart (rows that do not start on 16 bytes).
+// A thread has eight consecutive columns.  VEC: rows of dy and of the result start on 16 bytes.  Otherwise a row is read
+// as the 16-byte lines that hold the columns, and the columns of a finished run change places within the warp, through
+// shared memory, so that they are written side by side.
 template <class In, class Out, bool VEC>
-__global__ void __launch_bounds__(kBlock, VEC ? 1 : 3) k_sum_runs(const In* __restrict__ dy, Out* __restrict__ out, const __grid_constant__ GradArgs g) {
-  __shared__ int32_t skey[kMaxPlaces + 2], spos[kMaxPlaces];
+__global__ void __launch_bounds__(kBlock, VEC ? 1 : 3) k_sum_runs(const In* __restrict__ dy, const In* end, Out* __restrict__ out, const __grid_constant__ GradArgs g) {
+  __shared__ int32_t skey[kMaxPlaces + 2 * kMaxChunk + 2], spos[kMaxPlaces + kMaxChunk];
+  __shared__ float turn[VEC ? 1 : kBlock / 32][VEC ? 1 : 32 * 9];
   if (blockIdx.x >= g.chunk_blocks * g.slices) {
     fill_rows<Out, VEC>(g, out, blockIdx.x - g.chunk_blocks * g.slices);
     return;
@@ -405,66 +410,85 @@ __global__ void __launch_bounds__(kBlock, VEC ? 1 : 3) k_sum_runs(const In* __re
   const int64_t block = blockIdx.x / g.slices, slice = blockIdx.x - block * g.slices;
   const int groups = kBlock >> g.log_lanes, places = groups * g.chunk;
   const int64_t first = block * places;
-  for (int i = threadIdx.x; i < places; i += kBlock) {
-    const int64_t q = first + i;
-    skey[i + 1] = q < g.rows ? __ldg(g.key + q) : INT32_MAX;
-    spos[i] = q < g.rows ? __ldg(g.pos + q) : 0;
+  // keys from one chunk and one place in front to one chunk and one place behind
+  for (int i = threadIdx.x; i < places + 2 * g.chunk + 2; i += kBlock) {
+    const int64_t q = first - g.chunk - 1 + i;
+    skey[i] = q < 0 ? -1 : q < g.rows ? __ldg(g.key + q) : INT32_MAX;
   }
-  if (threadIdx.x == 0) skey[0] = first > 0 ? __ldg(g.key + first - 1) : -1;
-  if (threadIdx.x == 1) skey[places + 1] = first + places < g.rows ? __ldg(g.key + first + places) : INT32_MAX;
+  for (int i = threadIdx.x; i < places + g.chunk; i += kBlock) spos[i] = first + i < g.rows ? __ldg(g.pos + first + i) : 0;
   __syncthreads();
   const int lane = threadIdx.x & (g.lanes - 1), group = threadIdx.x >> g.log_lanes;
   const int64_t chunk = block * groups + group;
-  if (chunk >= g.chunks) return;
-  const int32_t *key = skey + 1 + group * g.chunk, *pos = spos + group * g.chunk;
-  const int64_t c0 = slice * (8 * g.lanes) + (VEC ? lane * 8 : lane);
-  auto col = [&](int j) { return c0 + (VEC ? j : j * g.lanes); };
-  if (c0 >= g.cols && !(lane == 0 && slice == 0)) return;
-  const bool mine = c0 < g.cols;
+  const int32_t *key = skey + g.chunk + 1 + group * g.chunk, *pos = spos + group * g.chunk;
+  const int64_t c0 = (slice * g.lanes + lane) * 8;
+  // threads without columns, or without a chunk, stay: the others of their warp exchange columns with them
+  const bool mine = c0 < g.cols && chunk < g.chunks;
   float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  int32_t now = key[0];
-  bool enters = now == key[-1];
-  auto flush = [&](bool leaves) {
-    if (!mine) return;
-    if (enters || leaves) {
-      float* p = g.part + (chunk * 2 + (enters ? 0 : 1)) * g.cols;
-      if (VEC) {
-        *(float4*)(p + c0) = make_float4(acc[0], acc[1], acc[2], acc[3]);
-        *(float4*)(p + c0 + 4) = make_float4(acc[4], acc[5], acc[6], acc[7]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (col(j) < g.cols) p[col(j)] = acc[j];
-      }
-    } else {
-      Out* p = out + (int64_t)now * g.cols;
+  if (key[0] >= g.vocab) return;  // nothing but tokens outside the table, or no chunk at all: a whole group
+  // The run that enters belongs to the chunk in front if it begins there and ends here: it is passed over.  The run
+  // that leaves is this chunk's, to its end, if it begins here and ends in the next one.
+  int begin = 0, stop = g.chunk;
+  bool enters = key[0] == key[-1];
+  if (enters && key[g.chunk] != key[0] && key[-g.chunk - 1] != key[0]) {
+    while (begin < g.chunk && key[begin] == key[0]) ++begin;
+    enters = false;
+  }
+  const int32_t last = key[g.chunk - 1];
+  bool leaves = key[g.chunk] == last;
+  if (leaves && key[2 * g.chunk] != last && !(key[0] == last && key[0] == key[-1])) {
+    while (key[stop] == last) ++stop;
+    leaves = false;
+  }
+  if (begin == stop) return;
+  int32_t now = key[begin];
+  if (now >= g.vocab) return;
+  auto flush = [&](bool to_part) {
+    if (enters || to_part) {
+      if (!mine) return;
+      float* p = g.part + (chunk * 2 + (enters ? 0 : 1)) * g.pitch + c0;
+      *(float4*)p = make_float4(acc[0], acc[1], acc[2], acc[3]);
+      *(float4*)(p + 4) = make_float4(acc[4], acc[5], acc[6], acc[7]);
+      return;
+    }
+    Out* p = out + (int64_t)now * g.cols;
+    if (VEC) {
       float v[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = g.scale * acc[j];
-      if (VEC) store8_whole(p + c0, v);
-      else
+      if (mine) store8_whole(p + c0, v);
+    } else if (g.lanes >= 32) {  // a warp is in one group: all of it is here
+      float* t = turn[threadIdx.x / 32];
+      const int l = threadIdx.x & 31;
+      const int64_t w0 = c0 - l * 8;  // the warp's first column
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (col(j) < g.cols) put(p + col(j), v[j]);
+      for (int j = 0; j < 8; ++j) t[l * 9 + j] = g.scale * acc[j];
+      __syncwarp();
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int i = j * 32 + l;
+        if (w0 + i < g.cols) put(p + w0 + i, t[i / 8 * 9 + i % 8]);
+      }
+      __syncwarp();
+    } else if (mine) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (c0 + j < g.cols) put(p + c0 + j, g.scale * acc[j]);
     }
   };
   constexpr int kFly = 4;
-  int i = 0;
-  for (; i < g.chunk && key[i] < g.vocab; i += kFly) {
-    float v[kFly][8];
-    Raw8<In> raw[kFly];
+  for (int i = begin; i < stop && key[i] < g.vocab; i += kFly) {
+    Raw8<In> raw[VEC ? kFly : 1];
+    Lines<In> lines[VEC ? 1 : kFly];
 #pragma unroll
     for (int k = 0; k < kFly; ++k) {
-      if (i + k >= g.chunk || key[i + k] >= g.vocab || !mine) continue;
-      const In* p = dy + (int64_t)pos[i + k] * g.ld;
-      if (VEC) raw[k] = load8(p + c0);
-      else
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[k][j] = col(j) < g.cols ? widen(__ldcs(p + col(j))) : 0.f;
+      if (i + k >= stop || key[i + k] >= g.vocab || !mine) continue;
+      const In* p = dy + (int64_t)pos[i + k] * g.ld + c0;
+      if (VEC) raw[VEC ? k : 0] = load8(p);
+      else lines[VEC ? 0 : k].fetch(p, end);
     }
 #pragma unroll
     for (int k = 0; k < kFly; ++k) {
-      if (i + k >= g.chunk || key[i + k] >= g.vocab) break;
+      if (i + k >= stop || key[i + k] >= g.vocab) break;
       if (key[i + k] != now) {
         flush(false);
         enters = false;
@@ -472,20 +496,21 @@ __global__ void __launch_bounds__(kBlock, VEC ? 1 : 3) k_sum_runs(const In* __re
 #pragma unroll
         for (int j = 0; j < 8; ++j) acc[j] = 0.f;
       }
-      if (VEC && mine) widen8(raw[k], v[k]);
       if (mine) {
+        float v[8];
+        if (VEC) widen8(raw[VEC ? k : 0], v);
+        else lines[VEC ? 0 : k].get(v);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) acc[j] += v[k][j];
+        for (int j = 0; j < 8; ++j) acc[j] += v[j];
       }
     }
   }
-  if (now >= g.vocab) return;  // nothing but tokens outside the table
-  const bool leaves = key[g.chunk - 1] == now && key[g.chunk] == now;
+  leaves = leaves && now == last;
   flush(leaves);
   if (leaves && !enters && lane == 0 && slice == 0) g.list[atomicAdd(g.crossing, 1)] = (int32_t)chunk;
 }
 
-// The runs that cross borders of chunks.  A block adds the parts of one run for 256 columns: its eight warps take equal
+// The long runs.  A block adds the parts of one run for 256 columns: its eight warps take equal
 // stretches of the run's chunks, their sums are added in the order of the warps.
 template <class Out>
 __global__ void __launch_bounds__(kBlock) k_join_runs(Out* __restrict__ out, const __grid_constant__ GradArgs g) {
@@ -507,7 +532,7 @@ __global__ void __launch_bounds__(kBlock) k_join_runs(Out* __restrict__ out, con
     const int64_t lo = chunk + 1 + m * warp / (kBlock / 32), hi = chunk + 1 + m * (warp + 1) / (kBlock / 32);
 #pragma unroll 4
     for (int64_t c = lo; c < hi; ++c) {
-      const float* p = g.part + c * 2 * g.cols + c0 + lane;
+      const float* p = g.part + c * 2 * g.pitch + c0 + lane;
 #pragma unroll
       for (int j = 0; j < 8; ++j)
         if (c0 + lane + j * 32 < g.cols) acc[j] += __ldg(p + j * 32);
@@ -517,7 +542,7 @@ __global__ void __launch_bounds__(kBlock) k_join_runs(Out* __restrict__ out, con
     __syncthreads();
     const int64_t c = c0 + threadIdx.x;
     if (c < g.cols) {
-      float total = __ldg(g.part + (chunk * 2 + 1) * g.cols + c);
+      float total = __ldg(g.part + (chunk * 2 + 1) * g.pitch + c);
 #pragma unroll
       for (int k = 0; k < kBlock / 32; ++k) total += sum[k][threadIdx.x];
       put(out + (int64_t)key * g.cols + c, g.scale * total);
@@ -528,8 +553,7 @@ __global__ void __launch_bounds__(kBlock) k_join_runs(Out* __restrict__ out, con
 
 // How the gradient is cut, and where its parts lie in the workspace.
 struct GradPlan {
-  int passes, digit, ranks;
-  bool spread;  // the sort in launches of its own passes, over many SMs
+  int passes, digit, ranks;  // of the sort of many tokens
   GradArgs g;
   int64_t keys_a, keys_b, touched, crossing, list, totals, part, bytes;  // byte offsets
   GradPlan(const CallDesc& d, int sm_count) : g{} {
@@ -537,10 +561,7 @@ struct GradPlan {
     while (bits < 31 && (d.vocab >> bits)) ++bits;
     passes = (bits + 8) / 9;
     digit = (bits + passes - 1) / passes;
-    ranks = 2;
-    while (ranks < kSortRanks && (int64_t)ranks * kSortBlock < d.rows) ranks *= 2;
-    spread = d.rows > kClusterTokens;
-    if (spread) ranks = (int)std::min<int64_t>(kPlaceBlocks, (d.rows + kSortBlock - 1) / kSortBlock);
+    ranks = (int)std::min<int64_t>(kPlaceBlocks, (d.rows + 2 * kSortBlock - 1) / (2 * kSortBlock));
     g.rows = d.rows;
     g.cols = d.cols;
     g.ld = d.ld;
@@ -554,9 +575,12 @@ struct GradPlan {
     }
     const int groups = kBlock / g.lanes;
     g.slices = std::max<int64_t>(1, (d.cols + 8 * g.lanes - 1) / (8 * g.lanes));
-    // chunks as long as they still give every SM two blocks
+    // Chunks as long as they still give every SM four blocks, or two where the rows are short (a block then has several
+    // chunks, and what a chunk costs besides its rows counts) or the zeros keep the SMs busy as well.
+    const bool filling = (d.vocab - d.rows) * (int64_t)dt_size(d.out_dt) > d.rows * (int64_t)dt_size(d.in_dt);
+    const int64_t blocks = sm_count * (filling || groups > 1 ? 2 : 4), least = d.rows > 2048 ? 16 : 8;
     g.chunk = std::min(kMaxChunk, kMaxPlaces / groups);
-    while (g.chunk > 8 && (d.rows + (int64_t)g.chunk * groups - 1) / ((int64_t)g.chunk * groups) * g.slices < sm_count * 2) g.chunk /= 2;
+    while (g.chunk > least && (d.rows + (int64_t)g.chunk * groups - 1) / ((int64_t)g.chunk * groups) * g.slices < blocks) g.chunk /= 2;
     g.chunks = (d.rows + g.chunk - 1) / g.chunk;
     g.chunk_blocks = (g.chunks + groups - 1) / groups;
     auto take = [&](int64_t n) {
@@ -571,7 +595,8 @@ struct GradPlan {
     crossing = take(4);
     list = take(g.chunks * 4);
     totals = take((int64_t)kPlaceBlocks * kBins * 4);
-    part = take(g.chunks * 2 * d.cols * 4);
+    g.pitch = (d.cols + 7) / 8 * 8;
+    part = take(g.chunks * 2 * g.pitch * 4);
   }
 };
 
@@ -597,15 +622,19 @@ cudaError_t launch_embedding(const LaunchCtx& c, const CallDesc& d, const void* 
   if (!n) return cudaSuccess;
   const int64_t in_bytes = (int64_t)dt_size(d.in_dt);
   const bool vec = d.cols % 8 == 0 && aligned16(table) && d.ld * in_bytes % 16 == 0;
-  const bool small = n < (int64_t)1 << 31;
-  const Divisor by_row(vec ? d.cols / 8 : d.cols);
-  const unsigned blocks = (unsigned)((n + 8 * kBlock * kUnits - 1) / (8 * kBlock * kUnits));
   with_types(d.in_dt, d.out_dt, d.ids_dt, [&](auto* i, auto* o, auto* id) {
     using In = std::remove_pointer_t<decltype(i)>;
     using Out = std::remove_pointer_t<decltype(o)>;
     using Id = std::remove_pointer_t<decltype(id)>;
-    auto* f = vec ? k_embedding<In, Out, Id, true> : k_embedding<In, Out, Id, false>;
-    f<<<blocks, kBlock, 0, c.stream>>>((const In*)table, (const Id*)ids, (Out*)out, n, d.cols, by_row, small, d.ld, d.vocab, (float)d.scale);
+    if (vec) {
+      const unsigned blocks = (unsigned)((n / 8 + kBlock * kUnits - 1) / (kBlock * kUnits));
+      k_embedding<In, Out, Id><<<blocks, kBlock, 0, c.stream>>>((const In*)table, (const Id*)ids, (Out*)out, n, d.cols, Divisor(d.cols / 8), n < (int64_t)1 << 31, d.ld, d.vocab, (float)d.scale);
+    } else {
+      const int64_t parts = (d.cols / 8 + kRowVecs) / kRowVecs, warps = d.rows * parts;
+      const unsigned blocks = (unsigned)((warps + kBlock / 32 - 1) / (kBlock / 32));
+      k_embedding_rows<In, Out, Id><<<blocks, kBlock, 0, c.stream>>>((const In*)table, (const In*)table + (d.vocab ? (d.vocab - 1) * d.ld + d.cols : 0), (const Id*)ids, (Out*)out, d.rows, d.cols,
+                                                                    (int)parts, Divisor(parts), d.ld, d.vocab, (float)d.scale);
+    }
   });
   ++*c.launches;
   return cudaGetLastError();
@@ -624,7 +653,7 @@ cudaError_t launch_embedding_grad(const LaunchCtx& c, const CallDesc& d, const v
   g.by_row = Divisor(vec ? d.cols / 8 : d.cols);
   g.small = n < (int64_t)1 << 31;
   const int64_t units = (n + 7) / 8;
-  const int64_t fill_blocks = (units + kBlock * kFillUnits - 1) / (kBlock * kFillUnits);
+  const int64_t fill_blocks = !vec && d.cols >= kFillRow ? (d.vocab + kBlock / 32 * kFillRows - 1) / (kBlock / 32 * kFillRows) : (units + kBlock * kFillUnits - 1) / (kBlock * kFillUnits);
   cudaError_t err = cudaSuccess;
   with_types(d.in_dt, d.out_dt, d.ids_dt, [&](auto* i, auto* o, auto* id) {
     using In = std::remove_pointer_t<decltype(i)>;
@@ -638,47 +667,26 @@ cudaError_t launch_embedding_grad(const LaunchCtx& c, const CallDesc& d, const v
       g.crossing = (int32_t*)(w + p.crossing);
       g.list = (int32_t*)(w + p.list);
       g.part = (float*)(w + p.part);
-      SortPass<Id> pass{};
-      pass.ids = (const Id*)ids;
-      pass.touched = (uint8_t*)(w + p.touched);
-      pass.rows = d.rows;
-      pass.vocab = d.vocab;
-      pass.digit = p.digit;
-      auto allow = [&](auto* f) { return cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(SortShared)); };  // of the current device
-      if (d.rows <= kSortBlock) {
-        k_sort_few_tokens<Id><<<1, kSortBlock, 0, c.stream>>>((const Id*)ids, (int)d.rows, d.vocab, (int32_t*)g.key, (int32_t*)g.pos, pass.touched, g.crossing);
-        ++*c.launches;
-      } else if (!p.spread) {
-        auto* sort = k_sort_tokens<Id>;
-        err = allow(sort);
+      if (d.rows <= kRankTokens) {
+        err = cudaMemsetAsync(w + p.touched, 0, (size_t)(p.crossing + 4 - p.touched), c.stream);
         if (err != cudaSuccess) return;
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3((unsigned)p.ranks);
-        cfg.blockDim = dim3(kSortBlock);
-        cfg.dynamicSmemBytes = sizeof(SortShared);
-        cfg.stream = c.stream;
-        cudaLaunchAttribute attr[1];
-        attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = (unsigned)p.ranks;
-        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-        cfg.attrs = attr;
-        cfg.numAttrs = 1;
-        err = cudaLaunchKernelEx(&cfg, sort, pass, p.passes, a, b, g.crossing);
-        if (err != cudaSuccess) return;
+        k_rank_tokens<Id><<<(unsigned)((d.rows + kRankPerBlock - 1) / kRankPerBlock), kRankBlock, 0, c.stream>>>((const Id*)ids, (int)d.rows, d.vocab, (int32_t*)g.key, (int32_t*)g.pos,
+                                                                                                             (uint8_t*)(w + p.touched));
         ++*c.launches;
       } else {
-        auto* count = k_count_tokens<Id>;
-        auto* place = k_place_tokens<Id>;
-        err = allow(count);
-        if (err == cudaSuccess) err = allow(place);
-        if (err != cudaSuccess) return;
+        SortPass<Id> pass{};
+        pass.ids = (const Id*)ids;
+        pass.touched = (uint8_t*)(w + p.touched);
+        pass.rows = d.rows;
+        pass.vocab = d.vocab;
+        pass.digit = p.digit;
         uint32_t* totals = (uint32_t*)(w + p.totals);
         for (int k = 0; k < p.passes; ++k) {
           pass.from = k == 0 ? nullptr : k % 2 ? a : b;
           pass.to = k % 2 ? b : a;
           pass.shift = k * p.digit;
-          count<<<p.ranks, kSortBlock, sizeof(SortShared), c.stream>>>(pass, totals, g.crossing);
-          place<<<p.ranks, kSortBlock, sizeof(SortShared), c.stream>>>(pass, totals);
+          k_count_tokens<Id><<<p.ranks, kSortBlock, 0, c.stream>>>(pass, totals, g.crossing);
+          k_place_tokens<Id><<<p.ranks, kSortBlock, 0, c.stream>>>(pass, totals);
           *c.launches += 2;
         }
       }
@@ -686,7 +694,7 @@ cudaError_t launch_embedding_grad(const LaunchCtx& c, const CallDesc& d, const v
       g.chunk_blocks = 0;
     }
     auto* sum = vec ? k_sum_runs<In, Out, true> : k_sum_runs<In, Out, false>;
-    sum<<<(unsigned)(g.chunk_blocks * g.slices + fill_blocks), kBlock, 0, c.stream>>>((const In*)dy, (Out*)out, g);
+    sum<<<(unsigned)(g.chunk_blocks * g.slices + fill_blocks), kBlock, 0, c.stream>>>((const In*)dy, (const In*)dy + (d.rows ? (d.rows - 1) * d.ld + d.cols : 0), (Out*)out, g);
     ++*c.launches;
     if (g.chunks > 1) {
       const int64_t most = g.chunks * ((d.cols + kBlock - 1) / kBlock);

@@ -12,9 +12,10 @@ namespace rx {
 namespace {
 
 constexpr int kBlock = 256;
-// Rows up to this long are one warp's, where there are enough of them (times with a block of 128 a row in brackets, f32:
-// 25000 x 4100 65.7 [87] us, 12500 x 8200 65.4 [71], 6000 x 16500 75 [72]; with twenty top tokens 126 [188], 147 [118]).
-constexpr int kWarpRow = 8192, kWarpRowTop = 6144;
+// Rows up to kWarpRow are one warp's where there are enough of them to keep the SMs busy: kWarpRows per SM, twice as many
+// for rows longer than kWarpLong.  (In brackets with a block of 128 a row: 25000 x 4100 f32 66 [87] us, with twenty top
+// tokens 126 [181]; 12000 x 16500 bf16 80 [84], with five 96 [135]; 6000 x 33000 bf16 88 [73], with five 101 [97].)
+constexpr int kWarpRow = 20000, kWarpLong = 8192, kWarpRows = 16;
 constexpr int kMaxRanksPerRow = 8;   // blocks of a cluster that share a row
 
 __device__ __forceinline__ float exp2_fast(float x) {  // within two units of the last place; results below 2^-126 are 0
@@ -203,13 +204,15 @@ struct Span {
 
 constexpr int kMaxLoose = 14;
 
-// ---- W = 8 or 32 lanes per row: rows of up to 1024 -----------------------------------------------------------------
+// ---- W = 8 or 32 lanes per row: rows of up to 512 (bf16) or 1024 (f32) -----------------------------------------------------------------
 // A row's elements sit in its lanes' registers, NE each, read one by one (eight lanes: a warp's four rows lie next to
 // each other).  TOP: the k-th largest value is bounded bit by bit, its upper 16 bits first -- among all elements, or, with
 // 32 lanes and k <= 32, among the lanes' largest, which is one vote a bit.  Where that leaves too many (most of the row
 // is equal), it is searched for to the last bit, and then the last index that is still wanted among the elements equal
 // to it.  What is left, little more than k, is ordered by counting.
-constexpr int kGroupRow = 1024, kNarrowRow = 256;
+constexpr int kNarrowRow = 256;
+template <class T>
+struct GroupRow { static constexpr int n = sizeof(T) == 4 ? 1024 : 512; };  // 16-bit loads one by one: 200000 x 1000 bf16 takes 173 us here, 113 with a warp's vectors
 template <int W>
 struct GroupCap { static constexpr int n = W == 8 ? 2 * kMaxTopK + 8 : 4 * kMaxTopK; };
 
@@ -333,17 +336,21 @@ __global__ void __launch_bounds__(kBlock, NE == 32 ? (W == 8 ? 2 : 3) : 4) k_log
   }
 }
 
-// ---- one warp per row: short rows -----------------------------------------------------------------------------------
-// TOP (top_k <= 32): the k-th largest of the 32 lanes' largest values bounds the k-th of the row from below, so a
-// second look at the row (it is in L1 by now) keeps little more than k candidates.
-constexpr int kWarpTop = 32;
+// ---- one warp per row: middling rows, many of them --------------------------------------------------------------------
+// TOP (top_k <= 32): while it streams, a lane notes the largest value of each of its stretches of vectors.  The k-th
+// largest of the 32 lanes' maxima bounds the k-th of the row from below, bit by bit with one vote each; only the stretches
+// that reach it are read again, their vectors spread over the lanes, and little more than k candidates are kept.
+constexpr int kWarpTop = 32, kWarpSpells = 16;
 constexpr int kWarpCap = 256 + kWarpTop + kMaxLoose;
 
 template <class T, class Id, bool TOP>
 __global__ void __launch_bounds__(kBlock) k_logprobs_warp(const T* __restrict__ logits, const Id* __restrict__ ids, int64_t rows, int64_t cols, int64_t ld, float scale, int top_k, LogProbsOut out) {
-  __shared__ uint64_t buf_[TOP ? kBlock / 32 : 1][kWarpCap], best_[TOP ? kBlock / 32 : 1][kWarpTop];
+  constexpr int kWarps = kBlock / 32, kFly = 4;
+  __shared__ uint64_t buf_[TOP ? kWarps : 1][kWarpCap], best_[TOP ? kWarps : 1][kWarpTop];
+  __shared__ float spell_[TOP ? kWarps : 1][TOP ? kWarpSpells * 32 : 1];
+  __shared__ uint16_t item_[TOP ? kWarps : 1][TOP ? kWarpSpells * 32 : 1];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t row = (int64_t)blockIdx.x * (kBlock / 32) + warp;
+  const int64_t row = (int64_t)blockIdx.x * kWarps + warp;
   if (row >= rows) return;
   const Span<T> sp(logits + row * ld, cols);
   const float c = scale * kLog2e;
@@ -355,21 +362,28 @@ __global__ void __launch_bounds__(kBlock) k_logprobs_warp(const T* __restrict__ 
     extra = widen(sp.x[sp.loose_at(lane)]);
     run.push1(extra);
   }
-  constexpr int kFly = 4;
-  const int vecs = (int)sp.vecs;
+  const int vecs = (int)sp.vecs, tiles = (vecs + 32 * kFly - 1) / (32 * kFly), per = TOP ? (tiles + kWarpSpells - 1) / kWarpSpells : tiles;
   const T* body = sp.x + sp.head;
-  for (int v0 = lane; v0 < vecs; v0 += 32 * kFly) {
-    Raw8<T> raw[kFly];
+  for (int g = 0, tile = 0; tile < tiles; ++g) {
+    float spell = -INFINITY;
+    for (const int stop = min(tiles, tile + per); tile < stop; ++tile) {
+      const int v0 = tile * 32 * kFly + lane;
+      Raw8<T> raw[kFly];
 #pragma unroll
-    for (int k = 0; k < kFly; ++k)
-      if (v0 + k * 32 < vecs) raw[k] = TOP ? load8_cached(body + (v0 + k * 32) * 8) : load8(body + (v0 + k * 32) * 8);
+      for (int k = 0; k < kFly; ++k)
+        if (v0 + k * 32 < vecs) raw[k] = TOP ? load8_cached(body + (v0 + k * 32) * 8) : load8(body + (v0 + k * 32) * 8);
 #pragma unroll
-    for (int k = 0; k < kFly; ++k) {
-      if (v0 + k * 32 >= vecs) break;
-      float v[8];
-      widen8(raw[k], v);
-      const float top = run.push(v);
-      if (TOP) mine = nan_max(mine, top);
+      for (int k = 0; k < kFly; ++k) {
+        if (v0 + k * 32 >= vecs) break;
+        float v[8];
+        widen8(raw[k], v);
+        const float top = run.push(v);
+        if (TOP) spell = nan_max(spell, top);
+      }
+    }
+    if (TOP) {
+      spell_[warp][g * 32 + lane] = spell;
+      mine = nan_max(mine, spell);
     }
   }
   const RowSum a = lanes_sum<32>(run.sum(), c);
@@ -377,12 +391,19 @@ __global__ void __launch_bounds__(kBlock) k_logprobs_warp(const T* __restrict__ 
   if (lane == 0) write_row(a, o, sp.x, ids, row, cols, out);
   if (TOP) {
     uint64_t *buf = buf_[warp], *best = best_[warp];
-    const uint32_t top_key = lane < vecs ? value_key(mine) : 0u;
+    const uint32_t top_key = lane < vecs ? value_key(mine) : 0u, before = (1u << lane) - 1;
     uint32_t reach = 0;
-    for (uint32_t bit = 1u << 31; bit >= 1u << 12; bit >>= 1)
+    for (uint32_t bit = 1u << 31; bit >= 1u << 16; bit >>= 1)
       if (__popc(__ballot_sync(~0u, top_key >= (reach | bit))) >= top_k) reach |= bit;
     // the same bound as a float: what is not below it is a candidate (NaN included; everything, where there is no bound)
     float least_value = key_value((uint64_t)reach << 32);
+    int items = 0;
+    for (int g = 0; g * per < tiles; ++g) {
+      const bool take = g * per * 32 * kFly + lane < vecs && !(spell_[warp][g * 32 + lane] < least_value);
+      const uint32_t who = __ballot_sync(~0u, take);
+      if (take) item_[warp][items + __popc(who & before)] = (uint16_t)(g * 32 + lane);
+      items += __popc(who);
+    }
     uint64_t least = 0;
     int n = 0;
     auto keep = [&](bool take, float v, int at) {  // all lanes together
@@ -391,7 +412,7 @@ __global__ void __launch_bounds__(kBlock) k_logprobs_warp(const T* __restrict__ 
       const uint64_t key = order_key(v, (uint32_t)at);
       take = take && key > least;
       who = __ballot_sync(~0u, take);
-      if (take) buf[n + __popc(who & ((1u << lane) - 1))] = key;
+      if (take) buf[n + __popc(who & before)] = key;
       n += __popc(who);
     };
     auto shrink = [&]() {
@@ -407,13 +428,15 @@ __global__ void __launch_bounds__(kBlock) k_logprobs_warp(const T* __restrict__ 
       __syncwarp();
     };
     keep(lane < loose && !(extra < least_value), extra, lane < loose ? (int)sp.loose_at(lane) : 0);
-    for (int v0 = 0; v0 < vecs; v0 += 32) {
-      const bool have = v0 + lane < vecs;
+    __syncwarp();
+    const int slots = items * per * kFly;
+    for (int s0 = 0; s0 < slots; s0 += 32) {
+      const int slot = s0 + lane, item = slot < slots ? item_[warp][slot / (per * kFly)] : 0, k = slot % (per * kFly);
+      const int tile = item / 32 * per + k / kFly, v0 = tile * 32 * kFly + k % kFly * 32 + item % 32;
+      const bool have = slot < slots && tile < tiles && v0 < vecs;
       float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      if (have) widen8(load8_cached(body + (v0 + lane) * 8), v);
-      const float top = nan_max3(nan_max3(v[0], v[1], v[2]), nan_max3(v[3], v[4], v[5]), nan_max(v[6], v[7]));
-      if (!__any_sync(~0u, have && !(top < least_value))) continue;
-      const int at = (int)sp.head + (v0 + lane) * 8;
+      if (have) widen8(load8_cached(body + v0 * 8), v);
+      const int at = (int)sp.head + v0 * 8;
 #pragma unroll
       for (int q = 0; q < 8; ++q) keep(have && !(v[q] < least_value), v[q], at + q);
       if (n > kWarpTop) shrink();
@@ -761,18 +784,18 @@ cudaError_t launch_logprobs(const LaunchCtx& c, const CallDesc& d, const void* l
   with_types(d.in_dt, d.ids_dt, [&](auto* i, auto* id) {
     using T = std::remove_pointer_t<decltype(i)>;
     using Id = std::remove_pointer_t<decltype(id)>;
-    if (d.cols <= kGroupRow) {
+    if (d.cols <= GroupRow<T>::n) {
       const int rows = kBlock / (d.cols <= kNarrowRow ? 8 : 32);
       const unsigned blocks = (unsigned)((d.rows + rows - 1) / rows);
       auto go = [&](auto* f) { f<<<blocks, kBlock, 0, c.stream>>>((const T*)logits, (const Id*)ids, d.rows, d.cols, d.ld, (float)d.scale, d.top_k, out); };
       if (d.cols <= 64) go(d.top_k ? k_logprobs_group<T, Id, true, 8, 8> : k_logprobs_group<T, Id, false, 8, 8>);
       else if (d.cols <= 128) go(d.top_k ? k_logprobs_group<T, Id, true, 8, 16> : k_logprobs_group<T, Id, false, 8, 16>);
       else if (d.cols <= kNarrowRow) go(d.top_k ? k_logprobs_group<T, Id, true, 8, 32> : k_logprobs_group<T, Id, false, 8, 32>);
-      else if (d.cols <= 512) go(d.top_k ? k_logprobs_group<T, Id, true, 32, 16> : k_logprobs_group<T, Id, false, 32, 16>);
-      else go(d.top_k ? k_logprobs_group<T, Id, true, 32, 32> : k_logprobs_group<T, Id, false, 32, 32>);
+      else if (d.cols <= 512 || sizeof(T) == 2) go(d.top_k ? k_logprobs_group<T, Id, true, 32, 16> : k_logprobs_group<T, Id, false, 32, 16>);
+      else if constexpr (sizeof(T) == 4) go(d.top_k ? k_logprobs_group<T, Id, true, 32, 32> : k_logprobs_group<T, Id, false, 32, 32>);
       return;
     }
-    if (d.cols <= (d.top_k ? kWarpRowTop : kWarpRow) && d.top_k <= kWarpTop && d.rows >= (int64_t)c.sm_count * 16) {
+    if (d.cols <= kWarpRow && d.top_k <= kWarpTop && d.rows >= (int64_t)c.sm_count * kWarpRows * (d.cols > kWarpLong ? 2 : 1)) {
       const unsigned blocks = (unsigned)((d.rows + kBlock / 32 - 1) / (kBlock / 32));
       auto* f = d.top_k ? k_logprobs_warp<T, Id, true> : k_logprobs_warp<T, Id, false>;
       f<<<blocks, kBlock, 0, c.stream>>>((const T*)logits, (const Id*)ids, d.rows, d.cols, d.ld, (float)d.scale, d.top_k, out);

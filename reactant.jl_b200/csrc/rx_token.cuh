@@ -48,6 +48,66 @@ __device__ __forceinline__ void store8(uint16_t* p, const float (&v)[8]) {
   __stcs((uint4*)p, make_uint4(bf16x2_bits(v[0], v[1]), bf16x2_bits(v[2], v[3]), bf16x2_bits(v[4], v[5]), bf16x2_bits(v[6], v[7])));
 }
 
+// Eight consecutive elements from any element's boundary: the 16-byte lines that hold them, fetched first and shifted
+// into place afterwards, so that several fetches can be in flight.  A line is read whole, up to 15 bytes in front of and
+// behind the elements; where that would reach past `end` (of the memory behind the operand) they are read one by one.
+template <class T>
+struct Lines {
+  uint4 w[sizeof(T) == 4 ? 3 : 2];
+  int shift;  // elements
+  __device__ __forceinline__ void fetch(const T* p, const T* end) {
+    const uintptr_t a = (uintptr_t)p;
+    shift = (int)(a % 16 / sizeof(T));
+    const uint4* line = (const uint4*)(a - a % 16);
+    constexpr int kWhole = sizeof(T) == 4 ? 2 : 1;
+    if ((uintptr_t)(line + kWhole + (shift ? 1 : 0)) <= (uintptr_t)end) {
+#pragma unroll
+      for (int k = 0; k < kWhole; ++k) w[k] = __ldg(line + k);
+      if (shift) w[kWhole] = __ldg(line + kWhole);
+    } else {
+      T one[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) one[k] = p + k < end ? __ldg(p + k) : T(0);
+      shift = 0;
+      if constexpr (sizeof(T) == 4) {
+        w[0] = make_uint4(__float_as_uint(one[0]), __float_as_uint(one[1]), __float_as_uint(one[2]), __float_as_uint(one[3]));
+        w[1] = make_uint4(__float_as_uint(one[4]), __float_as_uint(one[5]), __float_as_uint(one[6]), __float_as_uint(one[7]));
+      } else {
+        w[0] = make_uint4(one[0] | (uint32_t)one[1] << 16, one[2] | (uint32_t)one[3] << 16, one[4] | (uint32_t)one[5] << 16, one[6] | (uint32_t)one[7] << 16);
+      }
+    }
+  }
+  __device__ __forceinline__ void get(float (&v)[8]) const {
+    constexpr int kWords = sizeof(T) == 4 ? 12 : 8;
+    uint32_t x[kWords];
+#pragma unroll
+    for (int k = 0; k < kWords / 4; ++k) {
+      x[4 * k] = w[k].x;
+      x[4 * k + 1] = w[k].y;
+      x[4 * k + 2] = w[k].z;
+      x[4 * k + 3] = w[k].w;
+    }
+    const int words = sizeof(T) == 4 ? shift : shift >> 1;
+#pragma unroll
+    for (int k = 0; k + 2 < kWords; ++k)
+      if (words & 2) x[k] = x[k + 2];
+#pragma unroll
+    for (int k = 0; k + 1 < kWords; ++k)
+      if (words & 1) x[k] = x[k + 1];
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = __uint_as_float(x[k]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t y = shift & 1 ? __funnelshift_r(x[k], x[k + 1], 16) : x[k];
+        v[2 * k] = __uint_as_float(y << 16);
+        v[2 * k + 1] = __uint_as_float(y & 0xFFFF0000u);
+      }
+    }
+  }
+};
+
 // The same where the eight elements start on their own size (32 bytes for floats): one store a lane, whole sectors.
 __device__ __forceinline__ void store8_whole(float* p, const float (&v)[8]) {
   asm volatile("st.global.cs.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]) : "memory");

@@ -208,7 +208,7 @@ def test_operands_are_windows_or_copies(rx):
 
 
 # ---- GPU: the engine against the oracle ---------------------------------------------------------------------------------------
-SIZES = [(1, 1, 1), (1, 8, 5), (7, 33, 100), ((2, 3), 128, 50), (300, 1000, 999), (129, 2048, 40), (0, 8, 5), (5, 0, 7)]
+SIZES = [(1, 1, 1), (1, 8, 5), (7, 33, 100), ((2, 3), 128, 50), (300, 1000, 999), (129, 2048, 40), (0, 8, 5), (5, 0, 7), (33, 1029, 60), (1, 8191, 3), (40, 3, 9)]
 
 
 @pytest.mark.gpu
@@ -227,7 +227,7 @@ def test_embedding(rx, ref, client, tokens, features, vocab, et, out_et, ids_et)
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("et,out_et,ids_et", [("f32", "f32", "i64"), ("bf16", "f32", "i32"), ("bf16", "bf16", "i32")])
-@pytest.mark.parametrize("tokens,features,vocab", SIZES + [(5000, 24, 3), (4097, 65, 70000), (20000, 8, 300)])
+@pytest.mark.parametrize("tokens,features,vocab", SIZES + [(5000, 24, 3), (4097, 65, 70000), (20000, 8, 300), (8192, 300, 2000), (8193, 301, 20), (70000, 9, 5000)])
 def test_embedding_grad(rx, ref, client, tokens, features, vocab, et, out_et, ids_et):
     rng = np.random.default_rng(4)
     n = int(np.prod(tokens))
@@ -296,7 +296,7 @@ def masked_logits(rx, rng, shape, et, scale=3.0):
 
 
 LOGPROB_SIZES = [(1, 1, 1), (1, 8, 3), ((2, 3), 33, 5), (5, 1000, 64), (3, 1025, 20), (2, 50021, 7), (64, 259, 0), (0, 16, 2), (1, 131072, 32), (300, 64, 1),
-                 (37, 64, 64), (35, 128, 33), (33, 256, 20), (9, 257, 32), (5, 4096, 32), (2, 4097, 33)]
+                 (37, 64, 64), (35, 128, 33), (33, 256, 20), (9, 257, 32), (5, 4096, 32), (2, 4097, 33), (2400, 1030, 20), (2400, 513, 33), (4800, 8200, 3)]
 
 
 @pytest.mark.gpu
@@ -454,7 +454,7 @@ def test_step_repeats_itself_and_follows_its_key(rx, client):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("pattern", ["one", "two", "all different", "padding only", "runs of 33", "falling", "first and last"])
-@pytest.mark.parametrize("tokens,features", [(31, 8), (1024, 40), (8193, 8), (4000, 2056)])
+@pytest.mark.parametrize("tokens,features", [(31, 8), (1024, 40), (1025, 41), (8193, 8), (9000, 7), (4000, 2056), (4000, 2049)])
 def test_embedding_grad_patterns(rx, ref, client, pattern, tokens, features):
     """Runs that fill, cross and end at the borders of the pieces the work is cut into."""
     vocab = 9000
