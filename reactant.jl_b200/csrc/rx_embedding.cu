@@ -126,6 +126,7 @@ struct SortShared {
   uint32_t count[kSortWarps][kBins];
   uint32_t base[kBins];
   uint32_t warp_sum[kSortWarps];
+  int32_t seen[kBins];
 };
 
 // the lanes that have this lane's digit, by one vote a bit (one bit more than the digit where some lanes have none)
@@ -232,7 +233,12 @@ struct SortPass {
           if (!(same & below)) sh.count[warp][d] += __popc(same);
           to[at] = key[k];
           to[rows + at] = pos[k];
-          if (!from && key[k] < vocab && !touched[key[k]]) touched[key[k]] = 1;  // few lines take the marks of frequent ids: look first
+          // thousands of stores to the one byte of a frequent id would queue up (26 us instead of 8): a block marks
+          // an id again only when another one has taken its place among the last seen
+          if (!from && key[k] < vocab && sh.seen[key[k] % kBins] != key[k]) {
+            sh.seen[key[k] % kBins] = key[k];
+            touched[key[k]] = 1;
+          }
         }
         __syncwarp();
       }
@@ -289,7 +295,7 @@ __global__ void __launch_bounds__(kRankBlock) k_rank_tokens(const Id* __restrict
     if (lane == i && t < rows) {
       key[before[i]] = (int32_t)mine[i];
       pos[before[i]] = t;
-      if (mine[i] < (uint32_t)vocab && !touched[mine[i]]) touched[mine[i]] = 1;
+      if (mine[i] < (uint32_t)vocab) touched[mine[i]] = 1;
     }
   }
 }
@@ -307,6 +313,7 @@ template <class Id>
 __global__ void __launch_bounds__(kSortBlock) k_place_tokens(SortPass<Id> s, const uint32_t* __restrict__ totals) {
   __shared__ SortShared sh;
   s.own(blockIdx.x, gridDim.x);
+  sh.seen[threadIdx.x] = -1;  // (barriers follow)
   int32_t key[kHold], pos[kHold];
   s.fetch(s.lo, key);  // asked for ahead of the totals
   s.fetch_places(s.lo, pos);
@@ -338,9 +345,9 @@ struct GradArgs {
 
 constexpr int kMaxChunk = 128, kMaxPlaces = 1024, kFillUnits = 8;
 
-// Zeros for the rows that no token has.  Rows that are whole vectors, and short ones, go by units of eight consecutive
-// elements of the result, kFillUnits a thread, whose rows are all looked up before the first is written; long rows of an
-// odd length go by warps, a row at a time from its first element on a whole vector's boundary.
+// Zeros for the rows that no token has.  Rows that are whole vectors go by units of eight consecutive elements of the
+// result, kFillUnits a thread, whose rows are all looked up before the first is written; other long rows by warps, a row
+// at a time from its first element on a whole vector's boundary; other short ones by elements.
 constexpr int kFillRow = 256, kFillRows = 4;  // elements from which a row is a warp's; rows a warp
 
 template <class Out, bool VEC>
@@ -364,35 +371,20 @@ __device__ __forceinline__ void fill_rows(const GradArgs& g, Out* out, int64_t b
     }
     return;
   }
-  const int64_t n = g.vocab * g.cols, units = (n + 7) >> 3, per_row = g.cols >> 3;
+  constexpr int kUnit = VEC ? 8 : 1;
+  const int64_t units = g.vocab * g.cols / kUnit, per_row = g.cols / kUnit;
   const int64_t base = block * (kBlock * kFillUnits) + threadIdx.x;
-  auto row = [&](int64_t i) -> int64_t {  // of element i
-    if (VEC) return g.small ? g.by_row.quotient((uint32_t)(i >> 3)) : (i >> 3) / per_row;
-    return g.small ? g.by_row.quotient((uint32_t)i) : i / g.cols;
-  };
   bool free[kFillUnits];
 #pragma unroll
   for (int k = 0; k < kFillUnits; ++k) {
     const int64_t u = base + k * kBlock;
-    free[k] = u < units;
-    if (!free[k] || !g.touched) continue;
-    const int64_t t = row(u * 8);
-    uint32_t any = __ldg(g.touched + t);
-    if (!VEC) any |= __ldg(g.touched + row(min(u * 8 + 7, n - 1)));
-    free[k] = !any;
+    free[k] = u < units && !(g.touched && __ldg(g.touched + (g.small ? (int64_t)g.by_row.quotient((uint32_t)u) : u / per_row)));
   }
 #pragma unroll
   for (int k = 0; k < kFillUnits; ++k) {
-    const int64_t u = base + k * kBlock;
-    if (VEC) {
-      if (free[k]) store8_whole(out + u * 8, zero);
-    } else if (u < units) {
-      // a unit whose ends lie in rows without a token: so do its middle's, where a row is eight elements or longer
-      if (free[k] && u * 8 + 8 <= n && g.cols >= 8) store8_whole(out + u * 8, zero);
-      else
-        for (int64_t i = u * 8; i < min(u * 8 + 8, n); ++i)
-          if (!g.touched || !__ldg(g.touched + row(i))) put(out + i, 0.f);
-    }
+    if (!free[k]) continue;
+    if (VEC) store8_whole(out + (base + k * kBlock) * 8, zero);
+    else put(out + base + k * kBlock, 0.f);
   }
 }
 
@@ -652,8 +644,8 @@ cudaError_t launch_embedding_grad(const LaunchCtx& c, const CallDesc& d, const v
   const bool vec = vec_out && aligned16(dy) && d.ld * (int64_t)dt_size(d.in_dt) % 16 == 0;
   g.by_row = Divisor(vec ? d.cols / 8 : d.cols);
   g.small = n < (int64_t)1 << 31;
-  const int64_t units = (n + 7) / 8;
-  const int64_t fill_blocks = !vec && d.cols >= kFillRow ? (d.vocab + kBlock / 32 * kFillRows - 1) / (kBlock / 32 * kFillRows) : (units + kBlock * kFillUnits - 1) / (kBlock * kFillUnits);
+  const int64_t per = !vec && d.cols >= kFillRow ? kBlock / 32 * kFillRows : kBlock * kFillUnits, fills = !vec && d.cols >= kFillRow ? d.vocab : vec ? n / 8 : n;
+  const int64_t fill_blocks = (fills + per - 1) / per;
   cudaError_t err = cudaSuccess;
   with_types(d.in_dt, d.out_dt, d.ids_dt, [&](auto* i, auto* o, auto* id) {
     using In = std::remove_pointer_t<decltype(i)>;

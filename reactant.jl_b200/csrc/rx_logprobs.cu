@@ -707,42 +707,46 @@ struct GradRow {
 };
 
 template <class T, class Id, int TPR, bool VEC>
-__global__ void __launch_bounds__(kBlock) k_logprobs_grad(const T* __restrict__ logits, const Id* __restrict__ ids, int64_t rows, int64_t cols, int64_t ld, float scale, LogProbsGradIn in,
+__global__ void __launch_bounds__(kBlock, 4) k_logprobs_grad(const T* __restrict__ logits, const Id* __restrict__ ids, int64_t rows, int64_t cols, int64_t ld, float scale, LogProbsGradIn in,
                                                           T* __restrict__ out) {
   const int lane = threadIdx.x % TPR;
   const int64_t row = (int64_t)blockIdx.x * (kBlock / TPR) + threadIdx.x / TPR;
   if (row >= rows) return;
   const T* x = logits + row * ld;
   T* y = out + row * cols;
+  // elements in front of the first one on a 16-byte boundary (the same for both arrays)
+  const int64_t head = VEC ? min((int64_t)((16 - (uintptr_t)y % 16) % 16 / sizeof(T)), cols) : 0, vecs = VEC ? (cols - head) >> 3 : 0, tail = head + (vecs << 3);
+  const int64_t step = (int64_t)gridDim.y * TPR * kGradVecs;
+  int64_t v0 = (int64_t)blockIdx.y * TPR * kGradVecs + lane;
+  Raw8<T> raw[kGradVecs];
+  auto fetch = [&]() {
+#pragma unroll
+    for (int k = 0; k < kGradVecs; ++k)
+      if (v0 + k * TPR < vecs) raw[k] = load8(x + head + ((v0 + k * TPR) << 3));
+  };
+  if (VEC) fetch();  // in flight while the row's own values come
   GradRow r;
   r.c = scale;
   r.lse = __ldg(in.lse + row);
   r.h = __ldg(in.entropy + row);
   const int64_t id = (int64_t)__ldg(ids + row);
-  r.id = id >= 0 && id < cols ? (int32_t)id : -1;
-  const float g = in.dlogprob && r.id >= 0 ? __ldg(in.dlogprob + row) : 0.f;
+  const float arrived = in.dlogprob ? __ldg(in.dlogprob + row) : 0.f;
   r.gh = in.dentropy ? __ldg(in.dentropy + row) : 0.f;
-  r.a = (in.dlse ? __ldg(in.dlse + row) : 0.f) - g;
+  const float dlse = in.dlse ? __ldg(in.dlse + row) : 0.f;
+  r.id = id >= 0 && id < cols ? (int32_t)id : -1;
+  const float g = r.id >= 0 ? arrived : 0.f;
+  r.a = dlse - g;
   r.hot = g * scale;
   if (r.lse == -INFINITY) {  // a row without any probability has no gradient: every p becomes 0
     r.lse = INFINITY;
     r.id = -1;
   }
   if (VEC) {
-    // elements in front of the first one on a 16-byte boundary (the same for both arrays)
-    int64_t head = (int64_t)((16 - (uintptr_t)y % 16) % 16 / sizeof(T));
-    if (head > cols) head = cols;
-    const int64_t vecs = (cols - head) >> 3, tail = head + (vecs << 3);
     if (blockIdx.y == 0) {
       for (int64_t c = lane; c < head; c += TPR) put(y + c, r.one(widen(x[c]), (int32_t)c));
       for (int64_t c = tail + lane; c < cols; c += TPR) put(y + c, r.one(widen(x[c]), (int32_t)c));
     }
-    const int64_t step = (int64_t)gridDim.y * TPR * kGradVecs;
-    for (int64_t v0 = (int64_t)blockIdx.y * TPR * kGradVecs + lane; v0 < vecs; v0 += step) {
-      Raw8<T> raw[kGradVecs];
-#pragma unroll
-      for (int k = 0; k < kGradVecs; ++k)
-        if (v0 + k * TPR < vecs) raw[k] = load8(x + head + ((v0 + k * TPR) << 3));
+    while (v0 < vecs) {
 #pragma unroll
       for (int k = 0; k < kGradVecs; ++k) {
         if (v0 + k * TPR >= vecs) break;
@@ -758,6 +762,8 @@ __global__ void __launch_bounds__(kBlock) k_logprobs_grad(const T* __restrict__ 
         }
         store8(y + c, v);
       }
+      v0 += step;
+      fetch();
     }
   } else {
     for (int64_t c = (int64_t)blockIdx.y * TPR + lane; c < cols; c += (int64_t)gridDim.y * TPR) put(y + c, r.one(widen(x[c]), (int32_t)c));
