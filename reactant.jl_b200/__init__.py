@@ -322,9 +322,10 @@ class ConcreteRArray:
     def __dlpack__(self, *, stream=None, max_version=None, dl_device=None, copy=None):
         """Hand the array out without a copy, in its Julia shape (first dimension contiguous).  `stream` is the consumer's
         stream, which is made to wait for the work queued here: None or 1 the legacy default one, -1 no waiting."""
-        if copy or (dl_device is not None and tuple(dl_device) != self.__dlpack_device__()):
+        if copy or dl_device is not None and tuple(dl_device) != self.__dlpack_device__():
             raise BufferError("the array can only be handed out as it is, on its own device")
-        p = lib().RxBufferToDLPack(self._single().handle, (1 if stream is None else stream) & 0xFFFFFFFFFFFFFFFF)
+        buf = self.data[0] if len(self.data) == 1 and self.sharding is None else self._single()
+        p = lib().RxBufferToDLPack(buf.handle, (1 if stream is None else stream) & 0xFFFFFFFFFFFFFFFF)
         if not p:
             check()
         return _PyCapsule_New(p, b"dltensor", _dl_drop)
@@ -463,7 +464,8 @@ class Thunk:
         self.param_sharded_dim = [l.RxExecutableParameterShardedDim(handle, i) for i in range(self.num_parameters)]
         self.result_sharded_dim = [l.RxExecutableResultShardedDim(handle, i) for i in range(self.num_results)]
         self.param_alias = [l.RxExecutableParameterAlias(handle, i) for i in range(self.num_parameters)]
-        self._execute = l.XLAExecuteSharded
+        self._execute, self._error_code = l.XLAExecuteSharded, l.RxLastErrorCode
+        self._aliased = any(k >= 0 for k in self.param_alias)
         self._args_t = C.c_void_p * max(1, self.num_parameters)
         self._outs_t = C.c_void_p * max(1, self.num_results)
         mask_t = C.c_uint8 * max(1, self.num_parameters)
@@ -475,12 +477,13 @@ class Thunk:
         dev = args[0].data[0].device if args else self.client.addressable_devices[0]
         out = self._outs_t()
         self._execute(self.handle, len(args), self._args_t(*[a.data[0].handle for a in args]), dev.handle, self._masks[1 if donate else 0], self.num_results, out, None, None)
-        check()
+        if self._error_code():
+            check()
         bufs = [_Buffer(h, dev) for h in out[:self.num_results]]
         if self._result_info is None:
             self._result_info = [(ConcreteRArray if b.dims else ConcreteRNumber, tuple(reversed(b.dims)), b.dtype) for b in bufs]
         results = tuple(cls._of([b], shape, dtype) for b, (cls, shape, dtype) in zip(bufs, self._result_info))
-        if donate:
+        if donate and self._aliased:
             for a, k in zip(args, self.param_alias):
                 if 0 <= k < len(results):
                     a.data = results[k].data

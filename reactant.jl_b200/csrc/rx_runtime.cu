@@ -74,7 +74,8 @@ char* dup_cstr(const std::string& s) {
   return p;
 }
 
-constexpr size_t kMaxBusyBlocks = 4;  // blocks of one size that wait for another stream before an allocation waits with them
+// blocks of one size that wait for another stream before an allocation waits with them: a few calls' results
+constexpr size_t max_busy_blocks(size_t bytes) { return bytes <= ((size_t)16 << 20) ? 16 : 4; }
 
 size_t round_up(size_t b) { return b == 0 ? 256 : (b + 255) & ~(size_t)255; }
 
@@ -100,15 +101,18 @@ void* RxDevice::alloc(size_t bytes) {
       size_t take = blocks.size(), k = blocks.size();
       while (k > 0 && blocks[k - 1].busy) --k;
       if (k > 0) take = k - 1;  // the latest that only this device's stream has used
-      for (k = 0; take == blocks.size() && k < blocks.size(); ++k)
-        if (cudaEventQuery(blocks[k].busy) == cudaSuccess) take = k;
-      cudaGetLastError();  // "not ready" is no error
-      if (take == blocks.size() && (blocks.size() >= kMaxBusyBlocks || (bytes_limit > 0 && bytes_in_use + pool_bytes + (int64_t)rb > bytes_limit))) take = 0;
+      bool passed = false;
+      if (take == blocks.size()) {  // the one that has waited longest is the likeliest to be free
+        passed = cudaEventQuery(blocks[0].busy) == cudaSuccess;
+        if (passed) take = 0;
+        else cudaGetLastError();  // "not ready" is no error
+      }
+      if (take == blocks.size() && (blocks.size() >= max_busy_blocks(rb) || (bytes_limit > 0 && bytes_in_use + pool_bytes + (int64_t)rb > bytes_limit))) take = 0;
       if (take == blocks.size()) goto fresh;
       void* p = blocks[take].p;
       if (blocks[take].busy) {
-        cudaStreamWaitEvent(stream, blocks[take].busy, 0);  // at once, where it has passed already
-        cudaEventDestroy(blocks[take].busy);
+        if (!passed) cudaStreamWaitEvent(stream, blocks[take].busy, 0);
+        spare_events.push_back(blocks[take].busy);
       }
       blocks.erase(blocks.begin() + take);
       pool_bytes -= (int64_t)rb;
@@ -176,6 +180,31 @@ void RxDevice::trim() {
     }
 }
 
+cudaEvent_t RxDevice::take_event() {
+  {
+    std::lock_guard<std::mutex> lk(mu);
+    if (!spare_events.empty()) {
+      cudaEvent_t e = spare_events.back();
+      spare_events.pop_back();
+      return e;
+    }
+  }
+  cudaEvent_t e = nullptr;
+  if (cudaEventCreateWithFlags(&e, cudaEventDisableTiming) != cudaSuccess) {
+    cudaGetLastError();
+    return nullptr;
+  }
+  return e;
+}
+void RxDevice::give_event(cudaEvent_t e) {
+  if (closed.load()) {
+    cudaEventDestroy(e);
+    return;
+  }
+  std::lock_guard<std::mutex> lk(mu);
+  spare_events.push_back(e);
+}
+
 void RxDevice::hand_back(void* tensor) {
   auto* t = (rx::DLManagedTensor*)tensor;
   if (closed.load()) {  // everything that was queued has drained
@@ -185,8 +214,8 @@ void RxDevice::hand_back(void* tensor) {
   int cur = 0;
   cudaGetDevice(&cur);
   cudaSetDevice(ordinal);
-  Returned r{tensor, nullptr};
-  if (cudaEventCreateWithFlags(&r.done, cudaEventDisableTiming) != cudaSuccess || cudaEventRecord(r.done, stream) != cudaSuccess) {
+  Returned r{tensor, take_event()};
+  if (!r.done || cudaEventRecord(r.done, stream) != cudaSuccess) {
     cudaGetLastError();
     cudaStreamSynchronize(stream);
   }
@@ -214,7 +243,7 @@ void RxDevice::reap(bool all) {
   }
   cudaGetLastError();  // "not ready" is no error
   for (auto& r : done) {  // outside the lock: the owner's code runs here
-    if (r.done) cudaEventDestroy(r.done);
+    if (r.done) give_event(r.done);
     auto* t = (rx::DLManagedTensor*)r.tensor;
     if (t->deleter) t->deleter(t);
   }
@@ -1003,9 +1032,12 @@ void execute(RxExecutable* ex, const std::vector<RxDevice*>& devs, RxBuffer** ar
   for (size_t k = 0; k < devs.size(); ++k) {
     RxDevice* d = devs[k];
     CK(cudaSetDevice(d->ordinal));
-    auto es = std::make_shared<EventState>();
-    es->dev = d;
-    es->keep = d->shared_from_this();
+    std::shared_ptr<EventState> es;
+    if (future_results) {
+      es = std::make_shared<EventState>();
+      es->dev = d;
+      es->keep = d->shared_from_this();
+    }
     for (int j = 0; j < num_results; ++j) {
       const ResultBinding& rb = p.results[j];
       auto* b = own(new RxBuffer());
@@ -1147,6 +1179,8 @@ void FreeClient(RxClient* client) {
     d->trim();
     if (d->order) cudaEventDestroy(d->order);
     d->order = nullptr;
+    for (cudaEvent_t e : d->spare_events) cudaEventDestroy(e);
+    d->spare_events.clear();
     if (d->scratch) cudaFree(d->scratch);
     if (d->flush_buf) cudaFree(d->flush_buf);
     if (d->status) cudaFreeHost(d->status);
@@ -1338,17 +1372,17 @@ void handed_out_deleter(rx::DLManagedTensor* t) {
   int cur = 0;
   cudaGetDevice(&cur);
   if (cur != d->ordinal) cudaSetDevice(d->ordinal);
-  cudaEvent_t ev = nullptr;
-  if (cudaEventCreateWithFlags(&ev, cudaEventDisableTiming) != cudaSuccess || cudaEventRecord(ev, h->consumer) != cudaSuccess) {
+  cudaEvent_t ev = d->take_event();
+  if (!ev || cudaEventRecord(ev, h->consumer) != cudaSuccess) {
     cudaGetLastError();  // the consumer's stream is gone: everything it had queued is waited for instead
-    if (ev) cudaEventDestroy(ev);
+    if (ev) d->give_event(ev);
     cudaDeviceSynchronize();
   } else {
     std::lock_guard<std::mutex> g(h->st->pending_mu);
     if (h->st->pending) {  // another consumer's, or an all-reduce's: the new event stands for both
       cudaStreamWaitEvent(h->consumer, h->st->pending, 0);
       cudaEventRecord(ev, h->consumer);
-      cudaEventDestroy(h->st->pending);
+      d->give_event(h->st->pending);
     }
     h->st->pending = ev;
   }

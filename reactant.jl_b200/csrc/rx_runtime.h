@@ -88,6 +88,9 @@ struct RxDevice : std::enable_shared_from_this<RxDevice> {
   cudaEvent_t order = nullptr;             // recorded on `stream` when a consumer needs to wait for it and executions were queued since the last time
   uint64_t ordered = 0;                    // value of `enqueued` then
   std::atomic<uint64_t> enqueued{1};       // executions queued so far
+  std::vector<cudaEvent_t> spare_events;   // guarded by mu; without timing, like every event that takes part here
+  cudaEvent_t take_event();                // null, with the error cleared, when none can be made
+  void give_event(cudaEvent_t e);
   void hand_back(void* tensor);            // memory taken over is no longer used by anything that will be queued
   void reap(bool all);                     // owners whose memory is free now get it back
 
@@ -125,7 +128,7 @@ struct Storage {
     std::lock_guard<std::mutex> g(pending_mu);
     if (!pending) return;
     if (dev->stream) cudaStreamWaitEvent(dev->stream, pending, 0);
-    cudaEventDestroy(pending);
+    dev->give_event(pending);
     pending = nullptr;
   }
   ~Storage() {
