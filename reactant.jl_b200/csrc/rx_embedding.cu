@@ -260,6 +260,7 @@ constexpr int kRankTokens = 8192, kRankBlock = 512, kRankPerBlock = 4 * kRankBlo
 template <class Id>
 __global__ void __launch_bounds__(kRankBlock) k_rank_tokens(const Id* __restrict__ ids, int rows, int64_t vocab, int32_t* __restrict__ key, int32_t* __restrict__ pos, uint8_t* touched) {
   __shared__ __align__(16) uint32_t sh[kRankTokens];
+  pdl_release();
   const int vecs = (rows + 3) / 4, lane = threadIdx.x & 31;
 #pragma unroll 8
   for (int t = threadIdx.x; t < vecs * 4; t += kRankBlock) {
@@ -304,6 +305,8 @@ __global__ void __launch_bounds__(kRankBlock) k_rank_tokens(const Id* __restrict
 template <class Id>
 __global__ void __launch_bounds__(kSortBlock) k_count_tokens(SortPass<Id> s, uint32_t* totals, int32_t* crossing) {
   __shared__ SortShared sh;
+  pdl_wait();
+  pdl_release();
   if (!s.from) clear_touched(s.touched, s.vocab, crossing, blockIdx.x, gridDim.x);
   s.own(blockIdx.x, gridDim.x);
   int32_t key[kHold];
@@ -312,6 +315,8 @@ __global__ void __launch_bounds__(kSortBlock) k_count_tokens(SortPass<Id> s, uin
 template <class Id>
 __global__ void __launch_bounds__(kSortBlock) k_place_tokens(SortPass<Id> s, const uint32_t* __restrict__ totals) {
   __shared__ SortShared sh;
+  pdl_wait();
+  pdl_release();
   s.own(blockIdx.x, gridDim.x);
   sh.seen[threadIdx.x] = -1;  // (barriers follow)
   int32_t key[kHold], pos[kHold];
@@ -348,7 +353,7 @@ constexpr int kMaxChunk = 128, kMaxPlaces = 1024, kFillUnits = 8;
 // Zeros for the rows that no token has.  Rows that are whole vectors go by units of eight consecutive elements of the
 // result, kFillUnits a thread, whose rows are all looked up before the first is written; other long rows by warps, a row
 // at a time from its first element on a whole vector's boundary; other short ones by elements.
-constexpr int kFillRow = 256, kFillRows = 4;  // elements from which a row is a warp's; rows a warp
+constexpr int kFillRow = 256, kFillRows = 1;  // elements from which a row is a warp's; rows a warp
 
 template <class Out, bool VEC>
 __device__ __forceinline__ void fill_rows(const GradArgs& g, Out* out, int64_t block) {
@@ -395,6 +400,8 @@ template <class In, class Out, bool VEC>
 __global__ void __launch_bounds__(kBlock, VEC ? 1 : 3) k_sum_runs(const In* __restrict__ dy, const In* end, Out* __restrict__ out, const __grid_constant__ GradArgs g) {
   __shared__ int32_t skey[kMaxPlaces + 2 * kMaxChunk + 2], spos[kMaxPlaces + kMaxChunk];
   __shared__ float turn[VEC ? 1 : kBlock / 32][VEC ? 1 : 32 * 9];
+  pdl_wait();
+  pdl_release();
   if (blockIdx.x >= g.chunk_blocks * g.slices) {
     fill_rows<Out, VEC>(g, out, blockIdx.x - g.chunk_blocks * g.slices);
     return;
@@ -507,6 +514,7 @@ __global__ void __launch_bounds__(kBlock, VEC ? 1 : 3) k_sum_runs(const In* __re
 template <class Out>
 __global__ void __launch_bounds__(kBlock) k_join_runs(Out* __restrict__ out, const __grid_constant__ GradArgs g) {
   __shared__ float sum[kBlock / 32][kBlock];
+  pdl_wait();
   const int n = *g.crossing, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t slices = (g.cols + kBlock - 1) / kBlock, work = n * slices;
   for (int64_t w = blockIdx.x; w < work; w += gridDim.x) {
@@ -646,7 +654,25 @@ cudaError_t launch_embedding_grad(const LaunchCtx& c, const CallDesc& d, const v
   g.small = n < (int64_t)1 << 31;
   const int64_t per = !vec && d.cols >= kFillRow ? kBlock / 32 * kFillRows : kBlock * kFillUnits, fills = !vec && d.cols >= kFillRow ? d.vocab : vec ? n / 8 : n;
   const int64_t fill_blocks = (fills + per - 1) / per;
+  // Every kernel but the first may be set up while the one in front is still running: it waits for that one's results
+  // before it looks at anything.  The last lets nobody in ahead of its end, so what follows this call finds it done.
   cudaError_t err = cudaSuccess;
+  bool behind = false;
+  auto launch = [&](auto* kernel, int64_t blocks, int threads, auto... args) {
+    if (err != cudaSuccess) return;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)blocks);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.stream = c.stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = behind ? 1 : 0;
+    err = cudaLaunchKernelEx(&cfg, kernel, args...);
+    behind = true;
+    ++*c.launches;
+  };
   with_types(d.in_dt, d.out_dt, d.ids_dt, [&](auto* i, auto* o, auto* id) {
     using In = std::remove_pointer_t<decltype(i)>;
     using Out = std::remove_pointer_t<decltype(o)>;
@@ -661,10 +687,7 @@ cudaError_t launch_embedding_grad(const LaunchCtx& c, const CallDesc& d, const v
       g.part = (float*)(w + p.part);
       if (d.rows <= kRankTokens) {
         err = cudaMemsetAsync(w + p.touched, 0, (size_t)(p.crossing + 4 - p.touched), c.stream);
-        if (err != cudaSuccess) return;
-        k_rank_tokens<Id><<<(unsigned)((d.rows + kRankPerBlock - 1) / kRankPerBlock), kRankBlock, 0, c.stream>>>((const Id*)ids, (int)d.rows, d.vocab, (int32_t*)g.key, (int32_t*)g.pos,
-                                                                                                             (uint8_t*)(w + p.touched));
-        ++*c.launches;
+        launch(k_rank_tokens<Id>, (d.rows + kRankPerBlock - 1) / kRankPerBlock, kRankBlock, (const Id*)ids, (int)d.rows, d.vocab, (int32_t*)g.key, (int32_t*)g.pos, (uint8_t*)(w + p.touched));
       } else {
         SortPass<Id> pass{};
         pass.ids = (const Id*)ids;
@@ -677,22 +700,17 @@ cudaError_t launch_embedding_grad(const LaunchCtx& c, const CallDesc& d, const v
           pass.from = k == 0 ? nullptr : k % 2 ? a : b;
           pass.to = k % 2 ? b : a;
           pass.shift = k * p.digit;
-          k_count_tokens<Id><<<p.ranks, kSortBlock, 0, c.stream>>>(pass, totals, g.crossing);
-          k_place_tokens<Id><<<p.ranks, kSortBlock, 0, c.stream>>>(pass, totals);
-          *c.launches += 2;
+          launch(k_count_tokens<Id>, p.ranks, kSortBlock, pass, totals, g.crossing);
+          launch(k_place_tokens<Id>, p.ranks, kSortBlock, pass, (const uint32_t*)totals);
         }
       }
     } else {
       g.chunk_blocks = 0;
     }
-    auto* sum = vec ? k_sum_runs<In, Out, true> : k_sum_runs<In, Out, false>;
-    sum<<<(unsigned)(g.chunk_blocks * g.slices + fill_blocks), kBlock, 0, c.stream>>>((const In*)dy, (const In*)dy + (d.rows ? (d.rows - 1) * d.ld + d.cols : 0), (Out*)out, g);
-    ++*c.launches;
-    if (g.chunks > 1) {
-      const int64_t most = g.chunks * ((d.cols + kBlock - 1) / kBlock);
-      k_join_runs<Out><<<(unsigned)std::min<int64_t>(most, (int64_t)c.sm_count * 8), kBlock, 0, c.stream>>>((Out*)out, g);
-      ++*c.launches;
-    }
+    launch(vec ? k_sum_runs<In, Out, true> : k_sum_runs<In, Out, false>, g.chunk_blocks * g.slices + fill_blocks, kBlock, (const In*)dy,
+           (const In*)dy + (d.rows ? (d.rows - 1) * d.ld + d.cols : 0), (Out*)out, g);
+    // a run of at most two chunks' length never is a long one
+    if (g.chunks > 2) launch(k_join_runs<Out>, std::min<int64_t>(g.chunks * ((d.cols + kBlock - 1) / kBlock), (int64_t)c.sm_count * 8), kBlock, (Out*)out, g);
   });
   return err != cudaSuccess ? err : cudaGetLastError();
 }
