@@ -578,7 +578,7 @@ struct GradPlan {
     // Chunks as long as they still give every SM four blocks, or two where the rows are short (a block then has several
     // chunks, and what a chunk costs besides its rows counts) or the zeros keep the SMs busy as well.
     const bool filling = (d.vocab - d.rows) * (int64_t)dt_size(d.out_dt) > d.rows * (int64_t)dt_size(d.in_dt);
-    const int64_t blocks = sm_count * (filling || groups > 1 ? 2 : 4), least = d.rows > 2048 ? 16 : 8;
+    const int64_t blocks = sm_count * (filling || groups > 1 ? 2 : 4), least = d.rows > 2048 ? 16 : d.rows > 1024 ? 8 : 4;
     g.chunk = std::min(kMaxChunk, kMaxPlaces / groups);
     while (g.chunk > least && (d.rows + (int64_t)g.chunk * groups - 1) / ((int64_t)g.chunk * groups) * g.slices < blocks) g.chunk /= 2;
     g.chunks = (d.rows + g.chunk - 1) / g.chunk;
