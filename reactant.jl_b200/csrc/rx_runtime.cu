@@ -1414,8 +1414,7 @@ void* RxBufferToDLPack(RxBuffer* b, void* consumer_stream) {
     int cur = 0;
     cudaGetDevice(&cur);
     if (cur != d->ordinal) CK(cudaSetDevice(d->ordinal));
-    const bool late = b->st->pending != nullptr;
-    b->st->make_ready();
+    const bool late = b->st->make_ready();
     std::lock_guard<std::mutex> g(d->order_mu);
     if (!d->order) CK(cudaEventCreateWithFlags(&d->order, cudaEventDisableTiming));
     const uint64_t now = d->enqueued.load();

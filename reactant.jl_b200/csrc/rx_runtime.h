@@ -124,12 +124,13 @@ struct Storage {
   cudaEvent_t pending = nullptr;
   void* foreign = nullptr;  // the DLPack tensor that owns this memory, when it was taken over from another library
   Storage(RxDevice* d, void* p, size_t b) : dev(d), keep(d->shared_from_this()), ptr(p), bytes(b) {}
-  void make_ready() {  // call with the owning device current
+  bool make_ready() {  // call with the owning device current; whether there was anything to wait for
     std::lock_guard<std::mutex> g(pending_mu);
-    if (!pending) return;
+    if (!pending) return false;
     if (dev->stream) cudaStreamWaitEvent(dev->stream, pending, 0);
     dev->give_event(pending);
     pending = nullptr;
+    return true;
   }
   ~Storage() {
     if (pending && foreign) {

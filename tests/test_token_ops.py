@@ -325,19 +325,20 @@ def check_logprobs(got, want, x, temperature, top_k):
 @pytest.mark.gpu
 @pytest.mark.parametrize("et", ["f32", "bf16"])
 @pytest.mark.parametrize("pattern", ["equal", "rising", "falling", "two values", "zeros of both signs", "one finite", "nothing", "huge", "far apart", "lowest"])
-@pytest.mark.parametrize("vocab", [37, 250, 3001, 9001])
-def test_token_logprobs_patterns(rx, ref, client, pattern, vocab, et):
+@pytest.mark.parametrize("t,vocab", [(3, 37), (3, 250), (3, 600), (3, 3001), (3, 9001), (2400, 1500)])
+def test_token_logprobs_patterns(rx, ref, client, pattern, t, vocab, et):
     """Ties, orders that defeat a running threshold, rows that a mask empties, values at the ends of the range."""
-    t, lowest = 3, -3.3895313892515355e38  # the largest finite bf16
+    lowest = -3.3895313892515355e38  # the largest finite bf16
     rows = {"equal": np.full(vocab, 1.25), "rising": np.arange(vocab) * 0.125, "falling": np.arange(vocab) * -0.125, "two values": np.arange(vocab) % 2.0,
             "zeros of both signs": np.where(np.arange(vocab) % 3 == 0, 0.0, -0.0), "one finite": np.where(np.arange(vocab) == vocab - 2, -7.0, -np.inf), "nothing": np.full(vocab, -np.inf),
             "huge": np.where(np.arange(vocab) % 5 == 0, 1e30, -1e30), "far apart": np.arange(vocab) % 7 * 40.0, "lowest": np.where(np.arange(vocab) % 4 == 0, 1.0, lowest)}[pattern]
     x = np.broadcast_to(rows, (t, vocab)).astype(np.float32).astype(np_et(rx, et))
-    ids = np.array([0, vocab - 2, -1], np.int32)
+    ids = np.resize(np.array([0, vocab - 2, -1], np.int32), t)
     text = rx.programs.token_logprobs(t, vocab, et=et, top_k=20)
-    got, want = run(rx, client, text, [x, ids]), ref.run_module(text, [x.astype(np.float32), ids])
+    small = rx.programs.token_logprobs(3, vocab, et=et, top_k=20)  # all rows are alike
+    got, want = run(rx, client, text, [x, ids]), [np.resize(w, (t,) + w.shape[1:]) for w in ref.run_module(small, [x[:3].astype(np.float32), ids[:3]])]
     if pattern == "nothing":
-        assert (got[2] == -np.inf).all() and not got[1].any() and got[0].tolist() == [-np.inf, -np.inf, 0.0]
+        assert (got[2] == -np.inf).all() and not got[1].any() and np.array_equal(got[0], np.resize([-np.inf, -np.inf, 0.0], t))
         assert (got[3] == -np.inf).all() and (got[4] == np.arange(20)).all()
     else:
         check_logprobs(got, want, x, 1.0, 20)
@@ -345,14 +346,14 @@ def test_token_logprobs_patterns(rx, ref, client, pattern, vocab, et):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("bad", [np.nan, np.inf])
-@pytest.mark.parametrize("vocab", [40, 5000])
-def test_token_logprobs_not_finite(rx, ref, client, bad, vocab):
+@pytest.mark.parametrize("t,vocab", [(3, 40), (3, 300), (3, 5000), (2400, 1100)])
+def test_token_logprobs_not_finite(rx, ref, client, bad, t, vocab):
     """A row with a NaN or +inf has no probabilities; the rows around it are untouched; NaN ranks above everything."""
     rng = np.random.default_rng(7)
-    x = rng.standard_normal((3, vocab)).astype(np.float32)
+    x = rng.standard_normal((t, vocab)).astype(np.float32)
     x[1, vocab - 3] = bad
-    ids = np.array([1, 1, 1], np.int32)
-    text = rx.programs.token_logprobs(3, vocab, et="f32", top_k=4)
+    ids = np.ones(t, np.int32)
+    text = rx.programs.token_logprobs(t, vocab, et="f32", top_k=4)
     got, want = run(rx, client, text, [x, ids]), ref.run_module(text, [x, ids])
     assert np.isnan(got[0][1]) and np.isnan(got[1][1]) and np.isnan(got[2][1]) and np.isnan(got[3][1]).all()
     assert np.array_equal(got[4], want[4]) and got[4][1, 0] == vocab - 3
@@ -466,3 +467,125 @@ def test_embedding_grad_patterns(rx, ref, client, pattern, tokens, features):
     text = rx.programs.embedding_grad(vocab, features, tokens, et="f32")
     got, = run(rx, client, text, [dy, ids])
     assert np.array_equal(got, ref.run_module(text, [dy, ids])[0])
+
+
+@pytest.mark.gpu
+def test_empty_vocabulary(rx, client):
+    """Nothing to look up, nothing to choose from: rows of zeros, and rows without any probability."""
+    ids = np.array([0, -1, 3], np.int32)
+    got, = run(rx, client, rx.programs.embedding(0, 5, 3, et="f32"), [np.zeros((0, 5), np.float32), ids])
+    assert got.shape == (3, 5) and not got.any()
+    got, = run(rx, client, rx.programs.embedding_grad(0, 5, 3, et="f32"), [np.ones((3, 5), np.float32), ids])
+    assert got.shape == (0, 5)
+    lp, h, lse = run(rx, client, rx.programs.token_logprobs(3, 0, et="f32"), [np.zeros((3, 0), np.float32), ids])
+    assert not lp.any() and not h.any() and (lse == -np.inf).all()
+    z = np.zeros(3, np.float32)
+    got, = run(rx, client, rx.programs.token_logprobs_grad(3, 0, et="f32"), [np.zeros((3, 0), np.float32), ids, lse, h, z, z, z])
+    assert got.shape == (3, 0)
+
+
+def loop_module(n, trips, rate):
+    t = f"tensor<{n}xf32>"
+    return f"""module {{
+  func.func @main(%x: {t}, %key: tensor<2xi32>) -> {t} {{
+    %c0 = stablehlo.constant dense<0> : tensor<i64>
+    %c1 = stablehlo.constant dense<1> : tensor<i64>
+    %cn = stablehlo.constant dense<{trips}> : tensor<i64>
+    %one = stablehlo.constant dense<1.000000e+00> : {t}
+    %r:2 = stablehlo.while(%i = %c0, %a = %x) : tensor<i64>, {t}
+     cond {{
+      %p = stablehlo.compare LT, %i, %cn : (tensor<i64>, tensor<i64>) -> tensor<i1>
+      stablehlo.return %p : tensor<i1>
+    }} do {{
+      %n = stablehlo.add %i, %c1 : tensor<i64>
+      %b = stablehlo.add %a, %one : {t}
+      %d = stablehlo.custom_call @rx.dropout(%b, %key, %a) {{api_version = 4 : i32, backend_config = {{rate = {rate!r} : f64, site = 2 : i64}}}} : ({t}, tensor<2xi32>, {t}) -> {t}
+      stablehlo.return %n, %d : tensor<i64>, {t}
+    }}
+    return %r#1 : {t}
+  }}
+}}
+"""
+
+
+def test_calls_inside_a_loop_are_planned(rx):
+    d = rx.plan_describe(loop_module(100, 3, 0.25))
+    loop = next(s for s in d["steps"] if s["kind"] == "loop")
+    assert "dropout" in [s["kind"] for s in loop["body"]]
+
+
+@pytest.mark.gpu
+def test_calls_inside_a_loop(rx, ref, client):
+    x, key = np.arange(1000, dtype=np.float32), np.array([5, 6], np.int32)
+    for trips in (1, 2, 5):
+        text = loop_module(1000, trips, 0.25)
+        got, = run(rx, client, text, [x, key])
+        want = ref.run_module(text, [x, key])[0]
+        close(got, want, 8 * trips * U * np.abs(f64(want)))
+
+
+@pytest.mark.gpu
+def test_threads_share_a_device(rx, ref, client):
+    """Calls of several host threads at once, each with its own arrays, give what they give one after another."""
+    from concurrent.futures import ThreadPoolExecutor
+    rng = np.random.default_rng(13)
+    V, D, T = 5000, 72, 12000
+    text = rx.programs.embedding_grad(V, D, T, et="f32")
+    thunk = rx.compile(text, client)
+    sets = []
+    for _ in range(4):
+        dy, ids = rng.integers(-4, 5, (T, D)).astype(np.float32), some_ids(rng, T, V, "i32")
+        sets.append((rx.to_rarray(dy.T, client), rx.to_rarray(ids, client), ref.run_module(text, [dy, ids])[0]))
+
+    def work(k):
+        a, b, want = sets[k % 4]
+        return all(np.array_equal(np.asarray(thunk(a, b)).T, want) for _ in range(5))
+
+    with ThreadPoolExecutor(4) as pool:
+        assert all(pool.map(work, range(8)))
+
+
+@pytest.mark.gpu
+def test_offsets_beyond_32_bits(rx, client):
+    """More than 2^31 elements in the large operand or result: the last rows are what they are alone.  (Arrays are made on
+    the device and handed over; rows that are left out of the comparison are there for their addresses.)"""
+    torch = pytest.importorskip("torch")
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GB")
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(3)
+    cases = torch.device("cuda")
+    call = lambda text, *a: [torch.from_dlpack(o) for o in (lambda r: r if isinstance(r, tuple) else (r,))(rx.compile(text, client)(*[rx.from_dlpack(t.mT if t.dim() == 2 else t, client) for t in a]))]  # noqa: E731
+    same = lambda a, b: torch.equal(a.view(torch.int16) if a.dtype == torch.bfloat16 else a, b.view(torch.int16) if b.dtype == torch.bfloat16 else b)  # noqa: E731
+    T, V, tail = 16500, 131071, 700  # rows that do not start on 16 bytes
+    x = torch.randn(T, V, device=cases, dtype=torch.bfloat16, generator=gen)
+    ids = torch.randint(0, V, (T,), device=cases, generator=gen, dtype=torch.int32)
+    whole = call(rx.programs.token_logprobs(T, V, top_k=3), x, ids)
+    part = call(rx.programs.token_logprobs(tail, V, top_k=3), x[-tail:].clone(), ids[-tail:].clone())
+    for a, b in zip(whole, part):
+        a = a.mT if a.dim() == 2 else a
+        b = b.mT if b.dim() == 2 else b
+        if a.dtype == torch.int32:
+            assert torch.equal(a[-tail:], b)
+        else:
+            assert (a[-tail:] - b).abs().max() <= 64 * U * 16  # the two may be cut differently: 64 roundings of values up to 16
+    g = torch.randn(T, device=cases, generator=gen)
+    zero = torch.zeros_like(g)
+    grad = call(rx.programs.token_logprobs_grad(T, V), x, ids, whole[2], whole[1], g, zero, zero)[0].mT
+    want = call(rx.programs.token_logprobs_grad(tail, V), x[-tail:].clone(), ids[-tail:].clone(), whole[2][-tail:].clone(), whole[1][-tail:].clone(), g[-tail:].clone(), zero[-tail:].clone(), zero[-tail:].clone())[0].mT
+    assert same(grad[-tail:].contiguous(), want.contiguous())
+    # the same memory as activations to drop, and as a table
+    key = torch.tensor([7, 8], device=cases, dtype=torch.int32)
+    dropped = call(rx.programs.dropout((T, V), 0.5), x, key)[0].mT
+    n = 8 * 1000
+    flat = dropped.reshape(-1)[-n:].float()
+    kept = flat != 0
+    assert ((flat == 2 * x.reshape(-1)[-n:].float()) | ~kept).all() and 0.45 < kept.float().mean() < 0.55
+    del dropped, grad
+    looked = call(rx.programs.embedding(T, V, 40, scale=1.0), x, torch.arange(T - 40, T, device=cases, dtype=torch.int32))[0].mT
+    assert same(looked.contiguous(), x[-40:])
+    out = call(rx.programs.embedding(40, V, T), x[:40].clone(), (torch.arange(T, device=cases, dtype=torch.int32) % 40))[0].mT
+    assert same(out[-tail:].contiguous(), x[:40][(torch.arange(T, device=cases) % 40)[-tail:]])
+    del out
+    d = call(rx.programs.embedding_grad(T, V, 5, et="bf16", out_et="bf16"), x[:5].clone(), torch.tensor([T - 1, 0, T - 1, 77, -1], device=cases, dtype=torch.int32))[0].mT
+    assert same(d[T - 1].contiguous(), (x[0].float() + x[2].float()).to(torch.bfloat16)) and same(d[77].contiguous(), x[3]) and not d[-700:-1].any()
