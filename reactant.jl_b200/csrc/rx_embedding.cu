@@ -14,8 +14,11 @@ constexpr int kBlock = 256;
 //
 // Bound by memory: every distinct row is read, every row of the result written once.  The result is cut into units of
 // eight consecutive elements; a thread takes kUnits of them, a block apart, and asks for the ids and then the rows of
-// all of them before it stores.  Rows of the table and of the result start on 16 bytes, so a unit is a vector of one row.  65536 tokens of 2048 bf16 features: 72.9 us (one element a thread and a 64-bit division each: 361).
-constexpr int kUnits = 4;
+// all of them before it stores.  Rows of the table and of the result start on 16 bytes, so a unit is a vector of one row.
+// 65536 tokens of 2048 bf16 features out of 131072 rows: 71 us with two units a thread (one 88, four 73, eight 82; one
+// element a thread and a 64-bit division each 361), where the bytes alone need 54.  What is left is the way through L2:
+// with the whole table in there the same result takes 54.
+constexpr int kUnits = 2;
 
 template <class Id>
 __device__ __forceinline__ int64_t row_of(const Id* ids, int64_t t, int64_t vocab) {
