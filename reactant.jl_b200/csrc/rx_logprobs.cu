@@ -210,11 +210,28 @@ constexpr int kMaxLoose = 14;
 // 32 lanes and k <= 32, among the lanes' largest, which is one vote a bit.  Where that leaves too many (most of the row
 // is equal), it is searched for to the last bit, and then the last index that is still wanted among the elements equal
 // to it.  What is left, little more than k, is ordered by counting.
-constexpr int kNarrowRow = 256;
+constexpr int kNarrowRow = 256, kNarrowTopRow = 128;  // longest rows of eight lanes
 template <class T>
 struct GroupRow { static constexpr int n = sizeof(T) == 4 ? 1024 : 512; };  // 16-bit loads one by one: 200000 x 1000 bf16 takes 173 us here, 113 with a warp's vectors
 template <int W>
 struct GroupCap { static constexpr int n = W == 8 ? 2 * kMaxTopK + 8 : 4 * kMaxTopK; };
+
+// A bound from below on the k-th largest of the 32 lanes' keys (0: fewer lanes have one): for a small k the k-th itself,
+// largest by largest; otherwise its upper 16 bits, bit by bit with one vote each.
+__device__ __forceinline__ uint32_t bound_of_lanes(uint32_t key, int k) {
+  uint32_t bound = 0;
+  if (k <= 10) {
+    for (int left = k;;) {
+      bound = __reduce_max_sync(~0u, key);
+      left -= __popc(__ballot_sync(~0u, key == bound));
+      if (left <= 0 || bound == 0) return bound;
+      if (key == bound) key = 0;
+    }
+  }
+  for (uint32_t bit = 1u << 31; bit >= 1u << 16; bit >>= 1)
+    if (__popc(__ballot_sync(~0u, key >= (bound | bit))) >= k) bound |= bit;
+  return bound;
+}
 
 template <int W>
 __device__ __forceinline__ int lanes_count(int n) {
@@ -262,10 +279,7 @@ __global__ void __launch_bounds__(kBlock, NE == 32 ? (W == 8 ? 2 : 3) : 4) k_log
     int n = 0;
     bool done = false;
     if (W == 32 && top_k <= 32) {
-      const uint32_t best = lane < cols ? value_key(lane_top) : 0u;
-      uint32_t reach = 0;
-      for (uint32_t bit = 1u << 31; bit >= 1u << 16; bit >>= 1)
-        if (__popc(__ballot_sync(~0u, best >= (reach | bit))) >= top_k) reach |= bit;
+      const uint32_t reach = bound_of_lanes(lane < cols ? value_key(lane_top) : 0u, top_k);
       const float least = key_value((uint64_t)reach << 32);  // NaN, where there is no bound: nothing is below it
       done = true;
 #pragma unroll
@@ -391,10 +405,7 @@ __global__ void __launch_bounds__(kBlock) k_logprobs_warp(const T* __restrict__ 
   if (lane == 0) write_row(a, o, sp.x, ids, row, cols, out);
   if (TOP) {
     uint64_t *buf = buf_[warp], *best = best_[warp];
-    const uint32_t top_key = lane < vecs ? value_key(mine) : 0u, before = (1u << lane) - 1;
-    uint32_t reach = 0;
-    for (uint32_t bit = 1u << 31; bit >= 1u << 16; bit >>= 1)
-      if (__popc(__ballot_sync(~0u, top_key >= (reach | bit))) >= top_k) reach |= bit;
+    const uint32_t before = (1u << lane) - 1, reach = bound_of_lanes(lane < vecs ? value_key(mine) : 0u, top_k);
     // the same bound as a float: what is not below it is a candidate (NaN included; everything, where there is no bound)
     float least_value = key_value((uint64_t)reach << 32);
     int items = 0;
@@ -791,14 +802,23 @@ cudaError_t launch_logprobs(const LaunchCtx& c, const CallDesc& d, const void* l
     using T = std::remove_pointer_t<decltype(i)>;
     using Id = std::remove_pointer_t<decltype(id)>;
     if (d.cols <= GroupRow<T>::n) {
-      const int rows = kBlock / (d.cols <= kNarrowRow ? 8 : 32);
+      // with top tokens a warp a row pays earlier, its bound on the k-th costs so little (201615 x 203 f32, twelve: 214 us
+      // with eight lanes, 142 with 32; 500000 x 128, twenty: 280 and 323)
+      const bool wide = d.cols > (d.top_k && d.top_k <= 32 ? kNarrowTopRow : kNarrowRow);
+      const int rows = kBlock / (wide ? 32 : 8);
       const unsigned blocks = (unsigned)((d.rows + rows - 1) / rows);
       auto go = [&](auto* f) { f<<<blocks, kBlock, 0, c.stream>>>((const T*)logits, (const Id*)ids, d.rows, d.cols, d.ld, (float)d.scale, d.top_k, out); };
-      if (d.cols <= 64) go(d.top_k ? k_logprobs_group<T, Id, true, 8, 8> : k_logprobs_group<T, Id, false, 8, 8>);
-      else if (d.cols <= 128) go(d.top_k ? k_logprobs_group<T, Id, true, 8, 16> : k_logprobs_group<T, Id, false, 8, 16>);
-      else if (d.cols <= kNarrowRow) go(d.top_k ? k_logprobs_group<T, Id, true, 8, 32> : k_logprobs_group<T, Id, false, 8, 32>);
-      else if (d.cols <= 512 || sizeof(T) == 2) go(d.top_k ? k_logprobs_group<T, Id, true, 32, 16> : k_logprobs_group<T, Id, false, 32, 16>);
-      else if constexpr (sizeof(T) == 4) go(d.top_k ? k_logprobs_group<T, Id, true, 32, 32> : k_logprobs_group<T, Id, false, 32, 32>);
+      if (!wide) {
+        if (d.cols <= 64) go(d.top_k ? k_logprobs_group<T, Id, true, 8, 8> : k_logprobs_group<T, Id, false, 8, 8>);
+        else if (d.cols <= 128) go(d.top_k ? k_logprobs_group<T, Id, true, 8, 16> : k_logprobs_group<T, Id, false, 8, 16>);
+        else go(d.top_k ? k_logprobs_group<T, Id, true, 8, 32> : k_logprobs_group<T, Id, false, 8, 32>);
+      } else if (d.cols <= 256) {
+        go(k_logprobs_group<T, Id, true, 32, 8>);
+      } else if (d.cols <= 512 || sizeof(T) == 2) {
+        go(d.top_k ? k_logprobs_group<T, Id, true, 32, 16> : k_logprobs_group<T, Id, false, 32, 16>);
+      } else if constexpr (sizeof(T) == 4) {
+        go(d.top_k ? k_logprobs_group<T, Id, true, 32, 32> : k_logprobs_group<T, Id, false, 32, 32>);
+      }
       return;
     }
     if (d.cols <= kWarpRow && d.top_k <= kWarpTop && d.rows >= (int64_t)c.sm_count * kWarpRows * (d.cols > kWarpLong ? 2 : 1)) {
