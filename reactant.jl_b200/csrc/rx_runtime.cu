@@ -111,7 +111,10 @@ void* RxDevice::alloc(size_t bytes) {
       if (take == blocks.size()) goto fresh;
       void* p = blocks[take].p;
       if (blocks[take].busy) {
-        if (!passed) cudaStreamWaitEvent(stream, blocks[take].busy, 0);
+        if (!passed) {
+          cudaStreamWaitEvent(stream, blocks[take].busy, 0);
+          enqueued.fetch_add(1);  // whoever is handed this block next waits for that consumer too
+        }
         spare_events.push_back(blocks[take].busy);
       }
       blocks.erase(blocks.begin() + take);
@@ -1000,7 +1003,12 @@ void execute(RxExecutable* ex, const std::vector<RxDevice*>& devs, RxBuffer** ar
       }
     }
   }
-  for (RxDevice* d : order) d->enqueued.fetch_add(1);
+  // Counted when everything is queued, not before: an event that another thread records in between does not cover
+  // what is still to come.
+  struct Counted {
+    const std::vector<RxDevice*>& on;
+    ~Counted() { for (RxDevice* d : on) d->enqueued.fetch_add(1); }
+  } counted{order};
   run_steps(ex, p.steps, runs);
   // All-reduces still in flight on the communication stream: a result keeps the event (its future and its next user
   // wait for it), so the compute stream is free to start the next execution; anything else is joined now.

@@ -121,3 +121,35 @@ def test_donated_arrays_are_not_handed_out(rx, client):
     with pytest.raises(rx.ReactantError, match="donated"):
         old.__dlpack__()
     assert torch.from_dlpack(a).tolist() == [2.0] * 16
+
+
+def test_results_are_waited_for_while_another_thread_exports(rx, client):
+    """One thread takes its results to another stream while a second one keeps exporting an array of its own: what the
+    second thread waits for, recorded while the first one is still queueing work, must not pass for the first one's."""
+    import threading
+
+    n, steps = 1 << 24, 60
+    f = rx.compile(scale_module(n), client)
+    mine = rx.from_dlpack(torch.zeros(16, device="cuda"), client)
+    stop = threading.Event()
+
+    def export():
+        side = torch.cuda.Stream()
+        with torch.cuda.stream(side):
+            while not stop.is_set():
+                torch.from_dlpack(mine)
+
+    other = threading.Thread(target=export)
+    other.start()
+    try:
+        with torch.cuda.stream(torch.cuda.Stream()):
+            wrong = torch.zeros((), device="cuda", dtype=torch.int64)
+            for k in range(steps):
+                x = torch.full((n,), float(k + 1), device="cuda")
+                y = torch.from_dlpack(f(f(rx.from_dlpack(x, client))))
+                wrong += (y != 4.0 * (k + 1)).sum()
+            torch.cuda.current_stream().synchronize()
+    finally:
+        stop.set()
+        other.join()
+    assert wrong.item() == 0
