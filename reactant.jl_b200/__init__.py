@@ -419,7 +419,8 @@ def from_dlpack(x, client: Client | None = None, device: Device | None = None) -
     """An array of another library (a torch tensor, say) on one of this client's devices, as a ConcreteRArray over the
     same memory.  Its shape is the Julia shape, so its first dimension has to be the contiguous one: a row-major matrix
     is handed over as its transposed view.  The array has to be dense and start on a 16-byte boundary.  Work queued here
-    waits for what the producer's current stream holds; the memory goes back to its owner when the array is gone and
+    waits for what the producer's current stream holds (what is written to the memory later is waited for when it is handed
+    over again); the memory goes back to its owner when the array is gone and
     the work that uses it is done."""
     client = client or default_client()
     kind, ordinal = x.__dlpack_device__()
