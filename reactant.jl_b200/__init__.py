@@ -26,6 +26,7 @@ import ctypes as C
 import json
 import os
 import weakref
+from functools import cached_property
 
 import numpy as np
 
@@ -62,6 +63,11 @@ class Device:
     @property
     def local_id(self):
         return lib().PjRtDeviceGetLocalDeviceId(self.handle)
+
+    @cached_property
+    def dlpack(self):
+        """(kDLCUDA, ordinal): the device as the exchange of arrays names it."""
+        return (2, lib().PjRtDeviceGetLocalHardwareId(self.handle))
 
     @property
     def addressable(self):
@@ -317,7 +323,7 @@ class ConcreteRArray:
 
     # The array API's exchange of device arrays (DLPack): `torch.from_dlpack(y)` and the like see the same memory.
     def __dlpack_device__(self):
-        return (_DL_CUDA, lib().PjRtDeviceGetLocalHardwareId(self._single().device.handle))
+        return self._single().device.dlpack
 
     def __dlpack__(self, *, stream=None, max_version=None, dl_device=None, copy=None):
         """Hand the array out without a copy, in its Julia shape (first dimension contiguous).  `stream` is the consumer's
@@ -337,7 +343,6 @@ class ConcreteRArray:
 
 
 # DLPack capsules: the names and the rule that the consumer renames the capsule are the specification's.
-_DL_CUDA = 2
 _PyCapsule_New = C.pythonapi.PyCapsule_New
 _PyCapsule_New.restype, _PyCapsule_New.argtypes = C.py_object, [C.c_void_p, C.c_char_p, C.c_void_p]
 _PyCapsule_GetPointer = C.pythonapi.PyCapsule_GetPointer
@@ -423,11 +428,11 @@ def from_dlpack(x, client: Client | None = None, device: Device | None = None) -
     over again); the memory goes back to its owner when the array is gone and
     the work that uses it is done."""
     client = client or default_client()
-    kind, ordinal = x.__dlpack_device__()
     if device is None:
-        device = next((d for d in client.addressable_devices if kind == _DL_CUDA and lib().PjRtDeviceGetLocalHardwareId(d.handle) == ordinal), None)
+        where = tuple(int(v) for v in x.__dlpack_device__())
+        device = next((d for d in client.addressable_devices if d.dlpack == where), None)
         if device is None:
-            raise ReactantError(12, f"the array is on device ({int(kind)}, {ordinal}), which is not one of this client's")
+            raise ReactantError(12, f"the array is on device {where}, which is not one of this client's")
     capsule = x.__dlpack__(stream=lib().RxDeviceStream(device.handle))
     h = lib().RxBufferFromDLPack(device.handle, _PyCapsule_GetPointer(capsule, b"dltensor"))
     if not h:

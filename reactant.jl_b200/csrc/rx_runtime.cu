@@ -225,15 +225,67 @@ void RxDevice::hand_back(void* tensor) {
   {
     std::lock_guard<std::mutex> lk(mu);
     returned.push_back(r);
-    n_returned.store((int)returned.size());
+    n_returned.store((int)(returned.size() + parked.size()));
   }
   reap(false);
   cudaSetDevice(cur);
 }
 
+namespace {
+bool captured(cudaStream_t s) {  // into a graph; also when that cannot be told
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(s, &status) == cudaSuccess) return status != cudaStreamCaptureStatusNone;
+  cudaGetLastError();
+  return true;
+}
+
+// Memory of the pool is handed out again once the work queued so far has passed it; a graph would go on using it with
+// every replay.
+void not_captured(cudaStream_t s) {
+  if (captured(s)) throw Error(RX_ERR_ARG, "arrays cannot be exchanged, nor programs executed, on a stream that is being captured into a graph");
+}
+}  // namespace
+
+void RxDevice::leave_event(const std::shared_ptr<Storage>& st, cudaStream_t consumer) {  // this device is current
+  if (captured(consumer)) {
+    std::lock_guard<std::mutex> lk(mu);
+    parked.push_back({st, consumer});
+    n_returned.store((int)(returned.size() + parked.size()));
+    return;
+  }
+  cudaEvent_t ev = take_event();
+  if (!ev || cudaEventRecord(ev, consumer) != cudaSuccess) {
+    cudaGetLastError();  // the consumer's stream is gone: everything it had queued is waited for instead
+    if (ev) give_event(ev);
+    cudaDeviceSynchronize();
+    return;
+  }
+  std::lock_guard<std::mutex> g(st->pending_mu);
+  if (st->pending) {  // another consumer's, or an all-reduce's: the new event stands for both
+    cudaStreamWaitEvent(consumer, st->pending, 0);
+    cudaEventRecord(ev, consumer);
+    give_event(st->pending);
+  }
+  st->pending = ev;
+}
+
 void RxDevice::reap(bool all) {
   if (!n_returned.load()) return;
   std::vector<Returned> done;
+  std::vector<Parked> waiting;
+  {
+    std::lock_guard<std::mutex> lk(mu);
+    waiting.swap(parked);
+    n_returned.store((int)returned.size());
+  }
+  for (Parked& k : waiting) {  // a capture that goes on parks its memory again
+    int cur = 0;
+    cudaGetDevice(&cur);
+    if (cur != ordinal) cudaSetDevice(ordinal);
+    if (!all) leave_event(k.st, k.consumer);
+    k.st.reset();
+    if (cur != ordinal) cudaSetDevice(cur);
+  }
   {
     std::lock_guard<std::mutex> lk(mu);
     size_t kept = 0;
@@ -242,7 +294,7 @@ void RxDevice::reap(bool all) {
       else returned[kept++] = r;
     }
     returned.resize(kept);
-    n_returned.store((int)kept);
+    n_returned.store((int)(kept + parked.size()));
   }
   cudaGetLastError();  // "not ready" is no error
   for (auto& r : done) {  // outside the lock: the owner's code runs here
@@ -955,6 +1007,7 @@ void execute(RxExecutable* ex, const std::vector<RxDevice*>& devs, RxBuffer** ar
   for (RxDevice* d : order) {
     d->reap(false);
     held.emplace_back(d->exec_mu);
+    not_captured(d->stream);
   }
   std::vector<DevRun> runs(devs.size());
   for (size_t k = 0; k < devs.size(); ++k) {
@@ -1380,20 +1433,7 @@ void handed_out_deleter(rx::DLManagedTensor* t) {
   int cur = 0;
   cudaGetDevice(&cur);
   if (cur != d->ordinal) cudaSetDevice(d->ordinal);
-  cudaEvent_t ev = d->take_event();
-  if (!ev || cudaEventRecord(ev, h->consumer) != cudaSuccess) {
-    cudaGetLastError();  // the consumer's stream is gone: everything it had queued is waited for instead
-    if (ev) d->give_event(ev);
-    cudaDeviceSynchronize();
-  } else {
-    std::lock_guard<std::mutex> g(h->st->pending_mu);
-    if (h->st->pending) {  // another consumer's, or an all-reduce's: the new event stands for both
-      cudaStreamWaitEvent(h->consumer, h->st->pending, 0);
-      cudaEventRecord(ev, h->consumer);
-      d->give_event(h->st->pending);
-    }
-    h->st->pending = ev;
-  }
+  d->leave_event(h->st, h->consumer);
   h.reset();
   if (cur != d->ordinal) cudaSetDevice(cur);
 }
@@ -1422,15 +1462,23 @@ void* RxBufferToDLPack(RxBuffer* b, void* consumer_stream) {
     int cur = 0;
     cudaGetDevice(&cur);
     if (cur != d->ordinal) CK(cudaSetDevice(d->ordinal));
-    const bool late = b->st->make_ready();
+    not_captured(h->consumer);
+    unsigned long long id = 0;  // unlike the handle, never given to another stream
+    CK(cudaStreamGetId(h->consumer, &id));
+    b->st->make_ready();
     std::lock_guard<std::mutex> g(d->order_mu);
     if (!d->order) CK(cudaEventCreateWithFlags(&d->order, cudaEventDisableTiming));
     const uint64_t now = d->enqueued.load();
-    if (now != d->ordered || late) {
+    if (now != d->ordered) {
       CK(cudaEventRecord(d->order, d->stream));
       d->ordered = now;
+      d->waited = 0;
     }
-    CK(cudaStreamWaitEvent(h->consumer, d->order, 0));
+    if (d->waited != now || d->waited_id != id) {  // the results of one call: the first one's wait covers the others
+      CK(cudaStreamWaitEvent(h->consumer, d->order, 0));
+      d->waited = now;
+      d->waited_id = id;
+    }
     if (cur != d->ordinal) CK(cudaSetDevice(cur));
   }
   // the Julia view of the array: dims reversed, first dim contiguous
@@ -1454,6 +1502,7 @@ RxBuffer* RxBufferFromDLPack(RxDevice* d, void* tensor) {
   if (!d || !d->addressable) throw Error(RX_ERR_BAD_HANDLE, "device is null or not addressable from this process");
   if (!tensor) throw Error(RX_ERR_BAD_HANDLE, "null tensor");
   const rx::DLTensor& t = ((rx::DLManagedTensor*)tensor)->dl_tensor;
+  not_captured(d->stream);  // a producer that is being captured has drawn it into its graph
   if (t.device.device_type != rx::kDLCUDA || t.device.device_id != d->ordinal)
     throw Error(RX_ERR_ARG, "the array is not in the memory of CUDA device " + std::to_string(d->ordinal));
   DT dt = DT::INVALID;

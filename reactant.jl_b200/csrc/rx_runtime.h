@@ -34,6 +34,7 @@ struct MailTable {
   unsigned long long* peer[kMaxRanks];
 };
 
+struct Storage;
 struct RxDevice : std::enable_shared_from_this<RxDevice> {
   RxClient* client = nullptr;
   std::atomic<bool> closed{false};  // client freed: late buffer finalizers free straight to the driver
@@ -84,13 +85,20 @@ struct RxDevice : std::enable_shared_from_this<RxDevice> {
   struct Returned { void* tensor; cudaEvent_t done; };
   std::vector<Returned> returned;          // guarded by mu
   std::atomic<int> n_returned{0};
-  std::mutex order_mu;                     // guards the next two
+  // Memory whose consumer's stream was being captured into a graph when the consumer let go of it: no event can be
+  // recorded there until the capture has ended, and the memory stays out of use that long.
+  struct Parked { std::shared_ptr<Storage> st; cudaStream_t consumer; };
+  std::vector<Parked> parked;              // guarded by mu
+  std::mutex order_mu;                     // guards the next four
   cudaEvent_t order = nullptr;             // recorded on `stream` when a consumer needs to wait for it and executions were queued since the last time
   uint64_t ordered = 0;                    // value of `enqueued` then
-  std::atomic<uint64_t> enqueued{1};       // executions queued so far
+  uint64_t waited = 0;                     // the value of `ordered` that the stream with the following id has waited for last
+  unsigned long long waited_id = 0;
+  std::atomic<uint64_t> enqueued{1};       // executions, and waits for other streams, queued so far
   std::vector<cudaEvent_t> spare_events;   // guarded by mu; without timing, like every event that takes part here
   cudaEvent_t take_event();                // null, with the error cleared, when none can be made
   void give_event(cudaEvent_t e);
+  void leave_event(const std::shared_ptr<Storage>& st, cudaStream_t consumer);  // what `consumer` holds so far may still use the memory
   void hand_back(void* tensor);            // memory taken over is no longer used by anything that will be queued
   void reap(bool all);                     // owners whose memory is free now get it back
 
@@ -124,13 +132,13 @@ struct Storage {
   cudaEvent_t pending = nullptr;
   void* foreign = nullptr;  // the DLPack tensor that owns this memory, when it was taken over from another library
   Storage(RxDevice* d, void* p, size_t b) : dev(d), keep(d->shared_from_this()), ptr(p), bytes(b) {}
-  bool make_ready() {  // call with the owning device current; whether there was anything to wait for
+  void make_ready() {  // call with the owning device current
     std::lock_guard<std::mutex> g(pending_mu);
-    if (!pending) return false;
+    if (!pending) return;
     if (dev->stream) cudaStreamWaitEvent(dev->stream, pending, 0);
+    dev->enqueued.fetch_add(1);  // whoever waits for this device from now on waits for that too
     dev->give_event(pending);
     pending = nullptr;
-    return true;
   }
   ~Storage() {
     if (pending && foreign) {

@@ -153,3 +153,92 @@ def test_results_are_waited_for_while_another_thread_exports(rx, client):
         stop.set()
         other.join()
     assert wrong.item() == 0
+
+
+CAPTURE = """
+import gc, torch
+import __graft_entry__ as entry
+rx = entry.load_package()
+client = rx.default_client()
+n = 1 << 16
+f = rx.compile('''{module}''', client)
+x = torch.ones(n, device="cuda")
+a = rx.from_dlpack(x, client)
+side = torch.cuda.Stream()
+with torch.cuda.stream(side):
+    y = torch.from_dlpack(f(a))
+side.synchronize()
+
+
+def refused(act):
+    try:
+        act()
+    except rx.ReactantError as e:
+        assert "captured" in str(e), e
+        return
+    raise AssertionError("not refused")
+
+
+# in order: a consumer that is being captured; a result let go of on a stream that is being captured; a producer that is
+stream = torch.cuda.Stream()
+z = f(a)
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+w = torch.zeros(n, device="cuda")
+with torch.cuda.stream(stream):
+    g.capture_begin()
+    refused(lambda: torch.from_dlpack(z))
+    w += 1
+    g.capture_end()
+g.replay()
+torch.cuda.synchronize()
+assert (w == 1).all()
+
+where = y.data_ptr()
+with torch.cuda.stream(side):
+    g2 = torch.cuda.CUDAGraph()
+    g2.capture_begin()
+    w += 1
+    del y
+    gc.collect()
+    w += 1
+    g2.capture_end()
+g2.replay()
+torch.cuda.synchronize()
+assert (w == 3).all()
+for _ in range(4):
+    got = torch.from_dlpack(f(a))
+    torch.cuda.synchronize()
+    assert (got == 2).all()
+
+with torch.cuda.stream(stream):
+    g3 = torch.cuda.CUDAGraph()
+    g3.capture_begin()
+    refused(lambda: rx.from_dlpack(x, client))
+    refused(lambda: f(a))
+    try:
+        g3.capture_end()
+    except RuntimeError:
+        pass  # a stream that was drawn into the graph never came back to it
+torch.cuda.synchronize()
+for _ in range(4):
+    got = torch.from_dlpack(f(a))
+    torch.cuda.synchronize()
+    assert (got == 2).all()
+print("fine")
+"""
+
+
+def test_streams_under_capture_are_refused(tmp_path):
+    """Exchanging with, or executing on, a stream that is being captured into a graph is an error, and the device goes on
+    working afterwards.  In a process of its own: the last capture ends in an error of torch's."""
+    import os
+    import subprocess
+    import sys
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    script = tmp_path / "capture.py"
+    script.write_text(CAPTURE.replace("{module}", scale_module(1 << 16)))
+    env = dict(os.environ, PYTHONPATH=root)
+    r = subprocess.run([sys.executable, str(script)], cwd=root, env=env, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.strip().endswith("fine"), r.stdout + r.stderr
