@@ -31,7 +31,7 @@ from functools import cached_property
 import numpy as np
 
 from . import _lib, dist
-from ._lib import ReactantError, lib, check, take_string
+from ._lib import ReactantError, _call, lib, check, take_string
 
 try:
     import ml_dtypes
@@ -246,15 +246,10 @@ class NamedSharding:
 # ----------------------------------------------------------------------------
 # buffers and arrays  (src/Types.jl:155-263, src/ConcreteRArray.jl)
 # ----------------------------------------------------------------------------
-class _Buffer:
-    __slots__ = ("handle", "device", "_free", "__weakref__")
+class _Buffer(_call.Buffer):
+    """_Buffer(handle, device): freed with the object."""
 
-    def __init__(self, handle, device: Device):
-        self.handle, self.device, self._free = handle, device, lib().PjRtBufferFree
-
-    def __del__(self):
-        # (a weakref.finalize would do the same at several times the cost, on every result of every call)
-        self._free(self.handle)
+    __slots__ = ()
 
     @property
     def dims(self):
@@ -294,13 +289,6 @@ class ConcreteRArray:
         self.sharding = sharding
         self.replicated = replicated
 
-    @classmethod
-    def _of(cls, data, shape, dtype):
-        """An unsharded array from what is known to be in order already."""
-        a = cls.__new__(cls)
-        a.data, a.shape, a.dtype, a.sharding, a.replicated = data, shape, dtype, None, False
-        return a
-
     @property
     def ndim(self):
         return len(self.shape)
@@ -331,42 +319,12 @@ class ConcreteRArray:
         if copy or dl_device is not None and tuple(dl_device) != self.__dlpack_device__():
             raise BufferError("the array can only be handed out as it is, on its own device")
         buf = self.data[0] if len(self.data) == 1 and self.sharding is None else self._single()
-        p = lib().RxBufferToDLPack(buf.handle, (1 if stream is None else stream) & 0xFFFFFFFFFFFFFFFF)
-        if not p:
-            check()
-        return _PyCapsule_New(p, b"dltensor", _dl_drop)
+        return _call.hand_out(buf, 1 if stream is None else stream)
 
     def _single(self) -> "_Buffer":
         if len(self.data) != 1 or (self.sharding is not None and not self.replicated and self.sharding.sharded_dim() is not None):
             raise BufferError("an array spread over several devices has no single memory to exchange")
         return self.data[0]
-
-
-# DLPack capsules: the names and the rule that the consumer renames the capsule are the specification's.
-_PyCapsule_New = C.pythonapi.PyCapsule_New
-_PyCapsule_New.restype, _PyCapsule_New.argtypes = C.py_object, [C.c_void_p, C.c_char_p, C.c_void_p]
-_PyCapsule_GetPointer = C.pythonapi.PyCapsule_GetPointer
-_PyCapsule_GetPointer.restype, _PyCapsule_GetPointer.argtypes = C.c_void_p, [C.py_object, C.c_char_p]
-_PyCapsule_SetName = C.pythonapi.PyCapsule_SetName
-_PyCapsule_SetName.restype, _PyCapsule_SetName.argtypes = C.c_int, [C.py_object, C.c_char_p]
-_DL_USED = b"used_dltensor"
-
-
-_capsules = C.PyDLL(None)  # its own function objects: a capsule that is being destroyed is only an address
-_capsules.PyCapsule_IsValid.argtypes = _capsules.PyCapsule_GetPointer.argtypes = [C.c_void_p, C.c_char_p]
-_capsules.PyCapsule_GetPointer.restype = C.c_void_p
-
-
-@C.CFUNCTYPE(None, C.c_void_p)
-def _dl_drop_unused(capsule):
-    # a capsule that nobody consumed still owns its tensor, whose last field (after the 48 bytes of the tensor's
-    # description and the context) is its deleter
-    if _capsules.PyCapsule_IsValid(capsule, b"dltensor"):
-        tensor = _capsules.PyCapsule_GetPointer(capsule, b"dltensor")
-        C.CFUNCTYPE(None, C.c_void_p)(C.c_void_p.from_address(tensor + 56).value)(tensor)
-
-
-_dl_drop = C.cast(_dl_drop_unused, C.c_void_p)
 
 
 class ConcreteRNumber(ConcreteRArray):
@@ -434,11 +392,7 @@ def from_dlpack(x, client: Client | None = None, device: Device | None = None) -
         if device is None:
             raise ReactantError(12, f"the array is on device {where}, which is not one of this client's")
     capsule = x.__dlpack__(stream=lib().RxDeviceStream(device.handle))
-    h = lib().RxBufferFromDLPack(device.handle, _PyCapsule_GetPointer(capsule, b"dltensor"))
-    if not h:
-        check()
-    _PyCapsule_SetName(capsule, _DL_USED)
-    buf = _Buffer(h, device)
+    buf = _Buffer(_call.take_over(device.handle, capsule), device)
     dims = buf.dims
     cls = ConcreteRNumber if not dims else ConcreteRArray
     return cls([buf], tuple(reversed(dims)), buf.dtype)
@@ -470,30 +424,28 @@ class Thunk:
         self.param_sharded_dim = [l.RxExecutableParameterShardedDim(handle, i) for i in range(self.num_parameters)]
         self.result_sharded_dim = [l.RxExecutableResultShardedDim(handle, i) for i in range(self.num_results)]
         self.param_alias = [l.RxExecutableParameterAlias(handle, i) for i in range(self.num_parameters)]
-        self._execute, self._error_code = l.XLAExecuteSharded, l.RxLastErrorCode
         self._aliased = any(k >= 0 for k in self.param_alias)
-        self._args_t = C.c_void_p * max(1, self.num_parameters)
-        self._outs_t = C.c_void_p * max(1, self.num_results)
-        mask_t = C.c_uint8 * max(1, self.num_parameters)
-        self._masks = (mask_t(), mask_t(*[int(a >= 0) for a in self.param_alias]))
-        self._result_info = None  # (class, shape, dtype) of each result, known from the first call on
+        self._single = _call.Call(handle, self.num_parameters, self.num_results, bytes(self.num_parameters), bytes(int(a >= 0) for a in self.param_alias), _Buffer,
+                                  client.addressable_devices[0]) if self.num_partitions == 1 else None
 
     def _call_single(self, args, donate):
-        """The call on one device without waiting: no futures, and the results' shapes are looked up once."""
-        dev = args[0].data[0].device if args else self.client.addressable_devices[0]
-        out = self._outs_t()
-        self._execute(self.handle, len(args), self._args_t(*[a.data[0].handle for a in args]), dev.handle, self._masks[1 if donate else 0], self.num_results, out, None, None)
-        if self._error_code():
-            check()
-        bufs = [_Buffer(h, dev) for h in out[:self.num_results]]
-        if self._result_info is None:
-            self._result_info = [(ConcreteRArray if b.dims else ConcreteRNumber, tuple(reversed(b.dims)), b.dtype) for b in bufs]
-        results = tuple(cls._of([b], shape, dtype) for b, (cls, shape, dtype) in zip(bufs, self._result_info))
+        """The call on one device without waiting: no futures, and the results' shapes are looked up once.  None if an
+        argument is spread over several devices."""
+        r = self._single.run(args, donate)
+        if r is None:
+            return None
+        if self._single.results is None:
+            infos = tuple((ConcreteRArray if b.dims else ConcreteRNumber, tuple(reversed(b.dims)), np.dtype(b.dtype)) for b in r)
+            r = tuple(cls([b], shape, dtype) for b, (cls, shape, dtype) in zip(r, infos))
+            self._single.results = infos
+            if len(r) == 1:
+                r = r[0]
         if donate and self._aliased:
+            results = r if isinstance(r, tuple) else (r,)
             for a, k in zip(args, self.param_alias):
                 if 0 <= k < len(results):
                     a.data = results[k].data
-        return results[0] if len(results) == 1 else results
+        return r
 
     def describe(self) -> dict:
         return json.loads(take_string(lib().RxExecutableDescribe(self.handle)))
@@ -503,12 +455,13 @@ class Thunk:
         storage becomes the aliased result's) and, as Reactant does for mutated
         arguments (src/compiler/Codegen.jl:1116-1170), the argument objects are
         re-pointed at the new buffers, so `A` stays usable after `f(A, B)`."""
-        l = lib()
         if len(args) != self.num_parameters:
             raise ReactantError(12, f"thunk takes {self.num_parameters} arguments, got {len(args)}")
-        sharded = self.num_partitions > 1
-        if not sharded and not self.sync and all(len(a.data) == 1 for a in args):
-            return self._call_single(args, donate)
+        l, sharded = lib(), self.num_partitions > 1
+        if not sharded and not self.sync:
+            r = self._call_single(args, donate)
+            if r is not None:
+                return r
         ndev = len(self.client.addressable_devices) if sharded else 1
         for a in args:
             if len(a.data) != ndev:

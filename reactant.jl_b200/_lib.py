@@ -9,6 +9,11 @@ from __future__ import annotations
 import ctypes as C
 import os
 
+try:
+    from . import _call  # csrc/rx_python.cpp
+except ImportError as e:
+    raise ImportError(f"the extension module of the call path is missing: build it with `python reactant.jl_b200/build.py` ({e})") from e
+
 HERE = os.path.dirname(os.path.abspath(__file__))
 # RX_B200_LIB selects another build of the library (the bounds-checked one, say); the default is the in-tree build
 LIB_PATH = os.environ.get("RX_B200_LIB") or os.path.join(HERE, "librx_b200.so")
@@ -159,6 +164,7 @@ def lib():
             fn = getattr(_lib, name)
             fn.restype = res
             fn.argtypes = args
+        _call.bind(*(C.cast(getattr(_lib, n), C.c_void_p).value for n in ("XLAExecuteSharded", "RxLastErrorCode", "PjRtBufferFree", "RxBufferToDLPack", "RxBufferFromDLPack")), check)
     return _lib
 
 

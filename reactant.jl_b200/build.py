@@ -1,4 +1,4 @@
-"""Builds librx_b200.so (sm_100a) in-tree with nvcc.
+"""Builds librx_b200.so (sm_100a) in-tree with nvcc, and the extension module _call.so with the host compiler.
 
 Run as `python reactant.jl_b200/build.py`; `__graft_entry__.build()` calls
 `build()` below.  Objects are rebuilt only when a source or header is newer.
@@ -8,6 +8,7 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -59,6 +60,21 @@ def write_embedded_headers() -> None:
             f.write(new)
 
 
+def build_call(verbose: bool = False) -> str:
+    """_call.so: the extension module of the Python package's call path.  It links against nothing: _lib.py hands it the
+    library's entry points."""
+    src, out = os.path.join(CSRC, "rx_python.cpp"), os.path.join(HERE, "_call.so")
+    if _stale(out, [src, os.path.join(CSRC, "rx_dlpack.h"), os.path.join(HERE, "..", "include", "rx_b200.h")]):
+        cmd = [os.environ.get("CXX", "g++"), "-std=c++17", "-O2", "-Wall", "-Wno-missing-field-initializers", "-shared", "-fPIC", "-fvisibility=hidden", "-I", sysconfig.get_paths()["include"],
+               src, "-o", out]
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        if verbose or r.returncode:
+            sys.stderr.write(" ".join(cmd) + "\n" + r.stdout + r.stderr)
+        if r.returncode:
+            raise RuntimeError("failed: " + " ".join(cmd))
+    return out
+
+
 def build(verbose: bool = False, ptxas_info: bool = False, bounds: bool = False) -> str:
     """bounds=True builds librx_b200_bounds.so instead: the same library with -DRX_BOUNDS=1 (every element access of
     the chain kernels, the fused GEMM epilogues and the stencil stores checked against its buffer; select it with
@@ -99,6 +115,7 @@ def build(verbose: bool = False, ptxas_info: bool = False, bounds: bool = False)
         run(link)
     if ptxas_info:
         sys.stderr.write("\n".join(logs))
+    build_call(verbose)
     return out_path
 
 
