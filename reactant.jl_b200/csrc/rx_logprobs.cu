@@ -834,13 +834,25 @@ cudaError_t launch_logprobs(const LaunchCtx& c, const CallDesc& d, const void* l
       f<<<blocks, kBlock, 0, c.stream>>>((const T*)logits, (const Id*)ids, d.rows, d.cols, d.ld, (float)d.scale, d.top_k, out);
       return;
     }
-    // few rows: the blocks of a cluster share each, as long as that leaves a block two tiles, and blocks are large while
-    // there are fewer of them than SMs (4 x 131072 bf16: 9.9 us with blocks of 512, 12.6 with
-    // 128, between two events)
+    // Up to one row for every SM, blocks of 512, one to an SM, and as many to a row as the SMs allow (clusters of eight do
+    // not pack on more than half of them); beyond that blocks of 128, about six to an SM.  A block has at least one tile
+    // of its row, or two.  131072 bf16, twenty top tokens, us, with blocks of 512 by 1, 2, 4 and 8 a row [of 128]:
+    //   16 rows   14.6 12.6 10.6 16.7  [27.0 18.8 14.7 16.7]
+    //   64        15.1 12.7 20.8 34.7  [32.9 21.2 16.7 18.7]
+    //   148       16.4 23.3 41.3 65.9  [34.3 23.6 22.6 30.9]
+    //   200       27.4 33.1 53.1 86.0  [37.8 25.4 24.9 35.3]
+    //   512       52.0 74.0  122  204  [46.4 41.1 51.8 71.5]
+    //   1024      90.3  144  235  399  [68.3 72.2 88.4  128]
     auto go = [&](auto size) {
       constexpr int kLong = decltype(size)::value;
+      const int64_t sms = c.sm_count;
+      auto fits = [&](int ranks) {
+        if (d.cols < (int64_t)ranks * (kLong == 128 ? 2 : 1) * kLong * Fly<T>::n * 8) return false;
+        if (kLong != 128) return d.rows * ranks <= (ranks == 8 ? sms / 2 : sms);
+        return d.rows * ranks <= sms * (ranks == 2 ? 7 : ranks == 4 ? 6 : 0);
+      };
       int ranks = 1;
-      while (ranks < kMaxRanksPerRow && d.rows * ranks < (int64_t)c.sm_count * 8 && d.cols / (ranks * 2) >= (kLong == 128 ? 2 : 1) * kLong * Fly<T>::n * 8) ranks *= 2;
+      while (ranks < kMaxRanksPerRow && fits(ranks * 2)) ranks *= 2;
       cudaLaunchConfig_t cfg = {};
       cfg.gridDim = dim3((unsigned)(d.rows * ranks));
       cfg.blockDim = dim3(kLong);
@@ -854,7 +866,7 @@ cudaError_t launch_logprobs(const LaunchCtx& c, const CallDesc& d, const void* l
       auto* f = d.top_k ? k_logprobs_block<T, Id, true, kLong> : k_logprobs_block<T, Id, false, kLong>;
       err = cudaLaunchKernelEx(&cfg, f, (const T*)logits, (const Id*)ids, d.cols, d.ld, (float)d.scale, d.top_k, out);
     };
-    if (d.rows * kMaxRanksPerRow <= c.sm_count) go(std::integral_constant<int, 512>());
+    if (d.rows <= c.sm_count) go(std::integral_constant<int, 512>());
     else go(std::integral_constant<int, 128>());
   });
   ++*c.launches;
