@@ -470,6 +470,51 @@ def test_embedding_grad_patterns(rx, ref, client, pattern, tokens, features):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("et", ["f32", "bf16"])
+@pytest.mark.parametrize("pattern", ["random", "equal", "rising", "falling", "one finite", "lowest"])
+@pytest.mark.parametrize("t,vocab", [(2, 131079), (30, 65543), (70, 33001), (148, 16411), (149, 33001), (290, 17000)])
+def test_token_logprobs_of_few_rows(rx, ref, client, pattern, t, vocab, et):
+    """Rows that one, two, four or eight blocks share, with the top tokens anywhere among them."""
+    rng = np.random.default_rng(21)
+    i = np.arange(vocab)
+    rows = {"random": rng.standard_normal(vocab) * 3, "equal": np.full(vocab, 1.25), "rising": i * 2.0 ** -6, "falling": i * -2.0 ** -6,
+            "one finite": np.where(i == vocab - 2, -7.0, -np.inf), "lowest": np.where(i > vocab - 30, 1.0, -3.3895313892515355e38)}[pattern]
+    x = np.broadcast_to(rows, (t, vocab)).astype(np.float32).astype(np_et(rx, et))
+    ids = np.resize(np.array([0, vocab - 2, -1], np.int32), t)
+    n = min(t, 3)  # all rows are alike, and three of them have all the ids
+    for top_k in (0, 1, 24, 25, 64):
+        got = run(rx, client, rx.programs.token_logprobs(t, vocab, et=et, top_k=top_k), [x, ids])
+        small = rx.programs.token_logprobs(n, vocab, et=et, top_k=top_k)
+        want = ref.run_module(small, [x[:n].astype(np.float32), ids[:n]])
+        z = f64(x[:n])
+        bounds = logprob_bounds(z, z.max(-1), f64(want[1]))
+        want, (b_lse, b_ent, b_lp) = [np.resize(w, (t,) + w.shape[1:]) for w in want], [np.resize(b, t) for b in bounds]
+        close(got[2], want[2], b_lse, "lse")
+        close(got[1], want[1], b_ent, "entropy")
+        close(got[0], want[0], b_lp, "logprob")
+        if top_k:
+            assert np.array_equal(got[4], want[4])
+            close(got[3], want[3], b_lp[..., None], "top")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("features,et,out_et", [(257, "f32", "f32"), (512, "f32", "f32"), (1024, "bf16", "bf16"), (1001, "bf16", "f32")])
+@pytest.mark.parametrize("tokens", [1, 2, 31, 32, 33, 64, 65, 700, 1023, 1024, 1025])
+def test_embedding_grad_of_few_tokens(rx, ref, client, tokens, features, et, out_et):
+    """Rows are found among the sorted tokens: first, last, repeated and absent ones, at every length of the list's pieces."""
+    vocab = 2003
+    rng = np.random.default_rng(22)
+    for ids in (rng.integers(-1, vocab + 1, tokens), np.full(tokens, vocab - 1), np.zeros(tokens), np.arange(tokens) * 2, np.where(np.arange(tokens) % 2, 5, vocab), np.full(tokens, -1)):
+        ids = ids.astype(np.int32)
+        dy = rng.integers(-2, 3, (tokens, features)).astype(np.float32).astype(np_et(rx, et))
+        if out_et == "bf16":
+            dy[1:] = 0  # sums stay exact in the result's type
+        text = rx.programs.embedding_grad(vocab, features, tokens, et=et, out_et=out_et)
+        got, = run(rx, client, text, [dy, ids])
+        assert np.array_equal(f64(got), f64(ref.run_module(text, [dy.astype(np.float32), ids])[0]))
+
+
+@pytest.mark.gpu
 def test_empty_vocabulary(rx, client):
     """Nothing to look up, nothing to choose from: rows of zeros, and rows without any probability."""
     ids = np.array([0, -1, 3], np.int32)
