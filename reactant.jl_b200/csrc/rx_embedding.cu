@@ -413,13 +413,14 @@ __device__ __forceinline__ void fill_rows(const GradArgs& g, Out* out, int64_t b
   }
 }
 
-// A thread has eight consecutive columns.  VEC: rows of dy and of the result start on 16 bytes.  Otherwise a row is read
-// as the 16-byte lines that hold the columns, and the columns of a finished run change places within the warp, through
-// shared memory, so that they are written side by side.
-template <class In, class Out, bool VEC>
-__global__ void __launch_bounds__(kBlock, VEC ? 1 : 3) k_sum_runs(const In* __restrict__ dy, const In* end, Out* __restrict__ out, const __grid_constant__ GradArgs g) {
+// A thread has eight columns, STEP apart.  1: rows of dy and of the result start on 16 bytes, and the columns are vectors.
+// Otherwise STEP is a warp's width (or that of the threads that share a chunk, if fewer) and they are read and written one by
+// one, side by side with the neighbours' (22288 tokens, 1339 x 521 f32: the call 44 us; read as the 16-byte lines that hold eight
+// consecutive ones, and turned through shared memory to be written, 78).
+template <class In, class Out, int STEP>
+__global__ void __launch_bounds__(kBlock, STEP == 1 ? 1 : 4) k_sum_runs(const In* __restrict__ dy, Out* __restrict__ out, const __grid_constant__ GradArgs g) {
+  constexpr bool VEC = STEP == 1;
   __shared__ int32_t skey[kMaxPlaces + 2 * kMaxChunk + 2], spos[kMaxPlaces + kMaxChunk];
-  __shared__ float turn[VEC ? 1 : kBlock / 32][VEC ? 1 : 32 * 9];
   pdl_wait();
   pdl_release();
   if (blockIdx.x >= g.chunk_blocks * g.slices) {
@@ -439,9 +440,9 @@ __global__ void __launch_bounds__(kBlock, VEC ? 1 : 3) k_sum_runs(const In* __re
   const int lane = threadIdx.x & (g.lanes - 1), group = threadIdx.x >> g.log_lanes;
   const int64_t chunk = block * groups + group;
   const int32_t *key = skey + g.chunk + 1 + group * g.chunk, *pos = spos + group * g.chunk;
-  const int64_t c0 = (slice * g.lanes + lane) * 8;
-  // threads without columns, or without a chunk, stay: the others of their warp exchange columns with them
-  const bool mine = c0 < g.cols && chunk < g.chunks;
+  const int64_t c0 = (slice * g.lanes + (VEC ? lane : lane / STEP * STEP)) * 8 + (VEC ? 0 : lane % STEP);
+  if (chunk >= g.chunks || c0 >= g.cols) return;
+  const int live = (int)min((g.cols - c0 + STEP - 1) / STEP, (int64_t)8);  // columns
   float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   if (key[0] >= g.vocab) return;  // nothing but tokens outside the table, or no chunk at all: a whole group
   // The run that enters belongs to the chunk in front if it begins there and ends here: it is passed over.  The run
@@ -463,47 +464,43 @@ __global__ void __launch_bounds__(kBlock, VEC ? 1 : 3) k_sum_runs(const In* __re
   if (now >= g.vocab) return;
   auto flush = [&](bool to_part) {
     if (enters || to_part) {
-      if (!mine) return;
       float* p = g.part + (chunk * 2 + (enters ? 0 : 1)) * g.pitch + c0;
-      *(float4*)p = make_float4(acc[0], acc[1], acc[2], acc[3]);
-      *(float4*)(p + 4) = make_float4(acc[4], acc[5], acc[6], acc[7]);
+      if (VEC) {
+        *(float4*)p = make_float4(acc[0], acc[1], acc[2], acc[3]);
+        *(float4*)(p + 4) = make_float4(acc[4], acc[5], acc[6], acc[7]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (j < live) p[j * STEP] = acc[j];
+      }
       return;
     }
-    Out* p = out + (int64_t)now * g.cols;
+    Out* p = out + (int64_t)now * g.cols + c0;
     if (VEC) {
       float v[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = g.scale * acc[j];
-      if (mine) store8_whole(p + c0, v);
-    } else if (g.lanes >= 32) {  // a warp is in one group: all of it is here
-      float* t = turn[threadIdx.x / 32];
-      const int l = threadIdx.x & 31;
-      const int64_t w0 = c0 - l * 8;  // the warp's first column
-#pragma unroll
-      for (int j = 0; j < 8; ++j) t[l * 9 + j] = g.scale * acc[j];
-      __syncwarp();
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int i = j * 32 + l;
-        if (w0 + i < g.cols) put(p + w0 + i, t[i / 8 * 9 + i % 8]);
-      }
-      __syncwarp();
-    } else if (mine) {
+      store8_whole(p, v);
+    } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (c0 + j < g.cols) put(p + c0 + j, g.scale * acc[j]);
+        if (j < live) put(p + j * STEP, g.scale * acc[j]);
     }
   };
   constexpr int kFly = 4;
   for (int i = begin; i < stop && key[i] < g.vocab; i += kFly) {
     Raw8<In> raw[VEC ? kFly : 1];
-    Lines<In> lines[VEC ? 1 : kFly];
+    In one[VEC ? 1 : kFly][8];
 #pragma unroll
     for (int k = 0; k < kFly; ++k) {
-      if (i + k >= stop || key[i + k] >= g.vocab || !mine) continue;
+      if (i + k >= stop || key[i + k] >= g.vocab) continue;
       const In* p = dy + (int64_t)pos[i + k] * g.ld + c0;
-      if (VEC) raw[VEC ? k : 0] = load8(p);
-      else lines[VEC ? 0 : k].fetch(p, end);
+      if (VEC) {
+        raw[VEC ? k : 0] = load8(p);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) one[VEC ? 0 : k][j] = j < live ? __ldcs(p + j * STEP) : In(0);
+      }
     }
 #pragma unroll
     for (int k = 0; k < kFly; ++k) {
@@ -515,13 +512,15 @@ __global__ void __launch_bounds__(kBlock, VEC ? 1 : 3) k_sum_runs(const In* __re
 #pragma unroll
         for (int j = 0; j < 8; ++j) acc[j] = 0.f;
       }
-      if (mine) {
-        float v[8];
-        if (VEC) widen8(raw[VEC ? k : 0], v);
-        else lines[VEC ? 0 : k].get(v);
+      float v[8];
+      if (VEC) {
+        widen8(raw[VEC ? k : 0], v);
+      } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) acc[j] += v[j];
+        for (int j = 0; j < 8; ++j) v[j] = widen(one[VEC ? 0 : k][j]);
       }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[j] += v[j];
     }
   }
   leaves = leaves && now == last;
@@ -587,12 +586,16 @@ struct GradPlan {
     g.ld = d.ld;
     g.vocab = d.vocab;
     g.scale = (float)d.scale;
+    // As many threads as a row of up to 128 has columns by eight.  Longer rows are cut into slices of 256 to 2048 columns, the
+    // longest of those that leave nearly the fewest threads without columns.
+    auto width = [&](int lanes) { return (d.cols + 8 * lanes - 1) / (8 * lanes) * lanes; };
     g.lanes = 8;
+    while (g.lanes < 32 && g.lanes * 8 < d.cols) g.lanes *= 2;
+    if (g.lanes == 32)
+      for (int lanes = 64; lanes <= kBlock; lanes *= 2)
+        if (width(lanes) * 8 <= width(32) * 9) g.lanes = lanes;
     g.log_lanes = 3;
-    while (g.lanes < kBlock && g.lanes * 8 < d.cols) {
-      g.lanes *= 2;
-      ++g.log_lanes;
-    }
+    while (1 << g.log_lanes < g.lanes) ++g.log_lanes;
     const int groups = kBlock / g.lanes;
     g.slices = std::max<int64_t>(1, (d.cols + 8 * g.lanes - 1) / (8 * g.lanes));
     // Chunks as long as they still give every SM four blocks, or two where the rows are short (a block then has several
@@ -729,8 +732,7 @@ cudaError_t launch_embedding_grad(const LaunchCtx& c, const CallDesc& d, const v
     } else {
       g.chunk_blocks = 0;
     }
-    launch(vec ? k_sum_runs<In, Out, true> : k_sum_runs<In, Out, false>, g.chunk_blocks * g.slices + fill_blocks, kBlock, (const In*)dy,
-           (const In*)dy + (d.rows ? (d.rows - 1) * d.ld + d.cols : 0), (Out*)out, g);
+    launch(vec ? k_sum_runs<In, Out, 1> : g.lanes == 8 ? k_sum_runs<In, Out, 8> : g.lanes == 16 ? k_sum_runs<In, Out, 16> : k_sum_runs<In, Out, 32>, g.chunk_blocks * g.slices + fill_blocks, kBlock, (const In*)dy, (Out*)out, g);
     // a run of at most two chunks' length never is a long one
     if (g.chunks > 2) launch(k_join_runs<Out>, std::min<int64_t>(g.chunks * ((d.cols + kBlock - 1) / kBlock), (int64_t)c.sm_count * 8), kBlock, (Out*)out, g);
   });
