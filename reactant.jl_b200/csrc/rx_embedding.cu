@@ -255,17 +255,20 @@ __device__ __forceinline__ void clear_touched(uint8_t* touched, int64_t vocab, i
   if (rank == 0 && threadIdx.x == 0) *crossing = 0;
 }
 
-// Up to kRankTokens: every token's place is the number of tokens that come before it, counted outright.  A warp takes four
-// tokens and compares them with four keys a lane at a time; 8192 x 8192 comparisons are about 5 us of what the SMs issue,
-// 1024 x 1024 nothing, and one launch without any exchange between blocks replaces four.
-constexpr int kRankTokens = 8192, kRankBlock = 512, kRankPerBlock = 4 * kRankBlock / 32;
+// Up to kRankTokens: every token's place is the number of tokens that come before it, counted outright, which replaces
+// four launches by one without any exchange between blocks.  A warp takes four tokens and compares them with four keys a
+// lane at a time; `parts` warps share the keys, so that there is about a block to an SM, of 32 warps.  (8148 tokens: 15 us;
+// with half as many warps and no sharing 19; two blocks to an SM read the ids twice and take 16.6.  The comparisons are most of it.)
+constexpr int kRankTokens = 8192, kRankBlock = 1024, kRankWarps = kRankBlock / 32;
 
 template <class Id>
-__global__ void __launch_bounds__(kRankBlock) k_rank_tokens(const Id* __restrict__ ids, int rows, int64_t vocab, int32_t* __restrict__ key, int32_t* __restrict__ pos, uint8_t* touched,
+__global__ void __launch_bounds__(kRankBlock) k_rank_tokens(const Id* __restrict__ ids, int rows, int64_t vocab, int parts, int32_t* __restrict__ key, int32_t* __restrict__ pos, uint8_t* touched,
                                                             int32_t* crossing) {
   __shared__ __align__(16) uint32_t sh[kRankTokens];
+  __shared__ int count[4 * kRankWarps];
   pdl_release();
   if (blockIdx.x == 0 && threadIdx.x == 0) *crossing = 0;
+  if (threadIdx.x < 4 * kRankWarps) count[threadIdx.x] = 0;
   const int vecs = (rows + 3) / 4, lane = threadIdx.x & 31;
 #pragma unroll 8
   for (int t = threadIdx.x; t < vecs * 4; t += kRankBlock) {
@@ -277,32 +280,37 @@ __global__ void __launch_bounds__(kRankBlock) k_rank_tokens(const Id* __restrict
     sh[t] = k;
   }
   __syncthreads();
-  const int own = blockIdx.x * (kRankPerBlock / 4) + threadIdx.x / 32;
-  if (own >= vecs) return;
-  const uint4 m4 = ((const uint4*)sh)[own];
-  const uint32_t mine[4] = {m4.x, m4.y, m4.z, m4.w};
-  int before[4] = {0, 0, 0, 0};
+  const int groups = kRankWarps / parts, group = threadIdx.x / 32 / parts, part = threadIdx.x / 32 % parts;
+  const int own = blockIdx.x * groups + group;
+  if (own < vecs) {
+    const uint4 m4 = ((const uint4*)sh)[own];
+    const uint32_t mine[4] = {m4.x, m4.y, m4.z, m4.w};
+    int before[4] = {0, 0, 0, 0};
 #pragma unroll 2
-  for (int v = lane; v < vecs; v += 32) {
-    const uint4 k = ((const uint4*)sh)[v];
-    const uint32_t front = v < own;  // equal ids in front count, those behind do not
+    for (int v = part * 32 + lane; v < vecs; v += 32 * parts) {
+      const uint4 k = ((const uint4*)sh)[v];
+      const uint32_t front = v < own;  // equal ids in front count, those behind do not
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t limit = mine[i] + front;
+        before[i] += (k.x < limit) + (k.y < limit) + (k.z < limit) + (k.w < limit);
+      }
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t limit = mine[i] + front;
-      before[i] += (k.x < limit) + (k.y < limit) + (k.z < limit) + (k.w < limit);
+      before[i] = __reduce_add_sync(~0u, before[i]);
+      if (lane == i) atomicAdd(&count[group * 4 + i], before[i]);
     }
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    before[i] = __reduce_add_sync(~0u, before[i]);
-#pragma unroll
-    for (int j = 0; j < i; ++j) before[i] += mine[j] == mine[i];
-    const int t = own * 4 + i;
-    if (lane == i && t < rows) {
-      key[before[i]] = (int32_t)mine[i];
-      pos[before[i]] = t;
-      if (touched && mine[i] < (uint32_t)vocab) touched[mine[i]] = 1;
-    }
+  __syncthreads();
+  const int t = blockIdx.x * groups * 4 + threadIdx.x;
+  if (threadIdx.x < groups * 4 && t < rows) {
+    const uint32_t mine = sh[t];
+    int at = count[threadIdx.x];
+    for (int j = t & ~3; j < t; ++j) at += sh[j] == mine;  // those of its own four that come first
+    key[at] = (int32_t)mine;
+    pos[at] = t;
+    if (touched && mine < (uint32_t)vocab) touched[mine] = 1;
   }
 }
 
@@ -598,10 +606,9 @@ struct GradPlan {
     while (1 << g.log_lanes < g.lanes) ++g.log_lanes;
     const int groups = kBlock / g.lanes;
     g.slices = std::max<int64_t>(1, (d.cols + 8 * g.lanes - 1) / (8 * g.lanes));
-    // Chunks as long as they still give every SM four blocks, or two where the rows are short (a block then has several
-    // chunks, and what a chunk costs besides its rows counts) or the zeros keep the SMs busy as well.
-    const bool filling = (d.vocab - d.rows) * (int64_t)dt_size(d.out_dt) > d.rows * (int64_t)dt_size(d.in_dt);
-    const int64_t blocks = sm_count * (filling || groups > 1 ? 2 : 4), least = d.rows > 2048 ? 16 : d.rows > 1024 ? 8 : 4;
+    // Chunks as long as they still give every SM six blocks (8148 tokens, 5000 x 4775 bf16: 72 us, with two blocks 86, with
+    // eight 71; 65536 tokens, 131072 x 2048: 228, 232 and 234).
+    const int64_t blocks = sm_count * 6, least = d.rows > 2048 ? 16 : d.rows > 1024 ? 8 : 4;
     g.chunk = std::min(kMaxChunk, kMaxPlaces / groups);
     while (g.chunk > least && (d.rows + (int64_t)g.chunk * groups - 1) / ((int64_t)g.chunk * groups) * g.slices < blocks) g.chunk /= 2;
     g.chunks = (d.rows + g.chunk - 1) / g.chunk;
@@ -712,7 +719,10 @@ cudaError_t launch_embedding_grad(const LaunchCtx& c, const CallDesc& d, const v
       g.part = (float*)(w + p.part);
       if (d.rows <= kRankTokens) {
         if (!g.search) err = cudaMemsetAsync(w + p.touched, 0, (size_t)d.vocab, c.stream);
-        launch(k_rank_tokens<Id>, (d.rows + kRankPerBlock - 1) / kRankPerBlock, kRankBlock, (const Id*)ids, (int)d.rows, d.vocab, (int32_t*)g.key, (int32_t*)g.pos, (uint8_t*)g.touched, g.crossing);
+        int parts = 1;
+        while (parts < 8 && (d.rows + 4 * kRankWarps / (parts * 2) - 1) / (4 * kRankWarps / (parts * 2)) <= c.sm_count) parts *= 2;
+        const int per = 4 * kRankWarps / parts;
+        launch(k_rank_tokens<Id>, (d.rows + per - 1) / per, kRankBlock, (const Id*)ids, (int)d.rows, d.vocab, parts, (int32_t*)g.key, (int32_t*)g.pos, (uint8_t*)g.touched, g.crossing);
       } else {
         SortPass<Id> pass{};
         pass.ids = (const Id*)ids;
