@@ -498,6 +498,24 @@ def test_token_logprobs_of_few_rows(rx, ref, client, pattern, t, vocab, et):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("et", ["f32", "bf16"])
+@pytest.mark.parametrize("vocab", [1, 7, 8, 64, 65, 128, 129, 256, 257, 512, 513, 1024, 1025, 9000])
+def test_the_most_likely_token(rx, client, vocab, et):
+    """One top token: the lowest index of the largest value, of NaN where there is any, and of -inf where there is nothing else."""
+    i = np.arange(vocab)
+    rows = [np.full(vocab, 2.0), i % 2.0, -(i % 3.0), np.where(i % 2, 0.0, -0.0), np.where(i == vocab - 1, -7.0, -np.inf), np.full(vocab, -np.inf), i * 0.5, i * -0.5,
+            np.where(i >= vocab // 2, np.nan, 5.0), np.where(i == vocab - 1, np.nan, -np.inf), np.where(i >= vocab // 3, np.inf, 1.0), np.full(vocab, -3.3895313892515355e38)]
+    x = np.stack(rows).astype(np.float32).astype(np_et(rx, et))
+    got = run(rx, client, rx.programs.token_logprobs(len(rows), vocab, et=et, top_k=1), [x, np.zeros(len(rows), np.int32)])
+    z = f64(x)
+    want = [int(np.argmax(np.isnan(r))) if np.isnan(r).any() else int(np.argmax(r)) for r in z]
+    assert got[4][:, 0].tolist() == want
+    # the same number as the log probability of that token
+    again = run(rx, client, rx.programs.token_logprobs(len(rows), vocab, et=et, top_k=0), [x, np.array(want, np.int32)])
+    close(got[3][:, 0], again[0], 0.0, "top")
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("features,et,out_et", [(257, "f32", "f32"), (512, "f32", "f32"), (1024, "bf16", "bf16"), (1001, "bf16", "f32")])
 @pytest.mark.parametrize("tokens", [1, 2, 31, 32, 33, 64, 65, 700, 1023, 1024, 1025])
 def test_embedding_grad_of_few_tokens(rx, ref, client, tokens, features, et, out_et):
