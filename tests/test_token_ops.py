@@ -510,9 +510,13 @@ def test_the_most_likely_token(rx, client, vocab, et):
     z = f64(x)
     want = [int(np.argmax(np.isnan(r))) if np.isnan(r).any() else int(np.argmax(r)) for r in z]
     assert got[4][:, 0].tolist() == want
-    # the same number as the log probability of that token
+    # The same number as the log probability of that token, which another kernel may give: each is within its bound of the
+    # true one, so the two are within twice the bound of each other.
     again = run(rx, client, rx.programs.token_logprobs(len(rows), vocab, et=et, top_k=0), [x, np.array(want, np.int32)])
-    close(got[3][:, 0], again[0], 0.0, "top")
+    finite = np.isfinite(z.max(-1))
+    bound = np.zeros(len(rows))
+    bound[finite] = 2 * logprob_bounds(z[finite], z[finite].max(-1), f64(again[1])[finite])[2]
+    close(got[3][:, 0], again[0], bound, "top")
 
 
 @pytest.mark.gpu
