@@ -138,7 +138,9 @@ void CopyFromBuffer(RxClient* client, RxBuffer* buffer, void* data, size_t offse
  * takes the tensor over: its deleter is called once the buffer is freed and the
  * work queued with it is done.  The producer has to have ordered the device's
  * stream (RxDeviceStream) behind its own writes.  The array has to be dense and
- * start on a 16-byte boundary; other arrays are refused and stay the caller's. */
+ * start on a 16-byte boundary; other arrays are refused and stay the caller's.
+ * A consumer's or a device's stream that is being captured into a graph is an
+ * error, here and when a program is executed. */
 void* RxBufferToDLPack(RxBuffer* buffer, void* consumer_stream);
 RxBuffer* RxBufferFromDLPack(RxDevice* device, void* dl_managed_tensor);
 
