@@ -14,7 +14,7 @@ constexpr int kBlock = 256;
 //
 // Bound by memory: every distinct row is read, every row of the result written once.  The result is cut into units of
 // eight consecutive elements; a thread takes kUnits of them, a block apart, and asks for the ids and then the rows of
-// all of them before it stores.  Rows of the table and of the result start on 16 bytes, so a unit is a vector of one row.
+// all of them before it stores.  Rows of the table start on 16 bytes, those of the result on eight elements, so a unit is a vector of one row.
 // 65536 tokens of 2048 bf16 features out of 131072 rows: 71 us with two units a thread (one 88, four 73, eight 82; one
 // element a thread and a 64-bit division each 361), where the bytes alone need 54.  What is left is the way through L2:
 // with the whole table in there the same result takes 54.
@@ -59,7 +59,7 @@ __global__ void __launch_bounds__(kBlock) k_embedding(const In* __restrict__ tab
   }
 }
 
-// Rows that do not start on 16 bytes (an odd length, a window of a wider table): a warp takes kRowVecs vectors of a row of
+// Rows that do not start on 16 bytes (an odd length, a window of a wider table, a result off its vectors): a warp takes kRowVecs vectors of a row of
 // the result, cut at the result's vectors, and reads the 16-byte lines that hold the elements; the few in front of the
 // first vector and behind the last go one by one.  (65536 x 2047 bf16: 87 us, 2048 73; units across rows, each with its own
 // shift, took 184.)
@@ -421,7 +421,7 @@ __device__ __forceinline__ void fill_rows(const GradArgs& g, Out* out, int64_t b
   }
 }
 
-// A thread has eight columns, STEP apart.  1: rows of dy and of the result start on 16 bytes, and the columns are vectors.
+// A thread has eight columns, STEP apart.  1: rows of dy start on 16 bytes, those of the result on eight elements, and the columns are vectors.
 // Otherwise STEP is a warp's width (or that of the threads that share a chunk, if fewer) and they are read and written one by
 // one, side by side with the neighbours' (22288 tokens, 1339 x 521 f32: the call 44 us; read as the 16-byte lines that hold eight
 // consecutive ones, and turned through shared memory to be written, 78).
@@ -651,7 +651,7 @@ cudaError_t launch_embedding(const LaunchCtx& c, const CallDesc& d, const void* 
   const int64_t n = d.rows * d.cols;
   if (!n) return cudaSuccess;
   const int64_t in_bytes = (int64_t)dt_size(d.in_dt);
-  const bool vec = d.cols % 8 == 0 && aligned16(table) && d.ld * in_bytes % 16 == 0;
+  const bool vec = d.cols % 8 == 0 && aligned16(table) && d.ld * in_bytes % 16 == 0 && whole_stores(out, dt_size(d.out_dt));
   with_types(d.in_dt, d.out_dt, d.ids_dt, [&](auto* i, auto* o, auto* id) {
     using In = std::remove_pointer_t<decltype(i)>;
     using Out = std::remove_pointer_t<decltype(o)>;
@@ -678,7 +678,7 @@ cudaError_t launch_embedding_grad(const LaunchCtx& c, const CallDesc& d, const v
   GradArgs& g = p.g;
   char* w = (char*)workspace;
   const int64_t n = d.vocab * d.cols;
-  const bool vec_out = d.cols % 8 == 0;
+  const bool vec_out = d.cols % 8 == 0 && whole_stores(out, dt_size(d.out_dt));
   const bool vec = vec_out && aligned16(dy) && d.ld * (int64_t)dt_size(d.in_dt) % 16 == 0;
   g.by_row = Divisor(vec ? d.cols / 8 : d.cols);
   g.small = n < (int64_t)1 << 31;

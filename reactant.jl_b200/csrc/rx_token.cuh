@@ -108,7 +108,8 @@ struct Lines {
   }
 };
 
-// The same where the eight elements start on their own size (32 bytes for floats): one store a lane, whole sectors.
+// The same where the eight elements start on their own size (32 bytes for floats): one store a lane, whole sectors.  Blocks
+// of the pool start on 256 bytes, but memory taken over from another library on 16 only: launches ask `whole_stores` first.
 __device__ __forceinline__ void store8_whole(float* p, const float (&v)[8]) {
   asm volatile("st.global.cs.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]) : "memory");
 }
@@ -132,5 +133,6 @@ struct Divisor {
 };
 
 inline bool aligned16(const void* p) { return (uintptr_t)p % 16 == 0; }
+inline bool whole_stores(const void* out, size_t elem_bytes) { return (uintptr_t)out % (8 * elem_bytes) == 0; }
 
 }  // namespace rx

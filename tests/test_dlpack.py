@@ -242,3 +242,48 @@ def test_streams_under_capture_are_refused(tmp_path):
     env = dict(os.environ, PYTHONPATH=root)
     r = subprocess.run([sys.executable, str(script)], cwd=root, env=env, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and r.stdout.strip().endswith("fine"), r.stdout + r.stderr
+
+
+def carried_lookup(rows, features, trips, gradient=False):
+    """A loop that carries an array through lookups of its own rows (or through the gradient of one)."""
+    t = f"tensor<{rows}x{features}xf32>"
+    call = "rx.embedding_grad" if gradient else "rx.embedding"
+    return f"""module {{
+  func.func @main(%x: {t} {{tf.aliasing_output = 0 : i32}}, %ids: tensor<{rows}xi32>) -> {t} {{
+    %c0 = stablehlo.constant dense<0> : tensor<i64>
+    %c1 = stablehlo.constant dense<1> : tensor<i64>
+    %cn = stablehlo.constant dense<{trips}> : tensor<i64>
+    %r:2 = stablehlo.while(%i = %c0, %a = %x) : tensor<i64>, {t}
+     cond {{
+      %p = stablehlo.compare LT, %i, %cn : (tensor<i64>, tensor<i64>) -> tensor<i1>
+      stablehlo.return %p : tensor<i1>
+    }} do {{
+      %n = stablehlo.add %i, %c1 : tensor<i64>
+      %b = stablehlo.custom_call @{call}(%a, %ids) {{api_version = 4 : i32, backend_config = {{scale = 1.0 : f64}}}} : ({t}, tensor<{rows}xi32>) -> {t}
+      stablehlo.return %n, %b : tensor<i64>, {t}
+    }}
+    return %r#1 : {t}
+  }}
+}}
+"""
+
+
+@pytest.mark.parametrize("gradient", [False, True])
+@pytest.mark.parametrize("rows,features", [(6, 8), (40, 64), (700, 1024), (3000, 264)])
+@pytest.mark.parametrize("start", [4, 8])
+def test_loop_carries_an_array_off_its_vectors(rx, client, ref, rows, features, start, gradient):
+    """Memory of another library starts on 16 bytes, not on the eight elements that the lookup stores at once; a donated
+    argument that a loop carries may be what the body writes to from the second trip on."""
+    rng = np.random.default_rng(rows)
+    values = rng.integers(-4, 5, (rows, features)).astype(np.float32)
+    ids = rng.permutation(rows).astype(np.int32)  # a gradient of a permutation sums nothing: exact
+    ids[rows // 2] = -1
+    for trips in (1, 2, 3):
+        text = carried_lookup(rows, features, trips, gradient)
+        block = torch.full((rows * features + 16,), 7.0, device="cuda")
+        x = block[start:start + rows * features].view(rows, features)
+        x.copy_(torch.from_numpy(values))
+        a = rx.from_dlpack(x.mT, client)
+        got = torch.from_dlpack(rx.compile(text, client)(a, rx.to_rarray(ids, client))).mT
+        assert np.array_equal(got.cpu().numpy(), ref.run_module(text, [values, ids])[0])
+        assert (block[:start] == 7).all() and (block[start + rows * features:] == 7).all()
