@@ -261,6 +261,7 @@ void RxDevice::leave_event(const std::shared_ptr<Storage>& st, cudaStream_t cons
     cudaGetLastError();  // the consumer's stream is gone: everything it had queued is waited for instead
     if (ev) give_event(ev);
     cudaDeviceSynchronize();
+    st->lent.fetch_sub(1);
     return;
   }
   std::lock_guard<std::mutex> g(st->pending_mu);
@@ -270,6 +271,7 @@ void RxDevice::leave_event(const std::shared_ptr<Storage>& st, cudaStream_t cons
     give_event(st->pending);
   }
   st->pending = ev;
+  st->lent.fetch_sub(1);
 }
 
 void RxDevice::reap(bool all) {
@@ -1025,9 +1027,10 @@ void execute(RxExecutable* ex, const std::vector<RxDevice*>& devs, RxBuffer** ar
       const Slot& sl = p.slots[s];
       if (sl.kind == SlotK::Arg) {
         RxBuffer* b = args[k * nargs_per_dev + sl.arg_index];
+        const bool kept = !(donatable && donatable[sl.arg_index]) || b->st->shared();  // asked before the wait for what a consumer left
         b->st->make_ready();
-        if (sl.writable && !(donatable && donatable[sl.arg_index])) {
-          // the plan updates this argument in place but the caller keeps it: work on a private copy
+        if (sl.writable && kept) {
+          // the plan updates this argument in place but the caller, or another library, keeps it: work on a private copy
           size_t bytes = (size_t)sl.bytes();
           auto st = std::make_shared<Storage>(d, d->alloc(bytes), bytes);
           CK(cudaMemcpyAsync(st->ptr, b->st->ptr, bytes, cudaMemcpyDeviceToDevice, d->stream));
@@ -1432,7 +1435,10 @@ struct HandedOut {
 void handed_out_deleter(rx::DLManagedTensor* t) {
   std::unique_ptr<HandedOut> h((HandedOut*)t->manager_ctx);
   RxDevice* d = h->st->dev;
-  if (!h->ordered || d->closed.load()) return;
+  if (!h->ordered || d->closed.load()) {
+    h->st->lent.fetch_sub(1);
+    return;
+  }
   int cur = 0;
   cudaGetDevice(&cur);
   if (cur != d->ordinal) cudaSetDevice(d->ordinal);
@@ -1496,6 +1502,7 @@ void* RxBufferToDLPack(RxBuffer* b, void* consumer_stream) {
   h->t.dl_tensor = {b->st->ptr, {rx::kDLCUDA, d->ordinal}, (int32_t)n, dl_type(b->dt), h->shape.data(), h->strides.data(), 0};
   h->t.manager_ctx = h.get();
   h->t.deleter = handed_out_deleter;
+  h->st->lent.fetch_add(1);
   return &h.release()->t;
   API_END(nullptr)
 }

@@ -287,3 +287,60 @@ def test_loop_carries_an_array_off_its_vectors(rx, client, ref, rows, features, 
         got = torch.from_dlpack(rx.compile(text, client)(a, rx.to_rarray(ids, client))).mT
         assert np.array_equal(got.cpu().numpy(), ref.run_module(text, [values, ids])[0])
         assert (block[:start] == 7).all() and (block[start + rows * features:] == 7).all()
+
+
+def updated(n):
+    """An array whose first elements are replaced: in place, where the argument may be written."""
+    t = f"tensor<{n}xf32>"
+    return f"""module {{
+  func.func @main(%x: {t} {{tf.aliasing_output = 0 : i32}}, %v: tensor<4xf32>) -> {t} {{
+    %c0 = stablehlo.constant dense<0> : tensor<i32>
+    %0 = stablehlo.dynamic_update_slice %x, %v, %c0 : ({t}, tensor<4xf32>, tensor<i32>) -> {t}
+    return %0 : {t}
+  }}
+}}
+"""
+
+
+def test_donated_memory_that_another_library_sees_is_left_alone(rx, client):
+    """Donation ends an array's life here, not that of the tensor it came from or of the views that were handed out."""
+    n = 1 << 20
+    f = rx.compile(updated(n), client)
+    v = rx.to_rarray(np.full(4, 5, np.float32), client)
+    x = torch.ones(n, device="cuda")
+    a = rx.from_dlpack(x, client)
+    for k in range(2):  # the second time the argument is the first call's result
+        f(a, v)
+        got = torch.from_dlpack(a)
+        torch.cuda.synchronize()
+        assert (got[:4] == 5).all() and (got[4:] == 1).all() and (x == 1).all()
+        del got
+    b = rx.to_rarray(np.ones(n, np.float32), client)
+    for stream in (torch.cuda.current_stream(), torch.cuda.Stream()):
+        with torch.cuda.stream(stream):
+            view = torch.from_dlpack(b)
+            before = view.clone()
+            f(b, v)
+            torch.cuda.synchronize()
+            assert torch.equal(view, before)
+            del view
+            f(b, rx.to_rarray(np.full(4, 1, np.float32), client))
+    unordered = torch.from_dlpack(b.__dlpack__(stream=-1))
+    f(b, v)
+    torch.cuda.synchronize()
+    assert (unordered == 1).all()
+
+
+def test_donated_memory_that_nobody_sees_is_reused(rx, client):
+    """Handed out and let go of, or never: the result takes the argument's place."""
+    n = 1 << 20
+    f = rx.compile(updated(n), client)
+    v = rx.to_rarray(np.full(4, 5, np.float32), client)
+    b = rx.to_rarray(np.ones(n, np.float32), client)
+    view = torch.from_dlpack(b)
+    where = view.data_ptr()
+    b.__dlpack__()  # nobody takes it
+    del view
+    f(b, v)
+    again = torch.from_dlpack(b)
+    assert again.data_ptr() == where and again[:5].tolist() == [5, 5, 5, 5, 1]
