@@ -114,10 +114,7 @@ void* RxDevice::alloc(size_t bytes) {
       if (take == blocks.size()) goto fresh;
       void* p = blocks[take].p;
       if (blocks[take].busy) {
-        if (!passed) {
-          cudaStreamWaitEvent(stream, blocks[take].busy, 0);
-          enqueued.fetch_add(1);  // whoever is handed this block next waits for that consumer too
-        }
+        if (!passed) cudaStreamWaitEvent(stream, blocks[take].busy, 0);
         spare_events.push_back(blocks[take].busy);
       }
       blocks.erase(blocks.begin() + take);
@@ -1062,12 +1059,6 @@ void execute(RxExecutable* ex, const std::vector<RxDevice*>& devs, RxBuffer** ar
       }
     }
   }
-  // Counted when everything is queued, not before: an event that another thread records in between does not cover
-  // what is still to come.
-  struct Counted {
-    const std::vector<RxDevice*>& on;
-    ~Counted() { for (RxDevice* d : on) d->enqueued.fetch_add(1); }
-  } counted{order};
   run_steps(ex, p.steps, runs);
   // All-reduces still in flight on the communication stream: a result keeps the event (its future and its next user
   // wait for it), so the compute stream is free to start the next execution; anything else is joined now.
@@ -1472,22 +1463,13 @@ void* RxBufferToDLPack(RxBuffer* b, void* consumer_stream) {
     cudaGetDevice(&cur);
     if (cur != d->ordinal) CK(cudaSetDevice(d->ordinal));
     not_captured(h->consumer);
-    unsigned long long id = 0;  // unlike the handle, never given to another stream
-    CK(cudaStreamGetId(h->consumer, &id));
     b->st->make_ready();
     std::lock_guard<std::mutex> g(d->order_mu);
     if (!d->order) CK(cudaEventCreateWithFlags(&d->order, cudaEventDisableTiming));
-    const uint64_t now = d->enqueued.load();
-    if (now != d->ordered) {
-      CK(cudaEventRecord(d->order, d->stream));
-      d->ordered = now;
-      d->waited = 0;
-    }
-    if (d->waited != now || d->waited_id != id) {  // the results of one call: the first one's wait covers the others
-      CK(cudaStreamWaitEvent(h->consumer, d->order, 0));
-      d->waited = now;
-      d->waited_id = id;
-    }
+    // Every time, for the results of one call too (0.35 us each): only the stream itself knows what it holds.  Besides
+    // executions that is the wait for a producer, and whatever a caller queues on RxDeviceStream.
+    CK(cudaEventRecord(d->order, d->stream));
+    CK(cudaStreamWaitEvent(h->consumer, d->order, 0));
     if (cur != d->ordinal) CK(cudaSetDevice(cur));
   }
   // the Julia view of the array: dims reversed, first dim contiguous

@@ -89,12 +89,8 @@ struct RxDevice : std::enable_shared_from_this<RxDevice> {
   // recorded there until the capture has ended, and the memory stays out of use that long.
   struct Parked { std::shared_ptr<Storage> st; cudaStream_t consumer; };
   std::vector<Parked> parked;              // guarded by mu
-  std::mutex order_mu;                     // guards the next four
-  cudaEvent_t order = nullptr;             // recorded on `stream` when a consumer needs to wait for it and executions were queued since the last time
-  uint64_t ordered = 0;                    // value of `enqueued` then
-  uint64_t waited = 0;                     // the value of `ordered` that the stream with the following id has waited for last
-  unsigned long long waited_id = 0;
-  std::atomic<uint64_t> enqueued{1};       // executions, and waits for other streams, queued so far
+  std::mutex order_mu;                     // guards `order`
+  cudaEvent_t order = nullptr;             // recorded on `stream` for each consumer that has to wait for it
   std::vector<cudaEvent_t> spare_events;   // guarded by mu; without timing, like every event that takes part here
   cudaEvent_t take_event();                // null, with the error cleared, when none can be made
   void give_event(cudaEvent_t e);
@@ -139,7 +135,6 @@ struct Storage {
     std::lock_guard<std::mutex> g(pending_mu);
     if (!pending) return;
     if (dev->stream) cudaStreamWaitEvent(dev->stream, pending, 0);
-    dev->enqueued.fetch_add(1);  // whoever waits for this device from now on waits for that too
     dev->give_event(pending);
     pending = nullptr;
   }

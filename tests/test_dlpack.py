@@ -344,3 +344,55 @@ def test_donated_memory_that_nobody_sees_is_reused(rx, client):
     f(b, v)
     again = torch.from_dlpack(b)
     assert again.data_ptr() == where and again[:5].tolist() == [5, 5, 5, 5, 1]
+
+
+def busy_writes(x, value):
+    """Work that keeps the current stream busy for a while and then writes the value."""
+    big = torch.ones(4096, 4096, device="cuda")
+    for _ in range(12):
+        big = big @ big * 2.0 ** -12
+    return x.copy_(big.flatten()[:1].expand(x.numel()) * 0 + value)
+
+
+def test_an_imported_array_is_waited_for_where_it_is_handed_on(rx, client):
+    """Imported under the stream that writes it, handed on to another stream that has waited for this device before, with
+    no execution in between: that stream waits for the producer."""
+    n = 1 << 20
+    first, second, third = torch.cuda.Stream(), torch.cuda.Stream(), torch.cuda.Stream()
+    f = rx.compile(scale_module(n), client)
+    warm = rx.to_rarray(np.ones(n, np.float32), client)
+    for k in range(1, 6):
+        x = torch.zeros(n, device="cuda")
+        torch.cuda.synchronize()
+        with torch.cuda.stream(first):
+            torch.from_dlpack(f(warm)).sum()
+        with torch.cuda.stream(second):
+            busy_writes(x, k)
+            a = rx.from_dlpack(x, client)
+        for stream in (first, third):
+            with torch.cuda.stream(stream):
+                got = torch.from_dlpack(a).sum()
+            stream.synchronize()
+            assert got.item() == k * n
+        second.synchronize()
+
+
+def test_work_of_a_caller_on_the_device_stream_is_waited_for(rx, client):
+    """The device's stream is public: what a caller queues there itself is part of what a consumer waits for."""
+    n = 1 << 20
+    own = torch.cuda.ExternalStream(rx._lib.lib().RxDeviceStream(client.addressable_devices[0].handle))
+    f = rx.compile(scale_module(n), client)
+    a = f(rx.to_rarray(np.ones(n, np.float32), client))
+    side = torch.cuda.Stream()
+    for k in range(1, 4):
+        with torch.cuda.stream(side):
+            torch.from_dlpack(a).sum()
+        torch.cuda.synchronize()
+        view = torch.from_dlpack(a)
+        with torch.cuda.stream(own):
+            busy_writes(view, k)
+        with torch.cuda.stream(side):
+            got = torch.from_dlpack(a).sum()
+        side.synchronize()
+        assert got.item() == k * n
+        torch.cuda.synchronize()
