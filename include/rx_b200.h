@@ -133,7 +133,9 @@ void CopyFromBuffer(RxClient* client, RxBuffer* buffer, void* data, size_t offse
  * makes `consumer_stream` (a cudaStream_t; 1 = the legacy default stream, 2 = the
  * per-thread one, -1 = no ordering wanted) wait for the work queued so far.  The
  * consumer calls its deleter, after which the memory is used again only behind
- * what that stream held at that time.
+ * what that stream held at that time.  The stream has to exist until then; if the
+ * CUDA runtime reports that it does not, or that the handle means another stream
+ * (2, on another thread), the deleter waits for all work of the device.
  * RxBufferFromDLPack makes a buffer over the tensor's memory and, if it succeeds,
  * takes the tensor over: its deleter is called once the buffer is freed and the
  * work queued with it is done.  The producer has to have ordered the device's

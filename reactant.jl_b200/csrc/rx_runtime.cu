@@ -15,6 +15,7 @@
 
 #include "../../include/rx_b200.h"
 #include "rx_collective.h"
+#include "rx_consumer.h"
 #include "rx_dlpack.h"
 #include "rx_gemm.h"
 #include "rx_jit.h"
@@ -232,32 +233,50 @@ void RxDevice::hand_back(void* tensor) {
 }
 
 namespace {
-bool captured(cudaStream_t s) {  // into a graph; also when that cannot be told
-  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
-  if (cudaStreamIsCapturing(s, &status) == cudaSuccess) return status != cudaStreamCaptureStatusNone;
-  cudaGetLastError();
-  return true;
-}
+struct StreamQueries {
+  Query capturing(cudaStream_t s, bool* active) const {
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    const cudaError_t e = cudaStreamIsCapturing(s, &status);
+    *active = status != cudaStreamCaptureStatusNone;  // a capture that has become invalid has not ended either
+    if (e != cudaSuccess) cudaGetLastError();
+    return e == cudaSuccess ? Query::Ok : e == cudaErrorStreamCaptureImplicit ? Query::Implicit : Query::Failed;
+  }
+  Query id(cudaStream_t s, unsigned long long* id) const {
+    if (cudaStreamGetId(s, id) == cudaSuccess) return Query::Ok;
+    cudaGetLastError();
+    return Query::Failed;
+  }
+};
 
 // Memory of the pool is handed out again once the work queued so far has passed it; a graph would go on using it with
 // every replay.
 void not_captured(cudaStream_t s) {
-  if (captured(s)) throw Error(RX_ERR_ARG, "arrays cannot be exchanged, nor programs executed, on a stream that is being captured into a graph");
+  bool active = false;
+  const Query q = StreamQueries().capturing(s, &active);
+  if (q == Query::Failed) throw Error(RX_ERR_ARG, "the stream is not one of this process's CUDA streams");
+  if (q == Query::Implicit || active) throw Error(RX_ERR_ARG, "arrays cannot be exchanged, nor programs executed, on a stream that is being captured into a graph");
 }
 }  // namespace
 
-void RxDevice::leave_event(const std::shared_ptr<Storage>& st, cudaStream_t consumer) {  // this device is current
-  if (captured(consumer)) {
-    std::lock_guard<std::mutex> lk(mu);
-    parked.push_back({st, consumer});
-    n_returned.store((int)(returned.size() + parked.size()));
-    return;
+void RxDevice::leave_event(const std::shared_ptr<Storage>& st, cudaStream_t consumer, unsigned long long id) {  // this device is current
+  const Consumer state = consumer_state(StreamQueries(), consumer, id);
+  cudaEvent_t ev = nullptr;
+  if (state == Consumer::Present) {
+    ev = take_event();
+    if (ev && cudaEventRecord(ev, consumer) != cudaSuccess) {
+      cudaGetLastError();
+      give_event(ev);
+      ev = nullptr;
+    }
   }
-  cudaEvent_t ev = take_event();
-  if (!ev || cudaEventRecord(ev, consumer) != cudaSuccess) {
-    cudaGetLastError();  // the consumer's stream is gone: everything it had queued is waited for instead
-    if (ev) give_event(ev);
-    cudaDeviceSynchronize();
+  if (!ev) {
+    if (state == Consumer::Captured || cudaDeviceSynchronize() != cudaSuccess) {
+      cudaGetLastError();
+      std::lock_guard<std::mutex> lk(mu);
+      parked.push_back({st, consumer, id});
+      n_returned.store((int)(returned.size() + parked.size()));
+      return;
+    }
     st->lent.fetch_sub(1);
     return;
   }
@@ -284,7 +303,7 @@ void RxDevice::reap(bool all) {
     int cur = 0;
     cudaGetDevice(&cur);
     if (cur != ordinal) cudaSetDevice(ordinal);
-    if (!all) leave_event(k.st, k.consumer);
+    if (!all) leave_event(k.st, k.consumer, k.id);
     k.st.reset();
     if (cur != ordinal) cudaSetDevice(cur);
   }
@@ -1418,6 +1437,7 @@ struct HandedOut {
   std::vector<int64_t> shape, strides;
   std::shared_ptr<Storage> st;
   cudaStream_t consumer;
+  unsigned long long id = 0;  // of the stream
   bool ordered;
 };
 
@@ -1433,7 +1453,7 @@ void handed_out_deleter(rx::DLManagedTensor* t) {
   int cur = 0;
   cudaGetDevice(&cur);
   if (cur != d->ordinal) cudaSetDevice(d->ordinal);
-  d->leave_event(h->st, h->consumer);
+  d->leave_event(h->st, h->consumer, h->id);
   h.reset();
   if (cur != d->ordinal) cudaSetDevice(cur);
 }
@@ -1463,6 +1483,7 @@ void* RxBufferToDLPack(RxBuffer* b, void* consumer_stream) {
     cudaGetDevice(&cur);
     if (cur != d->ordinal) CK(cudaSetDevice(d->ordinal));
     not_captured(h->consumer);
+    CK(cudaStreamGetId(h->consumer, &h->id));
     b->st->make_ready();
     std::lock_guard<std::mutex> g(d->order_mu);
     if (!d->order) CK(cudaEventCreateWithFlags(&d->order, cudaEventDisableTiming));

@@ -87,14 +87,14 @@ struct RxDevice : std::enable_shared_from_this<RxDevice> {
   std::atomic<int> n_returned{0};
   // Memory whose consumer's stream was being captured into a graph when the consumer let go of it: no event can be
   // recorded there until the capture has ended, and the memory stays out of use that long.
-  struct Parked { std::shared_ptr<Storage> st; cudaStream_t consumer; };
+  struct Parked { std::shared_ptr<Storage> st; cudaStream_t consumer; unsigned long long id; };
   std::vector<Parked> parked;              // guarded by mu
   std::mutex order_mu;                     // guards `order`
   cudaEvent_t order = nullptr;             // recorded on `stream` for each consumer that has to wait for it
   std::vector<cudaEvent_t> spare_events;   // guarded by mu; without timing, like every event that takes part here
   cudaEvent_t take_event();                // null, with the error cleared, when none can be made
   void give_event(cudaEvent_t e);
-  void leave_event(const std::shared_ptr<Storage>& st, cudaStream_t consumer);  // what `consumer` holds so far may still use the memory
+  void leave_event(const std::shared_ptr<Storage>& st, cudaStream_t consumer, unsigned long long id);  // what `consumer` (the stream with that id) holds so far may still use the memory
   void hand_back(void* tensor);            // memory taken over is no longer used by anything that will be queued
   void reap(bool all);                     // owners whose memory is free now get it back
 

@@ -396,3 +396,39 @@ def test_work_of_a_caller_on_the_device_stream_is_waited_for(rx, client):
         side.synchronize()
         assert got.item() == k * n
         torch.cuda.synchronize()
+
+
+def test_per_thread_streams_of_different_threads(rx, client):
+    """Handed to one thread's own default stream and let go of on another thread, whose own is another stream: the memory is
+    used again behind everything."""
+    import threading
+
+    n = 1 << 12
+    f = rx.compile(scale_module(n), client)
+    x = rx.to_rarray(np.ones(n, np.float32), client)
+    base = client.addressable_devices[0].allocator_stats()["bytes_in_use"]
+    for _ in range(20):
+        held = [f(x).__dlpack__(stream=2)]
+        t = threading.Thread(target=held.clear)
+        t.start()
+        t.join()
+    assert client.addressable_devices[0].allocator_stats()["bytes_in_use"] == base
+    assert np.array_equal(np.asarray(f(x)), np.full(n, 2, np.float32))
+
+
+def test_stream_of_a_consumer_that_outlives_the_array(rx, client):
+    import ctypes
+
+    rt = ctypes.CDLL("libcudart.so.12")
+    stream = ctypes.c_void_p()
+    assert rt.cudaStreamCreateWithFlags(ctypes.byref(stream), 1) == 0
+    n = 1 << 12
+    f = rx.compile(scale_module(n), client)
+    x = rx.to_rarray(np.ones(n, np.float32), client)
+    base = client.addressable_devices[0].allocator_stats()["bytes_in_use"]
+    for _ in range(20):
+        capsule = f(x).__dlpack__(stream=stream.value)
+        del capsule
+    assert rt.cudaStreamDestroy(stream) == 0
+    assert client.addressable_devices[0].allocator_stats()["bytes_in_use"] == base
+    assert np.array_equal(np.asarray(f(x)), np.full(n, 2, np.float32))
