@@ -83,6 +83,16 @@ constexpr size_t kUnasked = (size_t)1 << 20;
 
 size_t round_up(size_t b) { return b == 0 ? 256 : (b + 255) & ~(size_t)255; }
 
+// Allocations and queries of events, allowed while some other stream of the process is being captured into a graph: what is
+// done here has nothing to do with that stream, and an array may be let go of at any time.  (In the default mode such a call is
+// an error that ends the capture.)
+struct BesideCaptures {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  BesideCaptures() { cudaThreadExchangeStreamCaptureMode(&mode); }
+  ~BesideCaptures() { cudaThreadExchangeStreamCaptureMode(&mode); }
+  BesideCaptures(const BesideCaptures&) = delete;
+};
+
 }  // namespace
 
 namespace rx {
@@ -107,6 +117,7 @@ void* RxDevice::alloc(size_t bytes) {
       if (k > 0) take = k - 1;  // the latest that only this device's stream has used
       bool passed = false;
       if (take == blocks.size() && rb > kUnasked) {  // the one that has waited longest is the likeliest to be free
+        BesideCaptures beside;
         passed = cudaEventQuery(blocks[0].busy) == cudaSuccess;
         if (passed) take = 0;
         else cudaGetLastError();  // "not ready" is no error
@@ -126,6 +137,7 @@ void* RxDevice::alloc(size_t bytes) {
     }
   }
 fresh:
+  BesideCaptures beside;
   if (bytes_limit > 0 && bytes_in_use + pool_bytes + (int64_t)rb > bytes_limit) trim();
   void* p = nullptr;
   CK(cudaSetDevice(ordinal));
@@ -193,6 +205,7 @@ cudaEvent_t RxDevice::take_event() {
       return e;
     }
   }
+  BesideCaptures beside;
   cudaEvent_t e = nullptr;
   if (cudaEventCreateWithFlags(&e, cudaEventDisableTiming) != cudaSuccess) {
     cudaGetLastError();
@@ -215,6 +228,7 @@ void RxDevice::hand_back(void* tensor) {
     if (t->deleter) t->deleter(t);
     return;
   }
+  BesideCaptures beside;
   int cur = 0;
   cudaGetDevice(&cur);
   cudaSetDevice(ordinal);
@@ -270,6 +284,7 @@ void RxDevice::leave_event(const std::shared_ptr<Storage>& st, cudaStream_t cons
     }
   }
   if (!ev) {
+    BesideCaptures beside;
     if (state == Consumer::Captured || cudaDeviceSynchronize() != cudaSuccess) {
       cudaGetLastError();
       std::lock_guard<std::mutex> lk(mu);
@@ -292,6 +307,7 @@ void RxDevice::leave_event(const std::shared_ptr<Storage>& st, cudaStream_t cons
 
 void RxDevice::reap(bool all) {
   if (!n_returned.load()) return;
+  BesideCaptures beside;
   std::vector<Returned> done;
   std::vector<Parked> waiting;
   {
@@ -1060,6 +1076,7 @@ void execute(RxExecutable* ex, const std::vector<RxDevice*>& devs, RxBuffer** ar
         auto& cs = ex->consts[d->local_id];
         auto it = cs.find((int)s);
         if (it == cs.end()) {
+          BesideCaptures beside;
           size_t bytes = (size_t)sl.bytes();
           auto st = std::make_shared<Storage>(d, d->alloc(bytes), bytes);
           CK(cudaMemcpyAsync(st->ptr, sl.init.data(), bytes, cudaMemcpyHostToDevice, d->stream));

@@ -432,3 +432,73 @@ def test_stream_of_a_consumer_that_outlives_the_array(rx, client):
     assert rt.cudaStreamDestroy(stream) == 0
     assert client.addressable_devices[0].allocator_stats()["bytes_in_use"] == base
     assert np.array_equal(np.asarray(f(x)), np.full(n, 2, np.float32))
+
+
+BESIDE = """
+import gc, threading, torch
+import __graft_entry__ as entry
+rx = entry.load_package()
+client = rx.default_client()
+n = 1 << 16
+f = rx.compile('''{module}''', client)
+held = [rx.from_dlpack(torch.ones(n, device="cuda"), client) for _ in range(4)]
+results = [f(a) for a in held]
+views = [torch.from_dlpack(f(a)) for a in held]
+torch.cuda.synchronize()
+w = torch.zeros(n, device="cuda")
+done = 0
+
+
+def captured(act):
+    global done
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        w.add_(1)
+        act()
+        gc.collect()
+        w.add_(1)
+    g.replay()
+    torch.cuda.synchronize()
+    done += 2
+    assert (w == done).all()
+
+
+def elsewhere():
+    global got
+    with torch.cuda.stream(torch.cuda.Stream()):
+        b = f(held[0])
+        got = torch.from_dlpack(f(b))
+        held.pop()  # (torch's own synchronisation is not allowed meanwhile)
+
+
+def thread():
+    t = threading.Thread(target=elsewhere)
+    t.start()
+    t.join()
+
+
+captured(held.pop)                       # an array that was taken over
+captured(results.pop)                    # one of the engine's own
+captured(views.pop)                      # a view, let go of on the stream that is captured
+captured(lambda: results.append(f(held[0])))
+captured(thread)
+assert (got == 4).all()
+for _ in range(4):
+    assert (torch.from_dlpack(f(held[0])) == 2).all()
+print("fine")
+"""
+
+
+def test_work_beside_a_capture(tmp_path):
+    """While a stream of another library is captured into a graph, arrays are let go of and programs run on the device's own
+    stream: the capture goes on and holds nothing of it."""
+    import os
+    import subprocess
+    import sys
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    script = tmp_path / "beside.py"
+    script.write_text(BESIDE.replace("{module}", scale_module(1 << 16)))
+    env = dict(os.environ, PYTHONPATH=root)
+    r = subprocess.run([sys.executable, str(script)], cwd=root, env=env, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.strip().endswith("fine"), r.stdout + r.stderr
