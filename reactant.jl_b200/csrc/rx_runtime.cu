@@ -1463,14 +1463,19 @@ struct HandedOut {
 void handed_out_deleter(rx::DLManagedTensor* t) {
   std::unique_ptr<HandedOut> h((HandedOut*)t->manager_ctx);
   RxDevice* d = h->st->dev;
-  if (!h->ordered || d->closed.load()) {
+  if (!h->ordered) {
     h->st->lent.fetch_sub(1);
     return;
   }
   int cur = 0;
   cudaGetDevice(&cur);
   if (cur != d->ordinal) cudaSetDevice(d->ordinal);
-  d->leave_event(h->st, h->consumer, h->id);
+  if (!d->closed.load()) {
+    d->leave_event(h->st, h->consumer, h->id);
+  } else {
+    if (h->st->foreign) cudaDeviceSynchronize();  // the owner may get it back next; memory of the pool goes to the driver, which waits itself
+    h->st->lent.fetch_sub(1);
+  }
   h.reset();
   if (cur != d->ordinal) cudaSetDevice(cur);
 }
@@ -1530,6 +1535,7 @@ void* RxBufferToDLPack(RxBuffer* b, void* consumer_stream) {
 RxBuffer* RxBufferFromDLPack(RxDevice* d, void* tensor) {
   API_BEGIN
   if (!d || !d->addressable) throw Error(RX_ERR_BAD_HANDLE, "device is null or not addressable from this process");
+  if (d->closed.load()) throw Error(RX_ERR_BAD_HANDLE, "the client that owns this device was freed");
   if (!tensor) throw Error(RX_ERR_BAD_HANDLE, "null tensor");
   const rx::DLTensor& t = ((rx::DLManagedTensor*)tensor)->dl_tensor;
   not_captured(d->stream);  // a producer that is being captured has drawn it into its graph

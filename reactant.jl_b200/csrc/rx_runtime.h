@@ -134,7 +134,8 @@ struct Storage {
   void make_ready() {  // call with the owning device current
     std::lock_guard<std::mutex> g(pending_mu);
     if (!pending) return;
-    if (dev->stream) cudaStreamWaitEvent(dev->stream, pending, 0);
+    if (!dev->closed.load()) cudaStreamWaitEvent(dev->stream, pending, 0);
+    else cudaEventSynchronize(pending);  // the client was freed: no stream is left to wait
     dev->give_event(pending);
     pending = nullptr;
   }

@@ -502,3 +502,34 @@ def test_work_beside_a_capture(tmp_path):
     env = dict(os.environ, PYTHONPATH=root)
     r = subprocess.run([sys.executable, str(script)], cwd=root, env=env, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and r.stdout.strip().endswith("fine"), r.stdout + r.stderr
+
+
+@pytest.mark.parametrize("first", ["view", "client"])
+def test_memory_outlives_its_client_until_its_consumer_is_done(rx, first):
+    """A consumer still reads a view when the client is closed and the array dropped: the owner gets its memory back behind
+    that read, whichever goes first."""
+    n = 1 << 20
+    side = torch.cuda.Stream()
+    for k in range(1, 4):
+        other = rx.Client(allowed_devices=[0])
+        x = torch.full((n,), float(k), device="cuda")
+        where = x.data_ptr()
+        a = rx.from_dlpack(x, other)
+        with torch.cuda.stream(side):
+            view = torch.from_dlpack(a)
+            busy_writes(torch.empty(4, device="cuda"), 0)
+            got = view.clone()
+        del x
+        if first == "view":
+            del view
+            other.close()
+        else:
+            other.close()
+            del view
+        del a
+        gc.collect()
+        again = torch.full((n,), -1.0, device="cuda")  # on the current stream, as the tensor was
+        torch.cuda.synchronize()
+        assert again.data_ptr() == where, "the owner did not get its memory back"
+        assert (got == k).all()
+        del again
