@@ -434,7 +434,7 @@ class Thunk:
         r = self._single.run(args, donate)
         if r is None:
             return None
-        if self._single.results is None:
+        if isinstance(r, list):  # buffers: the shapes were not known when this call began (another thread may know them by now)
             infos = tuple((ConcreteRArray if b.dims else ConcreteRNumber, tuple(reversed(b.dims)), np.dtype(b.dtype)) for b in r)
             r = tuple(cls([b], shape, dtype) for b, (cls, shape, dtype) in zip(r, infos))
             self._single.results = infos

@@ -324,3 +324,28 @@ def test_a_dimension_the_mesh_does_not_divide_is_replicated(rx):
     reduce needs no all-reduce and every device computes the whole sum."""
     p = rx.plan_describe(rx.programs.sinsum_add(1001, num_partitions=4))
     assert kinds(p) == ["reduce_full"] and p["steps"][0]["dims"] == [1001]
+
+
+def test_first_calls_of_two_threads_at_once(rx):
+    """Two threads make a program's first call together: the one that finds the results' shapes known by the time it returns
+    still gets arrays, not the buffers they are made from."""
+    class Buffer:
+        dims, dtype = (3, 2), np.dtype(np.float32)
+
+    class Single:
+        results = None
+
+        def __init__(self, n):
+            self.n = n
+
+        def run(self, args, donate):
+            made = [Buffer() for _ in range(self.n)]
+            self.results = tuple((rx.ConcreteRArray, (2, 3), np.dtype(np.float32)) for _ in made)  # the other thread's call
+            return made
+
+    for n in (1, 2):
+        thunk = rx.Thunk.__new__(rx.Thunk)
+        thunk._single, thunk._aliased, thunk.param_alias = Single(n), False, []
+        got = thunk._call_single((), True)
+        arrays = (got,) if n == 1 else got
+        assert len(arrays) == n and all(isinstance(a, rx.ConcreteRArray) and a.shape == (2, 3) for a in arrays)
