@@ -77,7 +77,8 @@ __global__ void __launch_bounds__(kBlock) k_embedding_rows(const In* __restrict_
   const In* x = table + (row < 0 ? 0 : row) * ld;
   Out* y = out + t * cols;
   constexpr int kWhole = 8 * sizeof(Out);
-  const int head = (int)min((int64_t)((kWhole - (uintptr_t)y % kWhole) % kWhole / sizeof(Out)), cols), vecs = (int)((cols - head) >> 3), rest = head + 8 * vecs;
+  const int head = (int)min((int64_t)((kWhole - (uintptr_t)y % kWhole) % kWhole / sizeof(Out)), cols), vecs = (int)((cols - head) >> 3);
+  const int64_t rest = head + 8 * (int64_t)vecs;  // with a lane's number on top it may pass 2^31
   if (part == 0 && lane < head) put(y + lane, row < 0 ? 0.f : scale * widen(__ldg(x + lane)));
   if (part == parts - 1 && rest + lane < cols) put(y + rest + lane, row < 0 ? 0.f : scale * widen(__ldg(x + rest + lane)));
   const int last = min(vecs, (part + 1) * kRowVecs);
@@ -397,7 +398,8 @@ __device__ __forceinline__ void fill_rows(const GradArgs& g, Out* out, int64_t b
       if (busy[k]) continue;
       Out* row = out + (first + k) * g.cols;
       constexpr int kWhole = 8 * sizeof(Out);
-      const int head = (int)((kWhole - (uintptr_t)row % kWhole) % kWhole / sizeof(Out)), vecs = (int)((g.cols - head) >> 3), rest = head + 8 * vecs;
+      const int head = (int)((kWhole - (uintptr_t)row % kWhole) % kWhole / sizeof(Out)), vecs = (int)((g.cols - head) >> 3);
+      const int64_t rest = head + 8 * (int64_t)vecs;
       if (lane < head) put(row + lane, 0.f);
       for (int v = lane; v < vecs; v += 32) store8_whole(row + head + 8 * v, zero);
       if (rest + lane < g.cols) put(row + rest + lane, 0.f);

@@ -2823,7 +2823,8 @@ struct Planner {
       }
       default: break;
     }
-    if (c.rows > INT32_MAX || c.vocab > INT32_MAX) throw Error(RX_ERR_TOO_LARGE, call_error(op, "more than 2^31 - 1 tokens or entries of the vocabulary"));
+    if (c.rows > INT32_MAX || c.vocab > INT32_MAX || (c.op != CallK::Dropout && c.cols > INT32_MAX))
+      throw Error(RX_ERR_TOO_LARGE, call_error(op, "more than 2^31 - 1 tokens, entries of the vocabulary or features"));
     for (int v : op.out) {
       shard[v] = s;
       const Type t = local_type(v);

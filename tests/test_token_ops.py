@@ -656,3 +656,37 @@ def test_offsets_beyond_32_bits(rx, client):
     del out
     d = call(rx.programs.embedding_grad(T, V, 5, et="bf16", out_et="bf16"), x[:5].clone(), torch.tensor([T - 1, 0, T - 1, 77, -1], device=cases, dtype=torch.int32))[0].mT
     assert same(d[T - 1].contiguous(), (x[0].float() + x[2].float()).to(torch.bfloat16)) and same(d[77].contiguous(), x[3]) and not d[-700:-1].any()
+
+
+def test_sizes_beyond_what_rows_are_counted_in(rx):
+    """Places inside a row, tokens and rows are 32-bit numbers: the largest are planned, longer ones refused."""
+    p, most = rx.programs, 2 ** 31 - 1
+    for build in (p.embedding, p.embedding_grad):
+        assert steps(rx, build(1, most, 1)) and steps(rx, build(most, 8, 1)) and steps(rx, build(8, 8, most))
+        for vocab, features, tokens in ((1, most + 1, 1), (2, most + 2, 3), (most + 1, 8, 1), (8, 8, most + 1)):
+            with pytest.raises(rx.ReactantError, match="2\\^31") as e:
+                rx.plan_describe(build(vocab, features, tokens))
+            assert e.value.code == 13
+    for build in (p.token_logprobs, p.token_logprobs_grad):
+        with pytest.raises(rx.ReactantError, match="2\\^31"):
+            rx.plan_describe(build(1, most + 1))
+    assert steps(rx, p.dropout((most + 1,), 0.5)) == ["dropout"]  # elements are counted in 64 bits
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("features", [2 ** 31 - 1, 2 ** 31 - 8, 2 ** 31 - 33])
+def test_longest_rows(rx, client, features):
+    """Rows whose last places are near 2^31: looked up, and their gradient with its zeros, whole and nothing behind them."""
+    torch = pytest.importorskip("torch")
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("needs 60 GB")
+    x = torch.randint(-2 ** 15, 2 ** 15, (2, features), device="cuda", dtype=torch.int16)
+    x &= 0x3FFF  # any finite positive number
+    table = x.view(torch.bfloat16)
+    call = lambda text, *a: torch.from_dlpack(rx.compile(text, client)(*[rx.from_dlpack(t.mT if t.dim() == 2 else t, client) for t in a])).mT  # noqa: E731
+    ids = torch.tensor([1, 0, 2], device="cuda", dtype=torch.int32)
+    got = call(rx.programs.embedding(2, features, 3), table, ids).view(torch.int16)
+    assert torch.equal(got[0], x[1]) and torch.equal(got[1], x[0]) and not got[2].any()
+    del got
+    got = call(rx.programs.embedding_grad(3, features, 2, out_et="bf16"), table, ids[:2].clone()).view(torch.int16)
+    assert torch.equal(got[0], x[1]) and torch.equal(got[1], x[0]) and not got[2].any()
