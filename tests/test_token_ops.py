@@ -690,3 +690,29 @@ def test_longest_rows(rx, client, features):
     del got
     got = call(rx.programs.embedding_grad(3, features, 2, out_et="bf16"), table, ids[:2].clone()).view(torch.int16)
     assert torch.equal(got[0], x[1]) and torch.equal(got[1], x[0]) and not got[2].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("et,t,vocab,temperature,peak", [("f32", 512, 50016, 0.7, 6.0), ("f32", 512, 50016, 1.0, 20.0), ("bf16", 256, 131072, 1.0, 6.0), ("f32", 2400, 4100, 1.0, 6.0), ("bf16", 5000, 16500, 0.7, 14.0),
+                                                        ("f32", 64, 65536, 1.0, 12.0), ("f32", 2000, 900, 1.0, 12.0)])
+def test_entropy_of_peaked_rows(rx, client, et, t, vocab, temperature, peak):
+    """One token stands out, by little or by much: the entropy is a small difference of larger numbers.  The definition
+    evaluated in 32 bits refers to the row's largest logit; a kernel in one pass cannot, and may lose as much again, and
+    the half step U of a sum that lies next to one."""
+    rng = np.random.default_rng(31)
+    x = (2.5 * rng.standard_normal((t, vocab))).astype(np.float32)
+    ids = rng.integers(0, vocab, t).astype(np.int32)
+    x[np.arange(t), ids] += np.float32(peak)
+    x = x.astype(np_et(rx, et))
+    got = run(rx, client, rx.programs.token_logprobs(t, vocab, et=et, temperature=temperature), [x, ids])[1]
+
+    def entropy(z):
+        d = z - z.max(-1, keepdims=True)
+        e = np.exp(d)
+        s = e.sum(-1)
+        return np.log(s) - (e * d).sum(-1) / s
+
+    want = entropy(f64(x) / temperature)
+    plain = entropy(x.astype(np.float32) / np.float32(temperature))
+    rms = lambda v: math.sqrt((v ** 2).mean())  # noqa: E731
+    assert rms(f64(got) - want) <= 2 * rms(f64(plain) - want) + U
