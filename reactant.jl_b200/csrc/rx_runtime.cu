@@ -123,6 +123,16 @@ void* RxDevice::alloc(size_t bytes) {
         else cudaGetLastError();  // "not ready" is no error
       }
       if (take == blocks.size() && (blocks.size() >= max_busy_blocks(rb) || (bytes_limit > 0 && bytes_in_use + pool_bytes + (int64_t)rb > bytes_limit))) take = 0;
+      if (take == 0 && !passed && blocks[0].busy) {
+        // the stream would wait for the oldest block's consumer: another one's may be done long since
+        BesideCaptures beside;
+        for (size_t j = 1; j < blocks.size() && !passed; ++j)
+          if (blocks[j].from != blocks[0].from && cudaEventQuery(blocks[j].busy) == cudaSuccess) {
+            take = j;
+            passed = true;
+          }
+        cudaGetLastError();
+      }
       if (take == blocks.size()) goto fresh;
       void* p = blocks[take].p;
       if (blocks[take].busy) {
@@ -159,7 +169,7 @@ fresh:
   return p;
 }
 
-void RxDevice::release(void* p, size_t bytes, cudaEvent_t busy) {
+void RxDevice::release(void* p, size_t bytes, cudaEvent_t busy, unsigned long long from) {
   if (!p) return;
   if (closed.load()) {  // pool and stream are gone: hand the block back to the driver
     cudaSetDevice(ordinal);
@@ -170,7 +180,7 @@ void RxDevice::release(void* p, size_t bytes, cudaEvent_t busy) {
   }
   size_t rb = round_up(bytes);
   std::lock_guard<std::mutex> lk(mu);
-  pool[rb].push_back({p, busy});
+  pool[rb].push_back({p, busy, from});
   bytes_in_use -= (int64_t)rb;
   pool_bytes += (int64_t)rb;
   peak_pool_bytes = std::max(peak_pool_bytes, pool_bytes);
@@ -302,6 +312,7 @@ void RxDevice::leave_event(const std::shared_ptr<Storage>& st, cudaStream_t cons
     give_event(st->pending);
   }
   st->pending = ev;
+  st->pending_from = id;
   st->lent.fetch_sub(1);
 }
 
@@ -1118,6 +1129,7 @@ void execute(RxExecutable* ex, const std::vector<RxDevice*>& devs, RxBuffer** ar
         std::lock_guard<std::mutex> g(st.pending_mu);
         if (st.pending) cudaEventDestroy(st.pending);
         st.pending = again;
+        st.pending_from = 0;
       }
       r.pending.erase(it);
     }

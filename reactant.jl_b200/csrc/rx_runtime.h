@@ -53,8 +53,9 @@ struct RxDevice : std::enable_shared_from_this<RxDevice> {
   // memory pool (exact-size free lists, stream ordered on `stream`)
   std::mutex mu;
   // A block that another stream may still be using carries that stream's event: it is handed out again once the event
-  // has passed, and only behind a wait for it when several such blocks of its size are waiting already.
-  struct Block { void* p; cudaEvent_t busy; };
+  // has passed, and only behind a wait for it when several such blocks of its size are waiting already, and no block that a
+  // different stream has used is free.
+  struct Block { void* p; cudaEvent_t busy; unsigned long long from; };  // from: the stream's id, 0 the communication stream
   std::map<size_t, std::vector<Block>> pool;
   int64_t num_allocs = 0, bytes_in_use = 0, peak_bytes_in_use = 0, largest_alloc = 0, bytes_limit = 0, pool_bytes = 0, peak_pool_bytes = 0;
   uint32_t* scratch = nullptr;
@@ -99,7 +100,7 @@ struct RxDevice : std::enable_shared_from_this<RxDevice> {
   void reap(bool all);                     // owners whose memory is free now get it back
 
   void* alloc(size_t bytes);
-  void release(void* p, size_t bytes, cudaEvent_t busy = nullptr);  // takes the event over
+  void release(void* p, size_t bytes, cudaEvent_t busy = nullptr, unsigned long long from = 0);  // takes the event over
   void trim();
   rx::LaunchCtx ctx() {
     rx::LaunchCtx c;
@@ -126,6 +127,7 @@ struct Storage {
   // event first.  A consumer that was handed the block (DLPack) leaves its stream's event here in the same way.
   std::mutex pending_mu;
   cudaEvent_t pending = nullptr;
+  unsigned long long pending_from = 0;  // the id of the consumer's stream
   void* foreign = nullptr;  // the DLPack tensor that owns this memory, when it was taken over from another library
   // Consumers that were handed this memory (DLPack) and have not let go of it, or whose last use no event covers yet.
   std::atomic<int> lent{0};
@@ -148,7 +150,7 @@ struct Storage {
       cudaSetDevice(cur);
     }
     if (foreign) dev->hand_back(foreign);
-    else dev->release(ptr, bytes, pending);
+    else dev->release(ptr, bytes, pending, pending_from);
   }
 };
 

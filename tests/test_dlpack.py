@@ -533,3 +533,29 @@ def test_memory_outlives_its_client_until_its_consumer_is_done(rx, first):
         assert again.data_ptr() == where, "the owner did not get its memory back"
         assert (got == k).all()
         del again
+
+
+@pytest.mark.parametrize("n", [1 << 12, 1 << 20, 1 << 23])
+def test_a_slow_consumer_does_not_hold_up_the_others(rx, client, n):
+    """Results of one size go to two streams, one of them busy for a long time: the device's stream never waits for that one
+    as long as the other's blocks are free."""
+    f = rx.compile(scale_module(n), client)
+    a = rx.to_rarray(np.ones(n, np.float32), client)
+    slow, fast = torch.cuda.Stream(), torch.cuda.Stream()
+    warm = [torch.from_dlpack(f(a)) for _ in range(20)]
+    torch.cuda.synchronize()
+    del warm
+    with torch.cuda.stream(slow):
+        for _ in range(3):
+            torch.from_dlpack(f(a)).sum()
+        torch.cuda._sleep(int(1e9))  # about half a second
+        torch.from_dlpack(f(a))
+        done = torch.cuda.Event()
+        done.record()
+    with torch.cuda.stream(fast):
+        for _ in range(60):
+            got = torch.from_dlpack(f(a))
+            fast.synchronize()
+    assert not done.query(), "the calls waited for the slow consumer"
+    assert (got == 2).all()
+    slow.synchronize()
