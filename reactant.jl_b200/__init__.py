@@ -26,12 +26,12 @@ import ctypes as C
 import json
 import os
 import weakref
-from functools import cached_property
+from functools import cache, cached_property
 
 import numpy as np
 
 from . import _lib, dist
-from ._lib import ReactantError, _call, lib, check, take_string
+from ._lib import ReactantError, lib, check, take_string
 
 try:
     import ml_dtypes
@@ -246,29 +246,37 @@ class NamedSharding:
 # ----------------------------------------------------------------------------
 # buffers and arrays  (src/Types.jl:155-263, src/ConcreteRArray.jl)
 # ----------------------------------------------------------------------------
-class _Buffer(_call.Buffer):
-    """_Buffer(handle, device): freed with the object."""
+@cache
+def _buffer_type():
+    class Buffer(_lib.call().Buffer):
+        """Buffer(handle, device): freed with the object."""
 
-    __slots__ = ()
+        __slots__ = ()
 
-    @property
-    def dims(self):
-        n = lib().BufferNDimensions(self.handle)
-        p = lib().BufferShape(self.handle)
-        return tuple(p[i] for i in range(n))
+        @property
+        def dims(self):
+            n = lib().BufferNDimensions(self.handle)
+            p = lib().BufferShape(self.handle)
+            return tuple(p[i] for i in range(n))
 
-    @property
-    def dtype(self):
-        return _NPTYPE[lib().BufferPrimitiveType(self.handle)]
+        @property
+        def dtype(self):
+            return _NPTYPE[lib().BufferPrimitiveType(self.handle)]
 
-    def to_host(self) -> np.ndarray:
-        out = np.empty(self.dims, dtype=self.dtype)
-        lib().BufferToHost(self.handle, out.ctypes.data_as(C.c_void_p))
-        check()
-        return out
+        def to_host(self) -> np.ndarray:
+            out = np.empty(self.dims, dtype=self.dtype)
+            lib().BufferToHost(self.handle, out.ctypes.data_as(C.c_void_p))
+            check()
+            return out
+
+    return Buffer
 
 
-def _upload(client: Client, device: Device, a: np.ndarray) -> _Buffer:
+def _buffer(handle, device: Device):
+    return _buffer_type()(handle, device)
+
+
+def _upload(client: Client, device: Device, a: np.ndarray):
     """Julia array -> device buffer with reversed dims and unchanged (column-major) bytes."""
     if a.dtype not in _PTYPE:
         raise ReactantError(3, f"unsupported element type {a.dtype}")
@@ -276,7 +284,7 @@ def _upload(client: Client, device: Device, a: np.ndarray) -> _Buffer:
     dims = (C.c_int64 * rm.ndim)(*rm.shape)
     h = lib().ArrayFromHostBuffer(client.handle, rm.ctypes.data_as(C.c_void_p), _PTYPE[a.dtype], rm.ndim, dims, device.handle)
     check()
-    return _Buffer(h, device)
+    return _buffer(h, device)
 
 
 class ConcreteRArray:
@@ -319,9 +327,9 @@ class ConcreteRArray:
         if copy or dl_device is not None and tuple(dl_device) != self.__dlpack_device__():
             raise BufferError("the array can only be handed out as it is, on its own device")
         buf = self.data[0] if len(self.data) == 1 and self.sharding is None else self._single()
-        return _call.hand_out(buf, 1 if stream is None else stream)
+        return _lib.call_path.hand_out(buf, 1 if stream is None else stream)
 
-    def _single(self) -> "_Buffer":
+    def _single(self):
         if len(self.data) != 1 or (self.sharding is not None and not self.replicated and self.sharding.sharded_dim() is not None):
             raise BufferError("an array spread over several devices has no single memory to exchange")
         return self.data[0]
@@ -392,7 +400,7 @@ def from_dlpack(x, client: Client | None = None, device: Device | None = None) -
         if device is None:
             raise ReactantError(12, f"the array is on device {where}, which is not one of this client's")
     capsule = x.__dlpack__(stream=lib().RxDeviceStream(device.handle))
-    buf = _Buffer(_call.take_over(device.handle, capsule), device)
+    buf = _buffer(_lib.call().take_over(device.handle, capsule), device)
     dims = buf.dims
     cls = ConcreteRNumber if not dims else ConcreteRArray
     return cls([buf], tuple(reversed(dims)), buf.dtype)
@@ -425,8 +433,8 @@ class Thunk:
         self.result_sharded_dim = [l.RxExecutableResultShardedDim(handle, i) for i in range(self.num_results)]
         self.param_alias = [l.RxExecutableParameterAlias(handle, i) for i in range(self.num_parameters)]
         self._aliased = any(k >= 0 for k in self.param_alias)
-        self._single = _call.Call(handle, self.num_parameters, self.num_results, bytes(self.num_parameters), bytes(int(a >= 0) for a in self.param_alias), _Buffer,
-                                  client.addressable_devices[0]) if self.num_partitions == 1 else None
+        self._single = _lib.call().Call(handle, self.num_parameters, self.num_results, bytes(self.num_parameters), bytes(int(a >= 0) for a in self.param_alias), _buffer_type(),
+                                        client.addressable_devices[0]) if self.num_partitions == 1 else None
 
     def _call_single(self, args, donate):
         """The call on one device without waiting: no futures, and the results' shapes are looked up once.  None if an
@@ -493,7 +501,7 @@ class Thunk:
             bufs = []
             for k in range(ndev):
                 dev = devs[k] if sharded else (args[0].data[0].device if args else devs[0])
-                bufs.append(_Buffer(out[k * nres + j], dev))
+                bufs.append(_buffer(out[k * nres + j], dev))
             dims = bufs[0].dims
             jl_shape = tuple(reversed(dims))
             dt = bufs[0].dtype

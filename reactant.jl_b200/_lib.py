@@ -1,18 +1,14 @@
 """ctypes binding of librx_b200.so: one prototype per symbol of include/rx_b200.h.
 
-The library is required: importing this module raises if it has not been
-built (python reactant.jl_b200/build.py).  There is no Python or CPU stand-in
-for any entry point.
+The library and, for arrays and calls, the extension module beside it are
+required: their first use raises if they have not been built (python
+reactant.jl_b200/build.py).  There is no Python or CPU stand-in for any entry
+point.
 """
 from __future__ import annotations
 
 import ctypes as C
 import os
-
-try:
-    from . import _call  # csrc/rx_python.cpp
-except ImportError as e:
-    raise ImportError(f"the extension module of the call path is missing: build it with `python reactant.jl_b200/build.py` ({e})") from e
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 # RX_B200_LIB selects another build of the library (the bounds-checked one, say); the default is the in-tree build
@@ -164,8 +160,24 @@ def lib():
             fn = getattr(_lib, name)
             fn.restype = res
             fn.argtypes = args
-        _call.bind(*(C.cast(getattr(_lib, n), C.c_void_p).value for n in ("XLAExecuteSharded", "RxLastErrorCode", "PjRtBufferFree", "RxBufferToDLPack", "RxBufferFromDLPack")), check)
     return _lib
+
+
+call_path = None
+
+
+def call():
+    """The extension module of arrays and calls (csrc/rx_python.cpp), bound to this library; planning does without it."""
+    global call_path
+    if call_path is None:
+        l = lib()
+        try:
+            from . import _call
+        except ImportError as e:
+            raise ImportError(f"the extension module of the call path is missing: build it with `python reactant.jl_b200/build.py` under this Python ({e})") from e
+        _call.bind(*(C.cast(getattr(l, n), C.c_void_p).value for n in ("XLAExecuteSharded", "RxLastErrorCode", "PjRtBufferFree", "RxBufferToDLPack", "RxBufferFromDLPack")), check)
+        call_path = _call
+    return call_path
 
 
 def check():

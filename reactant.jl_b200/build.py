@@ -1,4 +1,4 @@
-"""Builds librx_b200.so (sm_100a) in-tree with nvcc, and the extension module _call.so with the host compiler.
+"""Builds librx_b200.so (sm_100a) in-tree with nvcc, and the extension module _call with the host compiler.
 
 Run as `python reactant.jl_b200/build.py`; `__graft_entry__.build()` calls
 `build()` below.  Objects are rebuilt only when a source or header is newer.
@@ -61,9 +61,9 @@ def write_embedded_headers() -> None:
 
 
 def build_call(verbose: bool = False) -> str:
-    """_call.so: the extension module of the Python package's call path.  It links against nothing: _lib.py hands it the
-    library's entry points."""
-    src, out = os.path.join(CSRC, "rx_python.cpp"), os.path.join(HERE, "_call.so")
+    """The extension module of the Python package's call path, named for the interpreter that builds it (another version
+    does not load it).  It links against nothing: _lib.py hands it the library's entry points."""
+    src, out = os.path.join(CSRC, "rx_python.cpp"), os.path.join(HERE, "_call" + sysconfig.get_config_var("EXT_SUFFIX"))
     if _stale(out, [src, os.path.join(CSRC, "rx_dlpack.h"), os.path.join(HERE, "..", "include", "rx_b200.h")]):
         cmd = [os.environ.get("CXX", "g++"), "-std=c++17", "-O2", "-Wall", "-Wno-missing-field-initializers", "-shared", "-fPIC", "-fvisibility=hidden", "-I", sysconfig.get_paths()["include"],
                src, "-o", out]

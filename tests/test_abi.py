@@ -60,3 +60,33 @@ def test_client_creation_fails_loudly_without_a_device(rx):
 def test_only_gpu_backend_exists(rx):
     with pytest.raises(rx.ReactantError):
         rx.set_default_backend("cpu")
+
+
+def test_planning_needs_no_extension_module(rx):
+    """The package is imported, and modules are planned, without the extension module that arrays and calls need; those say
+    what is missing."""
+    import subprocess
+    import sys
+
+    program = """
+import sys
+import __graft_entry__ as entry
+name = entry.PKG_NAME + "._call"
+rx = entry.load_package()
+assert rx.plan_describe(rx.programs.embedding(8, 4, 3))["steps"][0]["kind"] == "embedding"
+assert name not in sys.modules, "loaded before it is needed"
+sys.modules[name] = None
+try:
+    rx._lib.call()
+except ImportError as e:
+    assert "build.py" in str(e), e
+    print("fine")
+"""
+    r = subprocess.run([sys.executable, "-c", program], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.strip() == "fine", r.stdout + r.stderr
+
+
+def test_extension_module_is_named_for_its_interpreter(rx):
+    import sysconfig
+
+    assert os.path.basename(rx._lib.call().__file__) == "_call" + sysconfig.get_config_var("EXT_SUFFIX")
