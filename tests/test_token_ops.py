@@ -716,3 +716,116 @@ def test_entropy_of_peaked_rows(rx, client, et, t, vocab, temperature, peak):
     plain = entropy(x.astype(np.float32) / np.float32(temperature))
     rms = lambda v: math.sqrt((v ** 2).mean())  # noqa: E731
     assert rms(f64(got) - want) <= 2 * rms(f64(plain) - want) + U
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("et", ["f32", "bf16"])
+@pytest.mark.parametrize("t,vocab,pitch,start", [(4, 1001, 1111, 7), (3, 64, 67, 0), (5, 130, 261, 3), (40, 999, 1001, 1), (2, 40003, 40010, 5), (1, 5000, 5003, 1), (300, 260, 263, 0), (6, 2048, 2056, 3), (7, 2048, 2052, 0)])
+def test_gradient_of_windows_of_wider_logits(rx, client, t, vocab, pitch, start, et):
+    """Logits that lie otherwise than their gradient does (another pitch, another start) give, bit for bit, what their copy gives."""
+    rng = np.random.default_rng(32)
+    wide = masked_logits(rx, rng, (t + 2, pitch), et)
+    x = np.ascontiguousarray(wide[1:t + 1, start:start + vocab])
+    ids = some_ids(rng, t, vocab, "i32")
+    lse, h, g, gh, gl = rng.standard_normal((5, t)).astype(np.float32)
+    lse += 12
+    base = rx.programs.token_logprobs_grad(t, vocab, et=et, temperature=0.8)
+    cut = base.replace(f"%arg0: tensor<{t}x{vocab}x{et}>", f"%arg0: tensor<{t + 2}x{pitch}x{et}>").replace(
+        "    %0 =", f"    %w = stablehlo.slice %arg0 [1:{t + 1}, {start}:{start + vocab}] : (tensor<{t + 2}x{pitch}x{et}>) -> tensor<{t}x{vocab}x{et}>\n    %0 =").replace(
+        "custom_call @rx.token_logprobs_grad(%arg0", "custom_call @rx.token_logprobs_grad(%w")
+    assert steps(rx, cut) == ["token_logprobs_grad"]  # read in place
+    a, = run(rx, client, cut, [wide, ids, lse, h, g, gh, gl])
+    b, = run(rx, client, base, [x, ids, lse, h, g, gh, gl])
+    assert np.array_equal(f64(a), f64(b)) and f64(a).any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("et", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,cols,residual", [(1, 7, False), (3, 5, True), (64, 129, True), (700, 1024, False), (33, 1001, False)])
+def test_dropout_of_windows(rx, ref, client, rows, cols, residual, et):
+    """Operands that start anywhere inside their arrays."""
+    rng = np.random.default_rng(33)
+    wide, r = values(rx, rng, (rows + 3, cols), et), values(rx, rng, (rows, cols), et)
+    key = np.array([3, -4], np.int32)
+    base = rx.programs.dropout((rows, cols), 0.4, et=et, site=2, residual=residual)
+    cut = base.replace(f"%arg0: tensor<{rows}x{cols}x{et}>", f"%arg0: tensor<{rows + 3}x{cols}x{et}>").replace(
+        "    %0 =", f"    %w = stablehlo.slice %arg0 [3:{rows + 3}, 0:{cols}] : (tensor<{rows + 3}x{cols}x{et}>) -> tensor<{rows}x{cols}x{et}>\n    %0 =").replace(
+        "custom_call @rx.dropout(%arg0", "custom_call @rx.dropout(%w")
+    assert steps(rx, cut) == ["dropout"]
+    more = [key] + ([r] if residual else [])
+    a, = run(rx, client, cut, [wide] + more)
+    b, = run(rx, client, base, [np.ascontiguousarray(wide[3:])] + more)
+    assert np.array_equal(f64(a), f64(b)) and f64(a).any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("et", ["f32", "bf16"])
+@pytest.mark.parametrize("nodes,node", [(2, 0), (2, 1), (4, 3), (8, 5)])
+@pytest.mark.parametrize("rows,cols,residual", [(8, 5, False), (16, 8, True), (64, 257, True), (8, 3001, False)])
+def test_dropout_of_a_share(rx, ref, rows, cols, residual, nodes, node, et):
+    """A process that holds one share of an array split over a mesh drops what the whole array's mask says.  (Nothing is
+    exchanged between the shares, so one device can be any of them.)"""
+    rng = np.random.default_rng(34)
+    client = rx.Client(node_id=node, num_nodes=nodes, allowed_devices=[0])
+    try:
+        x, r = values(rx, rng, (rows, cols), et), values(rx, rng, (rows, cols), et)
+        key = rng.integers(-2 ** 31, 2 ** 31, 2).astype(np.int32)
+        text = rx.programs.dropout((rows, cols), 0.3, et=et, site=9, residual=residual, num_partitions=nodes)
+        mesh = rx.Mesh(client.devices)
+        share = rows // nodes
+        mine = slice(node * share, (node + 1) * share)
+        split = rx.NamedSharding(mesh, (None, "x"))  # Julia's order of dims
+        arrays = [rx.from_local_shards([np.ascontiguousarray(v[mine].T)], (cols, rows), split, client) for v in ([x, r] if residual else [x])]
+        arrays.insert(1, rx.to_rarray(key, client, sharding=rx.NamedSharding(mesh, (None,))))
+        got = np.asarray(rx.compile(text, client)(*arrays).data[0].to_host()).reshape(share, cols)
+        keep = ref.dropout_mask(share * cols, key, 0.3, 9, first=node * share * cols).reshape(share, cols)
+        cut = math.floor(0.3 * 65536 + 0.5)
+        want = np.where(keep, f64(x[mine]) * (65536 / (65536 - cut)), 0) + (f64(r[mine]) if residual else 0)
+        close(f64(got), want, 2 * U * np.abs(f64(x[mine])) * 65536 / (65536 - cut) + 2 * HALF[et] * np.abs(want))
+        assert residual or np.array_equal(f64(got) != 0, keep & (f64(x[mine]) != 0))
+    finally:
+        client.close()
+
+
+def grad_on_the_device(rx, client, torch, ids, features, vocab, et="f32"):
+    """The gradient of whole numbers, whose sums are exact in any order, and torch's."""
+    n = ids.numel()
+    dy = torch.randint(-8, 9, (n, features), device="cuda", dtype=torch.int8).to(torch.float32 if et == "f32" else torch.bfloat16)
+    text = rx.programs.embedding_grad(vocab, features, n, et=et, ids_et="i32" if ids.dtype == torch.int32 else "i64")
+    got = torch.from_dlpack(rx.compile(text, client)(rx.from_dlpack(dy.mT, client), rx.from_dlpack(ids, client))).mT
+    want = torch.zeros(vocab, features, device="cuda")
+    live = (ids >= 0) & (ids < vocab)
+    want.index_add_(0, ids.clamp(0, vocab - 1).long(), dy.float() * live[:, None])
+    return torch.equal(got, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("features,et", [(2048, "bf16"), (2049, "f32"), (264, "f32"), (1500, "bf16")])
+@pytest.mark.parametrize("tokens", [17000, 33000, 66000, 140000])
+def test_embedding_grad_of_long_pieces(rx, client, tokens, features, et):
+    """Many tokens, whose sorted places are cut into long pieces: runs about as long as a piece, and as several, that begin
+    anywhere in one."""
+    torch = pytest.importorskip("torch")
+    rng = np.random.default_rng(35)
+    for piece in (32, 64, 128):
+        lengths = rng.choice([1, 2, piece - 1, piece, piece + 1, 2 * piece - 1, 2 * piece, 2 * piece + 1, 3 * piece + 5, 9 * piece], size=2 * tokens)
+        ids = np.repeat(np.arange(len(lengths)), lengths)[:tokens]
+        vocab = int(ids[-1]) + 3
+        ids = np.where(rng.random(tokens) < 0.001, vocab, rng.permutation(ids)).astype(np.int32)
+        assert grad_on_the_device(rx, client, torch, torch.from_numpy(ids).cuda(), features, vocab, et)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens,vocab,features,ids_et", [(9000, 2 ** 18 - 1, 8, "i32"), (9000, 2 ** 18, 8, "i64"), (70000, 2 ** 18 + 1, 5, "i32"), (20000, 2 ** 27, 1, "i32"), (10000, 2 ** 27 + 7, 2, "i64"), (8193, 1, 3, "i32"),
+                                                          (262144, 5000, 8, "i32"), (262177, 5000, 8, "i64"), (300000, 70000, 8, "i32"), (300000, 300000, 3, "i32"), (1000003, 9, 16, "i32")])
+def test_embedding_grad_of_long_sorts(rx, client, tokens, vocab, features, ids_et):
+    """Every number of passes of the sort, and more tokens than its warps hold in registers."""
+    torch = pytest.importorskip("torch")
+    rng = np.random.default_rng(36)
+    for spread in (1, 3):
+        ids = np.minimum((vocab * rng.random(tokens) ** spread).astype(np.int64), vocab - 1)
+        ids[rng.integers(0, tokens, 20)] = -1
+        ids[rng.integers(0, tokens, 20)] = vocab
+        ids[[0, -1]] = 0, vocab - 1
+        ids = torch.from_numpy(ids).cuda().to(torch.int32 if ids_et == "i32" else torch.int64)
+        assert grad_on_the_device(rx, client, torch, ids, features, vocab)
