@@ -360,7 +360,9 @@ struct GradArgs {
   int64_t chunks, chunk_blocks, slices;
   Divisor by_row;
   bool small;
-  bool search;  // few tokens: whether a row has one is looked up among the sorted tokens
+  bool search;   // few tokens: whether a row has one is looked up among the sorted tokens
+  bool by_rows;  // rows without a token are filled by a warp each
+  bool joined;   // k_join_runs follows
 };
 
 constexpr int kMaxChunk = 128, kMaxPlaces = 1024, kFillUnits = 8;
@@ -382,28 +384,22 @@ __device__ __forceinline__ bool has_token(const GradArgs& g, int64_t row) {  // 
 // Zeros for the rows that no token has.  Rows that are whole vectors go by units of eight consecutive elements of the
 // result, kFillUnits a thread, whose rows are all looked up before the first is written; other long rows, and those of a
 // few tokens, by warps, a row at a time from its first element on a whole vector's boundary; other short ones by elements.
-constexpr int kFillRow = 256, kFillRows = 1;  // elements from which a row is a warp's; rows a warp
+constexpr int kFillRow = 256;  // elements from which a row is a warp's
 
 template <class Out, bool VEC>
 __device__ __forceinline__ void fill_rows(const GradArgs& g, Out* out, int64_t block) {
   const float zero[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if ((!VEC || g.search) && g.cols >= kFillRow) {
+  if (g.by_rows) {
     const int lane = threadIdx.x & 31;
-    const int64_t first = (block * (kBlock / 32) + threadIdx.x / 32) * kFillRows;
-    uint32_t busy[kFillRows];
-#pragma unroll
-    for (int k = 0; k < kFillRows; ++k) busy[k] = first + k >= g.vocab || (g.search ? has_token(g, first + k) : g.touched && __ldg(g.touched + first + k));
-#pragma unroll
-    for (int k = 0; k < kFillRows; ++k) {
-      if (busy[k]) continue;
-      Out* row = out + (first + k) * g.cols;
-      constexpr int kWhole = 8 * sizeof(Out);
-      const int head = (int)((kWhole - (uintptr_t)row % kWhole) % kWhole / sizeof(Out)), vecs = (int)((g.cols - head) >> 3);
-      const int64_t rest = head + 8 * (int64_t)vecs;
-      if (lane < head) put(row + lane, 0.f);
-      for (int v = lane; v < vecs; v += 32) store8_whole(row + head + 8 * v, zero);
-      if (rest + lane < g.cols) put(row + rest + lane, 0.f);
-    }
+    const int64_t at = block * (kBlock / 32) + threadIdx.x / 32;
+    if (at >= g.vocab || (g.search ? has_token(g, at) : g.touched && __ldg(g.touched + at))) return;
+    Out* row = out + at * g.cols;
+    constexpr int kWhole = 8 * sizeof(Out);
+    const int head = (int)((kWhole - (uintptr_t)row % kWhole) % kWhole / sizeof(Out)), vecs = (int)((g.cols - head) >> 3);
+    const int64_t rest = head + 8 * (int64_t)vecs;
+    if (lane < head) put(row + lane, 0.f);
+    for (int v = lane; v < vecs; v += 32) store8_whole(row + head + 8 * v, zero);
+    if (rest + lane < g.cols) put(row + rest + lane, 0.f);
     return;
   }
   constexpr int kUnit = VEC ? 8 : 1;
@@ -432,7 +428,7 @@ __global__ void __launch_bounds__(kBlock, STEP == 1 ? 1 : 4) k_sum_runs(const In
   constexpr bool VEC = STEP == 1;
   __shared__ int32_t skey[kMaxPlaces + 2 * kMaxChunk + 2], spos[kMaxPlaces + kMaxChunk];
   pdl_wait();
-  pdl_release();
+  if (g.joined) pdl_release();
   if (blockIdx.x >= g.chunk_blocks * g.slices) {
     fill_rows<Out, VEC>(g, out, blockIdx.x - g.chunk_blocks * g.slices);
     return;
@@ -685,8 +681,9 @@ cudaError_t launch_embedding_grad(const LaunchCtx& c, const CallDesc& d, const v
   g.by_row = Divisor(vec ? d.cols / 8 : d.cols);
   g.small = n < (int64_t)1 << 31;
   g.search = d.rows > 0 && d.rows <= kSearchTokens && (vec ? d.cols * (int64_t)dt_size(d.out_dt) >= kSearchRow : d.cols >= kFillRow);
-  const bool by_rows = (!vec || g.search) && d.cols >= kFillRow;
-  const int64_t per = by_rows ? kBlock / 32 * kFillRows : kBlock * kFillUnits, fills = by_rows ? d.vocab : vec ? n / 8 : n;
+  g.by_rows = (!vec || g.search) && d.cols >= kFillRow;
+  g.joined = g.chunks > 2;  // a run of at most two chunks' length never is a long one
+  const int64_t per = g.by_rows ? kBlock / 32 : kBlock * kFillUnits, fills = g.by_rows ? d.vocab : vec ? n / 8 : n;
   const int64_t fill_blocks = (fills + per - 1) / per;
   // Every kernel but the first may be set up while the one in front is still running: it waits for that one's results
   // before it looks at anything.  The last lets nobody in ahead of its end, so what follows this call finds it done.
@@ -745,8 +742,7 @@ cudaError_t launch_embedding_grad(const LaunchCtx& c, const CallDesc& d, const v
       g.chunk_blocks = 0;
     }
     launch(vec ? k_sum_runs<In, Out, 1> : g.lanes == 8 ? k_sum_runs<In, Out, 8> : g.lanes == 16 ? k_sum_runs<In, Out, 16> : k_sum_runs<In, Out, 32>, g.chunk_blocks * g.slices + fill_blocks, kBlock, (const In*)dy, (Out*)out, g);
-    // a run of at most two chunks' length never is a long one
-    if (g.chunks > 2) launch(k_join_runs<Out>, std::min<int64_t>(g.chunks * ((d.cols + kBlock - 1) / kBlock), (int64_t)c.sm_count * 8), kBlock, (Out*)out, g);
+    if (g.joined) launch(k_join_runs<Out>, std::min<int64_t>(g.chunks * ((d.cols + kBlock - 1) / kBlock), (int64_t)c.sm_count * 8), kBlock, (Out*)out, g);
   });
   return err != cudaSuccess ? err : cudaGetLastError();
 }
