@@ -853,9 +853,7 @@ void with_types(DT in, DT ids, F f) {
 
 }  // namespace
 
-int64_t logprobs_workspace(const CallDesc&, int) { return 0; }
-
-cudaError_t launch_logprobs(const LaunchCtx& c, const CallDesc& d, const void* logits, const void* ids, const LogProbsOut& out, void*) {
+cudaError_t launch_logprobs(const LaunchCtx& c, const CallDesc& d, const void* logits, const void* ids, const LogProbsOut& out) {
   if (!d.rows) return cudaSuccess;
   cudaError_t err = cudaSuccess;
   with_types(d.in_dt, d.ids_dt, [&](auto* i, auto* id) {

@@ -636,21 +636,20 @@ void run_call(DevRun& r, const Step& st) {
     return (const char*)slot_ptr(r, slot) + c.off[k] * (int64_t)dt_size(r.plan->slots[slot].type.dt);
   };
   auto out = [&](size_t k) { return k < st.out_slot.size() ? slot_ptr(r, st.out_slot[k]) : nullptr; };
-  std::shared_ptr<Storage> work;
-  auto workspace = [&](int64_t bytes) -> void* {
-    if (!bytes) return nullptr;
-    work = std::make_shared<Storage>(d, d->alloc((size_t)bytes), (size_t)bytes);
-    return work->ptr;
-  };
   switch (c.op) {
     case CallK::Embedding: CK(launch_embedding(ctx, c, in(0), in(1), out(0))); break;
-    case CallK::EmbeddingGrad: CK(launch_embedding_grad(ctx, c, in(0), in(1), out(0), workspace(embedding_grad_workspace(c, d->sm_count)))); break;
+    case CallK::EmbeddingGrad: {
+      const size_t bytes = (size_t)embedding_grad_workspace(c, d->sm_count);
+      const auto work = bytes ? std::make_shared<Storage>(d, d->alloc(bytes), bytes) : nullptr;
+      CK(launch_embedding_grad(ctx, c, in(0), in(1), out(0), work ? work->ptr : nullptr));
+      break;
+    }
     case CallK::Dropout:
       CK(launch_dropout(ctx, c, in(0), in(1), st.leaf_slot.size() > 2 ? in(2) : nullptr, out(0), c.sharded ? (int64_t)d->global_id * c.cols : 0));
       break;
     case CallK::LogProbs: {
       const LogProbsOut o{(float*)out(0), (float*)out(1), (float*)out(2), (float*)out(3), (int32_t*)out(4)};
-      CK(launch_logprobs(ctx, c, in(0), in(1), o, workspace(logprobs_workspace(c, d->sm_count))));
+      CK(launch_logprobs(ctx, c, in(0), in(1), o));
       break;
     }
     case CallK::LogProbsGrad: {

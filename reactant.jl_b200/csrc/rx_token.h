@@ -69,8 +69,7 @@ struct LogProbsOut {
   float *logprob, *entropy, *lse, *top_value;
   int32_t* top_token;
 };
-cudaError_t launch_logprobs(const LaunchCtx& c, const CallDesc& d, const void* logits, const void* ids, const LogProbsOut& out, void* workspace);
-int64_t logprobs_workspace(const CallDesc& d, int sm_count);
+cudaError_t launch_logprobs(const LaunchCtx& c, const CallDesc& d, const void* logits, const void* ids, const LogProbsOut& out);
 struct LogProbsGradIn {
   const float *lse, *entropy, *dlogprob, *dentropy, *dlse;
 };
