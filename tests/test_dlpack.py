@@ -559,3 +559,26 @@ def test_a_slow_consumer_does_not_hold_up_the_others(rx, client, n):
     assert not done.query(), "the calls waited for the slow consumer"
     assert (got == 2).all()
     slow.synchronize()
+
+
+def test_reduction_of_an_array_that_is_still_being_written(rx, client):
+    """A full reduction may begin while the kernel in front of it ends; not while a producer still writes what it reads."""
+    n = 1 << 20
+    total = rx.compile(f"""module {{
+  func.func @main(%arg0: tensor<{n}xf32>) -> tensor<f32> {{
+    %c = stablehlo.constant dense<0.000000e+00> : tensor<f32>
+    %0 = stablehlo.reduce(%arg0 init: %c) applies stablehlo.add across dimensions = [0] : (tensor<{n}xf32>, tensor<f32>) -> tensor<f32>
+    return %0 : tensor<f32>
+  }}
+}}
+""", client)
+    own = rx.to_rarray(np.ones(n, np.float32), client)
+    side = torch.cuda.Stream()
+    for k in range(1, 5):
+        x = torch.zeros(n, device="cuda")
+        torch.cuda.synchronize()
+        total(own)
+        with torch.cuda.stream(side):
+            busy_writes(x, k)
+            a = rx.from_dlpack(x, client)
+        assert float(total(a)) == k * n
