@@ -142,7 +142,8 @@ void CopyFromBuffer(RxClient* client, RxBuffer* buffer, void* data, size_t offse
  * stream (RxDeviceStream) behind its own writes.  The array has to be dense and
  * start on a 16-byte boundary; other arrays are refused and stay the caller's.
  * Memory that another library sees, taken over or handed out and not let go of, is
- * never written by an execution: a donated argument over it is worked on as a copy.
+ * never written by an execution, nor is memory that another buffer or argument
+ * holds: a donated argument over it is worked on as a copy.
  * A consumer's or a device's stream that is being captured into a graph is an
  * error, here and when a program is executed. */
 void* RxBufferToDLPack(RxBuffer* buffer, void* consumer_stream);

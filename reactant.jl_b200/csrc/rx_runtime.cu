@@ -306,7 +306,6 @@ void RxDevice::leave_event(const std::shared_ptr<Storage>& st, cudaStream_t cons
       n_returned.store((int)(returned.size() + parked.size()));
       return;
     }
-    st->lent.fetch_sub(1);
     return;
   }
   std::lock_guard<std::mutex> g(st->pending_mu);
@@ -317,7 +316,6 @@ void RxDevice::leave_event(const std::shared_ptr<Storage>& st, cudaStream_t cons
   }
   st->pending = ev;
   st->pending_from = id;
-  st->lent.fetch_sub(1);
 }
 
 void RxDevice::reap(bool all) {
@@ -1039,6 +1037,14 @@ void check_arg(const Plan& p, int i, RxBuffer* b, RxDevice* d) {
   }
 }
 
+// Whether anything but one buffer holds the memory: another library that owns it or was handed it, another buffer (a result
+// that is an argument, returned as it came), an argument that was bound before this one.
+bool seen_elsewhere(const std::shared_ptr<Storage>& st) {
+  const bool others = st->foreign || st.use_count() > 1;
+  std::atomic_thread_fence(std::memory_order_acquire);  // what the last of them did before it let go has been done
+  return others;
+}
+
 // Runs the plan on `devs` (one program instance per device), args laid out [device][arg].
 void execute(RxExecutable* ex, const std::vector<RxDevice*>& devs, RxBuffer** args, int nargs_per_dev, const uint8_t* donatable,
              int num_results, RxBuffer** results, uint8_t* futures, RxFuture** future_results) {
@@ -1073,10 +1079,14 @@ void execute(RxExecutable* ex, const std::vector<RxDevice*>& devs, RxBuffer** ar
       const Slot& sl = p.slots[s];
       if (sl.kind == SlotK::Arg) {
         RxBuffer* b = args[k * nargs_per_dev + sl.arg_index];
-        const bool kept = !(donatable && donatable[sl.arg_index]) || b->st->shared();  // asked before the wait for what a consumer left
+        // asked before the wait for what a consumer left behind when it let go
+        bool kept = !(donatable && donatable[sl.arg_index]) || seen_elsewhere(b->st);
+        if (sl.writable && !kept)
+          for (int i = sl.arg_index + 1; i < nargs_per_dev; ++i) kept = kept || args[k * nargs_per_dev + i]->st == b->st;
         b->st->make_ready();
         if (sl.writable && kept) {
-          // the plan updates this argument in place but the caller, or another library, keeps it: work on a private copy
+          // the plan updates this argument in place but the caller, another array, argument or library keeps it: work on
+          // a private copy
           size_t bytes = (size_t)sl.bytes();
           auto st = std::make_shared<Storage>(d, d->alloc(bytes), bytes);
           CK(cudaMemcpyAsync(st->ptr, b->st->ptr, bytes, cudaMemcpyDeviceToDevice, d->stream));
@@ -1478,19 +1488,12 @@ struct HandedOut {
 void handed_out_deleter(rx::DLManagedTensor* t) {
   std::unique_ptr<HandedOut> h((HandedOut*)t->manager_ctx);
   RxDevice* d = h->st->dev;
-  if (!h->ordered) {
-    h->st->lent.fetch_sub(1);
-    return;
-  }
+  if (!h->ordered) return;
   int cur = 0;
   cudaGetDevice(&cur);
   if (cur != d->ordinal) cudaSetDevice(d->ordinal);
-  if (!d->closed.load()) {
-    d->leave_event(h->st, h->consumer, h->id);
-  } else {
-    if (h->st->foreign) cudaDeviceSynchronize();  // the owner may get it back next; memory of the pool goes to the driver, which waits itself
-    h->st->lent.fetch_sub(1);
-  }
+  if (!d->closed.load()) d->leave_event(h->st, h->consumer, h->id);
+  else if (h->st->foreign) cudaDeviceSynchronize();  // the owner may get it back next; memory of the pool goes to the driver, which waits itself
   h.reset();
   if (cur != d->ordinal) cudaSetDevice(cur);
 }
@@ -1542,7 +1545,6 @@ void* RxBufferToDLPack(RxBuffer* b, void* consumer_stream) {
   h->t.dl_tensor = {b->st->ptr, {rx::kDLCUDA, d->ordinal}, (int32_t)n, dl_type(b->dt), h->shape.data(), h->strides.data(), 0};
   h->t.manager_ctx = h.get();
   h->t.deleter = handed_out_deleter;
-  h->st->lent.fetch_add(1);
   return &h.release()->t;
   API_END(nullptr)
 }

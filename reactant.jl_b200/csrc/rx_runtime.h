@@ -129,9 +129,6 @@ struct Storage {
   cudaEvent_t pending = nullptr;
   unsigned long long pending_from = 0;  // the id of the consumer's stream
   void* foreign = nullptr;  // the DLPack tensor that owns this memory, when it was taken over from another library
-  // Consumers that were handed this memory (DLPack) and have not let go of it, or whose last use no event covers yet.
-  std::atomic<int> lent{0};
-  bool shared() const { return foreign || lent.load() > 0; }  // another library sees it: not to be written in place
   Storage(RxDevice* d, void* p, size_t b) : dev(d), keep(d->shared_from_this()), ptr(p), bytes(b) {}
   void make_ready() {  // call with the owning device current
     std::lock_guard<std::mutex> g(pending_mu);

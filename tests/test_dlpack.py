@@ -582,3 +582,49 @@ def test_reduction_of_an_array_that_is_still_being_written(rx, client):
             busy_writes(x, k)
             a = rx.from_dlpack(x, client)
         assert float(total(a)) == k * n
+
+
+def test_one_array_as_two_arguments_of_which_one_is_donated(rx, client):
+    """The other argument keeps its values while the donated one is updated."""
+    n = 1 << 16
+    t = f"tensor<{n}xf32>"
+    f = rx.compile(f"""module {{
+  func.func @main(%x: {t} {{tf.aliasing_output = 0 : i32}}, %v: tensor<4xf32>, %y: {t}) -> ({t}, {t}) {{
+    %c0 = stablehlo.constant dense<0> : tensor<i32>
+    %0 = stablehlo.dynamic_update_slice %x, %v, %c0 : ({t}, tensor<4xf32>, tensor<i32>) -> {t}
+    %1 = stablehlo.add %0, %y : {t}
+    return %0, %1 : {t}, {t}
+  }}
+}}
+""", client)
+    v = rx.to_rarray(np.full(4, 5, np.float32), client)
+    x = np.arange(n, dtype=np.float32)
+    want = x.copy()
+    want[:4] = 5
+    for again in range(2):
+        a = rx.to_rarray(x, client)
+        got = f(a, v, a)
+        assert np.array_equal(np.asarray(got[0]), want) and np.array_equal(np.asarray(got[1]), want + x)
+        b = rx.to_rarray(x, client)  # and as two
+        got = f(b, v, rx.to_rarray(x, client))
+        assert np.array_equal(np.asarray(got[0]), want) and np.array_equal(np.asarray(got[1]), want + x)
+        same = rx.ConcreteRArray(list(b.data), b.shape, b.dtype)  # two array objects of one buffer
+        got = f(b, v, same)
+        assert np.array_equal(np.asarray(got[1]), want + want)
+
+
+def test_an_argument_returned_as_it_came_survives_its_donation(rx, client):
+    """A result that is one of the arguments shares its memory; donating either leaves the other's values."""
+    n = 1 << 16
+    t = f"tensor<{n}xf32>"
+    same = rx.compile(f"module {{\n  func.func @main(%x: {t}) -> {t} {{\n    return %x : {t}\n  }}\n}}\n", client)
+    f = rx.compile(updated(n), client)
+    v = rx.to_rarray(np.full(4, 5, np.float32), client)
+    x = np.arange(n, dtype=np.float32)
+    a = rx.to_rarray(x, client)
+    b = same(a)
+    f(b, v)
+    assert np.array_equal(np.asarray(a), x) and np.asarray(b)[:4].tolist() == [5, 5, 5, 5]
+    c = same(a)
+    f(a, v)
+    assert np.array_equal(np.asarray(c), x) and np.asarray(a)[:4].tolist() == [5, 5, 5, 5]
