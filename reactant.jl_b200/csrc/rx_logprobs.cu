@@ -28,11 +28,6 @@ __device__ __forceinline__ float nan_max3(float a, float b, float c) {
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-__device__ __forceinline__ float warp_max(float v) {  // NaN if any lane has one
-  float r;
-  asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
-  return r;
-}
 // two floats in one 64-bit register, one instruction for both
 using Pair = uint64_t;
 __device__ __forceinline__ Pair pair(float lo, float hi) {
@@ -61,14 +56,16 @@ __device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
 // With c = log2(e) / temperature and a reference ref, one pass keeps
 //     s = sum 2^a,   w = sum 2^a a,   a = c (x - ref),
 // from which lse = ref / temperature + ln s and H = ln s - ln(2) w / s.  The reference need not be the maximum: it is
-// the largest value of the first vectors that a warp meets, and a lane's moves only when a logit lies 2^kSlack above it, so
-// the sums are almost never rescaled and cannot overflow.  How far below the maximum it may lie decides how much of H is lost
-// when ln s and w / s, both up to kSlack then, are subtracted: on 2048 rows of 50016 logits with one token standing out, H
-// is off by 3.9e-7 (rms; the definition in 32 bits 4.3e-7), with a slack of 16 and each lane's own first vector 1.6e-6 and 12e-6 at
-// most, for 1.5 % of the time.  x - ref is exact where it matters, whatever the size of the logits.
+// the maximum of the first vector a thread meets, and moves only when a logit lies 2^kSlack above it, so the sums are
+// almost never rescaled and cannot overflow.  How far below the maximum it may lie decides how much of H is lost when ln s
+// and w / s, both up to kSlack then, are subtracted, and how much of s and w is rounded away next to a large term; a vector's
+// eight terms are therefore added up before they join the sums.  On 2048 rows of 50016 logits with one token standing out, H is
+// off by 3.7e-7 (rms; the definition in 32 bits 4.3e-7) and 1.3e-6 at most; with a slack of 16 and every term added
+// singly 1.6e-6 and 12e-6, for 1 to 4 % less time (4096 x 131072 bf16 172 us, now 176; a slack of 6 takes 177).
+// x - ref is exact where it matters, whatever the size of the logits.
 // Arguments are cut at kFloor, where 2^a is 0 already: -inf, and a mask of the type's lowest value, add 0 and not
 // 0 * inf.  NaN and +inf go through (cut and maxima propagate NaN; inf - inf is NaN).
-constexpr float kSlack = 3.f, kFloor = -300.f;
+constexpr float kSlack = 8.f, kFloor = -300.f;
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 
 struct RowSum {
@@ -97,30 +94,23 @@ struct Running {
     ref = top;
     limit = top + slack;
   }
-  // The reference of a warp before anything is added: the largest of its first values, `top` of each lane.
-  __device__ __forceinline__ void start(float top) {
-    top = warp_max(top);
-    if (!(top <= ref)) {
-      ref = top;
-      limit = top + slack;
-    }
-  }
   __device__ __forceinline__ float push(const float (&v)[8]) {  // returns the largest
     const float top = nan_max3(nan_max3(v[0], v[1], v[2]), nan_max3(v[3], v[4], v[5]), nan_max(v[6], v[7]));
     if (!(top <= limit)) move(top);
     const Pair minus = pair(-ref, -ref), cc = pair(c, c);
-    Pair e[4], ea;
+    Pair vs, vw;  // of this vector
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       float a0, a1;
       split(mul2(add2(pair(v[2 * q], v[2 * q + 1]), minus), cc), a0, a1);
       a0 = nan_max(a0, kFloor);
       a1 = nan_max(a1, kFloor);
-      e[q] = pair(exp2_fast(a0), exp2_fast(a1));
-      ea = q == 0 ? mul2(e[q], pair(a0, a1)) : fma2(e[q], pair(a0, a1), ea);
+      const Pair e = pair(exp2_fast(a0), exp2_fast(a1));
+      vs = q == 0 ? e : add2(vs, e);
+      vw = q == 0 ? mul2(e, pair(a0, a1)) : fma2(e, pair(a0, a1), vw);
     }
-    s = add2(s, add2(add2(e[0], e[1]), add2(e[2], e[3])));  // a quarter of the roundings next to a large sum
-    w = add2(w, ea);
+    s = add2(s, vs);  // a quarter of the roundings next to a large sum
+    w = add2(w, vw);
     return top;
   }
   __device__ __forceinline__ void push1(float x) {
@@ -136,20 +126,6 @@ struct Running {
     return {ref, s0 + s1, w0 + w1};
   }
 };
-
-// the largest element of those of a lane's vectors that are there
-template <class R, int N, class There>
-__device__ __forceinline__ float largest_of(const R (&raw)[N], There there) {
-  float top = -INFINITY;
-#pragma unroll
-  for (int k = 0; k < N; ++k) {
-    if (!there(k)) break;
-    float v[8];
-    widen8(raw[k], v);
-    top = nan_max(top, nan_max3(nan_max3(v[0], v[1], v[2]), nan_max3(v[3], v[4], v[5]), nan_max(v[6], v[7])));
-  }
-  return top;
-}
 
 // The sums of W neighbouring lanes together, in all of them: one common reference, one rescaling per lane, and sums in
 // the order of a butterfly (the same in every lane: a + b is b + a).
@@ -406,7 +382,7 @@ constexpr int kWarpTop = 32, kWarpSpells = 16;
 constexpr int kWarpCap = 256 + kWarpTop + kMaxLoose;
 
 template <class T, class Id, bool TOP>
-__global__ void __launch_bounds__(kBlock, TOP ? 3 : 4) k_logprobs_warp(const T* __restrict__ logits, const Id* __restrict__ ids, int64_t rows, int64_t cols, int64_t ld, float scale, int top_k, LogProbsOut out) {
+__global__ void __launch_bounds__(kBlock, !TOP && sizeof(T) == 4 ? 4 : 0) k_logprobs_warp(const T* __restrict__ logits, const Id* __restrict__ ids, int64_t rows, int64_t cols, int64_t ld, float scale, int top_k, LogProbsOut out) {
   constexpr int kWarps = kBlock / 32, kFly = 4;
   __shared__ uint64_t buf_[TOP ? kWarps : 1][kWarpCap], best_[TOP ? kWarps : 1][kWarpTop];
   __shared__ float spell_[TOP ? kWarps : 1][TOP ? kWarpSpells * 32 : 1];
@@ -419,7 +395,11 @@ __global__ void __launch_bounds__(kBlock, TOP ? 3 : 4) k_logprobs_warp(const T* 
   Running run(c);
   float mine = -INFINITY;
   const int loose = sp.loose();
-  const float extra = lane < loose ? widen(sp.x[sp.loose_at(lane)]) : -INFINITY;
+  float extra = -INFINITY;
+  if (lane < loose) {
+    extra = widen(sp.x[sp.loose_at(lane)]);
+    run.push1(extra);
+  }
   const int vecs = (int)sp.vecs, tiles = (vecs + 32 * kFly - 1) / (32 * kFly), per = TOP ? (tiles + kWarpSpells - 1) / kWarpSpells : tiles;
   const T* body = sp.x + sp.head;
   for (int g = 0, tile = 0; tile < tiles; ++g) {
@@ -430,7 +410,6 @@ __global__ void __launch_bounds__(kBlock, TOP ? 3 : 4) k_logprobs_warp(const T* 
 #pragma unroll
       for (int k = 0; k < kFly; ++k)
         if (v0 + k * 32 < vecs) raw[k] = TOP ? load8_cached(body + (v0 + k * 32) * 8) : load8(body + (v0 + k * 32) * 8);
-      if (tile == 0) run.start(largest_of(raw, [&](int k) { return v0 + k * 32 < vecs; }));
 #pragma unroll
       for (int k = 0; k < kFly; ++k) {
         if (v0 + k * 32 >= vecs) break;
@@ -445,7 +424,6 @@ __global__ void __launch_bounds__(kBlock, TOP ? 3 : 4) k_logprobs_warp(const T* 
       mine = nan_max(mine, spell);
     }
   }
-  if (lane < loose) run.push1(extra);
   const RowSum a = lanes_sum<32>(run.sum(), c);
   const RowOut o(a, scale);
   if (lane == 0) write_row(a, o, sp.x, ids, row, cols, out);
@@ -600,7 +578,7 @@ __global__ void __launch_bounds__(kLong, kLong == 128 ? 6 : 1) k_logprobs_block(
   const int64_t lo = min(sp.vecs, share * rank), hi = min(sp.vecs, lo + share);
   const int tid = threadIdx.x, loose = rank == 0 ? sp.loose() : 0;
   Running run(c);
-  const float extra = tid < loose ? widen(sp.x[sp.loose_at(tid)]) : -INFINITY;
+  if (tid < loose) run.push1(widen(sp.x[sp.loose_at(tid)]));
   const int tiles = (int)((hi - lo + kTile - 1) / kTile), per = TOP ? max(1, (tiles + kSpells - 1) / kSpells) : max(1, tiles);
   uint32_t thread_top = 0;
   const int mine = (int)(hi - lo) - tid;  // vectors from this thread's first one to the end of the block's run
@@ -619,7 +597,6 @@ __global__ void __launch_bounds__(kLong, kLong == 128 ? 6 : 1) k_logprobs_block(
 #pragma unroll
       for (int k = 0; k < kFly; ++k)
         if (at + k * kLong < mine) next[k] = load8(body + (int64_t)(at + k * kLong) * 8);
-      if (tile == 0) run.start(largest_of(raw, [&](int k) { return k * kLong < mine; }));
 #pragma unroll
       for (int k = 0; k < kFly; ++k) {
         if (at - kTile + k * kLong >= mine) break;
@@ -636,7 +613,6 @@ __global__ void __launch_bounds__(kLong, kLong == 128 ? 6 : 1) k_logprobs_block(
       thread_top = max(thread_top, key);
     }
   }
-  if (tid < loose) run.push1(extra);
   RowSum a = lanes_sum<32>(run.sum(), c);
   if ((tid & 31) == 0) part[tid >> 5] = a;
   __syncthreads();
@@ -653,7 +629,10 @@ __global__ void __launch_bounds__(kLong, kLong == 128 ? 6 : 1) k_logprobs_block(
       const uint32_t key = t.spell[g][tid];
       if (key >= reach && key != 0u) t.item[atomicAdd(&t.n_items, 1)] = (uint16_t)(g * kLong + tid);
     }
-    if (tid < loose) t.buf[atomicAdd(&t.n, 1)] = order_key(extra, (uint32_t)sp.loose_at(tid));
+    if (tid < loose) {
+      const int64_t at = sp.loose_at(tid);
+      t.buf[atomicAdd(&t.n, 1)] = order_key(widen(sp.x[at]), (uint32_t)at);
+    }
     __syncthreads();
     const int slots = t.n_items * per * kFly;
     uint64_t least = reach ? ((uint64_t)reach << 32) - 1 : 0;  // a key has to be above this to be among the k best
